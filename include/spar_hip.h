@@ -102,6 +102,10 @@ enum SparHipReductionOp {
  * spar_hip_launch_axis_reduction_no_alloc (8 MiB). */
 #define SPAR_HIP_NO_ALLOC_SCRATCH_BYTES (8u << 20)
 
+/* Widest heads of the fused head norm and of attention. */
+#define SPAR_HIP_HEAD_NORM_MAX_EXTENT 256
+#define SPAR_HIP_ATTENTION_MAX_EXTENT 256
+
 /* Replaces struct SparCudaStatus (cuda_kernels.hpp:41-44). */
 struct SparHipStatus {
   int code;
@@ -140,6 +144,80 @@ struct SparHipAdamwTensor {
   uint64_t count;
   double first_correction;
   double second_correction;
+};
+
+/* Heads of a [batch, heads, tokens, extent] tensor: element (b, h, t, d) at
+ * data[b * strides[0] + h * strides[1] + t * strides[2] + d], of the call's
+ * dtype.  Any strides: a cache or projection of either order, or a block of a
+ * packed one, is read and written in place.  No reference counterpart (its
+ * attention copies heads into [batch, heads, tokens, extent] order first). */
+struct SparHipHeads {
+  void* data;
+  uint64_t strides[3]; /* batch, head, token */
+};
+
+/* How a head's first rotary_extent elements pair up for the rotation: element
+ * j with j + rotary_extent / 2, or 2j with 2j + 1 (the reference's layout,
+ * cuda_kernels.cu:663-687). */
+enum SparHipRotaryLayout {
+  SPAR_HIP_ROTARY_HALF = 0,
+  SPAR_HIP_ROTARY_INTERLEAVED = 1,
+};
+
+/* The rotation of token t of sequence b: pair j of a head turns by
+ * positions[b * position_stride + t] * frequencies[j] radians (the product in
+ * double, whatever the heads' dtype) and is multiplied by magnitude. */
+struct SparHipRotary {
+  const void* positions;     /* SPAR_HIP_INT32 or SPAR_HIP_INT64, device memory  */
+  uint64_t position_stride;  /* elements between sequences; 0: one row for all   */
+  int position_dtype;
+  const double* frequencies; /* rotary_extent / 2 values in device memory        */
+  uint64_t rotary_extent;    /* even, at most the heads' extent; the rest of a
+                                head is passed on                                */
+  double magnitude;          /* finite                                           */
+  int layout;                /* SparHipRotaryLayout                              */
+};
+
+/* One tensor of spar_hip_launch_head_norm_rotary_forward. */
+struct SparHipHeadNorm {
+  struct SparHipHeads output;
+  void* denominator; /* [batch, heads, tokens], contiguous: sqrt(mean(x * x) + eps);
+                        NULL where no backward follows */
+  struct SparHipHeads input;
+  const void* weight; /* [extent] */
+  uint64_t heads;
+};
+
+/* One tensor of spar_hip_launch_head_norm_rotary_backward. */
+struct SparHipHeadNormGradient {
+  struct SparHipHeads input_gradient;
+  void* weight_gradient; /* [extent] */
+  struct SparHipHeads output_gradient;
+  struct SparHipHeads input;
+  const void* weight;
+  const void* denominator; /* as the forward saved it */
+  uint64_t heads;
+};
+
+/* What an attention call computes: query_heads is a multiple of key_heads, and
+ * query head h reads key head h / (query_heads / key_heads).  Query i of
+ * sequence b is its token p = length(b) - queries + i, length(b) = lengths[b]
+ * clamped to [0, keys] (keys where lengths is NULL), and sees key j when
+ *   j <= p  and  (window == 0  or  p - j < window  or  j < sinks);
+ * queries with p < 0 see nothing. */
+struct SparHipAttention {
+  uint64_t batch;
+  uint64_t query_heads;
+  uint64_t key_heads;
+  uint64_t queries;    /* per sequence */
+  uint64_t keys;       /* per sequence */
+  uint64_t extent;     /* of a head; at most SPAR_HIP_ATTENTION_MAX_EXTENT */
+  uint64_t window;     /* newest keys a query sees; 0: all of them */
+  uint64_t sinks;      /* first keys that stay visible behind the window */
+  double scale;        /* of the scores; finite */
+  const void* lengths; /* [batch] in device memory, or NULL */
+  int length_dtype;    /* SPAR_HIP_INT32 or SPAR_HIP_INT64 */
+  int dtype;           /* of heads: SPAR_HIP_FLOAT32 or SPAR_HIP_FLOAT64 */
 };
 
 /* ---------------------------------------------------------------- runtime */
@@ -566,6 +644,76 @@ struct SparHipStatus spar_hip_launch_cross_entropy_backward(
     const void* row_log_sum, const int32_t* undefined_rows, const void* targets,
     uint64_t logits_rows, uint64_t classes, uint64_t sequence_length, int dtype,
     int target_dtype, int language_model, int device);
+
+/* ------------------------------------- attention: positions, norms, product */
+
+/* The entry points of this section allocate nothing and copy nothing from the
+ * host: they may be captured into a graph.  Outputs must not overlap inputs,
+ * unless an output names an input's very elements (the same data and strides)
+ * where that is said.  A workspace is device memory of at least the bytes its
+ * query returns, 16-byte aligned, free for others once the call's work is done:
+ * two calls that may run at once need one each. */
+
+/* output = the heads of `input` turned by their positions (inverse = 0), or by
+ * the opposite angles (inverse = 1: the gradient of the former).  The output may
+ * be the input itself.  Replaces the reference's rope kernel and launcher
+ * (cuda_kernels.cu:663-687, :1036-1067), which turn whole heads of interleaved
+ * pairs. */
+struct SparHipStatus spar_hip_launch_rotary(const struct SparHipHeads* output,
+                                            const struct SparHipHeads* input, uint64_t batch,
+                                            uint64_t heads, uint64_t tokens, uint64_t extent,
+                                            const struct SparHipRotary* rotary, int inverse,
+                                            int dtype, int device);
+
+/* RMSNorm of every head and the rotation of the result, for one or two tensors
+ * (a layer's queries and keys) in one launch:
+ *   d = sqrt(sum(x * x) / extent + epsilon), y = rotation((x / d) * weight).
+ * An output may be its part's input itself.  No reference counterpart. */
+struct SparHipStatus spar_hip_launch_head_norm_rotary_forward(
+    const struct SparHipHeadNorm* parts, int part_count, uint64_t batch, uint64_t tokens,
+    uint64_t extent, const struct SparHipRotary* rotary, double epsilon, int dtype, int device);
+
+/* Bytes of the backward's workspace, for `heads` heads in all parts together. */
+struct SparHipStatus spar_hip_head_norm_rotary_workspace(uint64_t* bytes, uint64_t batch,
+                                                         uint64_t tokens, uint64_t heads,
+                                                         uint64_t extent, int dtype);
+
+/* Its backward: the gradients of the inputs and the weights (sums over batch,
+ * heads and tokens in a fixed order).  An input gradient may be its part's
+ * output gradient itself. */
+struct SparHipStatus spar_hip_launch_head_norm_rotary_backward(
+    const struct SparHipHeadNormGradient* parts, int part_count, uint64_t batch, uint64_t tokens,
+    uint64_t extent, const struct SparHipRotary* rotary, void* workspace,
+    uint64_t workspace_bytes, int dtype, int device);
+
+/* Bytes of the workspace of the forward (backward = 0) or the backward (1). */
+struct SparHipStatus spar_hip_attention_workspace(uint64_t* bytes,
+                                                  const struct SparHipAttention* attention,
+                                                  int backward);
+
+/* output = softmax(scale * query key^T over the visible keys) value, and zeros
+ * for queries that see no key.  query and output have query_heads heads of
+ * `queries` tokens, key and value key_heads heads of `keys` tokens.  logsumexp
+ * [batch, query_heads, queries], contiguous, is kept for the backward (-inf where
+ * no key is seen); it may be NULL.  Keys and values that no query sees are not
+ * used, whatever they hold.  Replaces the reference's scores, mask and softmax
+ * over whole [queries, keys] matrices (nn/attention.cpp:122-135). */
+struct SparHipStatus spar_hip_launch_attention_forward(
+    const struct SparHipHeads* output, void* logsumexp, const struct SparHipHeads* query,
+    const struct SparHipHeads* key, const struct SparHipHeads* value,
+    const struct SparHipAttention* attention, void* workspace, uint64_t workspace_bytes,
+    int device);
+
+/* Its backward from the saved output and logsumexp: the gradients of query, key
+ * and value (zeros for queries that see nothing and for keys that no query
+ * sees), sums in a fixed order. */
+struct SparHipStatus spar_hip_launch_attention_backward(
+    const struct SparHipHeads* query_gradient, const struct SparHipHeads* key_gradient,
+    const struct SparHipHeads* value_gradient, const struct SparHipHeads* output_gradient,
+    const struct SparHipHeads* output, const void* logsumexp, const struct SparHipHeads* query,
+    const struct SparHipHeads* key, const struct SparHipHeads* value,
+    const struct SparHipAttention* attention, void* workspace, uint64_t workspace_bytes,
+    int device);
 
 /* ---------------------------------------------- optimizer and gradient norm */
 

@@ -1,0 +1,466 @@
+// Attention backward from the saved output and logsumexp: with P the weights,
+// dP = do v^T and delta = do . o per row,
+//   dS = P (dP - delta),  dq = scale dS k,  dk = scale dS^T q,  dv = P^T do.
+//
+// Two kernels, so that every gradient has one writer and sums in a fixed order.
+// query_kernel keeps 16 rows per wave and walks the keys they see (as the forward
+// does); it also leaves delta behind.  key_kernel keeps 16 keys per wave and walks
+// the rows that see them, the heads of a group among them.  Each recomputes S and
+// dP: seven products instead of the five that one kernel with shared sums of dq
+// would need, for results that do not depend on the order of workgroups.  In both,
+// P and dS pass from the products that yield them into those that consume them in
+// registers (attention.hpp).
+//
+// The sinks are seen by every later row, so their keys have thousands of rows
+// where others have the window's: rows behind a tile's own window are split over
+// `splits` workgroups that write parts, which sink_kernel adds in their order.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "attention.hpp"
+
+namespace spar_hip {
+namespace attention {
+namespace {
+
+template <typename T>
+struct Saved {
+  Heads<const T> query, key, value, output, output_gradient;
+  const T* logsumexp;  // [batch][query head][query]
+  T* delta;            // the same
+};
+
+template <typename T>
+struct Gradients {
+  Heads<T> query, key, value;
+  T* parts;         // [batch head][sink tile][split][dk, dv][64][extent]
+  uint32_t splits;  // of the rows behind a sink tile's window; 0: none
+  uint32_t sink_tiles;
+};
+
+// Query head, query and place among [batch][query head][query] of a row.
+struct Place {
+  uint32_t head, t;
+  uint64_t at;
+
+  __device__ __forceinline__ Place(const Call& call, uint32_t b, uint32_t key_head, uint32_t r) {
+    t = call.group.div(r);
+    head = key_head * call.group.divisor + (r - t * call.group.divisor);
+    at = (static_cast<uint64_t>(b) * call.key_heads * call.group.divisor + head) * call.queries +
+         t;
+  }
+  template <typename T>
+  __device__ __forceinline__ T* of(const Heads<T>& heads, uint32_t b) const {
+    return heads.data + b * heads.batch + head * heads.head + t * heads.token;
+  }
+};
+
+template <typename T, int DP, int KB>
+__global__ __launch_bounds__(kThreads) void query_kernel(Call call, Saved<T> saved,
+                                                         Heads<T> gradient, uint32_t row_tiles) {
+  constexpr int KT = KB * kBlock;
+  constexpr int W = Vec16<T>::width;
+  constexpr uint32_t kRows = kWaves * kBlock;
+  __shared__ Tile<T, KT, DP> keys, values;
+  const uint32_t batch_head = blockIdx.x % call.batch_heads;
+  const uint32_t row_tile = row_tiles - 1 - blockIdx.x / call.batch_heads;
+  const uint32_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave;
+  const int quarter = lane / kBlock, column = lane % kBlock;
+
+  const int32_t first = call.length(b) - call.queries;
+  const uint32_t begin_row = row_tile * kRows;
+  const uint32_t end_row = begin_row + kRows < call.rows ? begin_row + kRows : call.rows;
+  const int32_t low_token = call.token(begin_row, first);
+  const Keys seen(call, low_token < 0 ? 0 : low_token, call.token(end_row - 1, first));
+  const uint32_t tiles = seen.tiles(KT);
+
+  const uint32_t wave_row = begin_row + wave * kBlock;
+  const uint32_t wave_end = wave_row + kBlock < call.rows ? wave_row + kBlock : call.rows;
+  const int32_t oldest = call.token(wave_row, first);
+  const int32_t newest = wave_row < wave_end ? call.token(wave_end - 1, first) : -1;
+  const uint32_t r = wave_row + column;
+  const int32_t token = call.token(r, first);
+  const Place place(call, b, key_head, r < call.rows ? r : 0);
+  Operand<T, DP> q, g;
+  q.load(token < 0 ? nullptr : place.of(saved.query, b), call.extent, quarter);
+  g.load(token < 0 ? nullptr : place.of(saved.output_gradient, b), call.extent, quarter);
+  T delta = T(0), log_sum = T(0);
+  if (token >= 0) {
+    const T* out = place.of(saved.output, b);
+#pragma unroll
+    for (int s = 0; s < DP / (4 * W); ++s) {
+      T piece[W];
+      load_piece<T, W>(piece, out, 4 * W * s + W * quarter, call.extent);
+#pragma unroll
+      for (int i = 0; i < W; ++i) delta += piece[i] * g.value[s * W + i];
+    }
+    log_sum = saved.logsumexp[place.at] * static_cast<T>(kLog2E);
+  }
+  delta = quarter_sum(delta);
+  if (quarter == 0 && r < call.rows) saved.delta[place.at] = delta;
+  q.scale(static_cast<T>(call.scale * kLog2E));
+  Along<T, DP> dq;
+  dq.clear();
+  const T* key_base = saved.key.data + b * saved.key.batch + key_head * saved.key.head;
+  const T* value_base = saved.value.data + b * saved.value.batch + key_head * saved.value.head;
+
+  for (uint32_t i = 0; i < tiles; ++i) {
+    int32_t begin, end;
+    seen.tile(i, KT, begin, end);
+    __syncthreads();
+    keys.fill(call.extent, [&](uint32_t j) {
+      return begin + j < end ? key_base + (begin + j) * saved.key.token : nullptr;
+    });
+    values.fill(call.extent, [&](uint32_t j) {
+      return begin + j < end ? value_base + (begin + j) * saved.value.token : nullptr;
+    });
+    __syncthreads();
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const int32_t k0 = begin + kb * kBlock, k1 = k0 + kBlock - 1;
+      const bool any = k0 < end && k0 <= newest &&
+                       ((oldest < 0 ? 0 : oldest) - k1 < call.window || k0 < call.sinks);
+      if (!any) continue;
+      const bool whole = k1 <= oldest && k1 < end &&
+                         (newest - k0 < call.window || k1 < call.sinks);
+      typename Mma<T>::Acc s{0, 0, 0, 0}, dp{0, 0, 0, 0};
+#pragma unroll
+      for (int step = 0; step < DP / (4 * W); ++step) {
+        const auto k_piece = keys.along(kb * kBlock + column, step, quarter);
+        const auto v_piece = values.along(kb * kBlock + column, step, quarter);
+#pragma unroll
+        for (int n = 0; n < W; ++n) {
+          s = Mma<T>::step(k_piece[n], q.value[step * W + n], s);
+          dp = Mma<T>::step(v_piece[n], g.value[step * W + n], dp);
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int32_t at = k0 + Mma<T>::row_of(v, quarter);
+        const bool visible = whole | ((at < end) & call.sees(token, at));
+        const T ds = visible ? exp2_of(s[v] - log_sum) * (dp[v] - delta) : T(0);
+        dq.add(keys.value + (kb * kBlock + Mma<T>::row_of(v, quarter)) * keys.kPitch, column, ds);
+      }
+    }
+  }
+  if (r >= call.rows) return;
+  T* target = place.of(gradient, b);
+  dq.visit(quarter, [&](uint32_t d, auto& run) {
+    for (auto& x : run) x *= static_cast<T>(call.scale);
+    store_piece(target, d, call.extent, run);
+  });
+}
+
+constexpr uint32_t kKeyTile = kWaves * kBlock;
+
+template <typename T, int DP, int RB>
+__global__ __launch_bounds__(kThreads) void key_kernel(Call call, Saved<T> saved,
+                                                       Gradients<T> gradients,
+                                                       uint32_t sink_groups, uint32_t key_tiles) {
+  constexpr int RT = RB * kBlock;
+  constexpr int W = Vec16<T>::width;
+  __shared__ Tile<T, RT, DP> queries, output_gradients;
+  __shared__ T log_sums[RT], deltas[RT];
+  __shared__ int32_t tokens[RT];
+  const uint32_t batch_head = blockIdx.x % call.batch_heads;
+  const uint32_t rest = blockIdx.x / call.batch_heads;
+  // The splits of the sinks' later rows come first, then the tiles of keys.
+  const bool behind = rest < sink_groups;
+  const uint32_t tile = behind ? rest / gradients.splits : rest - sink_groups;
+  const uint32_t split = behind ? rest % gradients.splits : 0;
+  const uint32_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave;
+  const int quarter = lane / kBlock, column = lane % kBlock;
+
+  const int32_t length = call.length(b);
+  const int32_t first = length - call.queries;
+  const int32_t begin_key = static_cast<int32_t>(tile) * kKeyTile;
+  const int32_t end_key = begin_key + kKeyTile < length ? begin_key + kKeyTile : length;
+  // Tokens that see a key of the tile through the window, or behind it as sinks.
+  int32_t low = begin_key, high = end_key - 1 + call.window;  // [low, high)
+  if (high > length) high = length;
+  if (behind) {
+    low = high;
+    high = length;
+    if (begin_key >= call.sinks) low = high;
+  }
+  if (low < first) low = first;
+  if (low < 0) low = 0;
+  if (high < low || begin_key >= length) high = low;
+  uint32_t begin_row = static_cast<uint32_t>(low - first) * call.group.divisor;
+  uint32_t end_row = static_cast<uint32_t>(high - first) * call.group.divisor;
+  if (begin_row >= end_row) begin_row = end_row = 0;
+  uint32_t tiles = (end_row - begin_row + RT - 1) / RT;
+  uint32_t begin_tile = 0;
+  if (behind) {
+    begin_tile = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * split / gradients.splits);
+    tiles = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / gradients.splits);
+  }
+
+  const int32_t own = begin_key + wave * kBlock + column;
+  const int32_t wave_key = begin_key + wave * kBlock;
+  const bool keeps = own < length;
+  const T* key_base = saved.key.data + b * saved.key.batch + key_head * saved.key.head;
+  const T* value_base = saved.value.data + b * saved.value.batch + key_head * saved.value.head;
+  Operand<T, DP> k, x;
+  k.load(keeps ? key_base + own * saved.key.token : nullptr, call.extent, quarter);
+  x.load(keeps ? value_base + own * saved.value.token : nullptr, call.extent, quarter);
+  k.scale(static_cast<T>(call.scale * kLog2E));
+  Along<T, DP> dk, dv;
+  dk.clear();
+  dv.clear();
+
+  for (uint32_t i = begin_tile; i < tiles; ++i) {
+    const uint32_t row0 = begin_row + i * RT;
+    __syncthreads();
+    queries.fill(call.extent, [&](uint32_t j) -> const T* {
+      const uint32_t r = row0 + j;
+      return r < end_row ? Place(call, b, key_head, r).of(saved.query, b) : nullptr;
+    });
+    output_gradients.fill(call.extent, [&](uint32_t j) -> const T* {
+      const uint32_t r = row0 + j;
+      return r < end_row ? Place(call, b, key_head, r).of(saved.output_gradient, b) : nullptr;
+    });
+    if (threadIdx.x < RT) {
+      const uint32_t r = row0 + threadIdx.x;
+      const bool row = r < end_row;
+      const Place place(call, b, key_head, row ? r : begin_row);
+      tokens[threadIdx.x] = row ? call.token(r, first) : -1;
+      log_sums[threadIdx.x] = row ? saved.logsumexp[place.at] * static_cast<T>(kLog2E) : T(0);
+      deltas[threadIdx.x] = row ? saved.delta[place.at] : T(0);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const uint32_t block_row = row0 + rb * kBlock;
+      if (block_row >= end_row) break;
+      const uint32_t block_end =
+          block_row + kBlock < end_row ? block_row + kBlock : end_row;
+      const int32_t oldest = call.token(block_row, first);
+      const int32_t newest = call.token(block_end - 1, first);
+      const int32_t last_key = wave_key + kBlock - 1;
+      const bool any = wave_key < length && wave_key <= newest &&
+                       (oldest - last_key < call.window || wave_key < call.sinks);
+      if (!any) continue;
+      const bool whole = last_key <= oldest && block_end - block_row == kBlock &&
+                         (newest - wave_key < call.window || last_key < call.sinks);
+      typename Mma<T>::Acc s{0, 0, 0, 0}, dp{0, 0, 0, 0};
+#pragma unroll
+      for (int step = 0; step < DP / (4 * W); ++step) {
+        const auto q_piece = queries.along(rb * kBlock + column, step, quarter);
+        const auto g_piece = output_gradients.along(rb * kBlock + column, step, quarter);
+#pragma unroll
+        for (int n = 0; n < W; ++n) {
+          s = Mma<T>::step(q_piece[n], k.value[step * W + n], s);
+          dp = Mma<T>::step(g_piece[n], x.value[step * W + n], dp);
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int row = rb * kBlock + Mma<T>::row_of(v, quarter);
+        const bool visible = whole | call.sees(tokens[row], own);
+        const T p = visible ? exp2_of(s[v] - log_sums[row]) : T(0);
+        const T ds = visible ? p * (dp[v] - deltas[row]) : T(0);
+        dv.add(output_gradients.value + row * output_gradients.kPitch, column, p);
+        dk.add(queries.value + row * queries.kPitch, column, ds);
+      }
+    }
+  }
+
+  T* dk_target;
+  T* dv_target;
+  if (behind) {
+    T* part = gradients.parts +
+              ((static_cast<uint64_t>(batch_head) * gradients.sink_tiles + tile) *
+                   gradients.splits + split) * 2 * kKeyTile * call.extent;
+    dk_target = part + static_cast<uint64_t>(wave * kBlock + column) * call.extent;
+    dv_target = dk_target + static_cast<uint64_t>(kKeyTile) * call.extent;
+  } else {
+    if (own >= call.keys) return;
+    dk_target = gradients.key.data + b * gradients.key.batch + key_head * gradients.key.head +
+                own * gradients.key.token;
+    dv_target = gradients.value.data + b * gradients.value.batch +
+                key_head * gradients.value.head + own * gradients.value.token;
+  }
+  dk.visit(quarter, [&](uint32_t d, auto& run) {
+    for (auto& y : run) y *= static_cast<T>(call.scale);
+    store_piece(dk_target, d, call.extent, run);
+  });
+  dv.visit(quarter, [&](uint32_t d, auto& run) { store_piece(dv_target, d, call.extent, run); });
+}
+
+// dk and dv of the sinks: the window's part, as key_kernel wrote it, and the parts
+// of the later rows in their order.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sink_kernel(Call call, Gradients<T> gradients,
+                                                        uint32_t sinks) {
+  const uint64_t at = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const uint64_t per_head = static_cast<uint64_t>(sinks) * call.extent;
+  const uint64_t batch_head = at / per_head;
+  if (batch_head >= call.batch_heads) return;
+  const uint32_t within = static_cast<uint32_t>(at - batch_head * per_head);
+  const uint32_t key = within / call.extent, d = within % call.extent;
+  const uint64_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
+  const uint64_t stride = static_cast<uint64_t>(kKeyTile) * call.extent;
+  const T* part = gradients.parts +
+                  (batch_head * gradients.sink_tiles + key / kKeyTile) * gradients.splits * 2 *
+                      stride +
+                  static_cast<uint64_t>(key % kKeyTile) * call.extent + d;
+  T* dk = gradients.key.data + b * gradients.key.batch + key_head * gradients.key.head +
+          key * gradients.key.token + d;
+  T* dv = gradients.value.data + b * gradients.value.batch + key_head * gradients.value.head +
+          key * gradients.value.token + d;
+  T sum_k = *dk, sum_v = *dv;
+  for (uint32_t s = 0; s < gradients.splits; ++s) {
+    sum_k += part[2 * s * stride];
+    sum_v += part[(2 * s + 1) * stride];
+  }
+  *dk = sum_k;
+  *dv = sum_v;
+}
+
+// ---------------------------------------------------------------- launchers
+
+struct Plan {
+  uint32_t row_tiles, key_tiles, sink_tiles, splits;
+  uint64_t delta_bytes;  // a multiple of 16
+  uint64_t bytes;
+};
+
+// At most this many parts per sink tile.
+constexpr uint64_t kMostSplits = 64;
+
+Plan plan_of(const SparHipAttention& a) {
+  Plan plan{};
+  const uint64_t element = a.dtype == SPAR_HIP_FLOAT32 ? sizeof(float) : sizeof(double);
+  const uint64_t group = a.query_heads / a.key_heads;
+  plan.row_tiles = ceil_div_u32(a.queries * group, kWaves * kBlock);
+  plan.key_tiles = ceil_div_u32(a.keys, kKeyTile);
+  plan.delta_bytes =
+      (a.batch * a.query_heads * a.queries * element + 15) / 16 * 16;
+  const uint64_t sinks = std::min(a.sinks, a.keys);
+  // A split for as many later queries as a tile of keys has in its window.
+  if (a.window != 0 && sinks != 0 && a.keys > a.window) {
+    plan.sink_tiles = ceil_div_u32(sinks, kKeyTile);
+    const uint64_t later = std::min(a.queries, a.keys - a.window);
+    plan.splits = static_cast<uint32_t>(
+        std::min(kMostSplits, (later + a.window + kKeyTile - 1) / (a.window + kKeyTile)));
+  }
+  plan.bytes = plan.delta_bytes + a.batch * a.key_heads * plan.sink_tiles * plan.splits * 2 *
+                                      kKeyTile * a.extent * element;
+  return plan;
+}
+
+template <typename T>
+void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& query_gradient,
+           const SparHipHeads& key_gradient, const SparHipHeads& value_gradient,
+           const SparHipHeads& output_gradient, const SparHipHeads& output, const void* logsumexp,
+           const SparHipHeads& query, const SparHipHeads& key, const SparHipHeads& value,
+           void* workspace, hipStream_t stream) {
+  const Call call = call_of(a);
+  const Saved<T> saved{heads_of<const T>(query), heads_of<const T>(key), heads_of<const T>(value),
+                       heads_of<const T>(output), heads_of<const T>(output_gradient),
+                       static_cast<const T*>(logsumexp), static_cast<T*>(workspace)};
+  const Gradients<T> gradients{
+      heads_of<T>(query_gradient), heads_of<T>(key_gradient), heads_of<T>(value_gradient),
+      reinterpret_cast<T*>(static_cast<char*>(workspace) + plan.delta_bytes), plan.splits,
+      plan.sink_tiles};
+  const uint32_t sink_groups = plan.sink_tiles * plan.splits;
+  with_width(a.extent, [&](auto width) {
+    constexpr int DP = decltype(width)::value;
+    constexpr int KB = sizeof(T) == 4 ? 2 : 1;
+    if (call.rows != 0) {
+      query_kernel<T, DP, KB><<<plan.row_tiles * call.batch_heads, kThreads, 0, stream>>>(
+          call, saved, gradients.query, plan.row_tiles);
+    }
+    if (call.keys != 0) {
+      key_kernel<T, DP, KB>
+          <<<(plan.key_tiles + sink_groups) * call.batch_heads, kThreads, 0, stream>>>(
+              call, saved, gradients, sink_groups, plan.key_tiles);
+    }
+  });
+  if (sink_groups != 0) {
+    const uint32_t sinks = static_cast<uint32_t>(std::min(a.sinks, a.keys));
+    sink_kernel<T><<<ceil_div_u32(static_cast<uint64_t>(call.batch_heads) * sinks * a.extent,
+                                  kThreads),
+                     kThreads, 0, stream>>>(call, gradients, sinks);
+  }
+}
+
+bool fits(const SparHipAttention& a, const Plan& plan) {
+  const uint64_t batch_heads = a.batch * a.key_heads;
+  return (static_cast<uint64_t>(plan.key_tiles) +
+          static_cast<uint64_t>(plan.sink_tiles) * plan.splits) * batch_heads <= kIndex32Limit &&
+         static_cast<uint64_t>(plan.row_tiles) * batch_heads <= kIndex32Limit;
+}
+
+}  // namespace
+
+uint64_t forward_workspace(const SparHipAttention& a);  // attention_forward.hip
+
+}  // namespace attention
+}  // namespace spar_hip
+
+using namespace spar_hip;
+
+extern "C" SparHipStatus spar_hip_attention_workspace(uint64_t* bytes,
+                                                      const SparHipAttention* attention,
+                                                      int backward) {
+  if (bytes == nullptr || backward < 0 || backward > 1 || !attention::valid(attention)) {
+    return invalid();
+  }
+  *bytes = 0;
+  if (attention->batch == 0 || attention->query_heads == 0) return ok();
+  if (backward != 0) {
+    *bytes = attention::plan_of(*attention).bytes;
+  } else if (attention->queries != 0) {
+    *bytes = attention::forward_workspace(*attention);
+  }
+  return ok();
+}
+
+extern "C" SparHipStatus spar_hip_launch_attention_backward(
+    const SparHipHeads* query_gradient, const SparHipHeads* key_gradient,
+    const SparHipHeads* value_gradient, const SparHipHeads* output_gradient,
+    const SparHipHeads* output, const void* logsumexp, const SparHipHeads* query,
+    const SparHipHeads* key, const SparHipHeads* value, const SparHipAttention* attention,
+    void* workspace, uint64_t workspace_bytes, int device) {
+  if (!attention::valid(attention)) return invalid();
+  const SparHipAttention& a = *attention;
+  if (a.batch == 0 || a.query_heads == 0 || (a.queries == 0 && a.keys == 0)) return ok();
+  for (const SparHipHeads* heads :
+       {query_gradient, key_gradient, value_gradient, output_gradient, output, query, key, value}) {
+    if (heads == nullptr) return invalid();
+  }
+  if (a.queries != 0 &&
+      (query_gradient->data == nullptr || output_gradient->data == nullptr ||
+       output->data == nullptr || query->data == nullptr || logsumexp == nullptr)) {
+    return invalid();
+  }
+  if (a.keys != 0 && (key_gradient->data == nullptr || value_gradient->data == nullptr ||
+                      key->data == nullptr || value->data == nullptr)) {
+    return invalid();
+  }
+  const attention::Plan plan = attention::plan_of(a);
+  if (!attention::fits(a, plan) ||
+      (plan.bytes != 0 &&
+       (workspace == nullptr || workspace_bytes < plan.bytes || !aligned16(workspace)))) {
+    return invalid();
+  }
+  DeviceGuard guard;
+  if (enter(device, guard) != hipSuccess) return runtime(guard.error);
+  if (a.dtype == SPAR_HIP_FLOAT32) {
+    attention::start<float>(a, plan, *query_gradient, *key_gradient, *value_gradient,
+                            *output_gradient, *output, logsumexp, *query, *key, *value, workspace,
+                            guard.stream);
+  } else {
+    attention::start<double>(a, plan, *query_gradient, *key_gradient, *value_gradient,
+                             *output_gradient, *output, logsumexp, *query, *key, *value, workspace,
+                             guard.stream);
+  }
+  return finish(guard);
+}

@@ -1,0 +1,561 @@
+// Attention forward: o = softmax(scale q k^T over the visible keys) v in one pass
+// over the keys, with the running maximum and sum of the softmax per row.
+//
+// Scores are formed transposed, S^T = K Q^T, and so is the output, O^T = V^T P^T:
+// a lane then holds scores of one row only (its column), the row's maximum and sum
+// stay in that lane, the exponentials of S^T are the second product's operand as
+// they lie, and rescaling O takes no exchange between lanes (attention.hpp).
+// Scores carry scale * log2(e), folded into q, so that weights are powers of two.
+//
+// Two kernels.  tile_kernel: a workgroup of four waves with 16 or 32 rows each
+// shares tiles of keys and values in LDS; bound by the matrix units (4 extent
+// operations per visible pair).  token_kernel, for up to kTokenRows rows (a token
+// or a few per sequence): a workgroup's waves take different keys of the same 16
+// rows straight from memory into registers; bound by reading the visible cache.
+// Either splits the keys of a row tile over several workgroups where the rows alone
+// do not fill the chip; combine_kernel joins the parts in their order.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "attention.hpp"
+
+namespace spar_hip {
+namespace attention {
+namespace {
+
+// Where results go: the output itself, or one part per split of the keys.
+template <typename T>
+struct Results {
+  Heads<T> output;
+  T* logsumexp;
+  T* part_output;  // [split][batch][query head][query][extent]
+  T* part_weight;  // [split][batch][query head][query]: log2 of the sum
+  uint32_t splits;
+  uint64_t all_rows;  // batch * query heads * queries
+};
+
+// A row's running softmax and output.  `top` is the maximum so far of its scores,
+// the same in the four lanes that share the row; `total` each lane's own part.
+template <typename T, int DP>
+struct Row {
+  T top = lowest<T>();
+  T total = T(0);
+  Along<T, DP> out;
+
+  // Takes the scores of KB blocks of keys and turns them into weights.
+  template <int KB>
+  __device__ __forceinline__ void take(T (&score)[KB][4]) {
+    T high = lowest<T>();
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) high = score[kb][v] > high ? score[kb][v] : high;
+    }
+    high = quarter_max(high);
+    if (__any(high > top)) {
+      high = high > top ? high : top;
+      const T base = high == lowest<T>() ? T(0) : high;
+      const T shrink = exp2_of(top - base);
+      total *= shrink;
+      out.scale(shrink);
+      top = high;
+    }
+    const T base = top == lowest<T>() ? T(0) : top;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        score[kb][v] = exp2_of(score[kb][v] - base);
+        total += score[kb][v];
+      }
+    }
+  }
+};
+
+// Writes a finished row: `sum` is its whole total.
+template <typename T, int DP>
+__device__ __forceinline__ void write_row(const Call& call, const Results<T>& results, uint32_t b,
+                                          uint32_t key_head, uint32_t r, uint32_t split, T top,
+                                          T sum, const Along<T, DP>& out, int quarter) {
+  if (r >= call.rows) return;
+  const uint32_t t = call.group.div(r);
+  const uint32_t head = key_head * call.group.divisor + (r - t * call.group.divisor);
+  const T over = sum == T(0) ? T(0) : T(1) / sum;
+  const T weight = sum == T(0) ? lowest<T>() : top + log2_of(sum);
+  const uint64_t row =
+      (static_cast<uint64_t>(b) * call.key_heads * call.group.divisor + head) * call.queries + t;
+  T* target;
+  if (results.splits == 1) {
+    target = results.output.data + b * results.output.batch + head * results.output.head +
+             t * results.output.token;
+    if (quarter == 0 && results.logsumexp != nullptr) {
+      results.logsumexp[row] = weight * static_cast<T>(kLn2);
+    }
+  } else {
+    const uint64_t at = split * results.all_rows + row;
+    target = results.part_output + at * call.extent;
+    if (quarter == 0) results.part_weight[at] = weight;
+  }
+  out.visit(quarter, [&](uint32_t d, auto& run) {
+    for (auto& x : run) x *= over;
+    store_piece(target, d, call.extent, run);
+  });
+}
+
+template <typename T>
+__device__ __forceinline__ const T* head_row(const Heads<const T>& heads, const Call& call,
+                                             uint32_t b, uint32_t key_head, uint32_t r) {
+  const uint32_t t = call.group.div(r);
+  const uint32_t head = key_head * call.group.divisor + (r - t * call.group.divisor);
+  return heads.data + b * heads.batch + head * heads.head + t * heads.token;
+}
+
+// Workgroups of one key head follow each other at a distance of batch * key heads,
+// a multiple of the 8 dies in common sizes, so that they share a die's cache; the
+// last rows, which see most, come first.
+template <typename T, int DP, int MB, int KB>
+__global__ __launch_bounds__(kThreads) void tile_kernel(Call call, Results<T> results,
+                                                        Heads<const T> query, Heads<const T> key,
+                                                        Heads<const T> value, uint32_t row_tiles) {
+  constexpr int KT = KB * kBlock;
+  constexpr uint32_t kRows = kWaves * MB * kBlock;
+  __shared__ Tile<T, KT, DP> keys, values;
+  const uint32_t batch_head = blockIdx.x % call.batch_heads;
+  const uint32_t rest = blockIdx.x / call.batch_heads;
+  const uint32_t split = rest % results.splits;
+  const uint32_t row_tile = row_tiles - 1 - rest / results.splits;
+  const uint32_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave;
+  const int quarter = lane / kBlock, column = lane % kBlock;
+
+  const int32_t first = call.length(b) - call.queries;  // token of query 0
+  const uint32_t begin_row = row_tile * kRows;
+  const uint32_t end_row = begin_row + kRows < call.rows ? begin_row + kRows : call.rows;
+  const int32_t low_token = call.token(begin_row, first);
+  const Keys seen(call, low_token < 0 ? 0 : low_token, call.token(end_row - 1, first));
+  const uint32_t tiles = seen.tiles(KT);
+  const uint32_t begin_tile =
+      static_cast<uint32_t>(static_cast<uint64_t>(tiles) * split / results.splits);
+  const uint32_t end_tile =
+      static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / results.splits);
+
+  // This wave's rows and their tokens: all of them in the wave between `oldest`
+  // and `newest`.
+  const uint32_t wave_row = begin_row + wave * MB * kBlock;
+  const uint32_t wave_end =
+      wave_row + MB * kBlock < call.rows ? wave_row + MB * kBlock : call.rows;
+  const int32_t oldest = call.token(wave_row, first);
+  const int32_t newest = wave_row < wave_end ? call.token(wave_end - 1, first) : -1;
+  Operand<T, DP> q[MB];
+  Row<T, DP> row[MB];
+  int32_t token[MB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    const uint32_t r = wave_row + mb * kBlock + column;
+    token[mb] = call.token(r, first);
+    q[mb].load(token[mb] < 0 ? nullptr : head_row(query, call, b, key_head, r), call.extent,
+               quarter);
+    q[mb].scale(static_cast<T>(call.scale * kLog2E));
+    row[mb].out.clear();
+  }
+  const T* key_base = key.data + b * key.batch + key_head * key.head;
+  const T* value_base = value.data + b * value.batch + key_head * value.head;
+
+  for (uint32_t i = begin_tile; i < end_tile; ++i) {
+    int32_t begin, end;
+    seen.tile(i, KT, begin, end);
+    __syncthreads();
+    keys.fill(call.extent, [&](uint32_t j) {
+      return begin + j < end ? key_base + (begin + j) * key.token : nullptr;
+    });
+    values.fill(call.extent, [&](uint32_t j) {
+      return begin + j < end ? value_base + (begin + j) * value.token : nullptr;
+    });
+    __syncthreads();
+    bool any[KB];
+    bool some = false;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const int32_t k0 = begin + kb * kBlock, k1 = k0 + kBlock - 1;
+      any[kb] = k0 < end && k0 <= newest &&
+                ((oldest < 0 ? 0 : oldest) - k1 < call.window || k0 < call.sinks);
+      some |= any[kb];
+    }
+    if (!some) continue;
+    T score[MB][KB][4];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const int32_t k0 = begin + kb * kBlock, k1 = k0 + kBlock - 1;
+      typename Mma<T>::Acc s[MB];
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) s[mb] = typename Mma<T>::Acc{0, 0, 0, 0};
+      if (any[kb]) {
+#pragma unroll
+        for (int step = 0; step < DP / (4 * Operand<T, DP>::W); ++step) {
+          const auto piece = keys.along(kb * kBlock + column, step, quarter);
+#pragma unroll
+          for (int n = 0; n < Operand<T, DP>::W; ++n) {
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) {
+              s[mb] = Mma<T>::step(piece[n], q[mb].value[step * Operand<T, DP>::W + n], s[mb]);
+            }
+          }
+        }
+      }
+      const bool whole = any[kb] && k1 <= oldest && k1 < end &&
+                         (newest - k0 < call.window || k1 < call.sinks);
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int32_t at = k0 + Mma<T>::row_of(v, quarter);
+          const bool visible = whole | (any[kb] & (at < end) & call.sees(token[mb], at));
+          score[mb][kb][v] = visible ? s[mb][v] : lowest<T>();
+        }
+      }
+    }
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) row[mb].template take<KB>(score[mb]);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      if (!any[kb]) continue;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const T* from =
+            values.value + (kb * kBlock + Mma<T>::row_of(v, quarter)) * values.kPitch;
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) row[mb].out.add(from, column, score[mb][kb][v]);
+      }
+    }
+  }
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    write_row(call, results, b, key_head, wave_row + mb * kBlock + column, split, row[mb].top,
+              quarter_sum(row[mb].total), row[mb].out, quarter);
+  }
+}
+
+// Four waves with the same 16 rows and every fourth block of 16 keys, read into
+// the operands' layout from memory; at the end the waves' rows meet in LDS.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> results,
+                                                         Heads<const T> query, Heads<const T> key,
+                                                         Heads<const T> value,
+                                                         uint32_t row_tiles) {
+  constexpr int W = Vec16<T>::width;
+  constexpr int kPitch = DP + W;
+  __shared__ T outs[kWaves][kBlock][kPitch];
+  __shared__ T tops[kWaves][kBlock], totals[kWaves][kBlock];
+  const uint32_t batch_head = blockIdx.x % call.batch_heads;
+  const uint32_t rest = blockIdx.x / call.batch_heads;
+  const uint32_t split = rest % results.splits;
+  const uint32_t row_tile = row_tiles - 1 - rest / results.splits;
+  const uint32_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave;
+  const int quarter = lane / kBlock, column = lane % kBlock;
+
+  const int32_t first = call.length(b) - call.queries;
+  const uint32_t begin_row = row_tile * kBlock;
+  const uint32_t end_row = begin_row + kBlock < call.rows ? begin_row + kBlock : call.rows;
+  const int32_t oldest = call.token(begin_row, first);
+  const int32_t newest = call.token(end_row - 1, first);
+  const Keys seen(call, oldest < 0 ? 0 : oldest, newest);
+  const uint32_t blocks = seen.tiles(kBlock);
+  const uint32_t begin_block =
+      static_cast<uint32_t>(static_cast<uint64_t>(blocks) * split / results.splits);
+  const uint32_t end_block =
+      static_cast<uint32_t>(static_cast<uint64_t>(blocks) * (split + 1) / results.splits);
+
+  const uint32_t r = begin_row + column;
+  const int32_t token = call.token(r, first);
+  Operand<T, DP> q;
+  q.load(token < 0 ? nullptr : head_row(query, call, b, key_head, r), call.extent, quarter);
+  q.scale(static_cast<T>(call.scale * kLog2E));
+  Row<T, DP> row;
+  row.out.clear();
+  const T* key_base = key.data + b * key.batch + key_head * key.head;
+  const T* value_base = value.data + b * value.batch + key_head * value.head;
+
+  for (uint32_t i = begin_block + wave; i < end_block; i += kWaves) {
+    int32_t begin, end;
+    seen.tile(i, kBlock, begin, end);
+    Operand<T, DP> k;
+    const int32_t own = begin + column;
+    k.load(own < end ? key_base + own * key.token : nullptr, call.extent, quarter);
+    using Out = Along<T, DP>;
+    T v[4][DP / 16];  // pieces of the four keys whose weights this lane holds
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int32_t at = begin + Mma<T>::row_of(n, quarter);
+      const T* head = at < end ? value_base + at * value.token : nullptr;
+#pragma unroll
+      for (int c = 0; c < Out::kChunks; ++c) {
+        T piece[W];
+#pragma unroll
+        for (int j = 0; j < W; ++j) piece[j] = T(0);
+        if (head != nullptr) load_piece<T, W>(piece, head, 16 * W * c + W * column, call.extent);
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[n][c * W + j] = piece[j];
+      }
+      if constexpr (Out::kRest != 0) {
+        const uint32_t d = 16 * W * Out::kChunks + 2 * column;
+        v[n][Out::kChunks * W] = head != nullptr && d < call.extent ? head[d] : T(0);
+        v[n][Out::kChunks * W + 1] = head != nullptr && d + 1 < call.extent ? head[d + 1] : T(0);
+      }
+    }
+    typename Mma<T>::Acc s{0, 0, 0, 0};
+#pragma unroll
+    for (int step = 0; step < DP / 4; ++step) {
+      s = Mma<T>::step(k.value[step], q.value[step], s);
+    }
+    const int32_t last = begin + kBlock - 1;
+    const bool whole = last <= oldest && last < end &&
+                       (newest - begin < call.window || last < call.sinks);
+    T score[1][4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int32_t at = begin + Mma<T>::row_of(n, quarter);
+      const bool visible = whole | ((at < end) & call.sees(token, at));
+      score[0][n] = visible ? s[n] : lowest<T>();
+    }
+    row.template take<1>(score);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+#pragma unroll
+      for (int j = 0; j < DP / 16; ++j) {
+        row.out.block[j] = Mma<T>::step(v[n][j], score[0][n], row.out.block[j]);
+      }
+    }
+  }
+  const T total = quarter_sum(row.total);
+  if (quarter == 0) {
+    tops[wave][column] = row.top;
+    totals[wave][column] = total;
+  }
+  row.out.visit(quarter, [&](uint32_t d, auto& run) {
+    for (auto& x : run) {
+      outs[wave][column][d] = x;
+      ++d;
+    }
+  });
+  __syncthreads();
+  // Lane by lane over the rows' pieces: the waves in order.
+  constexpr int kPieces = DP / W;
+  for (int at = threadIdx.x; at < kBlock * kPieces; at += kThreads) {
+    const int c = at / kPieces, d = at % kPieces * W;
+    const uint32_t out_row = begin_row + c;
+    if (out_row >= call.rows) continue;
+    T top = tops[0][c];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) top = tops[w][c] > top ? tops[w][c] : top;
+    const T base = top == lowest<T>() ? T(0) : top;
+    T sum = T(0);
+    T run[W] = {};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const T shrink = exp2_of(tops[w][c] - base);
+      sum += totals[w][c] * shrink;
+#pragma unroll
+      for (int j = 0; j < W; ++j) run[j] += outs[w][c][d + j] * shrink;
+    }
+    const T over = sum == T(0) ? T(0) : T(1) / sum;
+#pragma unroll
+    for (int j = 0; j < W; ++j) run[j] *= over;
+    const uint32_t t = call.group.div(out_row);
+    const uint32_t head = key_head * call.group.divisor + (out_row - t * call.group.divisor);
+    const uint64_t place =
+        (static_cast<uint64_t>(b) * call.key_heads * call.group.divisor + head) * call.queries + t;
+    const T weight = sum == T(0) ? lowest<T>() : base + log2_of(sum);
+    T* target;
+    if (results.splits == 1) {
+      target = results.output.data + b * results.output.batch + head * results.output.head +
+               t * results.output.token;
+      if (d == 0 && results.logsumexp != nullptr) {
+        results.logsumexp[place] = weight * static_cast<T>(kLn2);
+      }
+    } else {
+      const uint64_t part = split * results.all_rows + place;
+      target = results.part_output + part * call.extent;
+      if (d == 0) results.part_weight[part] = weight;
+    }
+    store_piece(target, d, call.extent, run);
+  }
+}
+
+// The parts of a row: o = sum 2^(w - top) o_part / sum 2^(w - top), in their order.
+// 32 lanes per row, each an interleaved share of the head.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void combine_kernel(Call call, Results<T> results) {
+  constexpr int kLanes = 32;
+  const uint64_t row =
+      (static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x) / kLanes;
+  if (row >= results.all_rows) return;
+  T top = lowest<T>();
+  for (uint32_t s = 0; s < results.splits; ++s) {
+    const T w = results.part_weight[s * results.all_rows + row];
+    top = w > top || w != w ? w : top;
+  }
+  const T base = top == lowest<T>() ? T(0) : top;
+  T sum = T(0);
+  for (uint32_t s = 0; s < results.splits; ++s) {
+    sum += exp2_of(results.part_weight[s * results.all_rows + row] - base);
+  }
+  const T over = sum == T(0) ? T(0) : T(1) / sum;
+  const uint64_t batch_head = row / call.queries;
+  const uint32_t t = static_cast<uint32_t>(row - batch_head * call.queries);
+  const uint32_t heads = call.key_heads * call.group.divisor;
+  const uint64_t b = batch_head / heads, head = batch_head % heads;
+  T* target = results.output.data + b * results.output.batch + head * results.output.head +
+              t * results.output.token;
+  const uint32_t lane = threadIdx.x % kLanes;
+  if (lane == 0 && results.logsumexp != nullptr) {
+    results.logsumexp[row] =
+        (sum == T(0) ? lowest<T>() : base + log2_of(sum)) * static_cast<T>(kLn2);
+  }
+  for (uint32_t d = lane; d < call.extent; d += kLanes) {
+    T x = T(0);
+    for (uint32_t s = 0; s < results.splits; ++s) {
+      const uint64_t part = s * results.all_rows + row;
+      const T w = exp2_of(results.part_weight[part] - base) * over;
+      x += w * results.part_output[part * call.extent + d];
+    }
+    target[d] = x;
+  }
+}
+
+// ---------------------------------------------------------------- launchers
+
+// Up to this many rows per key head the waves share rows and split keys: a tile
+// of 64 rows would leave half of its matrix work unused.
+constexpr uint64_t kTokenRows = 32;
+
+// Workgroups that keep the chip's 256 CUs busy, and the fewest keys that repay
+// the writing and reading of a part.
+constexpr uint64_t kFullGrid = 512;
+constexpr uint64_t kTokenGrid = 1024;
+constexpr uint64_t kFewestKeys = 256;
+
+struct Plan {
+  bool token;
+  uint32_t blocks;     // of 16 rows per wave (tile_kernel)
+  uint32_t row_tiles;
+  uint32_t splits;
+  uint64_t rows;       // batch * query heads * queries
+  uint64_t bytes;
+};
+
+uint64_t element_size(const SparHipAttention& a) {
+  return a.dtype == SPAR_HIP_FLOAT32 ? sizeof(float) : sizeof(double);
+}
+
+Plan plan_of(const SparHipAttention& a) {
+  Plan plan{};
+  const uint64_t rows = a.queries * (a.query_heads / a.key_heads);
+  const uint64_t batch_heads = a.batch * a.key_heads;
+  plan.rows = a.batch * a.query_heads * a.queries;
+  plan.token = rows <= kTokenRows;
+  plan.blocks = 1;
+  uint64_t grid = kTokenGrid;
+  uint64_t seen = most_seen(a);
+  if (plan.token) {
+    plan.row_tiles = ceil_div_u32(rows, kBlock);
+  } else {
+    // Two blocks of rows per wave halve the reading of tiles; where they fit the
+    // registers and the grid stays full.
+    constexpr uint64_t kRows = kWaves * kBlock;
+    const bool narrow = a.extent <= 128 && a.dtype == SPAR_HIP_FLOAT32;
+    if (narrow && (rows + 2 * kRows - 1) / (2 * kRows) * batch_heads >= kFullGrid) {
+      plan.blocks = 2;
+    }
+    plan.row_tiles = ceil_div_u32(rows, kRows * plan.blocks);
+    grid = kFullGrid;
+    seen = std::min(a.keys, seen + kRows * plan.blocks / (a.query_heads / a.key_heads));
+  }
+  const uint64_t wanted = grid / std::max<uint64_t>(1, plan.row_tiles * batch_heads);
+  plan.splits = static_cast<uint32_t>(
+      std::max<uint64_t>(1, std::min(wanted, seen / kFewestKeys)));
+  if (plan.splits > 1) {
+    plan.bytes = plan.splits * plan.rows * (a.extent + 1) * element_size(a);
+  }
+  return plan;
+}
+
+template <typename T>
+void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& output,
+           void* logsumexp, const SparHipHeads& query, const SparHipHeads& key,
+           const SparHipHeads& value, void* workspace, hipStream_t stream) {
+  const Call call = call_of(a);
+  Results<T> results{heads_of<T>(output), static_cast<T*>(logsumexp), nullptr, nullptr,
+                     plan.splits, plan.rows};
+  if (plan.splits > 1) {
+    results.part_output = static_cast<T*>(workspace);
+    results.part_weight = results.part_output + plan.splits * plan.rows * a.extent;
+  }
+  const uint32_t grid = plan.row_tiles * call.batch_heads * plan.splits;
+  const auto q = heads_of<const T>(query), k = heads_of<const T>(key),
+             v = heads_of<const T>(value);
+  with_width(a.extent, [&](auto width) {
+    constexpr int DP = decltype(width)::value;
+    constexpr int KB = sizeof(T) == 4 ? 2 : 1;
+    if (plan.token) {
+      token_kernel<T, DP><<<grid, kThreads, 0, stream>>>(call, results, q, k, v, plan.row_tiles);
+      return;
+    }
+    if constexpr (sizeof(T) == 4 && DP <= 128) {
+      if (plan.blocks == 2) {
+        tile_kernel<T, DP, 2, KB>
+            <<<grid, kThreads, 0, stream>>>(call, results, q, k, v, plan.row_tiles);
+        return;
+      }
+    }
+    tile_kernel<T, DP, 1, KB><<<grid, kThreads, 0, stream>>>(call, results, q, k, v,
+                                                             plan.row_tiles);
+  });
+  if (plan.splits > 1) {
+    combine_kernel<T><<<ceil_div_u32(plan.rows * 32, kThreads), kThreads, 0, stream>>>(call,
+                                                                                    results);
+  }
+}
+
+}  // namespace
+
+uint64_t forward_workspace(const SparHipAttention& a) { return plan_of(a).bytes; }
+
+}  // namespace attention
+}  // namespace spar_hip
+
+using namespace spar_hip;
+
+extern "C" SparHipStatus spar_hip_launch_attention_forward(
+    const SparHipHeads* output, void* logsumexp, const SparHipHeads* query,
+    const SparHipHeads* key, const SparHipHeads* value, const SparHipAttention* attention,
+    void* workspace, uint64_t workspace_bytes, int device) {
+  if (!attention::valid(attention)) return invalid();
+  const SparHipAttention& a = *attention;
+  if (a.batch == 0 || a.query_heads == 0 || a.queries == 0) return ok();
+  if (output == nullptr || query == nullptr || key == nullptr || value == nullptr ||
+      output->data == nullptr || query->data == nullptr ||
+      (a.keys != 0 && (key->data == nullptr || value->data == nullptr))) {
+    return invalid();
+  }
+  const attention::Plan plan = attention::plan_of(a);
+  if (static_cast<uint64_t>(plan.row_tiles) * a.batch * a.key_heads * plan.splits >
+          kIndex32Limit ||
+      (plan.bytes != 0 &&
+       (workspace == nullptr || workspace_bytes < plan.bytes || !aligned16(workspace)))) {
+    return invalid();
+  }
+  DeviceGuard guard;
+  if (enter(device, guard) != hipSuccess) return runtime(guard.error);
+  if (a.dtype == SPAR_HIP_FLOAT32) {
+    attention::start<float>(a, plan, *output, logsumexp, *query, *key, *value, workspace,
+                            guard.stream);
+  } else {
+    attention::start<double>(a, plan, *output, logsumexp, *query, *key, *value, workspace,
+                             guard.stream);
+  }
+  return finish(guard);
+}

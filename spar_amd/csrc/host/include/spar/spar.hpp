@@ -2,6 +2,7 @@
 // src/spar.cppm:1-15, for the tensor/ops path this backend covers).
 #pragma once
 
+#include "spar/attention.hpp"
 #include "spar/core.hpp"
 #include "spar/loss.hpp"
 #include "spar/ops.hpp"

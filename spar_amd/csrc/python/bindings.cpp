@@ -320,6 +320,43 @@ PYBIND11_MODULE(_spar, m) {
         py::arg("epsilon") = 1.0e-5, py::call_guard<py::gil_scoped_release>());
   m.def("layer_norm", &spar::layer_norm, py::arg("input"), py::arg("weight"), py::arg("bias"),
         py::arg("epsilon") = 1.0e-5, py::call_guard<py::gil_scoped_release>());
+  py::enum_<spar::RotaryLayout>(m, "RotaryLayout")
+      .value("Half", spar::RotaryLayout::Half)
+      .value("Interleaved", spar::RotaryLayout::Interleaved);
+  py::class_<spar::RotaryScaling> scaling(m, "RotaryScaling");
+  py::enum_<spar::RotaryScaling::Kind>(scaling, "Kind")
+      .value("None_", spar::RotaryScaling::Kind::None)
+      .value("Linear", spar::RotaryScaling::Kind::Linear)
+      .value("Base", spar::RotaryScaling::Kind::Base)
+      .value("Parts", spar::RotaryScaling::Kind::Parts);
+  scaling
+      .def(py::init([](spar::RotaryScaling::Kind kind, double factor, double trained_tokens,
+                       double slow_turns, double fast_turns) {
+             return spar::RotaryScaling{kind, factor, trained_tokens, slow_turns, fast_turns};
+           }),
+           py::arg("kind") = spar::RotaryScaling::Kind::None, py::arg("factor") = 1.0,
+           py::arg("trained_tokens") = 0.0, py::arg("slow_turns") = 1.0,
+           py::arg("fast_turns") = 32.0)
+      .def_readwrite("kind", &spar::RotaryScaling::kind)
+      .def_readwrite("factor", &spar::RotaryScaling::factor)
+      .def_readwrite("trained_tokens", &spar::RotaryScaling::trained_tokens)
+      .def_readwrite("slow_turns", &spar::RotaryScaling::slow_turns)
+      .def_readwrite("fast_turns", &spar::RotaryScaling::fast_turns);
+  m.def("rotary_frequencies", &spar::rotary_frequencies, py::arg("rotary_extent"),
+        py::arg("base") = 10000.0, py::arg("scaling") = spar::RotaryScaling{});
+  m.def("rotary_magnitude", &spar::rotary_magnitude, py::arg("factor"));
+  m.def("rotary_embedding", &spar::rotary_embedding, py::arg("heads"), py::arg("positions"),
+        py::arg("frequencies"), py::arg("layout") = spar::RotaryLayout::Half,
+        py::arg("magnitude") = 1.0, py::call_guard<py::gil_scoped_release>());
+  m.def("query_key_norm_rotary", &spar::query_key_norm_rotary, py::arg("query"), py::arg("key"),
+        py::arg("query_weight"), py::arg("key_weight"), py::arg("positions"),
+        py::arg("frequencies"), py::arg("layout") = spar::RotaryLayout::Half,
+        py::arg("magnitude") = 1.0, py::arg("epsilon") = 1.0e-5,
+        py::call_guard<py::gil_scoped_release>());
+  m.def("window_attention", &spar::window_attention, py::arg("query"), py::arg("key"),
+        py::arg("value"), py::arg("window") = 0, py::arg("sinks") = 0,
+        py::arg("scale") = py::none(), py::arg("lengths") = py::none(),
+        py::call_guard<py::gil_scoped_release>());
   m.def("reduce_gradient_to_shape", [](const Tensor& g, const std::vector<std::int64_t>& s) {
     return spar::detail::reduce_gradient_to_shape(g, to_shape(s));
   });

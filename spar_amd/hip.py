@@ -21,6 +21,7 @@ EQUAL, NOT_EQUAL, LESS, LESS_EQUAL, GREATER, GREATER_EQUAL = 4, 5, 6, 7, 8, 9
 NEGATE, SQUARE, RECIPROCAL, EXP, LOG, SQRT, SIGMOID, SILU, TANH, GELU, GELU_DERIVATIVE = range(11)
 SUM, MEAN, MAX, ARGMAX = 0, 1, 2, 3
 MAX_RANK = 8
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
 
 BINARY_OPS = {"add": ADD, "subtract": SUBTRACT, "multiply": MULTIPLY, "divide": DIVIDE,
               "equal": EQUAL, "not_equal": NOT_EQUAL, "less": LESS, "less_equal": LESS_EQUAL,
@@ -55,6 +56,37 @@ class AdamwTensor(ctypes.Structure):
                 ("second_correction", ctypes.c_double)]
 
 
+class Heads(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("strides", ctypes.c_uint64 * 3)]
+
+
+class Rotary(ctypes.Structure):
+    _fields_ = [("positions", ctypes.c_void_p), ("position_stride", ctypes.c_uint64),
+                ("position_dtype", ctypes.c_int), ("frequencies", ctypes.c_void_p),
+                ("rotary_extent", ctypes.c_uint64), ("magnitude", ctypes.c_double),
+                ("layout", ctypes.c_int)]
+
+
+class HeadNorm(ctypes.Structure):
+    _fields_ = [("output", Heads), ("denominator", ctypes.c_void_p), ("input", Heads),
+                ("weight", ctypes.c_void_p), ("heads", ctypes.c_uint64)]
+
+
+class HeadNormGradient(ctypes.Structure):
+    _fields_ = [("input_gradient", Heads), ("weight_gradient", ctypes.c_void_p),
+                ("output_gradient", Heads), ("input", Heads), ("weight", ctypes.c_void_p),
+                ("denominator", ctypes.c_void_p), ("heads", ctypes.c_uint64)]
+
+
+class Attention(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_uint64), ("query_heads", ctypes.c_uint64),
+                ("key_heads", ctypes.c_uint64), ("queries", ctypes.c_uint64),
+                ("keys", ctypes.c_uint64), ("extent", ctypes.c_uint64),
+                ("window", ctypes.c_uint64), ("sinks", ctypes.c_uint64),
+                ("scale", ctypes.c_double), ("lengths", ctypes.c_void_p),
+                ("length_dtype", ctypes.c_int), ("dtype", ctypes.c_int)]
+
+
 class HipError(RuntimeError):
     def __init__(self, name: str, status: Status, message: str):
         super().__init__(f"{name} failed: {message} (code {status.code}, hip error {status.hip_error})")
@@ -68,6 +100,9 @@ _U32 = ctypes.c_uint32
 _I = ctypes.c_int
 _D = ctypes.c_double
 _U64P = ctypes.POINTER(ctypes.c_uint64)
+_HEADS = ctypes.POINTER(Heads)
+_ROTARY = ctypes.POINTER(Rotary)
+_ATTENTION = ctypes.POINTER(Attention)
 
 # name -> argument types (every entry point returns Status except error_string and
 # norm_max_extent)
@@ -129,6 +164,17 @@ SIGNATURES = {
                                        _U64, _U64, _U64, _I, _I, _I, _I],
     "spar_hip_launch_cross_entropy_backward": [_P, _P, _P, _P, _P, _P, _P, _U64, _U64, _U64, _I,
                                                _I, _I, _I],
+    "spar_hip_launch_rotary": [_HEADS, _HEADS, _U64, _U64, _U64, _U64, _ROTARY, _I, _I, _I],
+    "spar_hip_launch_head_norm_rotary_forward": [ctypes.POINTER(HeadNorm), _I, _U64, _U64, _U64,
+                                                 _ROTARY, _D, _I, _I],
+    "spar_hip_head_norm_rotary_workspace": [_U64P, _U64, _U64, _U64, _U64, _I],
+    "spar_hip_launch_head_norm_rotary_backward": [ctypes.POINTER(HeadNormGradient), _I, _U64, _U64,
+                                                  _U64, _ROTARY, _P, _U64, _I, _I],
+    "spar_hip_attention_workspace": [_U64P, _ATTENTION, _I],
+    "spar_hip_launch_attention_forward": [_HEADS, _P, _HEADS, _HEADS, _HEADS, _ATTENTION, _P, _U64,
+                                          _I],
+    "spar_hip_launch_attention_backward": [_HEADS, _HEADS, _HEADS, _HEADS, _HEADS, _P, _HEADS,
+                                           _HEADS, _HEADS, _ATTENTION, _P, _U64, _I],
     "spar_hip_gradient_norm_summary": [ctypes.POINTER(NormSummary), _P, _U64, _I, _I],
     "spar_hip_launch_gradient_norm_summary": [_P, _P, _U64, _I, _I],
     "spar_hip_launch_gradient_norm_summaries": [_P, _P, _U64P, _U64, _I, _I],
@@ -185,6 +231,55 @@ def status_of(name: str, *args) -> Status:
 def u64_array(values) -> ctypes.Array:
     values = [int(v) for v in values]
     return (ctypes.c_uint64 * max(len(values), 1))(*values)
+
+
+def heads(data, strides) -> Heads:
+    """A [batch, heads, tokens, extent] tensor: its first element's address and
+    its (batch, head, token) strides in elements."""
+    return Heads(data, tuple(strides))
+
+
+def rotary(positions, position_stride, position_dtype, frequencies, rotary_extent, magnitude=1.0,
+           layout=ROTARY_HALF) -> Rotary:
+    return Rotary(positions, position_stride, position_dtype, frequencies, rotary_extent,
+                  magnitude, layout)
+
+
+def head_norms(*parts):
+    """Parts of spar_hip_launch_head_norm_rotary_forward, each (output, output
+    strides, denominator, input, input strides, weight, heads)."""
+    return (HeadNorm * len(parts))(*(
+        HeadNorm(heads(output, output_strides), denominator, heads(source, strides), weight, count)
+        for output, output_strides, denominator, source, strides, weight, count in parts))
+
+
+def head_norm_gradients(*parts):
+    """Parts of spar_hip_launch_head_norm_rotary_backward, each (input gradient,
+    its strides, weight gradient, output gradient, its strides, input, its
+    strides, weight, denominator, heads)."""
+    return (HeadNormGradient * len(parts))(*(
+        HeadNormGradient(heads(dx, dx_strides), dw, heads(dy, dy_strides), heads(x, strides),
+                         weight, denominator, count)
+        for dx, dx_strides, dw, dy, dy_strides, x, strides, weight, denominator, count in parts))
+
+
+def head_norm_rotary_workspace(batch, tokens, heads, extent, dtype) -> int:
+    need = ctypes.c_uint64(0)
+    call("spar_hip_head_norm_rotary_workspace", ctypes.byref(need), batch, tokens, heads, extent,
+         dtype)
+    return need.value
+
+
+def attention(batch, query_heads, key_heads, queries, keys, extent, window, sinks, scale, lengths,
+              length_dtype, dtype) -> Attention:
+    return Attention(batch, query_heads, key_heads, queries, keys, extent, window, sinks, scale,
+                     lengths, length_dtype, dtype)
+
+
+def attention_workspace(shape, backward) -> int:
+    need = ctypes.c_uint64(0)
+    call("spar_hip_attention_workspace", ctypes.byref(need), shape, backward)
+    return need.value
 
 
 def dtype_tag(dtype) -> int:
