@@ -155,17 +155,21 @@ __device__ __forceinline__ T quarter_max(T x) {
   return x > z ? x : z;
 }
 
-// W neighbours of a head at d, zeros behind its extent.
-template <typename T, int W>
-__device__ __forceinline__ void load_piece(T (&x)[W], const T* head, uint32_t d, uint32_t extent) {
-  static_assert(W == Vec16<T>::width);
-  if (d + W <= extent) {
-    const auto v = loose_load(head + d);
-#pragma unroll
-    for (int i = 0; i < W; ++i) x[i] = v[i];
+// 16 bytes of a head at d, without a branch, so that a batch of them is in flight at
+// once: a piece behind the extent is read from the head's start, an element of a
+// piece that the extent cuts (EVEN says that it cuts none) from the head's end.
+// What stands there is finite where the head is, and meets zeros of the other
+// operand or is not written.
+template <bool EVEN, typename T>
+__device__ __forceinline__ typename Vec16<T>::type load_piece(const T* head, uint32_t d,
+                                                              uint32_t extent) {
+  if constexpr (EVEN) {
+    return loose_load(head + (d < extent ? d : 0));
   } else {
+    typename Vec16<T>::type v;
 #pragma unroll
-    for (int i = 0; i < W; ++i) x[i] = d + i < extent ? head[d + i] : T(0);
+    for (int i = 0; i < Vec16<T>::width; ++i) v[i] = head[d + i < extent ? d + i : extent - 1];
+    return v;
   }
 }
 
@@ -188,62 +192,67 @@ __device__ __forceinline__ void store_piece(T* head, uint32_t d, uint32_t extent
 }
 
 // Heads as a product's operand contracted along the head: lane l's pieces of row
-// l % 16.  `head` is that row, or null for a row of zeros.
+// l % 16.
 template <typename T, int DP>
 struct Operand {
   static constexpr int W = Vec16<T>::width;
   T value[DP / 4];
 
+  template <bool EVEN>
   __device__ __forceinline__ void load(const T* head, uint32_t extent, int quarter) {
 #pragma unroll
     for (int s = 0; s < DP / (4 * W); ++s) {
-      T piece[W];
-#pragma unroll
-      for (int i = 0; i < W; ++i) piece[i] = T(0);
-      if (head != nullptr) load_piece<T, W>(piece, head, 4 * W * s + W * quarter, extent);
+      const auto piece = load_piece<EVEN>(head, 4 * W * s + W * quarter, extent);
 #pragma unroll
       for (int i = 0; i < W; ++i) value[s * W + i] = piece[i];
     }
   }
-  __device__ __forceinline__ void scale(T factor) {
+  // Zeros behind the extent, and everywhere if the row is not `held`; times factor.
+  __device__ __forceinline__ void finish(bool held, uint32_t extent, int quarter, T factor) {
 #pragma unroll
-    for (int i = 0; i < DP / 4; ++i) value[i] *= factor;
+    for (int s = 0; s < DP / (4 * W); ++s) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const bool inside = held & (4 * W * s + W * quarter + i < extent);
+        value[s * W + i] = inside ? value[s * W + i] * factor : T(0);
+      }
+    }
   }
 };
 
 // A tile of ROWS heads in LDS, rows 16 bytes apart from a multiple of 128: 16
 // lanes that read one piece of 16 rows each, or 16 pieces of one row, fall into
-// different banks.
+// different banks.  The pieces pass through registers, so that the next tile is on
+// its way while the present one is used.
 template <typename T, int ROWS, int DP>
 struct Tile {
   static constexpr int W = Vec16<T>::width;
   static constexpr int kPitch = DP + W;
+  static constexpr int kPieces = DP / W;
+  static constexpr int kShare = ROWS * kPieces / kThreads;  // pieces per thread
+  static_assert(ROWS * kPieces % kThreads == 0);
   alignas(16) T value[ROWS * kPitch];
 
-  // head_of(row): the row's head, or null for zeros.  All threads of a workgroup.
-  template <typename HeadOf>
-  __device__ __forceinline__ void fill(uint32_t extent, HeadOf&& head_of) {
-    constexpr int kPieces = DP / W;
-    constexpr int kAll = ROWS * kPieces;
-    static_assert(kAll % kThreads == 0);
-    T piece[kAll / kThreads][W];
+  struct Stage {
+    typename Vec16<T>::type piece[kShare];
+
+    // head_of(row): the row's head.  All threads of a workgroup.
+    template <bool EVEN, typename HeadOf>
+    __device__ __forceinline__ void load(uint32_t extent, HeadOf&& head_of) {
 #pragma unroll
-    for (int j = 0; j < kAll / kThreads; ++j) {
-      const uint32_t at = threadIdx.x + j * kThreads;
-      const uint32_t row = at / kPieces, d = at % kPieces * W;
-      const T* head = head_of(row);
-#pragma unroll
-      for (int i = 0; i < W; ++i) piece[j][i] = T(0);
-      if (head != nullptr) load_piece<T, W>(piece[j], head, d, extent);
+      for (int j = 0; j < kShare; ++j) {
+        const uint32_t at = threadIdx.x + j * kThreads;
+        piece[j] = load_piece<EVEN>(head_of(at / kPieces), at % kPieces * W, extent);
+      }
     }
+  };
+
+  __device__ __forceinline__ void fill(const Stage& stage) {
 #pragma unroll
-    for (int j = 0; j < kAll / kThreads; ++j) {
+    for (int j = 0; j < kShare; ++j) {
       const uint32_t at = threadIdx.x + j * kThreads;
-      const uint32_t row = at / kPieces, d = at % kPieces * W;
-      typename Vec16<T>::type v;
-#pragma unroll
-      for (int i = 0; i < W; ++i) v[i] = piece[j][i];
-      *reinterpret_cast<typename Vec16<T>::type*>(value + row * kPitch + d) = v;
+      *reinterpret_cast<typename Vec16<T>::type*>(value + at / kPieces * kPitch +
+                                                  at % kPieces * W) = stage.piece[j];
     }
   }
 
@@ -318,9 +327,15 @@ struct Along {
   }
 };
 
-// Calls body(integral_constant<DP>) with the smallest padded width.
+// Waves per SIMD that a kernel's registers leave room for: one computes while the
+// other waits for its tile or takes exponentials.
+template <typename T, int DP>
+constexpr int tile_waves() {
+  return DP * sizeof(T) <= 512 ? 2 : 1;
+}
+
 template <typename Body>
-bool with_width(uint64_t extent, Body&& body) {
+void with_padded_width(uint64_t extent, Body&& body) {
   if (extent <= 32) {
     body(std::integral_constant<int, 32>{});
   } else if (extent <= 64) {
@@ -331,12 +346,18 @@ bool with_width(uint64_t extent, Body&& body) {
     body(std::integral_constant<int, 128>{});
   } else if (extent <= 192) {
     body(std::integral_constant<int, 192>{});
-  } else if (extent <= 256) {
-    body(std::integral_constant<int, 256>{});
   } else {
-    return false;
+    body(std::integral_constant<int, SPAR_HIP_ATTENTION_MAX_EXTENT>{});
   }
-  return true;
+}
+
+// Calls body(integral_constant<DP>, Policy<EVEN>) with the smallest padded
+// width, EVEN if 16-byte pieces divide the extent.
+template <typename T, typename Body>
+void with_width(uint64_t extent, Body&& body) {
+  with_policy(extent % Vec16<T>::width == 0, [&](auto even) {
+    with_padded_width(extent, [&](auto width) { body(width, even); });
+  });
 }
 
 inline bool valid(const SparHipAttention* a) {

@@ -56,8 +56,8 @@ struct Place {
   }
 };
 
-template <typename T, int DP, int KB>
-__global__ __launch_bounds__(kThreads) void query_kernel(Call call, Saved<T> saved,
+template <typename T, int DP, int KB, bool EVEN>
+__global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(Call call, Saved<T> saved,
                                                          Heads<T> gradient, uint32_t row_tiles) {
   constexpr int KT = KB * kBlock;
   constexpr int W = Vec16<T>::width;
@@ -85,39 +85,49 @@ __global__ __launch_bounds__(kThreads) void query_kernel(Call call, Saved<T> sav
   const int32_t token = call.token(r, first);
   const Place place(call, b, key_head, r < call.rows ? r : 0);
   Operand<T, DP> q, g;
-  q.load(token < 0 ? nullptr : place.of(saved.query, b), call.extent, quarter);
-  g.load(token < 0 ? nullptr : place.of(saved.output_gradient, b), call.extent, quarter);
-  T delta = T(0), log_sum = T(0);
-  if (token >= 0) {
-    const T* out = place.of(saved.output, b);
-#pragma unroll
-    for (int s = 0; s < DP / (4 * W); ++s) {
-      T piece[W];
-      load_piece<T, W>(piece, out, 4 * W * s + W * quarter, call.extent);
-#pragma unroll
-      for (int i = 0; i < W; ++i) delta += piece[i] * g.value[s * W + i];
-    }
+  T delta = T(0), log_sum;
+  {
+    Operand<T, DP> out;
+    q.template load<EVEN>(place.of(saved.query, b), call.extent, quarter);
+    g.template load<EVEN>(place.of(saved.output_gradient, b), call.extent, quarter);
+    out.template load<EVEN>(place.of(saved.output, b), call.extent, quarter);
     log_sum = saved.logsumexp[place.at] * static_cast<T>(kLog2E);
+    q.finish(token >= 0, call.extent, quarter, static_cast<T>(call.scale * kLog2E));
+    g.finish(token >= 0, call.extent, quarter, T(1));
+#pragma unroll
+    for (int i = 0; i < DP / 4; ++i) delta += out.value[i] * g.value[i];
   }
   delta = quarter_sum(delta);
   if (quarter == 0 && r < call.rows) saved.delta[place.at] = delta;
-  q.scale(static_cast<T>(call.scale * kLog2E));
   Along<T, DP> dq;
   dq.clear();
   const T* key_base = saved.key.data + b * saved.key.batch + key_head * saved.key.head;
   const T* value_base = saved.value.data + b * saved.value.batch + key_head * saved.value.head;
 
+  // Rows of a tile behind its run repeat the tile's first key; no row sees them.
+  typename Tile<T, KT, DP>::Stage next_keys, next_values;
+  const auto stage = [&](uint32_t i) {
+    int32_t begin, end;
+    seen.tile(i, KT, begin, end);
+    const auto at = [&](uint32_t j) {
+      const int32_t k = begin + static_cast<int32_t>(j);
+      return static_cast<uint64_t>(k < end ? k : begin);
+    };
+    next_keys.template load<EVEN>(call.extent,
+                                  [&](uint32_t j) { return key_base + at(j) * saved.key.token; });
+    next_values.template load<EVEN>(
+        call.extent, [&](uint32_t j) { return value_base + at(j) * saved.value.token; });
+  };
+  if (tiles != 0) stage(0);
+
   for (uint32_t i = 0; i < tiles; ++i) {
     int32_t begin, end;
     seen.tile(i, KT, begin, end);
     __syncthreads();
-    keys.fill(call.extent, [&](uint32_t j) {
-      return begin + j < end ? key_base + (begin + j) * saved.key.token : nullptr;
-    });
-    values.fill(call.extent, [&](uint32_t j) {
-      return begin + j < end ? value_base + (begin + j) * saved.value.token : nullptr;
-    });
+    keys.fill(next_keys);
+    values.fill(next_values);
     __syncthreads();
+    if (i + 1 < tiles) stage(i + 1);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       const int32_t k0 = begin + kb * kBlock, k1 = k0 + kBlock - 1;
@@ -156,8 +166,8 @@ __global__ __launch_bounds__(kThreads) void query_kernel(Call call, Saved<T> sav
 
 constexpr uint32_t kKeyTile = kWaves * kBlock;
 
-template <typename T, int DP, int RB>
-__global__ __launch_bounds__(kThreads) void key_kernel(Call call, Saved<T> saved,
+template <typename T, int DP, int RB, bool EVEN>
+__global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void key_kernel(Call call, Saved<T> saved,
                                                        Gradients<T> gradients,
                                                        uint32_t sink_groups, uint32_t key_tiles) {
   constexpr int RT = RB * kBlock;
@@ -207,33 +217,50 @@ __global__ __launch_bounds__(kThreads) void key_kernel(Call call, Saved<T> saved
   const T* key_base = saved.key.data + b * saved.key.batch + key_head * saved.key.head;
   const T* value_base = saved.value.data + b * saved.value.batch + key_head * saved.value.head;
   Operand<T, DP> k, x;
-  k.load(keeps ? key_base + own * saved.key.token : nullptr, call.extent, quarter);
-  x.load(keeps ? value_base + own * saved.value.token : nullptr, call.extent, quarter);
-  k.scale(static_cast<T>(call.scale * kLog2E));
+  {
+    const uint64_t at = static_cast<uint32_t>(own) < call.keys ? own : 0;
+    k.template load<EVEN>(key_base + at * saved.key.token, call.extent, quarter);
+    x.template load<EVEN>(value_base + at * saved.value.token, call.extent, quarter);
+    k.finish(keeps, call.extent, quarter, static_cast<T>(call.scale * kLog2E));
+    x.finish(keeps, call.extent, quarter, T(1));
+  }
   Along<T, DP> dk, dv;
   dk.clear();
   dv.clear();
 
+  // Rows of a tile behind the last repeat the tile's first; their token sees nothing.
+  typename Tile<T, RT, DP>::Stage next_queries, next_gradients;
+  T next_log_sum, next_delta;
+  int32_t next_token;
+  const auto stage = [&](uint32_t i) {
+    const uint32_t row0 = begin_row + i * RT;
+    const auto at = [&](uint32_t j) {
+      return Place(call, b, key_head, row0 + j < end_row ? row0 + j : row0);
+    };
+    next_queries.template load<EVEN>(call.extent,
+                                     [&](uint32_t j) { return at(j).of(saved.query, b); });
+    next_gradients.template load<EVEN>(
+        call.extent, [&](uint32_t j) { return at(j).of(saved.output_gradient, b); });
+    const uint32_t own_row = threadIdx.x % RT;
+    const Place place = at(own_row);
+    next_token = row0 + own_row < end_row ? call.token(row0 + own_row, first) : -1;
+    next_log_sum = saved.logsumexp[place.at];
+    next_delta = saved.delta[place.at];
+  };
+  if (begin_tile < tiles) stage(begin_tile);
+
   for (uint32_t i = begin_tile; i < tiles; ++i) {
     const uint32_t row0 = begin_row + i * RT;
     __syncthreads();
-    queries.fill(call.extent, [&](uint32_t j) -> const T* {
-      const uint32_t r = row0 + j;
-      return r < end_row ? Place(call, b, key_head, r).of(saved.query, b) : nullptr;
-    });
-    output_gradients.fill(call.extent, [&](uint32_t j) -> const T* {
-      const uint32_t r = row0 + j;
-      return r < end_row ? Place(call, b, key_head, r).of(saved.output_gradient, b) : nullptr;
-    });
+    queries.fill(next_queries);
+    output_gradients.fill(next_gradients);
     if (threadIdx.x < RT) {
-      const uint32_t r = row0 + threadIdx.x;
-      const bool row = r < end_row;
-      const Place place(call, b, key_head, row ? r : begin_row);
-      tokens[threadIdx.x] = row ? call.token(r, first) : -1;
-      log_sums[threadIdx.x] = row ? saved.logsumexp[place.at] * static_cast<T>(kLog2E) : T(0);
-      deltas[threadIdx.x] = row ? saved.delta[place.at] : T(0);
+      tokens[threadIdx.x] = next_token;
+      log_sums[threadIdx.x] = next_log_sum * static_cast<T>(kLog2E);
+      deltas[threadIdx.x] = next_delta;
     }
     __syncthreads();
+    if (i + 1 < tiles) stage(i + 1);
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       const uint32_t block_row = row0 + rb * kBlock;
@@ -370,15 +397,16 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& quer
       reinterpret_cast<T*>(static_cast<char*>(workspace) + plan.delta_bytes), plan.splits,
       plan.sink_tiles};
   const uint32_t sink_groups = plan.sink_tiles * plan.splits;
-  with_width(a.extent, [&](auto width) {
+  with_width<T>(a.extent, [&](auto width, auto even) {
     constexpr int DP = decltype(width)::value;
+    constexpr bool EVEN = decltype(even)::value;
     constexpr int KB = sizeof(T) == 4 ? 2 : 1;
     if (call.rows != 0) {
-      query_kernel<T, DP, KB><<<plan.row_tiles * call.batch_heads, kThreads, 0, stream>>>(
+      query_kernel<T, DP, KB, EVEN><<<plan.row_tiles * call.batch_heads, kThreads, 0, stream>>>(
           call, saved, gradients.query, plan.row_tiles);
     }
     if (call.keys != 0) {
-      key_kernel<T, DP, KB>
+      key_kernel<T, DP, KB, EVEN>
           <<<(plan.key_tiles + sink_groups) * call.batch_heads, kThreads, 0, stream>>>(
               call, saved, gradients, sink_groups, plan.key_tiles);
     }

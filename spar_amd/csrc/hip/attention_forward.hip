@@ -29,11 +29,15 @@ template <typename T>
 struct Results {
   Heads<T> output;
   T* logsumexp;
-  T* part_output;  // [split][batch][query head][query][extent]
+  T* part_output;  // [split][batch][query head][query][pitch]
   T* part_weight;  // [split][batch][query head][query]: log2 of the sum
   uint32_t splits;
+  uint32_t pitch;     // the extent rounded up to whole pieces
   uint64_t all_rows;  // batch * query heads * queries
 };
+
+// At most this many parts of a row: one for each thread that joins them.
+constexpr uint32_t kMostParts = kThreads;
 
 // A row's running softmax and output.  `top` is the maximum so far of its scores,
 // the same in the four lanes that share the row; `total` each lane's own part.
@@ -94,7 +98,7 @@ __device__ __forceinline__ void write_row(const Call& call, const Results<T>& re
     }
   } else {
     const uint64_t at = split * results.all_rows + row;
-    target = results.part_output + at * call.extent;
+    target = results.part_output + at * results.pitch;
     if (quarter == 0) results.part_weight[at] = weight;
   }
   out.visit(quarter, [&](uint32_t d, auto& run) {
@@ -103,9 +107,11 @@ __device__ __forceinline__ void write_row(const Call& call, const Results<T>& re
   });
 }
 
+// The head of row r, of some row where r is behind the last.
 template <typename T>
 __device__ __forceinline__ const T* head_row(const Heads<const T>& heads, const Call& call,
                                              uint32_t b, uint32_t key_head, uint32_t r) {
+  r = r < call.rows ? r : call.rows - 1;
   const uint32_t t = call.group.div(r);
   const uint32_t head = key_head * call.group.divisor + (r - t * call.group.divisor);
   return heads.data + b * heads.batch + head * heads.head + t * heads.token;
@@ -114,8 +120,8 @@ __device__ __forceinline__ const T* head_row(const Heads<const T>& heads, const 
 // Workgroups of one key head follow each other at a distance of batch * key heads,
 // a multiple of the 8 dies in common sizes, so that they share a die's cache; the
 // last rows, which see most, come first.
-template <typename T, int DP, int MB, int KB>
-__global__ __launch_bounds__(kThreads) void tile_kernel(Call call, Results<T> results,
+template <typename T, int DP, int MB, int KB, bool EVEN>
+__global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(Call call, Results<T> results,
                                                         Heads<const T> query, Heads<const T> key,
                                                         Heads<const T> value, uint32_t row_tiles) {
   constexpr int KT = KB * kBlock;
@@ -155,25 +161,37 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(Call call, Results<T> re
   for (int mb = 0; mb < MB; ++mb) {
     const uint32_t r = wave_row + mb * kBlock + column;
     token[mb] = call.token(r, first);
-    q[mb].load(token[mb] < 0 ? nullptr : head_row(query, call, b, key_head, r), call.extent,
-               quarter);
-    q[mb].scale(static_cast<T>(call.scale * kLog2E));
+    q[mb].template load<EVEN>(head_row(query, call, b, key_head, r), call.extent, quarter);
+    q[mb].finish(token[mb] >= 0, call.extent, quarter, static_cast<T>(call.scale * kLog2E));
     row[mb].out.clear();
   }
   const T* key_base = key.data + b * key.batch + key_head * key.head;
   const T* value_base = value.data + b * value.batch + key_head * value.head;
 
+  // Rows of a tile behind its run repeat the tile's first key; no row sees them.
+  typename Tile<T, KT, DP>::Stage next_keys, next_values;
+  const auto stage = [&](uint32_t i) {
+    int32_t begin, end;
+    seen.tile(i, KT, begin, end);
+    const auto at = [&](uint32_t j) {
+      const int32_t k = begin + static_cast<int32_t>(j);
+      return static_cast<uint64_t>(k < end ? k : begin);
+    };
+    next_keys.template load<EVEN>(call.extent,
+                                  [&](uint32_t j) { return key_base + at(j) * key.token; });
+    next_values.template load<EVEN>(call.extent,
+                                    [&](uint32_t j) { return value_base + at(j) * value.token; });
+  };
+  if (begin_tile < end_tile) stage(begin_tile);
+
   for (uint32_t i = begin_tile; i < end_tile; ++i) {
     int32_t begin, end;
     seen.tile(i, KT, begin, end);
     __syncthreads();
-    keys.fill(call.extent, [&](uint32_t j) {
-      return begin + j < end ? key_base + (begin + j) * key.token : nullptr;
-    });
-    values.fill(call.extent, [&](uint32_t j) {
-      return begin + j < end ? value_base + (begin + j) * value.token : nullptr;
-    });
+    keys.fill(next_keys);
+    values.fill(next_values);
     __syncthreads();
+    if (i + 1 < end_tile) stage(i + 1);
     bool any[KB];
     bool some = false;
 #pragma unroll
@@ -239,7 +257,7 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(Call call, Results<T> re
 
 // Four waves with the same 16 rows and every fourth block of 16 keys, read into
 // the operands' layout from memory; at the end the waves' rows meet in LDS.
-template <typename T, int DP>
+template <typename T, int DP, bool EVEN>
 __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> results,
                                                          Heads<const T> query, Heads<const T> key,
                                                          Heads<const T> value,
@@ -272,8 +290,8 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
   const uint32_t r = begin_row + column;
   const int32_t token = call.token(r, first);
   Operand<T, DP> q;
-  q.load(token < 0 ? nullptr : head_row(query, call, b, key_head, r), call.extent, quarter);
-  q.scale(static_cast<T>(call.scale * kLog2E));
+  q.template load<EVEN>(head_row(query, call, b, key_head, r), call.extent, quarter);
+  q.finish(token >= 0, call.extent, quarter, static_cast<T>(call.scale * kLog2E));
   Row<T, DP> row;
   row.out.clear();
   const T* key_base = key.data + b * key.batch + key_head * key.head;
@@ -282,28 +300,26 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
   for (uint32_t i = begin_block + wave; i < end_block; i += kWaves) {
     int32_t begin, end;
     seen.tile(i, kBlock, begin, end);
+    // Keys behind the run repeat its block's first; no row sees them.
+    const auto at_key = [&](int32_t k) { return static_cast<uint64_t>(k < end ? k : begin); };
     Operand<T, DP> k;
-    const int32_t own = begin + column;
-    k.load(own < end ? key_base + own * key.token : nullptr, call.extent, quarter);
+    k.template load<EVEN>(key_base + at_key(begin + column) * key.token, call.extent, quarter);
     using Out = Along<T, DP>;
     T v[4][DP / 16];  // pieces of the four keys whose weights this lane holds
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-      const int32_t at = begin + Mma<T>::row_of(n, quarter);
-      const T* head = at < end ? value_base + at * value.token : nullptr;
+      const T* head =
+          value_base + at_key(begin + Mma<T>::row_of(n, quarter)) * value.token;
 #pragma unroll
       for (int c = 0; c < Out::kChunks; ++c) {
-        T piece[W];
-#pragma unroll
-        for (int j = 0; j < W; ++j) piece[j] = T(0);
-        if (head != nullptr) load_piece<T, W>(piece, head, 16 * W * c + W * column, call.extent);
+        const auto piece = load_piece<EVEN>(head, 16 * W * c + W * column, call.extent);
 #pragma unroll
         for (int j = 0; j < W; ++j) v[n][c * W + j] = piece[j];
       }
       if constexpr (Out::kRest != 0) {
         const uint32_t d = 16 * W * Out::kChunks + 2 * column;
-        v[n][Out::kChunks * W] = head != nullptr && d < call.extent ? head[d] : T(0);
-        v[n][Out::kChunks * W + 1] = head != nullptr && d + 1 < call.extent ? head[d + 1] : T(0);
+        v[n][Out::kChunks * W] = head[d < call.extent ? d : 0];
+        v[n][Out::kChunks * W + 1] = head[d + 1 < call.extent ? d + 1 : 0];
       }
     }
     typename Mma<T>::Acc s{0, 0, 0, 0};
@@ -378,53 +394,88 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
       }
     } else {
       const uint64_t part = split * results.all_rows + place;
-      target = results.part_output + part * call.extent;
+      target = results.part_output + part * results.pitch;
       if (d == 0) results.part_weight[part] = weight;
     }
     store_piece(target, d, call.extent, run);
   }
 }
 
-// The parts of a row: o = sum 2^(w - top) o_part / sum 2^(w - top), in their order.
-// 32 lanes per row, each an interleaved share of the head.
+// The parts of a row: o = sum 2^(w - top) o_part / sum 2^(w - top).  A workgroup per
+// row: kLanes lanes side by side along the head, the splits dealt out to its runs,
+// whose sums meet in a tree.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void combine_kernel(Call call, Results<T> results) {
-  constexpr int kLanes = 32;
-  const uint64_t row =
-      (static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x) / kLanes;
-  if (row >= results.all_rows) return;
-  T top = lowest<T>();
-  for (uint32_t s = 0; s < results.splits; ++s) {
-    const T w = results.part_weight[s * results.all_rows + row];
-    top = w > top || w != w ? w : top;
+  constexpr int W = Vec16<T>::width;
+  constexpr uint32_t kLanes = SPAR_HIP_ATTENTION_MAX_EXTENT / W / 2;  // two pieces each
+  constexpr uint32_t kRuns = kThreads / kLanes;
+  __shared__ T weights[kMostParts];
+  __shared__ alignas(16) T outs[kRuns][SPAR_HIP_ATTENTION_MAX_EXTENT];
+  __shared__ T waves[kWaves];
+  const uint64_t row = blockIdx.x;
+  const uint32_t split = threadIdx.x;
+  const T weight = split < results.splits ? results.part_weight[split * results.all_rows + row]
+                                          : lowest<T>();
+  // A NaN weight (a row with a NaN score) stays one.
+  const auto larger = [](T a, T b) { return ((a > b) | (a != a)) ? a : b; };
+  T top = weight;
+#pragma unroll
+  for (int mask = kWave / 2; mask > 0; mask >>= 1) {
+    top = larger(top, __shfl_xor(top, mask, kWave));
   }
+  if (threadIdx.x % kWave == 0) waves[threadIdx.x / kWave] = top;
+  __syncthreads();
+  top = waves[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) top = larger(top, waves[w]);
   const T base = top == lowest<T>() ? T(0) : top;
+  weights[split] = exp2_of(weight - base);
+  __syncthreads();
   T sum = T(0);
-  for (uint32_t s = 0; s < results.splits; ++s) {
-    sum += exp2_of(results.part_weight[s * results.all_rows + row] - base);
-  }
+  for (uint32_t s = 0; s < results.splits; ++s) sum += weights[s];
   const T over = sum == T(0) ? T(0) : T(1) / sum;
+  const uint32_t lane = threadIdx.x % kLanes, run = threadIdx.x / kLanes;
+  typename Vec16<T>::type x[2] = {};
+#pragma unroll 4
+  for (uint32_t s = run; s < results.splits; s += kRuns) {
+    const T* part = results.part_output + (s * results.all_rows + row) * results.pitch;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t d = (lane + j * kLanes) * W;
+      if (d < results.pitch) {
+        x[j] += *reinterpret_cast<const typename Vec16<T>::type*>(part + d) * weights[s];
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    *reinterpret_cast<typename Vec16<T>::type*>(&outs[run][(lane + j * kLanes) * W]) = x[j];
+  }
+  for (uint32_t half = kRuns / 2; half > 0; half >>= 1) {
+    __syncthreads();
+    if (run < half) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t d = (lane + j * kLanes) * W;
+        x[j] += *reinterpret_cast<const typename Vec16<T>::type*>(&outs[run + half][d]);
+        *reinterpret_cast<typename Vec16<T>::type*>(&outs[run][d]) = x[j];
+      }
+    }
+  }
+  __syncthreads();
   const uint64_t batch_head = row / call.queries;
   const uint32_t t = static_cast<uint32_t>(row - batch_head * call.queries);
   const uint32_t heads = call.key_heads * call.group.divisor;
   const uint64_t b = batch_head / heads, head = batch_head % heads;
   T* target = results.output.data + b * results.output.batch + head * results.output.head +
               t * results.output.token;
-  const uint32_t lane = threadIdx.x % kLanes;
-  if (lane == 0 && results.logsumexp != nullptr) {
+  if (threadIdx.x < call.extent) target[threadIdx.x] = outs[0][threadIdx.x] * over;
+  if (threadIdx.x == 0 && results.logsumexp != nullptr) {
     results.logsumexp[row] =
         (sum == T(0) ? lowest<T>() : base + log2_of(sum)) * static_cast<T>(kLn2);
   }
-  for (uint32_t d = lane; d < call.extent; d += kLanes) {
-    T x = T(0);
-    for (uint32_t s = 0; s < results.splits; ++s) {
-      const uint64_t part = s * results.all_rows + row;
-      const T w = exp2_of(results.part_weight[part] - base) * over;
-      x += w * results.part_output[part * call.extent + d];
-    }
-    target[d] = x;
-  }
 }
+static_assert(kThreads >= SPAR_HIP_ATTENTION_MAX_EXTENT);
 
 // ---------------------------------------------------------------- launchers
 
@@ -443,6 +494,7 @@ struct Plan {
   uint32_t blocks;     // of 16 rows per wave (tile_kernel)
   uint32_t row_tiles;
   uint32_t splits;
+  uint32_t pitch;
   uint64_t rows;       // batch * query heads * queries
   uint64_t bytes;
 };
@@ -476,9 +528,11 @@ Plan plan_of(const SparHipAttention& a) {
   }
   const uint64_t wanted = grid / std::max<uint64_t>(1, plan.row_tiles * batch_heads);
   plan.splits = static_cast<uint32_t>(
-      std::max<uint64_t>(1, std::min(wanted, seen / kFewestKeys)));
+      std::max<uint64_t>(1, std::min({wanted, seen / kFewestKeys, uint64_t{kMostParts}})));
+  const uint64_t piece = 16 / element_size(a);
+  plan.pitch = static_cast<uint32_t>((a.extent + piece - 1) / piece * piece);
   if (plan.splits > 1) {
-    plan.bytes = plan.splits * plan.rows * (a.extent + 1) * element_size(a);
+    plan.bytes = plan.splits * plan.rows * (plan.pitch + 1) * element_size(a);
   }
   return plan;
 }
@@ -489,34 +543,36 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& outp
            const SparHipHeads& value, void* workspace, hipStream_t stream) {
   const Call call = call_of(a);
   Results<T> results{heads_of<T>(output), static_cast<T*>(logsumexp), nullptr, nullptr,
-                     plan.splits, plan.rows};
+                     plan.splits, plan.pitch, plan.rows};
   if (plan.splits > 1) {
     results.part_output = static_cast<T*>(workspace);
-    results.part_weight = results.part_output + plan.splits * plan.rows * a.extent;
+    results.part_weight = results.part_output + plan.splits * plan.rows * plan.pitch;
   }
   const uint32_t grid = plan.row_tiles * call.batch_heads * plan.splits;
   const auto q = heads_of<const T>(query), k = heads_of<const T>(key),
              v = heads_of<const T>(value);
-  with_width(a.extent, [&](auto width) {
+  with_width<T>(a.extent, [&](auto width, auto even) {
     constexpr int DP = decltype(width)::value;
+    constexpr bool EVEN = decltype(even)::value;
     constexpr int KB = sizeof(T) == 4 ? 2 : 1;
     if (plan.token) {
-      token_kernel<T, DP><<<grid, kThreads, 0, stream>>>(call, results, q, k, v, plan.row_tiles);
+      token_kernel<T, DP, EVEN>
+          <<<grid, kThreads, 0, stream>>>(call, results, q, k, v, plan.row_tiles);
       return;
     }
     if constexpr (sizeof(T) == 4 && DP <= 128) {
       if (plan.blocks == 2) {
-        tile_kernel<T, DP, 2, KB>
+        tile_kernel<T, DP, 2, KB, EVEN>
             <<<grid, kThreads, 0, stream>>>(call, results, q, k, v, plan.row_tiles);
         return;
       }
     }
-    tile_kernel<T, DP, 1, KB><<<grid, kThreads, 0, stream>>>(call, results, q, k, v,
-                                                             plan.row_tiles);
+    tile_kernel<T, DP, 1, KB, EVEN>
+        <<<grid, kThreads, 0, stream>>>(call, results, q, k, v, plan.row_tiles);
   });
   if (plan.splits > 1) {
-    combine_kernel<T><<<ceil_div_u32(plan.rows * 32, kThreads), kThreads, 0, stream>>>(call,
-                                                                                    results);
+    combine_kernel<T>
+        <<<static_cast<uint32_t>(plan.rows), kThreads, 0, stream>>>(call, results);
   }
 }
 
