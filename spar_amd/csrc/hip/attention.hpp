@@ -22,6 +22,9 @@
 
 #include <hip/hip_runtime.h>
 
+#include <initializer_list>
+#include <type_traits>
+
 #include "common.hpp"
 
 namespace spar_hip {
@@ -155,15 +158,21 @@ __device__ __forceinline__ T quarter_max(T x) {
   return x > z ? x : z;
 }
 
+// How a call's heads can be read in 16-byte pieces.
+enum class Reads {
+  Single,   // pieces do not divide the extent: element by element
+  Pieces,   // they do, at any address of an element
+  Aligned,  // and every head starts at a multiple of 16 bytes
+};
+
 // 16 bytes of a head at d, without a branch, so that a batch of them is in flight at
 // once: a piece behind the extent is read from the head's start, an element of a
-// piece that the extent cuts (EVEN says that it cuts none) from the head's end.
-// What stands there is finite where the head is, and meets zeros of the other
-// operand or is not written.
-template <bool EVEN, typename T>
+// piece that the extent cuts from the head's end.  What stands there is finite
+// where the head is, and meets zeros of the other operand or is not written.
+template <Reads READS, typename T>
 __device__ __forceinline__ typename Vec16<T>::type load_piece(const T* head, uint32_t d,
                                                               uint32_t extent) {
-  if constexpr (EVEN) {
+  if constexpr (READS != Reads::Single) {
     return loose_load(head + (d < extent ? d : 0));
   } else {
     typename Vec16<T>::type v;
@@ -198,11 +207,11 @@ struct Operand {
   static constexpr int W = Vec16<T>::width;
   T value[DP / 4];
 
-  template <bool EVEN>
+  template <Reads READS>
   __device__ __forceinline__ void load(const T* head, uint32_t extent, int quarter) {
 #pragma unroll
     for (int s = 0; s < DP / (4 * W); ++s) {
-      const auto piece = load_piece<EVEN>(head, 4 * W * s + W * quarter, extent);
+      const auto piece = load_piece<READS>(head, 4 * W * s + W * quarter, extent);
 #pragma unroll
       for (int i = 0; i < W; ++i) value[s * W + i] = piece[i];
     }
@@ -220,46 +229,98 @@ struct Operand {
   }
 };
 
-// A tile of ROWS heads in LDS, rows 16 bytes apart from a multiple of 128: 16
-// lanes that read one piece of 16 rows each, or 16 pieces of one row, fall into
-// different banks.  The pieces pass through registers, so that the next tile is on
-// its way while the present one is used.
-template <typename T, int ROWS, int DP>
+// Tiles of ROWS heads in LDS, two of them: one is used while the next one arrives.
+// Piece p of row r lies at piece p ^ (r % 8) of the row, so that 16 lanes that read
+// one piece of 16 rows each, and 16 lanes that read 16 pieces of one row, both
+// spread over all banks without padding: with that, aligned heads go from memory
+// to LDS directly, 64 neighbouring pieces of LDS per instruction, each lane asking
+// for the piece that belongs there.  Others pass through registers.
+template <typename T, int ROWS, int DP, Reads READS>
 struct Tile {
   static constexpr int W = Vec16<T>::width;
-  static constexpr int kPitch = DP + W;
   static constexpr int kPieces = DP / W;
   static constexpr int kShare = ROWS * kPieces / kThreads;  // pieces per thread
-  static_assert(ROWS * kPieces % kThreads == 0);
-  alignas(16) T value[ROWS * kPitch];
+  static constexpr bool kDirect = READS == Reads::Aligned;
+  static_assert(ROWS * kPieces % kThreads == 0 && kPieces % 8 == 0);
+  alignas(16) T value[2][ROWS * DP];
 
   struct Stage {
-    typename Vec16<T>::type piece[kShare];
-
-    // head_of(row): the row's head.  All threads of a workgroup.
-    template <bool EVEN, typename HeadOf>
-    __device__ __forceinline__ void load(uint32_t extent, HeadOf&& head_of) {
-#pragma unroll
-      for (int j = 0; j < kShare; ++j) {
-        const uint32_t at = threadIdx.x + j * kThreads;
-        piece[j] = load_piece<EVEN>(head_of(at / kPieces), at % kPieces * W, extent);
-      }
-    }
+    typename Vec16<T>::type piece[kDirect ? 1 : kShare];
   };
 
-  __device__ __forceinline__ void fill(const Stage& stage) {
+  // Starts the way of a tile into buffer `to`; head_of(row) is the row's head.  All
+  // threads of the workgroup.  It has arrived after finish() and a barrier.
+  template <typename HeadOf>
+  __device__ __forceinline__ void start(Stage& stage, int to, uint32_t extent,
+                                        HeadOf&& head_of) {
 #pragma unroll
     for (int j = 0; j < kShare; ++j) {
       const uint32_t at = threadIdx.x + j * kThreads;
-      *reinterpret_cast<typename Vec16<T>::type*>(value + at / kPieces * kPitch +
-                                                  at % kPieces * W) = stage.piece[j];
+      const uint32_t row = at / kPieces, piece = at % kPieces ^ row % 8;
+      if constexpr (kDirect) {
+        const uint32_t d = piece * W;
+        const T* from = head_of(row) + (d < extent ? d : 0);
+        const uint32_t wave_at = j * kThreads + threadIdx.x / kWave * kWave;
+        const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+            (__attribute__((address_space(3))) T*)(value[to])));
+        const uint32_t base = __builtin_amdgcn_readfirstlane(lds + wave_at * 16);
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                     :
+                     : "s"(base), "v"(from)
+                     : "memory");
+      } else {
+        stage.piece[j] = load_piece<READS>(head_of(row), piece * W, extent);
+      }
     }
   }
+  __device__ __forceinline__ void finish(const Stage& stage, int to) {
+    if constexpr (kDirect) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    } else {
+#pragma unroll
+      for (int j = 0; j < kShare; ++j) {
+        *reinterpret_cast<typename Vec16<T>::type*>(
+            value[to] + (threadIdx.x + j * kThreads) * W) = stage.piece[j];
+      }
+    }
+  }
+};
 
-  // The piece of row `row` that step group s contracts along the head.
-  __device__ __forceinline__ typename Vec16<T>::type along(int row, int s, int quarter) const {
-    return *reinterpret_cast<const typename Vec16<T>::type*>(value + row * kPitch + 4 * W * s +
-                                                             W * quarter);
+// Where a lane finds its pieces of a block of 16 rows of a tile.
+template <typename T, int DP>
+struct Lane {
+  static constexpr int W = Vec16<T>::width;
+  static constexpr int kChunks = DP / (16 * W);
+  static constexpr int kRest = DP % (16 * W) / 16;  // 0 or 2 blocks of 16
+  static_assert(kRest == 0 || kRest == 2);
+  using Piece = typename Vec16<T>::type;
+  int quarter, column;
+  int along_[2], across_[4], rest_[4];
+
+  __device__ __forceinline__ explicit Lane(int lane)
+      : quarter(lane / kBlock), column(lane % kBlock) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      along_[half] = column * DP + ((4 * half + quarter) ^ (column % 8)) * W;
+    }
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int row = Mma<T>::row_of(v, quarter);
+      across_[v] = row * DP + (column ^ (row % 8)) * W;
+      const int piece = 16 * kChunks + column * 2 / W;
+      rest_[v] = row * DP + (piece ^ (row % 8)) * W + column * 2 % W;
+    }
+  }
+  // Of row `column`, for group `step` of the contraction along the head.
+  __device__ __forceinline__ Piece along(const T* block, int step) const {
+    return *reinterpret_cast<const Piece*>(block + along_[step % 2] + step / 2 * 8 * W);
+  }
+  // Of row row_of(v, quarter), elements 16 W c + W column and on.
+  __device__ __forceinline__ Piece across(const T* block, int v, int c) const {
+    return *reinterpret_cast<const Piece*>(block + across_[v] + c * 16 * W);
+  }
+  __device__ __forceinline__ const T* rest(const T* block, int v) const {
+    return block + rest_[v];
   }
 };
 
@@ -268,9 +329,8 @@ struct Tile {
 template <typename T, int DP>
 struct Along {
   static constexpr int W = Vec16<T>::width;
-  static constexpr int kChunks = DP / (16 * W);
-  static constexpr int kRest = DP % (16 * W) / 16;  // 0 or 2 blocks
-  static_assert(kRest == 0 || kRest == 2);
+  static constexpr int kChunks = Lane<T, DP>::kChunks;
+  static constexpr int kRest = Lane<T, DP>::kRest;
   using Acc = typename Mma<T>::Acc;
   Acc block[DP / 16];
 
@@ -283,24 +343,6 @@ struct Along {
     for (int n = 0; n < DP / 16; ++n) {
 #pragma unroll
       for (int v = 0; v < 4; ++v) block[n][v] *= factor;
-    }
-  }
-  // += head^T weight for one head row (held in LDS, `row`) per quarter.
-  __device__ __forceinline__ void add(const T* row, int m, T weight) {
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      const auto piece =
-          *reinterpret_cast<const typename Vec16<T>::type*>(row + 16 * W * c + W * m);
-#pragma unroll
-      for (int n = 0; n < W; ++n) {
-        block[c * W + n] = Mma<T>::step(piece[n], weight, block[c * W + n]);
-      }
-    }
-    if constexpr (kRest != 0) {
-      const T* rest = row + 16 * W * kChunks + 2 * m;
-      const T first = rest[0], second = rest[1];
-      block[kChunks * W] = Mma<T>::step(first, weight, block[kChunks * W]);
-      block[kChunks * W + 1] = Mma<T>::step(second, weight, block[kChunks * W + 1]);
     }
   }
   // Calls body(d, values) for the runs of neighbours d a lane holds: of W values,
@@ -351,12 +393,109 @@ void with_padded_width(uint64_t extent, Body&& body) {
   }
 }
 
-// Calls body(integral_constant<DP>, Policy<EVEN>) with the smallest padded
-// width, EVEN if 16-byte pieces divide the extent.
+// COUNT pieces read from LDS AHEAD uses before their own: the reads' latency (about
+// 128 cycles) passes under the matrix instructions of the pieces before.  Left to
+// itself the compiler reads a piece right before its use, into registers that the
+// instructions before still occupy.  `queue` holds the first AHEAD on entry.
+template <int AHEAD, typename Piece>
+struct Queue {
+  static constexpr int kAhead = AHEAD;
+  Piece piece[AHEAD + 1];
+};
+
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0); }
+
+template <int AHEAD, typename Piece, typename Read>
+__device__ __forceinline__ void fill_queue(Queue<AHEAD, Piece>& queue, Read&& read) {
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) queue.piece[i] = read(i);
+}
+
+template <int COUNT, int AHEAD, typename Piece, typename Read, typename Use>
+__device__ __forceinline__ void run_queue(Queue<AHEAD, Piece>& queue, Read&& read, Use&& use) {
+  keep_order();
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i) {
+    if (i + AHEAD < COUNT) queue.piece[(i + AHEAD) % (AHEAD + 1)] = read(i + AHEAD);
+    keep_order();
+    use(i, queue.piece[i % (AHEAD + 1)]);
+    keep_order();
+  }
+}
+
+// out(i) += tile^T weight(i, .) for i < N: over BLOCKS blocks of 16 rows of a tile,
+// of each of which the lane has the weights of row_of(v, quarter), v < 4.
+template <int N, int BLOCKS, typename T, int DP>
+struct Across {
+  using L = Lane<T, DP>;
+  static constexpr int W = L::W;
+  static constexpr int kPerRow = L::kChunks + (L::kRest != 0);
+  static constexpr int kCount = BLOCKS * 4 * kPerRow;
+  static constexpr int kAhead = kCount < 2 ? kCount : 2;
+  const L& lane;
+  const T* rows;
+  Queue<kAhead, typename L::Piece> queue;
+
+  // Reads the first pieces.
+  __device__ __forceinline__ Across(const L& lane_, const T* rows_) : lane(lane_), rows(rows_) {
+    fill_queue(queue, [&](int i) { return read(i); });
+  }
+  __device__ __forceinline__ typename L::Piece read(int i) const {
+    const int block = i / (4 * kPerRow), v = i / kPerRow % 4, c = i % kPerRow;
+    const T* from = rows + block * kBlock * DP;
+    if (L::kRest != 0 && c == L::kChunks) {
+      const T* rest = lane.rest(from, v);
+      typename L::Piece piece{};
+      piece[0] = rest[0];
+      piece[1] = rest[1];
+      return piece;
+    }
+    return lane.across(from, v, c);
+  }
+  // weight(i, block, v)
+  template <typename Out, typename Weight>
+  __device__ __forceinline__ void run(Out&& out, Weight&& weight) {
+    run_queue<kCount>(
+        queue, [&](int i) { return read(i); },
+        [&](int at, const typename L::Piece& piece) {
+          const int b = at / (4 * kPerRow), v = at / kPerRow % 4, c = at % kPerRow;
+          const int pieces = L::kRest != 0 && c == L::kChunks ? 2 : W;
+#pragma unroll
+          for (int n = 0; n < W; ++n) {
+            if (n >= pieces) continue;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              auto& block = out(i).block[c * W + n];
+              block = Mma<T>::step(piece[n], weight(i, b, v), block);
+            }
+          }
+        });
+  }
+};
+
+template <typename T>
+bool reads_aligned(const SparHipHeads& heads) {
+  constexpr uint64_t W = Vec16<T>::width;
+  return aligned16(heads.data) && heads.strides[0] % W == 0 && heads.strides[1] % W == 0 &&
+         heads.strides[2] % W == 0;
+}
+
+// Calls body(integral_constant<DP>, integral_constant<READS>) with the smallest
+// padded width and the widest reads that all of `heads` allow.
 template <typename T, typename Body>
-void with_width(uint64_t extent, Body&& body) {
-  with_policy(extent % Vec16<T>::width == 0, [&](auto even) {
-    with_padded_width(extent, [&](auto width) { body(width, even); });
+void with_width(uint64_t extent, std::initializer_list<const SparHipHeads*> heads, Body&& body) {
+  Reads reads = extent % Vec16<T>::width == 0 ? Reads::Aligned : Reads::Single;
+  for (const SparHipHeads* h : heads) {
+    if (reads == Reads::Aligned && !reads_aligned<T>(*h)) reads = Reads::Pieces;
+  }
+  with_padded_width(extent, [&](auto width) {
+    if (reads == Reads::Aligned) {
+      body(width, std::integral_constant<Reads, Reads::Aligned>{});
+    } else if (reads == Reads::Pieces) {
+      body(width, std::integral_constant<Reads, Reads::Pieces>{});
+    } else {
+      body(width, std::integral_constant<Reads, Reads::Single>{});
+    }
   });
 }
 

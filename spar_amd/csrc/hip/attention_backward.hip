@@ -56,19 +56,42 @@ struct Place {
   }
 };
 
-template <typename T, int DP, int KB, bool EVEN>
+// s = a_rows a and dp = b_rows b of a block of 16 rows each, side by side: two sums
+// take turns in the matrix units.
+template <typename T, int DP>
+__device__ __forceinline__ void products(const Lane<T, DP>& lane, const T* a_rows,
+                                         const Operand<T, DP>& a, typename Mma<T>::Acc& s,
+                                         const T* b_rows, const Operand<T, DP>& b,
+                                         typename Mma<T>::Acc& dp) {
+  constexpr int W = Vec16<T>::width;
+  struct Pair {
+    typename Vec16<T>::type a, b;
+  };
+  const auto read = [&](int i) { return Pair{lane.along(a_rows, i), lane.along(b_rows, i)}; };
+  Queue<1, Pair> queue;
+  fill_queue(queue, read);
+  run_queue<DP / (4 * W)>(queue, read, [&](int i, const Pair& pair) {
+#pragma unroll
+    for (int n = 0; n < W; ++n) {
+      s = Mma<T>::step(pair.a[n], a.value[i * W + n], s);
+      dp = Mma<T>::step(pair.b[n], b.value[i * W + n], dp);
+    }
+  });
+}
+
+template <typename T, int DP, int KB, Reads READS>
 __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(Call call, Saved<T> saved,
                                                          Heads<T> gradient, uint32_t row_tiles) {
   constexpr int KT = KB * kBlock;
   constexpr int W = Vec16<T>::width;
   constexpr uint32_t kRows = kWaves * kBlock;
-  __shared__ Tile<T, KT, DP> keys, values;
+  __shared__ Tile<T, KT, DP, READS> keys, values;
   const uint32_t batch_head = blockIdx.x % call.batch_heads;
   const uint32_t row_tile = row_tiles - 1 - blockIdx.x / call.batch_heads;
   const uint32_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int lane = threadIdx.x % kWave;
-  const int quarter = lane / kBlock, column = lane % kBlock;
+  const Lane<T, DP> lane(threadIdx.x % kWave);
+  const int quarter = lane.quarter, column = lane.column;
 
   const int32_t first = call.length(b) - call.queries;
   const uint32_t begin_row = row_tile * kRows;
@@ -88,9 +111,9 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
   T delta = T(0), log_sum;
   {
     Operand<T, DP> out;
-    q.template load<EVEN>(place.of(saved.query, b), call.extent, quarter);
-    g.template load<EVEN>(place.of(saved.output_gradient, b), call.extent, quarter);
-    out.template load<EVEN>(place.of(saved.output, b), call.extent, quarter);
+    q.template load<READS>(place.of(saved.query, b), call.extent, quarter);
+    g.template load<READS>(place.of(saved.output_gradient, b), call.extent, quarter);
+    out.template load<READS>(place.of(saved.output, b), call.extent, quarter);
     log_sum = saved.logsumexp[place.at] * static_cast<T>(kLog2E);
     q.finish(token >= 0, call.extent, quarter, static_cast<T>(call.scale * kLog2E));
     g.finish(token >= 0, call.extent, quarter, T(1));
@@ -105,29 +128,33 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
   const T* value_base = saved.value.data + b * saved.value.batch + key_head * saved.value.head;
 
   // Rows of a tile behind its run repeat the tile's first key; no row sees them.
-  typename Tile<T, KT, DP>::Stage next_keys, next_values;
-  const auto stage = [&](uint32_t i) {
+  typename Tile<T, KT, DP, READS>::Stage next_keys, next_values;
+  const auto start = [&](uint32_t i) {
     int32_t begin, end;
     seen.tile(i, KT, begin, end);
     const auto at = [&](uint32_t j) {
       const int32_t k = begin + static_cast<int32_t>(j);
       return static_cast<uint64_t>(k < end ? k : begin);
     };
-    next_keys.template load<EVEN>(call.extent,
-                                  [&](uint32_t j) { return key_base + at(j) * saved.key.token; });
-    next_values.template load<EVEN>(
-        call.extent, [&](uint32_t j) { return value_base + at(j) * saved.value.token; });
+    keys.start(next_keys, i % 2, call.extent,
+               [&](uint32_t j) { return key_base + at(j) * saved.key.token; });
+    values.start(next_values, i % 2, call.extent,
+                 [&](uint32_t j) { return value_base + at(j) * saved.value.token; });
   };
-  if (tiles != 0) stage(0);
+  const auto finish = [&](uint32_t i) {
+    keys.finish(next_keys, i % 2);
+    values.finish(next_values, i % 2);
+  };
+  if (tiles != 0) {
+    start(0);
+    finish(0);
+  }
 
   for (uint32_t i = 0; i < tiles; ++i) {
     int32_t begin, end;
     seen.tile(i, KT, begin, end);
     __syncthreads();
-    keys.fill(next_keys);
-    values.fill(next_values);
-    __syncthreads();
-    if (i + 1 < tiles) stage(i + 1);
+    if (i + 1 < tiles) start(i + 1);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       const int32_t k0 = begin + kb * kBlock, k1 = k0 + kBlock - 1;
@@ -136,25 +163,22 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
       if (!any) continue;
       const bool whole = k1 <= oldest && k1 < end &&
                          (newest - k0 < call.window || k1 < call.sinks);
+      const T* key_rows = keys.value[i % 2] + kb * kBlock * DP;
+      const T* value_rows = values.value[i % 2] + kb * kBlock * DP;
       typename Mma<T>::Acc s{0, 0, 0, 0}, dp{0, 0, 0, 0};
-#pragma unroll
-      for (int step = 0; step < DP / (4 * W); ++step) {
-        const auto k_piece = keys.along(kb * kBlock + column, step, quarter);
-        const auto v_piece = values.along(kb * kBlock + column, step, quarter);
-#pragma unroll
-        for (int n = 0; n < W; ++n) {
-          s = Mma<T>::step(k_piece[n], q.value[step * W + n], s);
-          dp = Mma<T>::step(v_piece[n], g.value[step * W + n], dp);
-        }
-      }
+      products(lane, key_rows, q, s, value_rows, g, dp);
+      Across<1, 1, T, DP> across(lane, key_rows);
+      T ds[4];
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int32_t at = k0 + Mma<T>::row_of(v, quarter);
         const bool visible = whole | ((at < end) & call.sees(token, at));
-        const T ds = visible ? exp2_of(s[v] - log_sum) * (dp[v] - delta) : T(0);
-        dq.add(keys.value + (kb * kBlock + Mma<T>::row_of(v, quarter)) * keys.kPitch, column, ds);
+        const T toward = exp2_of(s[v] - log_sum) * (dp[v] - delta);
+        ds[v] = visible ? toward : T(0);
       }
+      across.run([&](int) -> auto& { return dq; }, [&](int, int, int v) { return ds[v]; });
     }
+    if (i + 1 < tiles) finish(i + 1);
   }
   if (r >= call.rows) return;
   T* target = place.of(gradient, b);
@@ -166,15 +190,15 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
 
 constexpr uint32_t kKeyTile = kWaves * kBlock;
 
-template <typename T, int DP, int RB, bool EVEN>
+template <typename T, int DP, int RB, Reads READS>
 __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void key_kernel(Call call, Saved<T> saved,
                                                        Gradients<T> gradients,
                                                        uint32_t sink_groups, uint32_t key_tiles) {
   constexpr int RT = RB * kBlock;
   constexpr int W = Vec16<T>::width;
-  __shared__ Tile<T, RT, DP> queries, output_gradients;
-  __shared__ T log_sums[RT], deltas[RT];
-  __shared__ int32_t tokens[RT];
+  __shared__ Tile<T, RT, DP, READS> queries, output_gradients;
+  __shared__ T log_sums[2][RT], deltas[2][RT];
+  __shared__ int32_t tokens[2][RT];
   const uint32_t batch_head = blockIdx.x % call.batch_heads;
   const uint32_t rest = blockIdx.x / call.batch_heads;
   // The splits of the sinks' later rows come first, then the tiles of keys.
@@ -183,8 +207,8 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void key_kernel(Ca
   const uint32_t split = behind ? rest % gradients.splits : 0;
   const uint32_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int lane = threadIdx.x % kWave;
-  const int quarter = lane / kBlock, column = lane % kBlock;
+  const Lane<T, DP> lane(threadIdx.x % kWave);
+  const int quarter = lane.quarter, column = lane.column;
 
   const int32_t length = call.length(b);
   const int32_t first = length - call.queries;
@@ -219,8 +243,8 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void key_kernel(Ca
   Operand<T, DP> k, x;
   {
     const uint64_t at = static_cast<uint32_t>(own) < call.keys ? own : 0;
-    k.template load<EVEN>(key_base + at * saved.key.token, call.extent, quarter);
-    x.template load<EVEN>(value_base + at * saved.value.token, call.extent, quarter);
+    k.template load<READS>(key_base + at * saved.key.token, call.extent, quarter);
+    x.template load<READS>(value_base + at * saved.value.token, call.extent, quarter);
     k.finish(keeps, call.extent, quarter, static_cast<T>(call.scale * kLog2E));
     x.finish(keeps, call.extent, quarter, T(1));
   }
@@ -229,38 +253,42 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void key_kernel(Ca
   dv.clear();
 
   // Rows of a tile behind the last repeat the tile's first; their token sees nothing.
-  typename Tile<T, RT, DP>::Stage next_queries, next_gradients;
+  typename Tile<T, RT, DP, READS>::Stage next_queries, next_gradients;
   T next_log_sum, next_delta;
   int32_t next_token;
-  const auto stage = [&](uint32_t i) {
+  const auto start = [&](uint32_t i) {
     const uint32_t row0 = begin_row + i * RT;
     const auto at = [&](uint32_t j) {
       return Place(call, b, key_head, row0 + j < end_row ? row0 + j : row0);
     };
-    next_queries.template load<EVEN>(call.extent,
-                                     [&](uint32_t j) { return at(j).of(saved.query, b); });
-    next_gradients.template load<EVEN>(
-        call.extent, [&](uint32_t j) { return at(j).of(saved.output_gradient, b); });
     const uint32_t own_row = threadIdx.x % RT;
     const Place place = at(own_row);
     next_token = row0 + own_row < end_row ? call.token(row0 + own_row, first) : -1;
     next_log_sum = saved.logsumexp[place.at];
     next_delta = saved.delta[place.at];
+    queries.start(next_queries, i % 2, call.extent,
+                  [&](uint32_t j) { return at(j).of(saved.query, b); });
+    output_gradients.start(next_gradients, i % 2, call.extent,
+                           [&](uint32_t j) { return at(j).of(saved.output_gradient, b); });
   };
-  if (begin_tile < tiles) stage(begin_tile);
+  const auto finish = [&](uint32_t i) {
+    if (threadIdx.x < RT) {
+      tokens[i % 2][threadIdx.x] = next_token;
+      log_sums[i % 2][threadIdx.x] = next_log_sum * static_cast<T>(kLog2E);
+      deltas[i % 2][threadIdx.x] = next_delta;
+    }
+    queries.finish(next_queries, i % 2);
+    output_gradients.finish(next_gradients, i % 2);
+  };
+  if (begin_tile < tiles) {
+    start(begin_tile);
+    finish(begin_tile);
+  }
 
   for (uint32_t i = begin_tile; i < tiles; ++i) {
     const uint32_t row0 = begin_row + i * RT;
     __syncthreads();
-    queries.fill(next_queries);
-    output_gradients.fill(next_gradients);
-    if (threadIdx.x < RT) {
-      tokens[threadIdx.x] = next_token;
-      log_sums[threadIdx.x] = next_log_sum * static_cast<T>(kLog2E);
-      deltas[threadIdx.x] = next_delta;
-    }
-    __syncthreads();
-    if (i + 1 < tiles) stage(i + 1);
+    if (i + 1 < tiles) start(i + 1);
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       const uint32_t block_row = row0 + rb * kBlock;
@@ -275,27 +303,28 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void key_kernel(Ca
       if (!any) continue;
       const bool whole = last_key <= oldest && block_end - block_row == kBlock &&
                          (newest - wave_key < call.window || last_key < call.sinks);
+      const T* query_rows = queries.value[i % 2] + rb * kBlock * DP;
+      const T* gradient_rows = output_gradients.value[i % 2] + rb * kBlock * DP;
       typename Mma<T>::Acc s{0, 0, 0, 0}, dp{0, 0, 0, 0};
-#pragma unroll
-      for (int step = 0; step < DP / (4 * W); ++step) {
-        const auto q_piece = queries.along(rb * kBlock + column, step, quarter);
-        const auto g_piece = output_gradients.along(rb * kBlock + column, step, quarter);
-#pragma unroll
-        for (int n = 0; n < W; ++n) {
-          s = Mma<T>::step(q_piece[n], k.value[step * W + n], s);
-          dp = Mma<T>::step(g_piece[n], x.value[step * W + n], dp);
-        }
-      }
+      products(lane, query_rows, k, s, gradient_rows, x, dp);
+      Across<1, 1, T, DP> across_gradients(lane, gradient_rows);
+      T p[4], ds[4];
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int row = rb * kBlock + Mma<T>::row_of(v, quarter);
-        const bool visible = whole | call.sees(tokens[row], own);
-        const T p = visible ? exp2_of(s[v] - log_sums[row]) : T(0);
-        const T ds = visible ? p * (dp[v] - deltas[row]) : T(0);
-        dv.add(output_gradients.value + row * output_gradients.kPitch, column, p);
-        dk.add(queries.value + row * queries.kPitch, column, ds);
+        const bool visible = whole | call.sees(tokens[i % 2][row], own);
+        const T weight = exp2_of(s[v] - log_sums[i % 2][row]);
+        const T toward = weight * (dp[v] - deltas[i % 2][row]);
+        p[v] = visible ? weight : T(0);
+        ds[v] = visible ? toward : T(0);
       }
+      across_gradients.run([&](int) -> auto& { return dv; },
+                           [&](int, int, int v) { return p[v]; });
+      Across<1, 1, T, DP> across_queries(lane, query_rows);
+      across_queries.run([&](int) -> auto& { return dk; },
+                         [&](int, int, int v) { return ds[v]; });
     }
+    if (i + 1 < tiles) finish(i + 1);
   }
 
   T* dk_target;
@@ -397,16 +426,17 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& quer
       reinterpret_cast<T*>(static_cast<char*>(workspace) + plan.delta_bytes), plan.splits,
       plan.sink_tiles};
   const uint32_t sink_groups = plan.sink_tiles * plan.splits;
-  with_width<T>(a.extent, [&](auto width, auto even) {
+  with_width<T>(a.extent, {&output_gradient, &output, &query, &key, &value},
+                [&](auto width, auto reads) {
     constexpr int DP = decltype(width)::value;
-    constexpr bool EVEN = decltype(even)::value;
+    constexpr Reads READS = decltype(reads)::value;
     constexpr int KB = sizeof(T) == 4 ? 2 : 1;
     if (call.rows != 0) {
-      query_kernel<T, DP, KB, EVEN><<<plan.row_tiles * call.batch_heads, kThreads, 0, stream>>>(
+      query_kernel<T, DP, KB, READS><<<plan.row_tiles * call.batch_heads, kThreads, 0, stream>>>(
           call, saved, gradients.query, plan.row_tiles);
     }
     if (call.keys != 0) {
-      key_kernel<T, DP, KB, EVEN>
+      key_kernel<T, DP, KB, READS>
           <<<(plan.key_tiles + sink_groups) * call.batch_heads, kThreads, 0, stream>>>(
               call, saved, gradients, sink_groups, plan.key_tiles);
     }

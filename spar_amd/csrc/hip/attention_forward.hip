@@ -120,21 +120,21 @@ __device__ __forceinline__ const T* head_row(const Heads<const T>& heads, const 
 // Workgroups of one key head follow each other at a distance of batch * key heads,
 // a multiple of the 8 dies in common sizes, so that they share a die's cache; the
 // last rows, which see most, come first.
-template <typename T, int DP, int MB, int KB, bool EVEN>
-__global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(Call call, Results<T> results,
-                                                        Heads<const T> query, Heads<const T> key,
-                                                        Heads<const T> value, uint32_t row_tiles) {
+template <typename T, int DP, int MB, int KB, Reads READS>
+__global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(
+    Call call, Results<T> results, Heads<const T> query, Heads<const T> key, Heads<const T> value,
+    uint32_t row_tiles) {
   constexpr int KT = KB * kBlock;
+  constexpr int W = Vec16<T>::width;
   constexpr uint32_t kRows = kWaves * MB * kBlock;
-  __shared__ Tile<T, KT, DP> keys, values;
+  __shared__ Tile<T, KT, DP, READS> keys, values;
   const uint32_t batch_head = blockIdx.x % call.batch_heads;
   const uint32_t rest = blockIdx.x / call.batch_heads;
   const uint32_t split = rest % results.splits;
   const uint32_t row_tile = row_tiles - 1 - rest / results.splits;
   const uint32_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int lane = threadIdx.x % kWave;
-  const int quarter = lane / kBlock, column = lane % kBlock;
+  const Lane<T, DP> lane(threadIdx.x % kWave);
 
   const int32_t first = call.length(b) - call.queries;  // token of query 0
   const uint32_t begin_row = row_tile * kRows;
@@ -146,6 +146,27 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(C
       static_cast<uint32_t>(static_cast<uint64_t>(tiles) * split / results.splits);
   const uint32_t end_tile =
       static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / results.splits);
+  const T* key_base = key.data + b * key.batch + key_head * key.head;
+  const T* value_base = value.data + b * value.batch + key_head * value.head;
+  // Rows of a tile behind its run repeat the tile's first key; no row sees them.
+  typename Tile<T, KT, DP, READS>::Stage next_keys, next_values;
+  const auto start = [&](uint32_t i) {
+    int32_t begin, end;
+    seen.tile(i, KT, begin, end);
+    const auto at = [&](uint32_t j) {
+      const int32_t k = begin + static_cast<int32_t>(j);
+      return static_cast<uint64_t>(k < end ? k : begin);
+    };
+    keys.start(next_keys, i % 2, call.extent,
+               [&](uint32_t j) { return key_base + at(j) * key.token; });
+    values.start(next_values, i % 2, call.extent,
+                 [&](uint32_t j) { return value_base + at(j) * value.token; });
+  };
+  const auto finish = [&](uint32_t i) {
+    keys.finish(next_keys, i % 2);
+    values.finish(next_values, i % 2);
+  };
+  if (begin_tile < end_tile) start(begin_tile);
 
   // This wave's rows and their tokens: all of them in the wave between `oldest`
   // and `newest`.
@@ -159,105 +180,78 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(C
   int32_t token[MB];
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
-    const uint32_t r = wave_row + mb * kBlock + column;
+    const uint32_t r = wave_row + mb * kBlock + lane.column;
     token[mb] = call.token(r, first);
-    q[mb].template load<EVEN>(head_row(query, call, b, key_head, r), call.extent, quarter);
-    q[mb].finish(token[mb] >= 0, call.extent, quarter, static_cast<T>(call.scale * kLog2E));
+    q[mb].template load<READS>(head_row(query, call, b, key_head, r), call.extent, lane.quarter);
+    q[mb].finish(token[mb] >= 0, call.extent, lane.quarter,
+                 static_cast<T>(call.scale * kLog2E));
     row[mb].out.clear();
   }
-  const T* key_base = key.data + b * key.batch + key_head * key.head;
-  const T* value_base = value.data + b * value.batch + key_head * value.head;
-
-  // Rows of a tile behind its run repeat the tile's first key; no row sees them.
-  typename Tile<T, KT, DP>::Stage next_keys, next_values;
-  const auto stage = [&](uint32_t i) {
-    int32_t begin, end;
-    seen.tile(i, KT, begin, end);
-    const auto at = [&](uint32_t j) {
-      const int32_t k = begin + static_cast<int32_t>(j);
-      return static_cast<uint64_t>(k < end ? k : begin);
-    };
-    next_keys.template load<EVEN>(call.extent,
-                                  [&](uint32_t j) { return key_base + at(j) * key.token; });
-    next_values.template load<EVEN>(call.extent,
-                                    [&](uint32_t j) { return value_base + at(j) * value.token; });
-  };
-  if (begin_tile < end_tile) stage(begin_tile);
+  if (begin_tile < end_tile) finish(begin_tile);
 
   for (uint32_t i = begin_tile; i < end_tile; ++i) {
     int32_t begin, end;
     seen.tile(i, KT, begin, end);
     __syncthreads();
-    keys.fill(next_keys);
-    values.fill(next_values);
-    __syncthreads();
-    if (i + 1 < end_tile) stage(i + 1);
-    bool any[KB];
-    bool some = false;
+    if (i + 1 < end_tile) start(i + 1);
+    const int32_t last = begin + KT - 1;
+    const bool any = begin <= newest && ((oldest < 0 ? 0 : oldest) - last < call.window ||
+                                         begin < call.sinks);
+    if (any) {
+      const T* key_rows = keys.value[i % 2];
+      const T* value_rows = values.value[i % 2];
+      typename Mma<T>::Acc s[KB][MB];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      const int32_t k0 = begin + kb * kBlock, k1 = k0 + kBlock - 1;
-      any[kb] = k0 < end && k0 <= newest &&
-                ((oldest < 0 ? 0 : oldest) - k1 < call.window || k0 < call.sinks);
-      some |= any[kb];
-    }
-    if (!some) continue;
-    T score[MB][KB][4];
+      for (int n = 0; n < KB; ++n) {
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      const int32_t k0 = begin + kb * kBlock, k1 = k0 + kBlock - 1;
-      typename Mma<T>::Acc s[MB];
+        for (int mb = 0; mb < MB; ++mb) s[n][mb] = typename Mma<T>::Acc{0, 0, 0, 0};
+      }
+      const auto read = [&](int i) { return lane.along(key_rows + i % KB * kBlock * DP, i / KB); };
+      Queue<2, typename Vec16<T>::type> queue;
+      fill_queue(queue, read);
+      run_queue<KB * DP / (4 * W)>(queue, read,
+                                   [&](int i, const typename Vec16<T>::type& piece) {
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb) s[mb] = typename Mma<T>::Acc{0, 0, 0, 0};
-      if (any[kb]) {
+        for (int x = 0; x < W; ++x) {
 #pragma unroll
-        for (int step = 0; step < DP / (4 * Operand<T, DP>::W); ++step) {
-          const auto piece = keys.along(kb * kBlock + column, step, quarter);
-#pragma unroll
-          for (int n = 0; n < Operand<T, DP>::W; ++n) {
-#pragma unroll
-            for (int mb = 0; mb < MB; ++mb) {
-              s[mb] = Mma<T>::step(piece[n], q[mb].value[step * Operand<T, DP>::W + n], s[mb]);
-            }
+          for (int mb = 0; mb < MB; ++mb) {
+            auto& score = s[i % KB][mb];
+            score = Mma<T>::step(piece[x], q[mb].value[i / KB * W + x], score);
           }
         }
-      }
-      const bool whole = any[kb] && k1 <= oldest && k1 < end &&
-                         (newest - k0 < call.window || k1 < call.sinks);
+      });
+      Across<MB, KB, T, DP> across(lane, value_rows);
+      const bool whole = last <= oldest && last < end &&
+                         (newest - begin < call.window || last < call.sinks);
+      T score[MB][KB][4];
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const int32_t at = k0 + Mma<T>::row_of(v, quarter);
-          const bool visible = whole | (any[kb] & (at < end) & call.sees(token[mb], at));
-          score[mb][kb][v] = visible ? s[mb][v] : lowest<T>();
+        for (int n = 0; n < KB; ++n) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int32_t at = begin + n * kBlock + Mma<T>::row_of(v, lane.quarter);
+            const bool visible = whole | ((at < end) & call.sees(token[mb], at));
+            score[mb][n][v] = visible ? s[n][mb][v] : lowest<T>();
+          }
         }
+        row[mb].template take<KB>(score[mb]);
       }
+      across.run([&](int mb) -> auto& { return row[mb].out; },
+                 [&](int mb, int n, int v) { return score[mb][n][v]; });
     }
-#pragma unroll
-    for (int mb = 0; mb < MB; ++mb) row[mb].template take<KB>(score[mb]);
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      if (!any[kb]) continue;
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const T* from =
-            values.value + (kb * kBlock + Mma<T>::row_of(v, quarter)) * values.kPitch;
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) row[mb].out.add(from, column, score[mb][kb][v]);
-      }
-    }
+    if (i + 1 < end_tile) finish(i + 1);
   }
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
-    write_row(call, results, b, key_head, wave_row + mb * kBlock + column, split, row[mb].top,
-              quarter_sum(row[mb].total), row[mb].out, quarter);
+    write_row(call, results, b, key_head, wave_row + mb * kBlock + lane.column, split,
+              row[mb].top, quarter_sum(row[mb].total), row[mb].out, lane.quarter);
   }
 }
 
 // Four waves with the same 16 rows and every fourth block of 16 keys, read into
 // the operands' layout from memory; at the end the waves' rows meet in LDS.
-template <typename T, int DP, bool EVEN>
+template <typename T, int DP, Reads READS>
 __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> results,
                                                          Heads<const T> query, Heads<const T> key,
                                                          Heads<const T> value,
@@ -290,7 +284,7 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
   const uint32_t r = begin_row + column;
   const int32_t token = call.token(r, first);
   Operand<T, DP> q;
-  q.template load<EVEN>(head_row(query, call, b, key_head, r), call.extent, quarter);
+  q.template load<READS>(head_row(query, call, b, key_head, r), call.extent, quarter);
   q.finish(token >= 0, call.extent, quarter, static_cast<T>(call.scale * kLog2E));
   Row<T, DP> row;
   row.out.clear();
@@ -303,7 +297,7 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
     // Keys behind the run repeat its block's first; no row sees them.
     const auto at_key = [&](int32_t k) { return static_cast<uint64_t>(k < end ? k : begin); };
     Operand<T, DP> k;
-    k.template load<EVEN>(key_base + at_key(begin + column) * key.token, call.extent, quarter);
+    k.template load<READS>(key_base + at_key(begin + column) * key.token, call.extent, quarter);
     using Out = Along<T, DP>;
     T v[4][DP / 16];  // pieces of the four keys whose weights this lane holds
 #pragma unroll
@@ -312,7 +306,7 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
           value_base + at_key(begin + Mma<T>::row_of(n, quarter)) * value.token;
 #pragma unroll
       for (int c = 0; c < Out::kChunks; ++c) {
-        const auto piece = load_piece<EVEN>(head, 16 * W * c + W * column, call.extent);
+        const auto piece = load_piece<READS>(head, 16 * W * c + W * column, call.extent);
 #pragma unroll
         for (int j = 0; j < W; ++j) v[n][c * W + j] = piece[j];
       }
@@ -551,23 +545,25 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& outp
   const uint32_t grid = plan.row_tiles * call.batch_heads * plan.splits;
   const auto q = heads_of<const T>(query), k = heads_of<const T>(key),
              v = heads_of<const T>(value);
-  with_width<T>(a.extent, [&](auto width, auto even) {
+  with_width<T>(a.extent, {&query, &key, &value}, [&](auto width, auto reads) {
     constexpr int DP = decltype(width)::value;
-    constexpr bool EVEN = decltype(even)::value;
+    constexpr Reads READS = decltype(reads)::value;
     constexpr int KB = sizeof(T) == 4 ? 2 : 1;
     if (plan.token) {
-      token_kernel<T, DP, EVEN>
+      // It reads pieces at any address alike.
+      constexpr Reads kReads = READS == Reads::Aligned ? Reads::Pieces : READS;
+      token_kernel<T, DP, kReads>
           <<<grid, kThreads, 0, stream>>>(call, results, q, k, v, plan.row_tiles);
       return;
     }
     if constexpr (sizeof(T) == 4 && DP <= 128) {
       if (plan.blocks == 2) {
-        tile_kernel<T, DP, 2, KB, EVEN>
+        tile_kernel<T, DP, 2, KB, READS>
             <<<grid, kThreads, 0, stream>>>(call, results, q, k, v, plan.row_tiles);
         return;
       }
     }
-    tile_kernel<T, DP, 1, KB, EVEN>
+    tile_kernel<T, DP, 1, KB, READS>
         <<<grid, kThreads, 0, stream>>>(call, results, q, k, v, plan.row_tiles);
   });
   if (plan.splits > 1) {
