@@ -246,30 +246,56 @@ struct Tile {
 
   struct Stage {
     typename Vec16<T>::type piece[kDirect ? 1 : kShare];
+    uint32_t offset[kDirect ? kShare : 1];  // bytes, of a tile of ROWS rows
   };
 
-  // Starts the way of a tile into buffer `to`; head_of(row) is the row's head.  All
-  // threads of the workgroup.  It has arrived after finish() and a barrier.
-  template <typename HeadOf>
-  __device__ __forceinline__ void start(Stage& stage, int to, uint32_t extent,
-                                        HeadOf&& head_of) {
+  // offset_of(row): elements from a tile's base to the head of its row.  The offsets
+  // of the rows in whole tiles, which most are, are computed once.
+  template <typename OffsetOf>
+  __device__ __forceinline__ void prepare(Stage& stage, uint32_t extent, OffsetOf&& offset_of) {
+    if constexpr (kDirect) {
 #pragma unroll
-    for (int j = 0; j < kShare; ++j) {
-      const uint32_t at = threadIdx.x + j * kThreads;
-      const uint32_t row = at / kPieces, piece = at % kPieces ^ row % 8;
-      if constexpr (kDirect) {
-        const uint32_t d = piece * W;
-        const T* from = head_of(row) + (d < extent ? d : 0);
-        const uint32_t wave_at = j * kThreads + threadIdx.x / kWave * kWave;
-        const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
-            (__attribute__((address_space(3))) T*)(value[to])));
-        const uint32_t base = __builtin_amdgcn_readfirstlane(lds + wave_at * 16);
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+      for (int j = 0; j < kShare; ++j) stage.offset[j] = bytes_at(j, extent, offset_of);
+    }
+  }
+  template <typename OffsetOf>
+  __device__ __forceinline__ static uint32_t bytes_at(int j, uint32_t extent,
+                                                      OffsetOf&& offset_of) {
+    const uint32_t at = threadIdx.x + j * kThreads;
+    const uint32_t row = at / kPieces, d = (at % kPieces ^ row % 8) * W;
+    return static_cast<uint32_t>(offset_of(row) + (d < extent ? d : 0)) * sizeof(T);
+  }
+
+  // Starts the way of the tile at `base` into buffer `to`; offset_of is asked where
+  // the tile is not `whole`.  All threads of the workgroup.  The tile has arrived
+  // after finish() and a barrier.
+  template <typename OffsetOf>
+  __device__ __forceinline__ void start(Stage& stage, int to, const T* base, bool whole,
+                                        uint32_t extent, OffsetOf&& offset_of) {
+    if constexpr (kDirect) {
+      const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+      const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+                               (__attribute__((address_space(3))) T*)(value[to]))) +
+                           wave * kWave * 16;
+      const auto load = [&](int j, uint32_t offset) {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                      :
-                     : "s"(base), "v"(from)
+                     : "s"(lds + j * kThreads * 16), "v"(offset), "s"(base)
                      : "memory");
+      };
+      if (whole) {
+#pragma unroll
+        for (int j = 0; j < kShare; ++j) load(j, stage.offset[j]);
       } else {
-        stage.piece[j] = load_piece<READS>(head_of(row), piece * W, extent);
+#pragma unroll
+        for (int j = 0; j < kShare; ++j) load(j, bytes_at(j, extent, offset_of));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kShare; ++j) {
+        const uint32_t at = threadIdx.x + j * kThreads;
+        const uint32_t row = at / kPieces, piece = at % kPieces ^ row % 8;
+        stage.piece[j] = load_piece<READS>(base + offset_of(row), piece * W, extent);
       }
     }
   }
@@ -473,22 +499,29 @@ struct Across {
   }
 };
 
+// Whether heads go to LDS directly: pieces at multiples of 16 bytes, and the rows of
+// a tile (of up to 32 tokens and all heads of a group) within 2^32 bytes.
 template <typename T>
-bool reads_aligned(const SparHipHeads& heads) {
+bool reads_aligned(const SparHipHeads& heads, uint64_t group) {
   constexpr uint64_t W = Vec16<T>::width;
+  constexpr uint64_t kMost = uint64_t{1} << 24;
   return aligned16(heads.data) && heads.strides[0] % W == 0 && heads.strides[1] % W == 0 &&
-         heads.strides[2] % W == 0;
+         heads.strides[2] % W == 0 && heads.strides[2] <= kMost &&
+         (group <= 1 || heads.strides[1] <= kMost * 8 / (group - 1));
 }
 
 // Calls body(integral_constant<DP>, integral_constant<READS>) with the smallest
 // padded width and the widest reads that all of `heads` allow.
 template <typename T, typename Body>
-void with_width(uint64_t extent, std::initializer_list<const SparHipHeads*> heads, Body&& body) {
-  Reads reads = extent % Vec16<T>::width == 0 ? Reads::Aligned : Reads::Single;
+void with_width(const SparHipAttention& a, std::initializer_list<const SparHipHeads*> heads,
+                Body&& body) {
+  Reads reads = a.extent % Vec16<T>::width == 0 ? Reads::Aligned : Reads::Single;
   for (const SparHipHeads* h : heads) {
-    if (reads == Reads::Aligned && !reads_aligned<T>(*h)) reads = Reads::Pieces;
+    if (reads == Reads::Aligned && !reads_aligned<T>(*h, a.query_heads / a.key_heads)) {
+      reads = Reads::Pieces;
+    }
   }
-  with_padded_width(extent, [&](auto width) {
+  with_padded_width(a.extent, [&](auto width) {
     if (reads == Reads::Aligned) {
       body(width, std::integral_constant<Reads, Reads::Aligned>{});
     } else if (reads == Reads::Pieces) {

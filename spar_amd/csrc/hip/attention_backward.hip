@@ -129,17 +129,17 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
 
   // Rows of a tile behind its run repeat the tile's first key; no row sees them.
   typename Tile<T, KT, DP, READS>::Stage next_keys, next_values;
+  keys.prepare(next_keys, call.extent, [&](uint32_t j) { return j * saved.key.token; });
+  values.prepare(next_values, call.extent, [&](uint32_t j) { return j * saved.value.token; });
   const auto start = [&](uint32_t i) {
     int32_t begin, end;
     seen.tile(i, KT, begin, end);
-    const auto at = [&](uint32_t j) {
-      const int32_t k = begin + static_cast<int32_t>(j);
-      return static_cast<uint64_t>(k < end ? k : begin);
-    };
-    keys.start(next_keys, i % 2, call.extent,
-               [&](uint32_t j) { return key_base + at(j) * saved.key.token; });
-    values.start(next_values, i % 2, call.extent,
-                 [&](uint32_t j) { return value_base + at(j) * saved.value.token; });
+    const uint64_t rows = end - begin;
+    const auto at = [&](uint64_t j) { return j < rows ? j : 0; };
+    keys.start(next_keys, i % 2, key_base + begin * saved.key.token, rows >= KT, call.extent,
+               [&](uint32_t j) { return at(j) * saved.key.token; });
+    values.start(next_values, i % 2, value_base + begin * saved.value.token, rows >= KT,
+                 call.extent, [&](uint32_t j) { return at(j) * saved.value.token; });
   };
   const auto finish = [&](uint32_t i) {
     keys.finish(next_keys, i % 2);
@@ -170,11 +170,14 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
       Across<1, 1, T, DP> across(lane, key_rows);
       T ds[4];
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int32_t at = k0 + Mma<T>::row_of(v, quarter);
-        const bool visible = whole | ((at < end) & call.sees(token, at));
-        const T toward = exp2_of(s[v] - log_sum) * (dp[v] - delta);
-        ds[v] = visible ? toward : T(0);
+      for (int v = 0; v < 4; ++v) ds[v] = exp2_of(s[v] - log_sum) * (dp[v] - delta);
+      if (!whole) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int32_t at = k0 + Mma<T>::row_of(v, quarter);
+          const bool visible = (at < end) & call.sees(token, at);
+          ds[v] = visible ? ds[v] : T(0);
+        }
       }
       across.run([&](int) -> auto& { return dq; }, [&](int, int, int v) { return ds[v]; });
     }
@@ -256,20 +259,38 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void key_kernel(Ca
   typename Tile<T, RT, DP, READS>::Stage next_queries, next_gradients;
   T next_log_sum, next_delta;
   int32_t next_token;
+  // Offsets of a tile's rows from the first head of the query of its first row,
+  // `extra` heads behind which that row is.
+  const uint32_t group = call.group.divisor;
+  const T* query_base = saved.query.data + b * saved.query.batch +
+                        static_cast<uint64_t>(key_head) * group * saved.query.head;
+  const T* gradient_base = saved.output_gradient.data + b * saved.output_gradient.batch +
+                           static_cast<uint64_t>(key_head) * group * saved.output_gradient.head;
+  const auto offset = [&](const Heads<const T>& heads, uint32_t j) {
+    const uint32_t t = call.group.div(j);
+    return t * heads.token + (j - t * group) * heads.head;
+  };
+  const bool even = RT % group == 0;
+  queries.prepare(next_queries, call.extent,
+                  [&](uint32_t j) { return offset(saved.query, j); });
+  output_gradients.prepare(next_gradients, call.extent,
+                           [&](uint32_t j) { return offset(saved.output_gradient, j); });
   const auto start = [&](uint32_t i) {
     const uint32_t row0 = begin_row + i * RT;
-    const auto at = [&](uint32_t j) {
-      return Place(call, b, key_head, row0 + j < end_row ? row0 + j : row0);
-    };
     const uint32_t own_row = threadIdx.x % RT;
-    const Place place = at(own_row);
-    next_token = row0 + own_row < end_row ? call.token(row0 + own_row, first) : -1;
+    const bool row = row0 + own_row < end_row;
+    const Place place(call, b, key_head, row ? row0 + own_row : row0);
+    next_token = row ? call.token(row0 + own_row, first) : -1;
     next_log_sum = saved.logsumexp[place.at];
     next_delta = saved.delta[place.at];
-    queries.start(next_queries, i % 2, call.extent,
-                  [&](uint32_t j) { return at(j).of(saved.query, b); });
-    output_gradients.start(next_gradients, i % 2, call.extent,
-                           [&](uint32_t j) { return at(j).of(saved.output_gradient, b); });
+    const uint32_t t0 = call.group.div(row0), extra = row0 - t0 * group;
+    const bool whole = even && row0 + RT <= end_row;
+    const auto at = [&](uint32_t j) { return extra + (row0 + j < end_row ? j : 0); };
+    queries.start(next_queries, i % 2, query_base + t0 * saved.query.token, whole, call.extent,
+                  [&](uint32_t j) { return offset(saved.query, at(j)); });
+    output_gradients.start(next_gradients, i % 2,
+                           gradient_base + t0 * saved.output_gradient.token, whole, call.extent,
+                           [&](uint32_t j) { return offset(saved.output_gradient, at(j)); });
   };
   const auto finish = [&](uint32_t i) {
     if (threadIdx.x < RT) {
@@ -312,11 +333,17 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void key_kernel(Ca
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int row = rb * kBlock + Mma<T>::row_of(v, quarter);
-        const bool visible = whole | call.sees(tokens[i % 2][row], own);
-        const T weight = exp2_of(s[v] - log_sums[i % 2][row]);
-        const T toward = weight * (dp[v] - deltas[i % 2][row]);
-        p[v] = visible ? weight : T(0);
-        ds[v] = visible ? toward : T(0);
+        p[v] = exp2_of(s[v] - log_sums[i % 2][row]);
+        ds[v] = p[v] * (dp[v] - deltas[i % 2][row]);
+      }
+      if (!whole) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const bool visible =
+              call.sees(tokens[i % 2][rb * kBlock + Mma<T>::row_of(v, quarter)], own);
+          p[v] = visible ? p[v] : T(0);
+          ds[v] = visible ? ds[v] : T(0);
+        }
       }
       across_gradients.run([&](int) -> auto& { return dv; },
                            [&](int, int, int v) { return p[v]; });
@@ -426,7 +453,7 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& quer
       reinterpret_cast<T*>(static_cast<char*>(workspace) + plan.delta_bytes), plan.splits,
       plan.sink_tiles};
   const uint32_t sink_groups = plan.sink_tiles * plan.splits;
-  with_width<T>(a.extent, {&output_gradient, &output, &query, &key, &value},
+  with_width<T>(a, {&output_gradient, &output, &query, &key, &value},
                 [&](auto width, auto reads) {
     constexpr int DP = decltype(width)::value;
     constexpr Reads READS = decltype(reads)::value;

@@ -150,17 +150,17 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(
   const T* value_base = value.data + b * value.batch + key_head * value.head;
   // Rows of a tile behind its run repeat the tile's first key; no row sees them.
   typename Tile<T, KT, DP, READS>::Stage next_keys, next_values;
+  keys.prepare(next_keys, call.extent, [&](uint32_t j) { return j * key.token; });
+  values.prepare(next_values, call.extent, [&](uint32_t j) { return j * value.token; });
   const auto start = [&](uint32_t i) {
     int32_t begin, end;
     seen.tile(i, KT, begin, end);
-    const auto at = [&](uint32_t j) {
-      const int32_t k = begin + static_cast<int32_t>(j);
-      return static_cast<uint64_t>(k < end ? k : begin);
-    };
-    keys.start(next_keys, i % 2, call.extent,
-               [&](uint32_t j) { return key_base + at(j) * key.token; });
-    values.start(next_values, i % 2, call.extent,
-                 [&](uint32_t j) { return value_base + at(j) * value.token; });
+    const uint64_t rows = end - begin;
+    const auto at = [&](uint64_t j) { return j < rows ? j : 0; };
+    keys.start(next_keys, i % 2, key_base + begin * key.token, rows >= KT, call.extent,
+               [&](uint32_t j) { return at(j) * key.token; });
+    values.start(next_values, i % 2, value_base + begin * value.token, rows >= KT,
+                 call.extent, [&](uint32_t j) { return at(j) * value.token; });
   };
   const auto finish = [&](uint32_t i) {
     keys.finish(next_keys, i % 2);
@@ -229,14 +229,25 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(
 #pragma unroll
         for (int n = 0; n < KB; ++n) {
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const int32_t at = begin + n * kBlock + Mma<T>::row_of(v, lane.quarter);
-            const bool visible = whole | ((at < end) & call.sees(token[mb], at));
-            score[mb][n][v] = visible ? s[n][mb][v] : lowest<T>();
+          for (int v = 0; v < 4; ++v) score[mb][n][v] = s[n][mb][v];
+        }
+      }
+      if (!whole) {
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+#pragma unroll
+          for (int n = 0; n < KB; ++n) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              const int32_t at = begin + n * kBlock + Mma<T>::row_of(v, lane.quarter);
+              const bool visible = (at < end) & call.sees(token[mb], at);
+              score[mb][n][v] = visible ? score[mb][n][v] : lowest<T>();
+            }
           }
         }
-        row[mb].template take<KB>(score[mb]);
       }
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) row[mb].template take<KB>(score[mb]);
       across.run([&](int mb) -> auto& { return row[mb].out; },
                  [&](int mb, int n, int v) { return score[mb][n][v]; });
     }
@@ -545,7 +556,7 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& outp
   const uint32_t grid = plan.row_tiles * call.batch_heads * plan.splits;
   const auto q = heads_of<const T>(query), k = heads_of<const T>(key),
              v = heads_of<const T>(value);
-  with_width<T>(a.extent, {&query, &key, &value}, [&](auto width, auto reads) {
+  with_width<T>(a, {&query, &key, &value}, [&](auto width, auto reads) {
     constexpr int DP = decltype(width)::value;
     constexpr Reads READS = decltype(reads)::value;
     constexpr int KB = sizeof(T) == 4 ? 2 : 1;
