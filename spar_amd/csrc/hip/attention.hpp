@@ -144,18 +144,33 @@ __device__ __forceinline__ T lowest() {
   return -static_cast<T>(__builtin_huge_val());
 }
 
-// Sums and maxima over the four quarters of a wave, which hold one column's rows.
+// Sums and maxima over the four quarters of a wave, which hold one column's rows: the
+// halves and then the quarters of a half change places in registers, each lane
+// combining both.  A maximum passes over NaN.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_fmaxf(a, b); }
+__device__ __forceinline__ double larger(double a, double b) { return __builtin_fmax(a, b); }
+
+template <typename Combine>
+__device__ __forceinline__ float over_quarters(float x, Combine&& combine) {
+  const uint32_t a = __float_as_uint(x);
+  const auto halves = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  const uint32_t h = __float_as_uint(combine(__uint_as_float(halves[0]),
+                                             __uint_as_float(halves[1])));
+  const auto quarters = __builtin_amdgcn_permlane16_swap(h, h, false, false);
+  return combine(__uint_as_float(quarters[0]), __uint_as_float(quarters[1]));
+}
+template <typename Combine>
+__device__ __forceinline__ double over_quarters(double x, Combine&& combine) {
+  x = combine(x, __shfl_xor(x, 32, kWave));
+  return combine(x, __shfl_xor(x, 16, kWave));
+}
 template <typename T>
 __device__ __forceinline__ T quarter_sum(T x) {
-  x += __shfl_xor(x, 16, kWave);
-  return x + __shfl_xor(x, 32, kWave);
+  return over_quarters(x, [](T a, T b) { return a + b; });
 }
 template <typename T>
 __device__ __forceinline__ T quarter_max(T x) {
-  const T y = __shfl_xor(x, 16, kWave);
-  x = x > y ? x : y;
-  const T z = __shfl_xor(x, 32, kWave);
-  return x > z ? x : z;
+  return over_quarters(x, [](T a, T b) { return larger(a, b); });
 }
 
 // How a call's heads can be read in 16-byte pieces.

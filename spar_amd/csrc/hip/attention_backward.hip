@@ -193,10 +193,15 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
 
 constexpr uint32_t kKeyTile = kWaves * kBlock;
 
+// Blocks of 16 keys that share a tile's waves, for so many sinks in the tile.
+__host__ __device__ inline int sink_blocks(int32_t sinks) {
+  return sinks <= kBlock ? 1 : sinks <= 2 * kBlock ? 2 : kWaves;
+}
+
 template <typename T, int DP, int RB, Reads READS>
 __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void key_kernel(Call call, Saved<T> saved,
                                                        Gradients<T> gradients,
-                                                       uint32_t sink_groups, uint32_t key_tiles) {
+                                                       uint32_t key_tiles) {
   constexpr int RT = RB * kBlock;
   constexpr int W = Vec16<T>::width;
   __shared__ Tile<T, RT, DP, READS> queries, output_gradients;
@@ -204,10 +209,10 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void key_kernel(Ca
   __shared__ int32_t tokens[2][RT];
   const uint32_t batch_head = blockIdx.x % call.batch_heads;
   const uint32_t rest = blockIdx.x / call.batch_heads;
-  // The splits of the sinks' later rows come first, then the tiles of keys.
-  const bool behind = rest < sink_groups;
-  const uint32_t tile = behind ? rest / gradients.splits : rest - sink_groups;
-  const uint32_t split = behind ? rest % gradients.splits : 0;
+  // The tiles of keys come first, the short splits of the sinks' later rows last.
+  const bool behind = rest >= key_tiles;
+  const uint32_t tile = behind ? (rest - key_tiles) / gradients.splits : rest;
+  const uint32_t split = behind ? (rest - key_tiles) % gradients.splits : 0;
   const uint32_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const Lane<T, DP> lane(threadIdx.x % kWave);
@@ -238,8 +243,12 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void key_kernel(Ca
     tiles = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / gradients.splits);
   }
 
-  const int32_t own = begin_key + wave * kBlock + column;
-  const int32_t wave_key = begin_key + wave * kBlock;
+  // Behind the window a tile with few sinks gives its waves the same keys and every
+  // second or fourth block of rows.
+  const int key_blocks = behind ? sink_blocks(call.sinks - begin_key) : kWaves;
+  const int32_t wave_key = begin_key + wave % key_blocks * kBlock;
+  const uint32_t turns = kWaves / key_blocks, turn = wave / key_blocks;
+  const int32_t own = wave_key + column;
   const bool keeps = own < length;
   const T* key_base = saved.key.data + b * saved.key.batch + key_head * saved.key.head;
   const T* value_base = saved.value.data + b * saved.value.batch + key_head * saved.value.head;
@@ -314,6 +323,7 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void key_kernel(Ca
     for (int rb = 0; rb < RB; ++rb) {
       const uint32_t block_row = row0 + rb * kBlock;
       if (block_row >= end_row) break;
+      if ((i * RB + rb) % turns != turn) continue;
       const uint32_t block_end =
           block_row + kBlock < end_row ? block_row + kBlock : end_row;
       const int32_t oldest = call.token(block_row, first);
@@ -357,6 +367,7 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void key_kernel(Ca
   T* dk_target;
   T* dv_target;
   if (behind) {
+    if (own >= call.sinks) return;
     T* part = gradients.parts +
               ((static_cast<uint64_t>(batch_head) * gradients.sink_tiles + tile) *
                    gradients.splits + split) * 2 * kKeyTile * call.extent;
@@ -389,18 +400,23 @@ __global__ __launch_bounds__(kThreads) void sink_kernel(Call call, Gradients<T> 
   const uint32_t key = within / call.extent, d = within % call.extent;
   const uint64_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
   const uint64_t stride = static_cast<uint64_t>(kKeyTile) * call.extent;
+  const uint32_t tile = key / kKeyTile;
+  const int blocks = sink_blocks(static_cast<int32_t>(sinks - tile * kKeyTile));
   const T* part = gradients.parts +
-                  (batch_head * gradients.sink_tiles + key / kKeyTile) * gradients.splits * 2 *
-                      stride +
+                  (batch_head * gradients.sink_tiles + tile) * gradients.splits * 2 * stride +
                   static_cast<uint64_t>(key % kKeyTile) * call.extent + d;
   T* dk = gradients.key.data + b * gradients.key.batch + key_head * gradients.key.head +
           key * gradients.key.token + d;
   T* dv = gradients.value.data + b * gradients.value.batch + key_head * gradients.value.head +
           key * gradients.value.token + d;
   T sum_k = *dk, sum_v = *dv;
+  const uint64_t turn = static_cast<uint64_t>(blocks) * kBlock * call.extent;
+#pragma unroll 4
   for (uint32_t s = 0; s < gradients.splits; ++s) {
-    sum_k += part[2 * s * stride];
-    sum_v += part[(2 * s + 1) * stride];
+    for (int t = 0; t < kWaves / blocks; ++t) {
+      sum_k += part[2 * s * stride + t * turn];
+      sum_v += part[(2 * s + 1) * stride + t * turn];
+    }
   }
   *dk = sum_k;
   *dv = sum_v;
@@ -414,8 +430,10 @@ struct Plan {
   uint64_t bytes;
 };
 
-// At most this many parts per sink tile.
-constexpr uint64_t kMostSplits = 64;
+// At most this many splits per sink tile, each of this part of the rows that a tile
+// of keys has in its window.
+constexpr uint64_t kMostSplits = 256;
+constexpr uint64_t kSplitShare = 2;
 
 Plan plan_of(const SparHipAttention& a) {
   Plan plan{};
@@ -426,12 +444,12 @@ Plan plan_of(const SparHipAttention& a) {
   plan.delta_bytes =
       (a.batch * a.query_heads * a.queries * element + 15) / 16 * 16;
   const uint64_t sinks = std::min(a.sinks, a.keys);
-  // A split for as many later queries as a tile of keys has in its window.
   if (a.window != 0 && sinks != 0 && a.keys > a.window) {
     plan.sink_tiles = ceil_div_u32(sinks, kKeyTile);
     const uint64_t later = std::min(a.queries, a.keys - a.window);
-    plan.splits = static_cast<uint32_t>(
-        std::min(kMostSplits, (later + a.window + kKeyTile - 1) / (a.window + kKeyTile)));
+    const uint64_t share = (a.window + kKeyTile) / kSplitShare;
+    plan.splits =
+        static_cast<uint32_t>(std::min(kMostSplits, (later + share - 1) / share));
   }
   plan.bytes = plan.delta_bytes + a.batch * a.key_heads * plan.sink_tiles * plan.splits * 2 *
                                       kKeyTile * a.extent * element;
@@ -465,7 +483,7 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& quer
     if (call.keys != 0) {
       key_kernel<T, DP, KB, READS>
           <<<(plan.key_tiles + sink_groups) * call.batch_heads, kThreads, 0, stream>>>(
-              call, saved, gradients, sink_groups, plan.key_tiles);
+              call, saved, gradients, plan.key_tiles);
     }
   });
   if (sink_groups != 0) {

@@ -39,38 +39,40 @@ struct Results {
 // At most this many parts of a row: one for each thread that joins them.
 constexpr uint32_t kMostParts = kThreads;
 
-// A row's running softmax and output.  `top` is the maximum so far of its scores,
-// the same in the four lanes that share the row; `total` each lane's own part.
+// A row's running softmax and output: weights are 2^(score - base), `total` each
+// lane's own part of their sum.  The base follows the row's maximum only when that
+// has grown by 2^kSlack, so that the output is rarely rescaled; sums of weights up
+// to 2^kSlack lose nothing in floating point.
 template <typename T, int DP>
 struct Row {
-  T top = lowest<T>();
+  static constexpr int kSlack = 8;
+  T base = lowest<T>();  // the same in the four lanes that share the row
   T total = T(0);
   Along<T, DP> out;
 
   // Takes the scores of KB blocks of keys and turns them into weights.
   template <int KB>
   __device__ __forceinline__ void take(T (&score)[KB][4]) {
-    T high = lowest<T>();
+    T high = score[0][0];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
-      for (int v = 0; v < 4; ++v) high = score[kb][v] > high ? score[kb][v] : high;
+      for (int v = kb == 0 ? 1 : 0; v < 4; ++v) high = larger(high, score[kb][v]);
     }
     high = quarter_max(high);
-    if (__any(high > top)) {
-      high = high > top ? high : top;
-      const T base = high == lowest<T>() ? T(0) : high;
-      const T shrink = exp2_of(top - base);
+    if (__any(high > base + kSlack)) {
+      high = larger(high, base);
+      const T shrink = exp2_of(base - (high == lowest<T>() ? T(0) : high));
       total *= shrink;
       out.scale(shrink);
-      top = high;
+      base = high;
     }
-    const T base = top == lowest<T>() ? T(0) : top;
+    const T from = base == lowest<T>() ? T(0) : base;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        score[kb][v] = exp2_of(score[kb][v] - base);
+        score[kb][v] = exp2_of(score[kb][v] - from);
         total += score[kb][v];
       }
     }
@@ -80,13 +82,13 @@ struct Row {
 // Writes a finished row: `sum` is its whole total.
 template <typename T, int DP>
 __device__ __forceinline__ void write_row(const Call& call, const Results<T>& results, uint32_t b,
-                                          uint32_t key_head, uint32_t r, uint32_t split, T top,
+                                          uint32_t key_head, uint32_t r, uint32_t split, T base,
                                           T sum, const Along<T, DP>& out, int quarter) {
   if (r >= call.rows) return;
   const uint32_t t = call.group.div(r);
   const uint32_t head = key_head * call.group.divisor + (r - t * call.group.divisor);
   const T over = sum == T(0) ? T(0) : T(1) / sum;
-  const T weight = sum == T(0) ? lowest<T>() : top + log2_of(sum);
+  const T weight = sum == T(0) ? lowest<T>() : base + log2_of(sum);
   const uint64_t row =
       (static_cast<uint64_t>(b) * call.key_heads * call.group.divisor + head) * call.queries + t;
   T* target;
@@ -256,7 +258,7 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
     write_row(call, results, b, key_head, wave_row + mb * kBlock + lane.column, split,
-              row[mb].top, quarter_sum(row[mb].total), row[mb].out, lane.quarter);
+              row[mb].base, quarter_sum(row[mb].total), row[mb].out, lane.quarter);
   }
 }
 
@@ -353,7 +355,7 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
   }
   const T total = quarter_sum(row.total);
   if (quarter == 0) {
-    tops[wave][column] = row.top;
+    tops[wave][column] = row.base;
     totals[wave][column] = total;
   }
   row.out.visit(quarter, [&](uint32_t d, auto& run) {
@@ -406,9 +408,75 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
   }
 }
 
-// The parts of a row: o = sum 2^(w - top) o_part / sum 2^(w - top).  A workgroup per
-// row: kLanes lanes side by side along the head, the splits dealt out to its runs,
-// whose sums meet in a tree.
+// The parts of a row: o = sum 2^(w - top) o_part / sum 2^(w - top), w the log2 of a
+// part's sum.  Few parts: kLanes lanes side by side along a row's head take them in
+// their order.
+constexpr uint32_t kFewParts = 8;
+
+template <typename T>
+__device__ __forceinline__ T* output_row(const Call& call, const Results<T>& results,
+                                         uint64_t row) {
+  const uint64_t batch_head = row / call.queries;
+  const uint32_t t = static_cast<uint32_t>(row - batch_head * call.queries);
+  const uint32_t heads = call.key_heads * call.group.divisor;
+  const uint64_t b = batch_head / heads, head = batch_head % heads;
+  return results.output.data + b * results.output.batch + head * results.output.head +
+         t * results.output.token;
+}
+
+// The larger, or a NaN (the weight of a row with a NaN score).
+template <typename T>
+__device__ __forceinline__ T top_of(T a, T b) {
+  return ((a > b) | (a != a)) ? a : b;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void combine_few_kernel(Call call, Results<T> results) {
+  constexpr int W = Vec16<T>::width;
+  constexpr uint32_t kLanes = 32;
+  const uint64_t row = static_cast<uint64_t>(blockIdx.x) * (kThreads / kLanes) +
+                       threadIdx.x / kLanes;
+  if (row >= results.all_rows) return;
+  T weight[kFewParts];
+  T top = lowest<T>();
+#pragma unroll
+  for (uint32_t s = 0; s < kFewParts; ++s) {
+    weight[s] = s < results.splits ? results.part_weight[s * results.all_rows + row]
+                                   : lowest<T>();
+    top = top_of(weight[s], top);
+  }
+  const T base = top == lowest<T>() ? T(0) : top;
+  T sum = T(0);
+#pragma unroll
+  for (uint32_t s = 0; s < kFewParts; ++s) {
+    weight[s] = exp2_of(weight[s] - base);
+    sum += weight[s];
+  }
+  const T over = sum == T(0) ? T(0) : T(1) / sum;
+  T* target = output_row(call, results, row);
+  const uint32_t lane = threadIdx.x % kLanes;
+  for (uint32_t d = lane * W; d < call.extent; d += kLanes * W) {
+    typename Vec16<T>::type x = {};
+#pragma unroll
+    for (uint32_t s = 0; s < kFewParts; ++s) {
+      if (s < results.splits) {
+        const T* part = results.part_output + (s * results.all_rows + row) * results.pitch;
+        x += *reinterpret_cast<const typename Vec16<T>::type*>(part + d) * weight[s];
+      }
+    }
+    T run[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) run[i] = x[i] * over;
+    store_piece(target, d, call.extent, run);
+  }
+  if (lane == 0 && results.logsumexp != nullptr) {
+    results.logsumexp[row] =
+        (sum == T(0) ? lowest<T>() : base + log2_of(sum)) * static_cast<T>(kLn2);
+  }
+}
+
+// Many parts: a workgroup per row, the parts dealt out to its runs of lanes, whose
+// sums meet in a tree.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void combine_kernel(Call call, Results<T> results) {
   constexpr int W = Vec16<T>::width;
@@ -421,18 +489,16 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(Call call, Results<T>
   const uint32_t split = threadIdx.x;
   const T weight = split < results.splits ? results.part_weight[split * results.all_rows + row]
                                           : lowest<T>();
-  // A NaN weight (a row with a NaN score) stays one.
-  const auto larger = [](T a, T b) { return ((a > b) | (a != a)) ? a : b; };
   T top = weight;
 #pragma unroll
   for (int mask = kWave / 2; mask > 0; mask >>= 1) {
-    top = larger(top, __shfl_xor(top, mask, kWave));
+    top = top_of(__shfl_xor(top, mask, kWave), top);
   }
   if (threadIdx.x % kWave == 0) waves[threadIdx.x / kWave] = top;
   __syncthreads();
   top = waves[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) top = larger(top, waves[w]);
+  for (int w = 1; w < kWaves; ++w) top = top_of(waves[w], top);
   const T base = top == lowest<T>() ? T(0) : top;
   weights[split] = exp2_of(weight - base);
   __syncthreads();
@@ -468,12 +534,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(Call call, Results<T>
     }
   }
   __syncthreads();
-  const uint64_t batch_head = row / call.queries;
-  const uint32_t t = static_cast<uint32_t>(row - batch_head * call.queries);
-  const uint32_t heads = call.key_heads * call.group.divisor;
-  const uint64_t b = batch_head / heads, head = batch_head % heads;
-  T* target = results.output.data + b * results.output.batch + head * results.output.head +
-              t * results.output.token;
+  T* target = output_row(call, results, row);
   if (threadIdx.x < call.extent) target[threadIdx.x] = outs[0][threadIdx.x] * over;
   if (threadIdx.x == 0 && results.logsumexp != nullptr) {
     results.logsumexp[row] =
@@ -520,11 +581,12 @@ Plan plan_of(const SparHipAttention& a) {
   if (plan.token) {
     plan.row_tiles = ceil_div_u32(rows, kBlock);
   } else {
-    // Two blocks of rows per wave halve the reading of tiles; where they fit the
-    // registers and the grid stays full.
+    // Two blocks of rows per wave halve the reading of tiles and share the softmax's
+    // exchanges; where they fit the registers and fill the grid, with splits if need be.
     constexpr uint64_t kRows = kWaves * kBlock;
     const bool narrow = a.extent <= 128 && a.dtype == SPAR_HIP_FLOAT32;
-    if (narrow && (rows + 2 * kRows - 1) / (2 * kRows) * batch_heads >= kFullGrid) {
+    const uint64_t tiles = (rows + 2 * kRows - 1) / (2 * kRows) * batch_heads;
+    if (narrow && tiles * std::max<uint64_t>(1, seen / kFewestKeys) >= kFullGrid) {
       plan.blocks = 2;
     }
     plan.row_tiles = ceil_div_u32(rows, kRows * plan.blocks);
@@ -577,7 +639,10 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& outp
     tile_kernel<T, DP, 1, KB, READS>
         <<<grid, kThreads, 0, stream>>>(call, results, q, k, v, plan.row_tiles);
   });
-  if (plan.splits > 1) {
+  if (plan.splits > 1 && plan.splits <= kFewParts) {
+    combine_few_kernel<T>
+        <<<ceil_div_u32(plan.rows * 32, kThreads), kThreads, 0, stream>>>(call, results);
+  } else if (plan.splits > 1) {
     combine_kernel<T>
         <<<static_cast<uint32_t>(plan.rows), kThreads, 0, stream>>>(call, results);
   }
