@@ -38,8 +38,12 @@ typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 template <typename T> struct Mma;
 
-// float32 runs at 157 TFLOP/s, twice what the vector units do without packed
-// instructions; products and sums are IEEE single.
+// float32 reaches 154 TFLOP/s, twice what the vector units do without packed
+// instructions; products and sums are IEEE single.  Vector instructions of any wave
+// take their time, 4 cycles each, from the same pipeline (one per matrix instruction
+// leaves 138 TFLOP/s, two 124), so the kernels count them: products start from what
+// would be subtracted from them, masks are formed for tiles at an edge alone, and
+// addresses move in scalar registers.
 template <> struct Mma<float> {
   using Acc = f32x4;
   __device__ static __forceinline__ Acc step(float a, float b, Acc c) {
@@ -254,9 +258,10 @@ template <typename T, int ROWS, int DP, Reads READS>
 struct Tile {
   static constexpr int W = Vec16<T>::width;
   static constexpr int kPieces = DP / W;
-  static constexpr int kShare = ROWS * kPieces / kThreads;  // pieces per thread
+  static constexpr int kAll = ROWS * kPieces;
+  static constexpr int kShare = (kAll + kThreads - 1) / kThreads;  // pieces per thread
   static constexpr bool kDirect = READS == Reads::Aligned;
-  static_assert(ROWS * kPieces % kThreads == 0 && kPieces % 8 == 0);
+  static_assert(kAll % kWave == 0 && kPieces % 8 == 0);
   alignas(16) T value[2][ROWS * DP];
 
   struct Stage {
@@ -273,6 +278,10 @@ struct Tile {
       for (int j = 0; j < kShare; ++j) stage.offset[j] = bytes_at(j, extent, offset_of);
     }
   }
+  // Whether share j of this wave lies in the tile (the last may not).
+  __device__ __forceinline__ static bool holds(int j, uint32_t wave) {
+    return (j + 1) * kThreads <= kAll || j * kThreads + wave * kWave < kAll;
+  }
   template <typename OffsetOf>
   __device__ __forceinline__ static uint32_t bytes_at(int j, uint32_t extent,
                                                       OffsetOf&& offset_of) {
@@ -287,8 +296,8 @@ struct Tile {
   template <typename OffsetOf>
   __device__ __forceinline__ void start(Stage& stage, int to, const T* base, bool whole,
                                         uint32_t extent, OffsetOf&& offset_of) {
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if constexpr (kDirect) {
-      const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
       const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
                                (__attribute__((address_space(3))) T*)(value[to]))) +
                            wave * kWave * 16;
@@ -300,17 +309,23 @@ struct Tile {
       };
       if (whole) {
 #pragma unroll
-        for (int j = 0; j < kShare; ++j) load(j, stage.offset[j]);
+        for (int j = 0; j < kShare; ++j) {
+          if (holds(j, wave)) load(j, stage.offset[j]);
+        }
       } else {
 #pragma unroll
-        for (int j = 0; j < kShare; ++j) load(j, bytes_at(j, extent, offset_of));
+        for (int j = 0; j < kShare; ++j) {
+          if (holds(j, wave)) load(j, bytes_at(j, extent, offset_of));
+        }
       }
     } else {
 #pragma unroll
       for (int j = 0; j < kShare; ++j) {
         const uint32_t at = threadIdx.x + j * kThreads;
         const uint32_t row = at / kPieces, piece = at % kPieces ^ row % 8;
-        stage.piece[j] = load_piece<READS>(base + offset_of(row), piece * W, extent);
+        if (holds(j, wave)) {
+          stage.piece[j] = load_piece<READS>(base + offset_of(row), piece * W, extent);
+        }
       }
     }
   }
@@ -320,8 +335,10 @@ struct Tile {
     } else {
 #pragma unroll
       for (int j = 0; j < kShare; ++j) {
-        *reinterpret_cast<typename Vec16<T>::type*>(
-            value[to] + (threadIdx.x + j * kThreads) * W) = stage.piece[j];
+        if (holds(j, __builtin_amdgcn_readfirstlane(threadIdx.x / kWave))) {
+          *reinterpret_cast<typename Vec16<T>::type*>(
+              value[to] + (threadIdx.x + j * kThreads) * W) = stage.piece[j];
+        }
       }
     }
   }
@@ -410,11 +427,17 @@ struct Along {
   }
 };
 
-// Waves per SIMD that a kernel's registers leave room for: one computes while the
-// other waits for its tile or takes exponentials.
+// Blocks of 16 rows in a tile of keys or queries.
+template <typename T, int DP>
+constexpr int tile_blocks() {
+  return DP * sizeof(T) <= 256 ? 2 : 1;
+}
+
+// Waves per SIMD that a kernel's registers are to leave room for.
 template <typename T, int DP>
 constexpr int tile_waves() {
-  return DP * sizeof(T) <= 512 ? 2 : 1;
+  const int row = DP * sizeof(T);
+  return (row <= 256 ? 4 : row <= 512 ? 3 : row <= 768 ? 2 : 1) - (sizeof(T) == 8 && row <= 512);
 }
 
 template <typename Body>
@@ -464,9 +487,9 @@ __device__ __forceinline__ void run_queue(Queue<AHEAD, Piece>& queue, Read&& rea
   }
 }
 
-// out(i) += tile^T weight(i, .) for i < N: over BLOCKS blocks of 16 rows of a tile,
-// of each of which the lane has the weights of row_of(v, quarter), v < 4.
-template <int N, int BLOCKS, typename T, int DP>
+// out += tile^T weights: over BLOCKS blocks of 16 rows of a tile, of each of which the
+// lane has the weights of row_of(v, quarter), v < 4.
+template <int BLOCKS, typename T, int DP>
 struct Across {
   using L = Lane<T, DP>;
   static constexpr int W = L::W;
@@ -493,9 +516,9 @@ struct Across {
     }
     return lane.across(from, v, c);
   }
-  // weight(i, block, v)
-  template <typename Out, typename Weight>
-  __device__ __forceinline__ void run(Out&& out, Weight&& weight) {
+  // weight(block, v)
+  template <typename Weight>
+  __device__ __forceinline__ void run(Along<T, DP>& out, Weight&& weight) {
     run_queue<kCount>(
         queue, [&](int i) { return read(i); },
         [&](int at, const typename L::Piece& piece) {
@@ -504,11 +527,7 @@ struct Across {
 #pragma unroll
           for (int n = 0; n < W; ++n) {
             if (n >= pieces) continue;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-              auto& block = out(i).block[c * W + n];
-              block = Mma<T>::step(piece[n], weight(i, b, v), block);
-            }
+            out.block[c * W + n] = Mma<T>::step(piece[n], weight(b, v), out.block[c * W + n]);
           }
         });
   }

@@ -56,7 +56,7 @@ struct Place {
   }
 };
 
-// s = a_rows a and dp = b_rows b of a block of 16 rows each, side by side: two sums
+// s += a_rows a and dp += b_rows b of a block of 16 rows each, side by side: two sums
 // take turns in the matrix units.
 template <typename T, int DP>
 __device__ __forceinline__ void products(const Lane<T, DP>& lane, const T* a_rows,
@@ -122,6 +122,8 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
   }
   delta = quarter_sum(delta);
   if (quarter == 0 && r < call.rows) saved.delta[place.at] = delta;
+  // What is subtracted from scores and from dP, where their products start.
+  const typename Mma<T>::Acc from_log_sum = -log_sum, from_delta = -delta;
   Along<T, DP> dq;
   dq.clear();
   const T* key_base = saved.key.data + b * saved.key.batch + key_head * saved.key.head;
@@ -165,12 +167,12 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
                          (newest - k0 < call.window || k1 < call.sinks);
       const T* key_rows = keys.value[i % 2] + kb * kBlock * DP;
       const T* value_rows = values.value[i % 2] + kb * kBlock * DP;
-      typename Mma<T>::Acc s{0, 0, 0, 0}, dp{0, 0, 0, 0};
+      typename Mma<T>::Acc s = from_log_sum, dp = from_delta;
       products(lane, key_rows, q, s, value_rows, g, dp);
-      Across<1, 1, T, DP> across(lane, key_rows);
+      Across<1, T, DP> across(lane, key_rows);
       T ds[4];
 #pragma unroll
-      for (int v = 0; v < 4; ++v) ds[v] = exp2_of(s[v] - log_sum) * (dp[v] - delta);
+      for (int v = 0; v < 4; ++v) ds[v] = exp2_of(s[v]) * dp[v];
       if (!whole) {
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
@@ -179,7 +181,7 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
           ds[v] = visible ? ds[v] : T(0);
         }
       }
-      across.run([&](int) -> auto& { return dq; }, [&](int, int, int v) { return ds[v]; });
+      across.run(dq, [&](int, int v) { return ds[v]; });
     }
     if (i + 1 < tiles) finish(i + 1);
   }
@@ -193,19 +195,25 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
 
 constexpr uint32_t kKeyTile = kWaves * kBlock;
 
+// Its operands and sums take a third more registers than the other kernels'.
+template <typename T, int DP>
+constexpr int key_waves() {
+  return DP * sizeof(T) <= 256 ? 3 : DP * sizeof(T) <= 512 ? 2 : 1;
+}
+
 // Blocks of 16 keys that share a tile's waves, for so many sinks in the tile.
 __host__ __device__ inline int sink_blocks(int32_t sinks) {
   return sinks <= kBlock ? 1 : sinks <= 2 * kBlock ? 2 : kWaves;
 }
 
 template <typename T, int DP, int RB, Reads READS>
-__global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void key_kernel(Call call, Saved<T> saved,
+__global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(Call call, Saved<T> saved,
                                                        Gradients<T> gradients,
                                                        uint32_t key_tiles) {
   constexpr int RT = RB * kBlock;
   constexpr int W = Vec16<T>::width;
   __shared__ Tile<T, RT, DP, READS> queries, output_gradients;
-  __shared__ T log_sums[2][RT], deltas[2][RT];
+  __shared__ alignas(16) T from_log_sums[2][RT], from_deltas[2][RT];  // negated
   __shared__ int32_t tokens[2][RT];
   const uint32_t batch_head = blockIdx.x % call.batch_heads;
   const uint32_t rest = blockIdx.x / call.batch_heads;
@@ -304,8 +312,8 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void key_kernel(Ca
   const auto finish = [&](uint32_t i) {
     if (threadIdx.x < RT) {
       tokens[i % 2][threadIdx.x] = next_token;
-      log_sums[i % 2][threadIdx.x] = next_log_sum * static_cast<T>(kLog2E);
-      deltas[i % 2][threadIdx.x] = next_delta;
+      from_log_sums[i % 2][threadIdx.x] = next_log_sum * static_cast<T>(-kLog2E);
+      from_deltas[i % 2][threadIdx.x] = -next_delta;
     }
     queries.finish(next_queries, i % 2);
     output_gradients.finish(next_gradients, i % 2);
@@ -336,15 +344,20 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void key_kernel(Ca
                          (newest - wave_key < call.window || last_key < call.sinks);
       const T* query_rows = queries.value[i % 2] + rb * kBlock * DP;
       const T* gradient_rows = output_gradients.value[i % 2] + rb * kBlock * DP;
-      typename Mma<T>::Acc s{0, 0, 0, 0}, dp{0, 0, 0, 0};
-      products(lane, query_rows, k, s, gradient_rows, x, dp);
-      Across<1, 1, T, DP> across_gradients(lane, gradient_rows);
-      T p[4], ds[4];
+      typename Mma<T>::Acc s, dp;
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int row = rb * kBlock + Mma<T>::row_of(v, quarter);
-        p[v] = exp2_of(s[v] - log_sums[i % 2][row]);
-        ds[v] = p[v] * (dp[v] - deltas[i % 2][row]);
+        s[v] = from_log_sums[i % 2][row];
+        dp[v] = from_deltas[i % 2][row];
+      }
+      products(lane, query_rows, k, s, gradient_rows, x, dp);
+      Across<1, T, DP> across_gradients(lane, gradient_rows);
+      T p[4], ds[4];
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        p[v] = exp2_of(s[v]);
+        ds[v] = p[v] * dp[v];
       }
       if (!whole) {
 #pragma unroll
@@ -355,11 +368,9 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void key_kernel(Ca
           ds[v] = visible ? ds[v] : T(0);
         }
       }
-      across_gradients.run([&](int) -> auto& { return dv; },
-                           [&](int, int, int v) { return p[v]; });
-      Across<1, 1, T, DP> across_queries(lane, query_rows);
-      across_queries.run([&](int) -> auto& { return dk; },
-                         [&](int, int, int v) { return ds[v]; });
+      across_gradients.run(dv, [&](int, int v) { return p[v]; });
+      Across<1, T, DP> across_queries(lane, query_rows);
+      across_queries.run(dk, [&](int, int v) { return ds[v]; });
     }
     if (i + 1 < tiles) finish(i + 1);
   }
@@ -475,13 +486,14 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& quer
                 [&](auto width, auto reads) {
     constexpr int DP = decltype(width)::value;
     constexpr Reads READS = decltype(reads)::value;
-    constexpr int KB = sizeof(T) == 4 ? 2 : 1;
+    constexpr int kBlocks = tile_blocks<T, DP>();
+    constexpr int kKeyBlocks = sizeof(T) == 4 && DP <= 128 ? 2 : 1;
     if (call.rows != 0) {
-      query_kernel<T, DP, KB, READS><<<plan.row_tiles * call.batch_heads, kThreads, 0, stream>>>(
+      query_kernel<T, DP, kBlocks, READS><<<plan.row_tiles * call.batch_heads, kThreads, 0, stream>>>(
           call, saved, gradients.query, plan.row_tiles);
     }
     if (call.keys != 0) {
-      key_kernel<T, DP, KB, READS>
+      key_kernel<T, DP, kKeyBlocks, READS>
           <<<(plan.key_tiles + sink_groups) * call.batch_heads, kThreads, 0, stream>>>(
               call, saved, gradients, plan.key_tiles);
     }

@@ -40,17 +40,22 @@ struct Results {
 constexpr uint32_t kMostParts = kThreads;
 
 // A row's running softmax and output: weights are 2^(score - base), `total` each
-// lane's own part of their sum.  The base follows the row's maximum only when that
-// has grown by 2^kSlack, so that the output is rarely rescaled; sums of weights up
-// to 2^kSlack lose nothing in floating point.
+// lane's own part of their sum.  Scores come with the base already taken off: their
+// product starts from `start`.  The base follows the row's maximum only when that has
+// grown by 2^kSlack, so that the output is rarely rescaled; sums of weights up to
+// 2^kSlack lose nothing in floating point.
 template <typename T, int DP>
 struct Row {
   static constexpr int kSlack = 8;
-  T base = lowest<T>();  // the same in the four lanes that share the row
+  typename Mma<T>::Acc start{0, 0, 0, 0};  // -base; the same in the row's four lanes
+  T limit = lowest<T>();  // of scores: kSlack, or the lowest before the first is seen
   T total = T(0);
   Along<T, DP> out;
 
-  // Takes the scores of KB blocks of keys and turns them into weights.
+  // The base, and the lowest value where no score has been seen.
+  __device__ __forceinline__ T top() const { return limit == lowest<T>() ? limit : -start[0]; }
+
+  // Turns the scores of KB blocks of keys into weights.
   template <int KB>
   __device__ __forceinline__ void take(T (&score)[KB][4]) {
     T high = score[0][0];
@@ -59,20 +64,26 @@ struct Row {
 #pragma unroll
       for (int v = kb == 0 ? 1 : 0; v < 4; ++v) high = larger(high, score[kb][v]);
     }
-    high = quarter_max(high);
-    if (__any(high > base + kSlack)) {
-      high = larger(high, base);
-      const T shrink = exp2_of(base - (high == lowest<T>() ? T(0) : high));
+    if (__any(high > limit)) {
+      high = quarter_max(high);
+      const bool grows = high > limit;
+      const T step = grows ? high : T(0);
+      const T shrink = limit == lowest<T>() ? T(1) : exp2_of(-step);
       total *= shrink;
       out.scale(shrink);
-      base = high;
+      start -= step;
+      limit = grows ? T(kSlack) : limit;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) score[kb][v] -= step;
+      }
     }
-    const T from = base == lowest<T>() ? T(0) : base;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        score[kb][v] = exp2_of(score[kb][v] - from);
+        score[kb][v] = exp2_of(score[kb][v]);
         total += score[kb][v];
       }
     }
@@ -122,13 +133,13 @@ __device__ __forceinline__ const T* head_row(const Heads<const T>& heads, const 
 // Workgroups of one key head follow each other at a distance of batch * key heads,
 // a multiple of the 8 dies in common sizes, so that they share a die's cache; the
 // last rows, which see most, come first.
-template <typename T, int DP, int MB, int KB, Reads READS>
+template <typename T, int DP, int KB, Reads READS>
 __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(
     Call call, Results<T> results, Heads<const T> query, Heads<const T> key, Heads<const T> value,
     uint32_t row_tiles) {
   constexpr int KT = KB * kBlock;
   constexpr int W = Vec16<T>::width;
-  constexpr uint32_t kRows = kWaves * MB * kBlock;
+  constexpr uint32_t kRows = kWaves * kBlock;
   __shared__ Tile<T, KT, DP, READS> keys, values;
   const uint32_t batch_head = blockIdx.x % call.batch_heads;
   const uint32_t rest = blockIdx.x / call.batch_heads;
@@ -172,23 +183,18 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(
 
   // This wave's rows and their tokens: all of them in the wave between `oldest`
   // and `newest`.
-  const uint32_t wave_row = begin_row + wave * MB * kBlock;
+  const uint32_t wave_row = begin_row + wave * kBlock;
   const uint32_t wave_end =
-      wave_row + MB * kBlock < call.rows ? wave_row + MB * kBlock : call.rows;
+      wave_row + kBlock < call.rows ? wave_row + kBlock : call.rows;
   const int32_t oldest = call.token(wave_row, first);
   const int32_t newest = wave_row < wave_end ? call.token(wave_end - 1, first) : -1;
-  Operand<T, DP> q[MB];
-  Row<T, DP> row[MB];
-  int32_t token[MB];
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
-    const uint32_t r = wave_row + mb * kBlock + lane.column;
-    token[mb] = call.token(r, first);
-    q[mb].template load<READS>(head_row(query, call, b, key_head, r), call.extent, lane.quarter);
-    q[mb].finish(token[mb] >= 0, call.extent, lane.quarter,
-                 static_cast<T>(call.scale * kLog2E));
-    row[mb].out.clear();
-  }
+  const uint32_t r = wave_row + lane.column;
+  const int32_t token = call.token(r, first);
+  Operand<T, DP> q;
+  q.template load<READS>(head_row(query, call, b, key_head, r), call.extent, lane.quarter);
+  q.finish(token >= 0, call.extent, lane.quarter, static_cast<T>(call.scale * kLog2E));
+  Row<T, DP> row;
+  row.out.clear();
   if (begin_tile < end_tile) finish(begin_tile);
 
   for (uint32_t i = begin_tile; i < end_tile; ++i) {
@@ -202,64 +208,46 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(
     if (any) {
       const T* key_rows = keys.value[i % 2];
       const T* value_rows = values.value[i % 2];
-      typename Mma<T>::Acc s[KB][MB];
+      typename Mma<T>::Acc s[KB];
 #pragma unroll
-      for (int n = 0; n < KB; ++n) {
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) s[n][mb] = typename Mma<T>::Acc{0, 0, 0, 0};
-      }
-      const auto read = [&](int i) { return lane.along(key_rows + i % KB * kBlock * DP, i / KB); };
+      for (int n = 0; n < KB; ++n) s[n] = row.start;
+      const auto read = [&](int p) { return lane.along(key_rows + p % KB * kBlock * DP, p / KB); };
       Queue<2, typename Vec16<T>::type> queue;
       fill_queue(queue, read);
       run_queue<KB * DP / (4 * W)>(queue, read,
-                                   [&](int i, const typename Vec16<T>::type& piece) {
+                                   [&](int p, const typename Vec16<T>::type& piece) {
 #pragma unroll
         for (int x = 0; x < W; ++x) {
-#pragma unroll
-          for (int mb = 0; mb < MB; ++mb) {
-            auto& score = s[i % KB][mb];
-            score = Mma<T>::step(piece[x], q[mb].value[i / KB * W + x], score);
-          }
+          s[p % KB] = Mma<T>::step(piece[x], q.value[p / KB * W + x], s[p % KB]);
         }
       });
-      Across<MB, KB, T, DP> across(lane, value_rows);
+      Across<KB, T, DP> across(lane, value_rows);
       const bool whole = last <= oldest && last < end &&
                          (newest - begin < call.window || last < call.sinks);
-      T score[MB][KB][4];
+      T score[KB][4];
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb) {
+      for (int n = 0; n < KB; ++n) {
 #pragma unroll
-        for (int n = 0; n < KB; ++n) {
-#pragma unroll
-          for (int v = 0; v < 4; ++v) score[mb][n][v] = s[n][mb][v];
-        }
+        for (int v = 0; v < 4; ++v) score[n][v] = s[n][v];
       }
       if (!whole) {
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
+        for (int n = 0; n < KB; ++n) {
 #pragma unroll
-          for (int n = 0; n < KB; ++n) {
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              const int32_t at = begin + n * kBlock + Mma<T>::row_of(v, lane.quarter);
-              const bool visible = (at < end) & call.sees(token[mb], at);
-              score[mb][n][v] = visible ? score[mb][n][v] : lowest<T>();
-            }
+          for (int v = 0; v < 4; ++v) {
+            const int32_t at = begin + n * kBlock + Mma<T>::row_of(v, lane.quarter);
+            const bool visible = (at < end) & call.sees(token, at);
+            score[n][v] = visible ? score[n][v] : lowest<T>();
           }
         }
       }
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) row[mb].template take<KB>(score[mb]);
-      across.run([&](int mb) -> auto& { return row[mb].out; },
-                 [&](int mb, int n, int v) { return score[mb][n][v]; });
+      row.template take<KB>(score);
+      across.run(row.out, [&](int n, int v) { return score[n][v]; });
     }
     if (i + 1 < end_tile) finish(i + 1);
   }
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
-    write_row(call, results, b, key_head, wave_row + mb * kBlock + lane.column, split,
-              row[mb].base, quarter_sum(row[mb].total), row[mb].out, lane.quarter);
-  }
+  write_row(call, results, b, key_head, r, split, row.top(), quarter_sum(row.total), row.out,
+            lane.quarter);
 }
 
 // Four waves with the same 16 rows and every fourth block of 16 keys, read into
@@ -329,7 +317,7 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
         v[n][Out::kChunks * W + 1] = head[d + 1 < call.extent ? d + 1 : 0];
       }
     }
-    typename Mma<T>::Acc s{0, 0, 0, 0};
+    typename Mma<T>::Acc s = row.start;
 #pragma unroll
     for (int step = 0; step < DP / 4; ++step) {
       s = Mma<T>::step(k.value[step], q.value[step], s);
@@ -355,7 +343,7 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
   }
   const T total = quarter_sum(row.total);
   if (quarter == 0) {
-    tops[wave][column] = row.base;
+    tops[wave][column] = row.top();
     totals[wave][column] = total;
   }
   row.out.visit(quarter, [&](uint32_t d, auto& run) {
@@ -557,7 +545,6 @@ constexpr uint64_t kFewestKeys = 256;
 
 struct Plan {
   bool token;
-  uint32_t blocks;     // of 16 rows per wave (tile_kernel)
   uint32_t row_tiles;
   uint32_t splits;
   uint32_t pitch;
@@ -575,23 +562,15 @@ Plan plan_of(const SparHipAttention& a) {
   const uint64_t batch_heads = a.batch * a.key_heads;
   plan.rows = a.batch * a.query_heads * a.queries;
   plan.token = rows <= kTokenRows;
-  plan.blocks = 1;
   uint64_t grid = kTokenGrid;
   uint64_t seen = most_seen(a);
   if (plan.token) {
     plan.row_tiles = ceil_div_u32(rows, kBlock);
   } else {
-    // Two blocks of rows per wave halve the reading of tiles and share the softmax's
-    // exchanges; where they fit the registers and fill the grid, with splits if need be.
     constexpr uint64_t kRows = kWaves * kBlock;
-    const bool narrow = a.extent <= 128 && a.dtype == SPAR_HIP_FLOAT32;
-    const uint64_t tiles = (rows + 2 * kRows - 1) / (2 * kRows) * batch_heads;
-    if (narrow && tiles * std::max<uint64_t>(1, seen / kFewestKeys) >= kFullGrid) {
-      plan.blocks = 2;
-    }
-    plan.row_tiles = ceil_div_u32(rows, kRows * plan.blocks);
+    plan.row_tiles = ceil_div_u32(rows, kRows);
     grid = kFullGrid;
-    seen = std::min(a.keys, seen + kRows * plan.blocks / (a.query_heads / a.key_heads));
+    seen = std::min(a.keys, seen + kRows / (a.query_heads / a.key_heads));
   }
   const uint64_t wanted = grid / std::max<uint64_t>(1, plan.row_tiles * batch_heads);
   plan.splits = static_cast<uint32_t>(
@@ -621,7 +600,6 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& outp
   with_width<T>(a, {&query, &key, &value}, [&](auto width, auto reads) {
     constexpr int DP = decltype(width)::value;
     constexpr Reads READS = decltype(reads)::value;
-    constexpr int KB = sizeof(T) == 4 ? 2 : 1;
     if (plan.token) {
       // It reads pieces at any address alike.
       constexpr Reads kReads = READS == Reads::Aligned ? Reads::Pieces : READS;
@@ -629,14 +607,7 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& outp
           <<<grid, kThreads, 0, stream>>>(call, results, q, k, v, plan.row_tiles);
       return;
     }
-    if constexpr (sizeof(T) == 4 && DP <= 128) {
-      if (plan.blocks == 2) {
-        tile_kernel<T, DP, 2, KB, READS>
-            <<<grid, kThreads, 0, stream>>>(call, results, q, k, v, plan.row_tiles);
-        return;
-      }
-    }
-    tile_kernel<T, DP, 1, KB, READS>
+    tile_kernel<T, DP, tile_blocks<T, DP>(), READS>
         <<<grid, kThreads, 0, stream>>>(call, results, q, k, v, plan.row_tiles);
   });
   if (plan.splits > 1 && plan.splits <= kFewParts) {
