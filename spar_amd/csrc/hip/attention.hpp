@@ -248,10 +248,15 @@ struct Operand {
   }
 };
 
+// What a piece's place in its row is mixed with.
+template <int PIECES>
+constexpr int kMix = PIECES % 16 == 0 ? 16 : 8;
+
 // Tiles of ROWS heads in LDS, two of them: one is used while the next one arrives.
-// Piece p of row r lies at piece p ^ (r % 8) of the row, so that 16 lanes that read
-// one piece of 16 rows each, and 16 lanes that read 16 pieces of one row, both
-// spread over all banks without padding: with that, aligned heads go from memory
+// Piece p of row r lies at piece p ^ (r % 16) of the row (r % 8 where 16 pieces do not
+// divide a row), so that 16 lanes that read one piece of 16 rows each, and 16 lanes
+// that read 16 pieces of one row, both spread over the 64 banks without padding (with
+// r % 8 every such read takes half as long again): so aligned heads go from memory
 // to LDS directly, 64 neighbouring pieces of LDS per instruction, each lane asking
 // for the piece that belongs there.  Others pass through registers.
 template <typename T, int ROWS, int DP, Reads READS>
@@ -286,7 +291,7 @@ struct Tile {
   __device__ __forceinline__ static uint32_t bytes_at(int j, uint32_t extent,
                                                       OffsetOf&& offset_of) {
     const uint32_t at = threadIdx.x + j * kThreads;
-    const uint32_t row = at / kPieces, d = (at % kPieces ^ row % 8) * W;
+    const uint32_t row = at / kPieces, d = (at % kPieces ^ row % kMix<kPieces>) * W;
     return static_cast<uint32_t>(offset_of(row) + (d < extent ? d : 0)) * sizeof(T);
   }
 
@@ -322,7 +327,7 @@ struct Tile {
 #pragma unroll
       for (int j = 0; j < kShare; ++j) {
         const uint32_t at = threadIdx.x + j * kThreads;
-        const uint32_t row = at / kPieces, piece = at % kPieces ^ row % 8;
+        const uint32_t row = at / kPieces, piece = at % kPieces ^ row % kMix<kPieces>;
         if (holds(j, wave)) {
           stage.piece[j] = load_piece<READS>(base + offset_of(row), piece * W, extent);
         }
@@ -353,25 +358,27 @@ struct Lane {
   static_assert(kRest == 0 || kRest == 2);
   using Piece = typename Vec16<T>::type;
   int quarter, column;
-  int along_[2], across_[4], rest_[4];
+  static constexpr int kMixed = kMix<DP / W>;
+  int along_[kMixed / 4], across_[4], rest_[4];
 
   __device__ __forceinline__ explicit Lane(int lane)
       : quarter(lane / kBlock), column(lane % kBlock) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      along_[half] = column * DP + ((4 * half + quarter) ^ (column % 8)) * W;
+    for (int s = 0; s < kMixed / 4; ++s) {
+      along_[s] = column * DP + ((4 * s + quarter) ^ (column % kMixed)) * W;
     }
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const int row = Mma<T>::row_of(v, quarter);
-      across_[v] = row * DP + (column ^ (row % 8)) * W;
+      across_[v] = row * DP + (column ^ (row % kMixed)) * W;
       const int piece = 16 * kChunks + column * 2 / W;
-      rest_[v] = row * DP + (piece ^ (row % 8)) * W + column * 2 % W;
+      rest_[v] = row * DP + (piece ^ (row % kMixed)) * W + column * 2 % W;
     }
   }
   // Of row `column`, for group `step` of the contraction along the head.
   __device__ __forceinline__ Piece along(const T* block, int step) const {
-    return *reinterpret_cast<const Piece*>(block + along_[step % 2] + step / 2 * 8 * W);
+    return *reinterpret_cast<const Piece*>(block + along_[step % (kMixed / 4)] +
+                                           step / (kMixed / 4) * kMixed * W);
   }
   // Of row row_of(v, quarter), elements 16 W c + W column and on.
   __device__ __forceinline__ Piece across(const T* block, int v, int c) const {

@@ -294,12 +294,13 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(Cal
                            [&](uint32_t j) { return offset(saved.output_gradient, j); });
   const auto start = [&](uint32_t i) {
     const uint32_t row0 = begin_row + i * RT;
-    const uint32_t own_row = threadIdx.x % RT;
-    const bool row = row0 + own_row < end_row;
-    const Place place(call, b, key_head, row ? row0 + own_row : row0);
-    next_token = row ? call.token(row0 + own_row, first) : -1;
-    next_log_sum = saved.logsumexp[place.at];
-    next_delta = saved.delta[place.at];
+    if (threadIdx.x < RT) {
+      const bool row = row0 + threadIdx.x < end_row;
+      const Place place(call, b, key_head, row ? row0 + threadIdx.x : row0);
+      next_token = row ? first + static_cast<int32_t>(place.t) : -1;
+      next_log_sum = saved.logsumexp[place.at];
+      next_delta = saved.delta[place.at];
+    }
     const uint32_t t0 = call.group.div(row0), extra = row0 - t0 * group;
     const bool whole = even && row0 + RT <= end_row;
     const auto at = [&](uint32_t j) { return extra + (row0 + j < end_row ? j : 0); };
