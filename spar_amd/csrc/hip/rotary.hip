@@ -280,11 +280,31 @@ struct NormParts {
   uint32_t heads[2];  // of each; heads[1] is 0 for one part
 };
 
+// The sum over LANES neighbouring lanes, in each of them, without LDS: lanes of a quad
+// change places, then quads of a half row and half rows mirror (their lanes hold equal
+// sums by then), then rows and halves of the wave swap.
+template <int CONTROL>
+__device__ __forceinline__ float moved(float x) {
+  return __uint_as_float(
+      __builtin_amdgcn_update_dpp(0, __float_as_uint(x), CONTROL, 0xf, 0xf, true));
+}
+template <int CONTROL>
+__device__ __forceinline__ double moved(double x) {
+  return __hiloint2double(
+      __builtin_amdgcn_update_dpp(0, __double2hiint(x), CONTROL, 0xf, 0xf, true),
+      __builtin_amdgcn_update_dpp(0, __double2loint(x), CONTROL, 0xf, 0xf, true));
+}
+
 template <typename T, int LANES>
-__device__ __forceinline__ T group_sum(T value) {
-#pragma unroll
-  for (int mask = LANES / 2; mask > 0; mask >>= 1) value += __shfl_xor(value, mask, kWave);
-  return value;
+__device__ __forceinline__ T group_sum(T x) {
+  static_assert(LANES >= 8 && LANES <= kWave);
+  x += moved<0xb1>(x);   // quad_perm 1 0 3 2
+  x += moved<0x4e>(x);   // quad_perm 2 3 0 1
+  x += moved<0x141>(x);  // row_half_mirror
+  if constexpr (LANES >= 16) x += moved<0x140>(x);  // row_mirror
+  if constexpr (LANES >= 32) x += __shfl_xor(x, 16, kWave);
+  if constexpr (LANES >= 64) x += __shfl_xor(x, 32, kWave);
+  return x;
 }
 
 template <typename T>
@@ -293,59 +313,58 @@ __device__ __forceinline__ T square_sum(const T (&x)[8]) {
          ((x[4] * x[4] + x[5] * x[5]) + (x[6] * x[6] + x[7] * x[7]));
 }
 
-// LANES lanes per head, a unit each (none where a head has fewer), for K heads
-// of one token: the heads of both parts counted through, so that a token's
-// queries and keys share cos, sin and the launch.
+// LANES lanes per head, a unit each (none where a head has fewer), for K heads of one
+// token of one part: cos, sin and the weight once for the K.  Groups of lanes count
+// through the first part's head groups and then the second's, so that a token's
+// queries and keys share the launch.
 template <typename T, bool HALF, bool NT, int LANES, int K>
 __global__ __launch_bounds__(kThreads) void norm_forward_kernel(NormParts<T> parts, Turn turn,
                                                                 Rows rows, uint32_t items,
                                                                 uint32_t units, FastDiv by_groups,
-                                                                T epsilon) {
+                                                                uint32_t first_groups, T epsilon) {
   const uint32_t item = (blockIdx.x * kThreads + threadIdx.x) / LANES;
   const uint32_t u = threadIdx.x % LANES;
   if (item >= items) return;
   const uint32_t row = by_groups.div(item);
-  const uint32_t group = item - row * by_groups.divisor;
+  uint32_t group = item - row * by_groups.divisor;
   uint64_t b, t;
   rows.split(row, b, t);
-  const bool holds = u < units;
   Unit unit{0, 0, 0, 0, kPassed};
-  if (holds) unit = unit_at<HALF>(u, turn.half, turn.extent);
-  const uint32_t heads = parts.heads[0] + parts.heads[1];
-  T x[K][8];
+  if (u < units) unit = unit_at<HALF>(u, turn.half, turn.extent);
+  const bool other = group >= first_groups;
+  const NormPart<T>& part = parts.part[other ? 1 : 0];
+  const uint32_t heads = parts.heads[other ? 1 : 0];
+  const uint32_t groups = other ? by_groups.divisor - first_groups : first_groups;
+  if (other) group -= first_groups;
+  const T* source = part.input.data + b * part.input.batch + t * part.input.token;
+  T* target = part.output.data + b * part.output.batch + t * part.output.token;
+  T x[K][8], w[8];
+  // A head behind the last is read as the last, and not written.
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const uint32_t head = group + k * by_groups.divisor;
-    if (head < heads) {
-      const bool other = head >= parts.heads[0];
-      const NormPart<T>& part = parts.part[other ? 1 : 0];
-      const uint32_t own = other ? head - parts.heads[0] : head;
-      load_unit<T, NT>(x[k], part.input.data + b * part.input.batch + t * part.input.token +
-                                 own * part.input.head, unit);
-    }
+    const uint32_t head = group + k * groups;
+    load_unit<T, NT>(x[k], source + (head < heads ? head : heads - 1) * part.input.head, unit);
   }
+  load_unit<T, false>(w, part.weight, unit);
   T c[4], s[4];
   unit_turn(turn, unit, b, t, c, s);
+  T d[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const uint32_t head = group + k * by_groups.divisor;
-    if (head >= heads) break;  // the same for all lanes of a head
-    const bool other = head >= parts.heads[0];
-    const NormPart<T>& part = parts.part[other ? 1 : 0];
-    const uint32_t own = other ? head - parts.heads[0] : head;
-    const T mean = group_sum<T, LANES>(square_sum(x[k])) / static_cast<T>(turn.extent);
-    const T d = sqrt(mean + epsilon);
-    const T over = T(1) / d;
-    if (u == 0 && part.denominator != nullptr) {
-      part.denominator[(b * parts.heads[other ? 1 : 0] + own) * rows.tokens + t] = d;
-    }
-    T w[8];
-    load_unit<T, false>(w, part.weight, unit);
+    d[k] = sqrt(group_sum<T, LANES>(square_sum(x[k])) / static_cast<T>(turn.extent) + epsilon);
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const T over = T(1) / d[k];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[k][i] = (x[k][i] * over) * w[i];
     turn_unit<T, HALF>(x[k], unit, c, s);
-    store_unit<T, NT>(part.output.data + b * part.output.batch + t * part.output.token +
-                          own * part.output.head, x[k], unit);
+    const uint32_t head = group + k * groups;
+    if (head >= heads) continue;
+    if (u == 0 && part.denominator != nullptr) {
+      part.denominator[(b * heads + head) * rows.tokens + t] = d[k];
+    }
+    store_unit<T, NT>(target + head * part.output.head, x[k], unit);
   }
 }
 
@@ -364,26 +383,35 @@ struct NormGradientParts {
   uint32_t heads[2];
 };
 
-// The same lanes walk the rows in a grid-stride; each keeps the weight gradients
-// of its unit for both parts, which the workgroup adds up at the end into one
-// row [2, extent] of `partials`.
+// Workgroups of the first part, then of the second; their groups of lanes walk the
+// part's rows and head groups in a grid-stride.  Each lane keeps the weight gradient
+// of its unit, which the workgroup adds up at the end into its row of `partials`.
 template <typename T, bool HALF, bool NT, int LANES, int K>
-__global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormGradientParts<T> parts,
-                                                                 Turn turn, Rows rows,
-                                                                 uint64_t items, uint32_t units,
-                                                                 uint32_t groups, T* partials) {
+__global__ __launch_bounds__(kThreads, 3) void norm_backward_kernel(NormGradientParts<T> parts,
+                                                                    Turn turn, Rows rows,
+                                                                    uint64_t all_rows,
+                                                                    uint32_t units,
+                                                                    uint32_t first_blocks,
+                                                                    T* partials) {
   constexpr uint32_t kGroups = kThreads / LANES;
+  const bool other = blockIdx.x >= first_blocks;
+  const NormGradientPart<T>& part = parts.part[other ? 1 : 0];
+  const uint32_t heads = parts.heads[other ? 1 : 0];
+  const uint32_t groups = (heads + K - 1) / K;
+  const uint32_t block = other ? blockIdx.x - first_blocks : blockIdx.x;
+  const uint32_t blocks = other ? gridDim.x - first_blocks : first_blocks;
   const uint32_t u = threadIdx.x % LANES;
   const bool holds = u < units;
   Unit unit{0, 0, 0, 0, kPassed};
   if (holds) unit = unit_at<HALF>(u, turn.half, turn.extent);
-  const uint32_t heads = parts.heads[0] + parts.heads[1];
   const T per_extent = T(1) / static_cast<T>(turn.extent);
-  T sums[2][8] = {};
+  T sums[8] = {}, w[8];
+  load_unit<T, false>(w, part.weight, unit);
   // Items of a group lie a stride apart: its row and head group advance by the
   // stride's quotient and remainder, with no division in the loop.
-  const uint64_t stride = static_cast<uint64_t>(gridDim.x) * kGroups;
-  uint64_t item = static_cast<uint64_t>(blockIdx.x) * kGroups + threadIdx.x / LANES;
+  const uint64_t items = all_rows * groups;
+  const uint64_t stride = static_cast<uint64_t>(blocks) * kGroups;
+  uint64_t item = static_cast<uint64_t>(block) * kGroups + threadIdx.x / LANES;
   uint64_t row = item / groups;
   uint32_t group = static_cast<uint32_t>(item - row * groups);
   const uint64_t row_step = stride / groups;
@@ -391,51 +419,46 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormGradientPar
   for (; item < items; item += stride) {
     uint64_t b, t;
     rows.split(row, b, t);
-    T c[4], s[4];
-    T x[K][8], g[K][8];
+    const T* source = part.input.data + b * part.input.batch + t * part.input.token;
+    const T* gradient = part.output_gradient.data + b * part.output_gradient.batch +
+                        t * part.output_gradient.token;
+    T x[K][8], g[K][8], over[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const uint32_t head = group + k * groups;
-      if (head < heads) {
-        const bool other = head >= parts.heads[0];
-        const NormGradientPart<T>& part = parts.part[other ? 1 : 0];
-        const uint32_t own = other ? head - parts.heads[0] : head;
-        load_unit<T, NT>(x[k], part.input.data + b * part.input.batch + t * part.input.token +
-                                   own * part.input.head, unit);
-        load_unit<T, NT>(g[k], part.output_gradient.data + b * part.output_gradient.batch +
-                                   t * part.output_gradient.token +
-                                   own * part.output_gradient.head, unit);
-      }
+      const uint32_t head = group + k * groups < heads ? group + k * groups : heads - 1;
+      load_unit<T, NT>(x[k], source + head * part.input.head, unit);
+      load_unit<T, NT>(g[k], gradient + head * part.output_gradient.head, unit);
+      over[k] = part.denominator[(b * heads + head) * rows.tokens + t];
     }
+    T c[4], s[4];
     unit_turn(turn, unit, b, t, c, s);
+    T mean[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const uint32_t head = group + k * groups;
-      if (head >= heads) break;
-      const bool other = head >= parts.heads[0];
-      const NormGradientPart<T>& part = parts.part[other ? 1 : 0];
-      const uint32_t own = other ? head - parts.heads[0] : head;
-      const T over =
-          T(1) / part.denominator[(b * parts.heads[other ? 1 : 0] + own) * rows.tokens + t];
+      // A head behind the last adds nothing.
+      const bool counts = group + k * groups < heads;
+      over[k] = T(1) / over[k];
       turn_unit<T, HALF>(g[k], unit, c, s);
-      T w[8];
-      load_unit<T, false>(w, part.weight, unit);
       T dot = T(0);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[k][i] *= over;
+        x[k][i] *= over[k];
         const T gx = g[k][i] * x[k][i];
-        sums[0][i] += other ? T(0) : gx;
-        sums[1][i] += other ? gx : T(0);
+        sums[i] += counts ? gx : T(0);
         g[k][i] *= w[i];
-        dot += g[k][i] * x[k][i];
+        dot += gx * w[i];
       }
-      const T mean = group_sum<T, LANES>(dot) * per_extent;
+      mean[k] = group_sum<T, LANES>(dot) * per_extent;
+    }
+    T* target = part.input_gradient.data + b * part.input_gradient.batch +
+                t * part.input_gradient.token;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[k][i] = (g[k][i] - x[k][i] * mean) * over;
-      store_unit<T, NT>(part.input_gradient.data + b * part.input_gradient.batch +
-                            t * part.input_gradient.token + own * part.input_gradient.head,
-                        g[k], unit);
+    for (int k = 0; k < K; ++k) {
+      const uint32_t head = group + k * groups;
+      if (head >= heads) continue;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[k][i] = (g[k][i] - x[k][i] * mean[k]) * over[k];
+      store_unit<T, NT>(target + head * part.input_gradient.head, g[k], unit);
     }
     row += row_step;
     group += group_step;
@@ -448,61 +471,54 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormGradientPar
 #pragma unroll
   for (int mask = kWave / 2; mask >= LANES; mask >>= 1) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sums[0][i] += __shfl_xor(sums[0][i], mask, kWave);
-      sums[1][i] += __shfl_xor(sums[1][i], mask, kWave);
-    }
+    for (int i = 0; i < 8; ++i) sums[i] += __shfl_xor(sums[i], mask, kWave);
   }
   constexpr int kWaves = kThreads / kWave;
-  __shared__ T shared[kWaves][2][LANES][9];
+  __shared__ T shared[kWaves][LANES][9];
   const int wave = threadIdx.x / kWave;
   if (threadIdx.x % kWave < LANES) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      shared[wave][0][u][i] = sums[0][i];
-      shared[wave][1][u][i] = sums[1][i];
-    }
+    for (int i = 0; i < 8; ++i) shared[wave][u][i] = sums[i];
   }
   __syncthreads();
-  if (wave < 2 && threadIdx.x % kWave < LANES && holds) {
-    T total[8];
+  if (threadIdx.x < LANES && holds) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      total[i] = shared[0][wave][u][i];
+      sums[i] = shared[0][u][i];
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) total[i] += shared[w][wave][u][i];
+      for (int w = 1; w < kWaves; ++w) sums[i] += shared[w][u][i];
     }
-    store_unit<T, false>(
-        partials + (static_cast<uint64_t>(blockIdx.x) * 2 + wave) * turn.extent, total, unit);
+    store_unit<T, false>(partials + static_cast<uint64_t>(blockIdx.x) * turn.extent, sums, unit);
   }
 }
 
-// Columns of the partial rows added up in their order: 16 columns per workgroup,
-// 64 lanes to a column, each a run of rows, then the runs in a tree.
+// The columns of a part's partial rows added up in their order (blockIdx.y: the part):
+// 16 columns per workgroup, 64 lanes to a column, each a run of rows, then the runs in
+// a tree.
 template <typename T>
 __global__ __launch_bounds__(1024) void norm_weight_kernel(T* first, T* second, const T* partials,
-                                                           uint32_t rows, uint32_t extent) {
+                                                           uint32_t first_rows,
+                                                           uint32_t second_rows,
+                                                           uint32_t extent) {
   __shared__ T shared[64][17];
+  const bool other = blockIdx.y != 0;
+  const uint32_t rows = other ? second_rows : first_rows;
+  const T* from = partials + (other ? static_cast<uint64_t>(first_rows) * extent : 0);
   const uint32_t lane = threadIdx.x % 16, run = threadIdx.x / 16;
   const uint32_t column = blockIdx.x * 16 + lane;
   const uint32_t per = (rows + 63) / 64;
   T sum = T(0);
-  if (column < 2 * extent) {
+  if (column < extent) {
     const uint32_t begin = run * per, end = begin + per < rows ? begin + per : rows;
 #pragma unroll 4
-    for (uint32_t r = begin; r < end; ++r) {
-      sum += partials[static_cast<uint64_t>(r) * 2 * extent + column];
-    }
+    for (uint32_t r = begin; r < end; ++r) sum += from[static_cast<uint64_t>(r) * extent + column];
   }
   shared[run][lane] = sum;
   for (uint32_t half = 32; half > 0; half >>= 1) {
     __syncthreads();
     if (run < half) shared[run][lane] += shared[run + half][lane];
   }
-  if (run == 0 && column < 2 * extent) {
-    T* target = column < extent ? first : second;
-    if (target != nullptr) target[column < extent ? column : column - extent] = shared[0][lane];
-  }
+  if (run == 0 && column < extent) (other ? second : first)[column] = shared[0][lane];
 }
 
 // ---------------------------------------------------------------- launchers
@@ -606,8 +622,8 @@ static_assert((SPAR_HIP_HEAD_NORM_MAX_EXTENT + 7) / 8 + 1 <= kWave);
 template <typename T, bool HALF, bool NT, int LANES, int K>
 void launch_norm_forward(const NormParts<T>& parts, uint64_t batch, uint64_t tokens,
                          const Turn& turn, double epsilon, hipStream_t stream) {
-  const uint32_t heads = parts.heads[0] + parts.heads[1];
-  const uint32_t groups = (heads + K - 1) / K;
+  const uint32_t first_groups = (parts.heads[0] + K - 1) / K;
+  const uint32_t groups = first_groups + (parts.heads[1] + K - 1) / K;
   FastDiv by_groups;
   by_groups.init(groups);
   const uint64_t most = (kIndex32Limit / LANES - kThreads) / groups;
@@ -617,7 +633,7 @@ void launch_norm_forward(const NormParts<T>& parts, uint64_t batch, uint64_t tok
     norm_forward_kernel<T, HALF, NT, LANES, K>
         <<<ceil_div_u32(static_cast<uint64_t>(items) * LANES, kThreads), kThreads, 0, stream>>>(
             parts, turn, rows_at(first, batch, tokens), items,
-            units_of(turn.half, turn.extent), by_groups, static_cast<T>(epsilon));
+            units_of(turn.half, turn.extent), by_groups, first_groups, static_cast<T>(epsilon));
   }
 }
 
@@ -650,13 +666,21 @@ void start_norm_forward(const SparHipHeadNorm* parts, int part_count, uint64_t b
   });
 }
 
-// Workgroups of the backward, one row of partial weight gradients each: as many
-// as the heads fill, at most four per CU.
-constexpr uint64_t kMostPartials = 1024;
+// Workgroups of the backward, one row of partial weight gradients each: as many as the
+// heads fill, at most three per CU, which is what their registers let a CU hold (with
+// four, the fourth waits for the others to end).
+constexpr uint64_t kMostPartials = 768;
 
 uint32_t partial_rows(uint64_t batch, uint64_t tokens, uint64_t heads) {
   const uint64_t wanted = (batch * tokens * heads + 7) / 8;
   return static_cast<uint32_t>(wanted < kMostPartials ? wanted : kMostPartials);
+}
+
+// Of these, the first part's: by its share of the heads, at least one for a part that
+// has any (`heads` is their sum).
+uint32_t first_rows_of(uint32_t partials, uint64_t first, uint64_t heads) {
+  const uint32_t share = static_cast<uint32_t>(partials * first / heads);
+  return first != 0 && share == 0 ? 1 : share;
 }
 
 template <typename T>
@@ -673,6 +697,10 @@ void start_norm_backward(const SparHipHeadNormGradient* parts, int part_count, u
   }
   const uint32_t heads = all.heads[0] + all.heads[1];
   const uint32_t partials = partial_rows(batch, tokens, heads);
+  const uint32_t first = partials == 0 ? 0 : first_rows_of(partials, all.heads[0], heads);
+  const uint32_t second = all.heads[1] == 0 || partials == 0 ? 0
+                          : partials > first                 ? partials - first
+                                                             : 1;
   const uint32_t units = units_of(turn.half, turn.extent);
   const bool stream_out =
       stream_output(batch * tokens * heads * static_cast<uint64_t>(turn.extent) * sizeof(T));
@@ -684,11 +712,10 @@ void start_norm_backward(const SparHipHeadNormGradient* parts, int part_count, u
           constexpr int kMany = 8 / sizeof(T);
           const auto launch = [&](auto many) {
             constexpr int K = decltype(many)::value;
-            const uint32_t groups = (heads + K - 1) / K;
             norm_backward_kernel<T, decltype(half)::value, decltype(nt)::value, kLanes, K>
-                <<<partials, kThreads, 0, stream>>>(all, turn, rows_at(0, batch, tokens),
-                                                    batch * tokens * groups, units, groups,
-                                                    static_cast<T*>(workspace));
+                <<<first + second, kThreads, 0, stream>>>(all, turn, rows_at(0, batch, tokens),
+                                                          batch * tokens, units, first,
+                                                          static_cast<T*>(workspace));
           };
           if (batch * tokens * heads * kLanes >= kMany * kMostPartials * kThreads) {
             launch(std::integral_constant<int, kMany>{});
@@ -699,10 +726,11 @@ void start_norm_backward(const SparHipHeadNormGradient* parts, int part_count, u
       });
     });
   }
-  norm_weight_kernel<T><<<ceil_div_u32(2 * turn.extent, 16), 1024, 0, stream>>>(
+  const dim3 grid(ceil_div_u32(turn.extent, 16), part_count);
+  norm_weight_kernel<T><<<grid, 1024, 0, stream>>>(
       static_cast<T*>(parts[0].weight_gradient),
       part_count > 1 ? static_cast<T*>(parts[1].weight_gradient) : nullptr,
-      static_cast<const T*>(workspace), partials, turn.extent);
+      static_cast<const T*>(workspace), first, second, turn.extent);
 }
 
 bool valid_head_norm(int part_count, uint64_t extent, const SparHipRotary* rotary, int dtype) {

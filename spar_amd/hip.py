@@ -67,15 +67,24 @@ class Rotary(ctypes.Structure):
                 ("layout", ctypes.c_int)]
 
 
+def _words(*names):
+    """Fields of 64 bits each; a name in brackets is a SparHipHeads."""
+    fields = []
+    for name in names:
+        parts = ([name[0]] + [f"{name[0]}_{axis}_stride" for axis in ("batch", "head", "token")]
+                 if isinstance(name, tuple) else [name])
+        fields += [(part, ctypes.c_uint64) for part in parts]
+    return fields
+
+
+# Flat, since nested structures take several times as long to make.
 class HeadNorm(ctypes.Structure):
-    _fields_ = [("output", Heads), ("denominator", ctypes.c_void_p), ("input", Heads),
-                ("weight", ctypes.c_void_p), ("heads", ctypes.c_uint64)]
+    _fields_ = _words(("output",), "denominator", ("input",), "weight", "heads")
 
 
 class HeadNormGradient(ctypes.Structure):
-    _fields_ = [("input_gradient", Heads), ("weight_gradient", ctypes.c_void_p),
-                ("output_gradient", Heads), ("input", Heads), ("weight", ctypes.c_void_p),
-                ("denominator", ctypes.c_void_p), ("heads", ctypes.c_uint64)]
+    _fields_ = _words(("input_gradient",), "weight_gradient", ("output_gradient",), ("input",),
+                      "weight", "denominator", "heads")
 
 
 class Attention(ctypes.Structure):
@@ -248,19 +257,20 @@ def rotary(positions, position_stride, position_dtype, frequencies, rotary_exten
 def head_norms(*parts):
     """Parts of spar_hip_launch_head_norm_rotary_forward, each (output, output
     strides, denominator, input, input strides, weight, heads)."""
-    return (HeadNorm * len(parts))(*(
-        HeadNorm(heads(output, output_strides), denominator, heads(source, strides), weight, count)
-        for output, output_strides, denominator, source, strides, weight, count in parts))
+    return (HeadNorm * len(parts))(*[
+        HeadNorm(output or 0, *output_strides, denominator or 0, source or 0, *strides,
+                 weight or 0, count)
+        for output, output_strides, denominator, source, strides, weight, count in parts])
 
 
 def head_norm_gradients(*parts):
     """Parts of spar_hip_launch_head_norm_rotary_backward, each (input gradient,
     its strides, weight gradient, output gradient, its strides, input, its
     strides, weight, denominator, heads)."""
-    return (HeadNormGradient * len(parts))(*(
-        HeadNormGradient(heads(dx, dx_strides), dw, heads(dy, dy_strides), heads(x, strides),
-                         weight, denominator, count)
-        for dx, dx_strides, dw, dy, dy_strides, x, strides, weight, denominator, count in parts))
+    return (HeadNormGradient * len(parts))(*[
+        HeadNormGradient(dx or 0, *dx_strides, dw or 0, dy or 0, *dy_strides, x or 0, *strides,
+                         weight or 0, denominator or 0, count)
+        for dx, dx_strides, dw, dy, dy_strides, x, strides, weight, denominator, count in parts])
 
 
 def head_norm_rotary_workspace(batch, tokens, heads, extent, dtype) -> int:
