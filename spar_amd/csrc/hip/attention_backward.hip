@@ -11,9 +11,10 @@
 // P and dS pass from the products that yield them into those that consume them in
 // registers (attention.hpp).
 //
-// The sinks are seen by every later row, so their keys have thousands of rows
-// where others have the window's: rows behind a tile's own window are split over
-// `splits` workgroups that write parts, which sink_kernel adds in their order.
+// Rows of a tile of keys are split over several workgroups where the tiles alone do
+// not fill the chip; and the sinks, which every later row sees, have thousands of
+// rows where other keys have the window's: those behind a tile's own window are split
+// too.  Splits write parts, which join_kernel adds in their order.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -31,12 +32,27 @@ struct Saved {
   T* delta;            // the same
 };
 
+// How the rows of tiles of keys are split, and where the parts lie: of every tile's
+// window (none for one split), then of the rows behind the windows of the sinks' tiles.
 template <typename T>
-struct Gradients {
-  Heads<T> query, key, value;
-  T* parts;         // [batch head][sink tile][split][dk, dv][64][extent]
-  uint32_t splits;  // of the rows behind a sink tile's window; 0: none
-  uint32_t sink_tiles;
+struct Splits {
+  T* parts;  // [batch head][tile][split][dk, dv][64][extent], and the same of the sinks
+  uint32_t key_tiles, main;    // splits of a tile's window: at least 1
+  uint32_t sink_tiles, later;  // splits of the rows behind it
+  uint32_t extent;
+
+  __device__ __forceinline__ uint64_t size() const;  // of a part
+  __device__ __forceinline__ T* main_part(uint32_t batch_head, uint32_t tile,
+                                          uint32_t split) const {
+    return parts + ((static_cast<uint64_t>(batch_head) * key_tiles + tile) * main + split) * size();
+  }
+  __device__ __forceinline__ T* later_part(uint32_t batch_heads, uint32_t batch_head,
+                                           uint32_t tile, uint32_t split) const {
+    T* const behind =
+        main == 1 ? parts : parts + static_cast<uint64_t>(batch_heads) * key_tiles * main * size();
+    return behind +
+           ((static_cast<uint64_t>(batch_head) * sink_tiles + tile) * later + split) * size();
+  }
 };
 
 // Query head, query and place among [batch][query head][query] of a row.
@@ -206,10 +222,16 @@ __host__ __device__ inline int sink_blocks(int32_t sinks) {
   return sinks <= kBlock ? 1 : sinks <= 2 * kBlock ? 2 : kWaves;
 }
 
+template <typename T>
+__device__ __forceinline__ uint64_t Splits<T>::size() const {
+  return static_cast<uint64_t>(2 * kKeyTile) * extent;
+}
+
 template <typename T, int DP, int RB, Reads READS>
 __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(Call call, Saved<T> saved,
-                                                       Gradients<T> gradients,
-                                                       uint32_t key_tiles) {
+                                                       Heads<T> key_gradient,
+                                                       Heads<T> value_gradient,
+                                                       Splits<T> splits) {
   constexpr int RT = RB * kBlock;
   constexpr int W = Vec16<T>::width;
   __shared__ Tile<T, RT, DP, READS> queries, output_gradients;
@@ -218,9 +240,11 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(Cal
   const uint32_t batch_head = blockIdx.x % call.batch_heads;
   const uint32_t rest = blockIdx.x / call.batch_heads;
   // The tiles of keys come first, the short splits of the sinks' later rows last.
-  const bool behind = rest >= key_tiles;
-  const uint32_t tile = behind ? (rest - key_tiles) / gradients.splits : rest;
-  const uint32_t split = behind ? (rest - key_tiles) % gradients.splits : 0;
+  const uint32_t main_groups = splits.key_tiles * splits.main;
+  const bool behind = rest >= main_groups;
+  const uint32_t parts = behind ? splits.later : splits.main;
+  const uint32_t tile = (behind ? rest - main_groups : rest) / parts;
+  const uint32_t split = (behind ? rest - main_groups : rest) % parts;
   const uint32_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const Lane<T, DP> lane(threadIdx.x % kWave);
@@ -245,11 +269,9 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(Cal
   uint32_t end_row = static_cast<uint32_t>(high - first) * call.group.divisor;
   if (begin_row >= end_row) begin_row = end_row = 0;
   uint32_t tiles = (end_row - begin_row + RT - 1) / RT;
-  uint32_t begin_tile = 0;
-  if (behind) {
-    begin_tile = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * split / gradients.splits);
-    tiles = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / gradients.splits);
-  }
+  const uint32_t begin_tile =
+      static_cast<uint32_t>(static_cast<uint64_t>(tiles) * split / parts);
+  tiles = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / parts);
 
   // Behind the window a tile with few sinks gives its waves the same keys and every
   // second or fourth block of rows.
@@ -378,19 +400,17 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(Cal
 
   T* dk_target;
   T* dv_target;
-  if (behind) {
-    if (own >= call.sinks) return;
-    T* part = gradients.parts +
-              ((static_cast<uint64_t>(batch_head) * gradients.sink_tiles + tile) *
-                   gradients.splits + split) * 2 * kKeyTile * call.extent;
+  if (own >= static_cast<int32_t>(behind ? call.sinks : call.keys)) return;
+  if (behind || splits.main > 1) {
+    T* part = behind ? splits.later_part(call.batch_heads, batch_head, tile, split)
+                     : splits.main_part(batch_head, tile, split);
     dk_target = part + static_cast<uint64_t>(wave * kBlock + column) * call.extent;
     dv_target = dk_target + static_cast<uint64_t>(kKeyTile) * call.extent;
   } else {
-    if (own >= call.keys) return;
-    dk_target = gradients.key.data + b * gradients.key.batch + key_head * gradients.key.head +
-                own * gradients.key.token;
-    dv_target = gradients.value.data + b * gradients.value.batch +
-                key_head * gradients.value.head + own * gradients.value.token;
+    dk_target = key_gradient.data + b * key_gradient.batch + key_head * key_gradient.head +
+                own * key_gradient.token;
+    dv_target = value_gradient.data + b * value_gradient.batch + key_head * value_gradient.head +
+                own * value_gradient.token;
   }
   dk.visit(quarter, [&](uint32_t d, auto& run) {
     for (auto& y : run) y *= static_cast<T>(call.scale);
@@ -399,72 +419,112 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(Cal
   dv.visit(quarter, [&](uint32_t d, auto& run) { store_piece(dv_target, d, call.extent, run); });
 }
 
-// dk and dv of the sinks: the window's part, as key_kernel wrote it, and the parts
-// of the later rows in their order.
+// dk and dv of the first `keys` keys from their parts in a fixed order: eight lanes to
+// an element take every eighth part each, and their sums meet in a tree.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sink_kernel(Call call, Gradients<T> gradients,
-                                                        uint32_t sinks) {
-  const uint64_t at = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const uint64_t per_head = static_cast<uint64_t>(sinks) * call.extent;
-  const uint64_t batch_head = at / per_head;
-  if (batch_head >= call.batch_heads) return;
-  const uint32_t within = static_cast<uint32_t>(at - batch_head * per_head);
+__global__ __launch_bounds__(kThreads) void join_kernel(Call call, Heads<T> key_gradient,
+                                                        Heads<T> value_gradient,
+                                                        Splits<T> splits, uint32_t keys) {
+  constexpr uint32_t kRuns = 8, kLanes = kThreads / kRuns;
+  __shared__ T sums[2][kRuns][kLanes];
+  const uint32_t lane = threadIdx.x % kLanes, run = threadIdx.x / kLanes;
+  const uint64_t per_head = static_cast<uint64_t>(keys) * call.extent;
+  const uint64_t at = static_cast<uint64_t>(blockIdx.x) * kLanes + lane;
+  const bool inside = at < per_head * call.batch_heads;
+  const uint32_t batch_head = inside ? static_cast<uint32_t>(at / per_head) : 0;
+  const uint32_t within = inside ? static_cast<uint32_t>(at - batch_head * per_head) : 0;
   const uint32_t key = within / call.extent, d = within % call.extent;
-  const uint64_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
-  const uint64_t stride = static_cast<uint64_t>(kKeyTile) * call.extent;
+  const uint32_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
   const uint32_t tile = key / kKeyTile;
-  const int blocks = sink_blocks(static_cast<int32_t>(sinks - tile * kKeyTile));
-  const T* part = gradients.parts +
-                  (batch_head * gradients.sink_tiles + tile) * gradients.splits * 2 * stride +
-                  static_cast<uint64_t>(key % kKeyTile) * call.extent + d;
-  T* dk = gradients.key.data + b * gradients.key.batch + key_head * gradients.key.head +
-          key * gradients.key.token + d;
-  T* dv = gradients.value.data + b * gradients.value.batch + key_head * gradients.value.head +
-          key * gradients.value.token + d;
-  T sum_k = *dk, sum_v = *dv;
-  const uint64_t turn = static_cast<uint64_t>(blocks) * kBlock * call.extent;
+  const uint64_t row = static_cast<uint64_t>(call.extent);
+  const uint64_t value_part = kKeyTile * row;
+  T* dk = key_gradient.data + b * key_gradient.batch + key_head * key_gradient.head +
+          key * key_gradient.token + d;
+  T* dv = value_gradient.data + b * value_gradient.batch + key_head * value_gradient.head +
+          key * value_gradient.token + d;
+  T sum_k = T(0), sum_v = T(0);
+  if (splits.main > 1) {
+    const T* from = splits.main_part(batch_head, tile, 0) + key % kKeyTile * row + d;
 #pragma unroll 4
-  for (uint32_t s = 0; s < gradients.splits; ++s) {
-    for (int t = 0; t < kWaves / blocks; ++t) {
-      sum_k += part[2 * s * stride + t * turn];
-      sum_v += part[(2 * s + 1) * stride + t * turn];
+    for (uint32_t s = run; s < splits.main; s += kRuns) {
+      sum_k += from[s * splits.size()];
+      sum_v += from[s * splits.size() + value_part];
+    }
+  } else if (run == 0 && inside) {
+    sum_k = *dk;
+    sum_v = *dv;
+  }
+  if (splits.later != 0 && key < static_cast<uint32_t>(call.sinks)) {
+    const int blocks = sink_blocks(call.sinks - static_cast<int32_t>(tile * kKeyTile));
+    const uint32_t turns = kWaves / blocks;
+    const T* from = splits.later_part(call.batch_heads, batch_head, tile, 0) +
+                    key % kKeyTile * row + d;
+#pragma unroll 4
+    for (uint32_t s = run; s < splits.later * turns; s += kRuns) {
+      const uint64_t part = s / turns * splits.size() + s % turns * blocks * kBlock * row;
+      sum_k += from[part];
+      sum_v += from[part + value_part];
     }
   }
-  *dk = sum_k;
-  *dv = sum_v;
+  sums[0][run][lane] = sum_k;
+  sums[1][run][lane] = sum_v;
+  for (uint32_t half = kRuns / 2; half > 0; half >>= 1) {
+    __syncthreads();
+    if (run < half) {
+      sums[0][run][lane] += sums[0][run + half][lane];
+      sums[1][run][lane] += sums[1][run + half][lane];
+    }
+  }
+  if (run == 0 && inside) {
+    *dk = sums[0][0][lane];
+    *dv = sums[1][0][lane];
+  }
 }
 
 // ---------------------------------------------------------------- launchers
 
 struct Plan {
-  uint32_t row_tiles, key_tiles, sink_tiles, splits;
+  uint32_t row_tiles, key_tiles, main, sink_tiles, later;
   uint64_t delta_bytes;  // a multiple of 16
   uint64_t bytes;
 };
 
-// At most this many splits per sink tile, each of this part of the rows that a tile
-// of keys has in its window.
-constexpr uint64_t kMostSplits = 256;
-constexpr uint64_t kSplitShare = 2;
+// At most this many splits of the rows behind a sink tile's window, each of this part
+// of the rows that a tile of keys has in its window.
+constexpr uint64_t kMostLater = 256;
+constexpr uint64_t kLaterShare = 2;
+// Workgroups that fill the chip, and the fewest rows that repay a part.
+constexpr uint64_t kFullGrid = 512;
+constexpr uint64_t kFewestRows = 64;
 
 Plan plan_of(const SparHipAttention& a) {
   Plan plan{};
   const uint64_t element = a.dtype == SPAR_HIP_FLOAT32 ? sizeof(float) : sizeof(double);
   const uint64_t group = a.query_heads / a.key_heads;
+  const uint64_t batch_heads = a.batch * a.key_heads;
   plan.row_tiles = ceil_div_u32(a.queries * group, kWaves * kBlock);
   plan.key_tiles = ceil_div_u32(a.keys, kKeyTile);
+  plan.main = 1;
   plan.delta_bytes =
       (a.batch * a.query_heads * a.queries * element + 15) / 16 * 16;
+  const uint64_t rows =
+      group * (a.window == 0 ? a.queries : std::min(a.queries, a.window + kKeyTile));
+  if (plan.key_tiles != 0) {
+    plan.main = static_cast<uint32_t>(std::max<uint64_t>(
+        1, std::min(kFullGrid / (plan.key_tiles * batch_heads), rows / kFewestRows)));
+  }
   const uint64_t sinks = std::min(a.sinks, a.keys);
   if (a.window != 0 && sinks != 0 && a.keys > a.window) {
     plan.sink_tiles = ceil_div_u32(sinks, kKeyTile);
-    const uint64_t later = std::min(a.queries, a.keys - a.window);
-    const uint64_t share = (a.window + kKeyTile) / kSplitShare;
-    plan.splits =
-        static_cast<uint32_t>(std::min(kMostSplits, (later + share - 1) / share));
+    const uint64_t behind = std::min(a.queries, a.keys - a.window);
+    const uint64_t share = (a.window + kKeyTile) / kLaterShare;
+    plan.later = static_cast<uint32_t>(std::min(
+        kMostLater, std::max((behind + share - 1) / share,
+                             std::min<uint64_t>(plan.main, behind * group / kFewestRows))));
   }
-  plan.bytes = plan.delta_bytes + a.batch * a.key_heads * plan.sink_tiles * plan.splits * 2 *
-                                      kKeyTile * a.extent * element;
+  const uint64_t parts = (plan.main > 1 ? uint64_t{plan.key_tiles} * plan.main : 0) +
+                         uint64_t{plan.sink_tiles} * plan.later;
+  plan.bytes = plan.delta_bytes + batch_heads * parts * 2 * kKeyTile * a.extent * element;
   return plan;
 }
 
@@ -478,11 +538,11 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& quer
   const Saved<T> saved{heads_of<const T>(query), heads_of<const T>(key), heads_of<const T>(value),
                        heads_of<const T>(output), heads_of<const T>(output_gradient),
                        static_cast<const T*>(logsumexp), static_cast<T*>(workspace)};
-  const Gradients<T> gradients{
-      heads_of<T>(query_gradient), heads_of<T>(key_gradient), heads_of<T>(value_gradient),
-      reinterpret_cast<T*>(static_cast<char*>(workspace) + plan.delta_bytes), plan.splits,
-      plan.sink_tiles};
-  const uint32_t sink_groups = plan.sink_tiles * plan.splits;
+  const Heads<T> dk = heads_of<T>(key_gradient), dv = heads_of<T>(value_gradient);
+  const Splits<T> splits{
+      reinterpret_cast<T*>(static_cast<char*>(workspace) + plan.delta_bytes), plan.key_tiles,
+      plan.main, plan.sink_tiles, plan.later, call.extent};
+  const uint32_t key_groups = plan.key_tiles * plan.main + plan.sink_tiles * plan.later;
   with_width<T>(a, {&output_gradient, &output, &query, &key, &value},
                 [&](auto width, auto reads) {
     constexpr int DP = decltype(width)::value;
@@ -490,27 +550,29 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& quer
     constexpr int kBlocks = tile_blocks<T, DP>();
     constexpr int kKeyBlocks = sizeof(T) == 4 && DP <= 128 ? 2 : 1;
     if (call.rows != 0) {
-      query_kernel<T, DP, kBlocks, READS><<<plan.row_tiles * call.batch_heads, kThreads, 0, stream>>>(
-          call, saved, gradients.query, plan.row_tiles);
+      query_kernel<T, DP, kBlocks, READS>
+          <<<plan.row_tiles * call.batch_heads, kThreads, 0, stream>>>(
+              call, saved, heads_of<T>(query_gradient), plan.row_tiles);
     }
     if (call.keys != 0) {
       key_kernel<T, DP, kKeyBlocks, READS>
-          <<<(plan.key_tiles + sink_groups) * call.batch_heads, kThreads, 0, stream>>>(
-              call, saved, gradients, plan.key_tiles);
+          <<<key_groups * call.batch_heads, kThreads, 0, stream>>>(call, saved, dk, dv, splits);
     }
   });
-  if (sink_groups != 0) {
-    const uint32_t sinks = static_cast<uint32_t>(std::min(a.sinks, a.keys));
-    sink_kernel<T><<<ceil_div_u32(static_cast<uint64_t>(call.batch_heads) * sinks * a.extent,
-                                  kThreads),
-                     kThreads, 0, stream>>>(call, gradients, sinks);
+  const uint32_t joined = plan.main > 1     ? call.keys
+                          : plan.later != 0 ? static_cast<uint32_t>(std::min(a.sinks, a.keys))
+                                            : 0;
+  if (joined != 0) {
+    join_kernel<T><<<ceil_div_u32(static_cast<uint64_t>(call.batch_heads) * joined * a.extent,
+                                  kThreads / 8),
+                     kThreads, 0, stream>>>(call, dk, dv, splits, joined);
   }
 }
 
 bool fits(const SparHipAttention& a, const Plan& plan) {
   const uint64_t batch_heads = a.batch * a.key_heads;
-  return (static_cast<uint64_t>(plan.key_tiles) +
-          static_cast<uint64_t>(plan.sink_tiles) * plan.splits) * batch_heads <= kIndex32Limit &&
+  return (static_cast<uint64_t>(plan.key_tiles) * plan.main +
+          static_cast<uint64_t>(plan.sink_tiles) * plan.later) * batch_heads <= kIndex32Limit &&
          static_cast<uint64_t>(plan.row_tiles) * batch_heads <= kIndex32Limit;
 }
 

@@ -539,9 +539,10 @@ constexpr uint64_t kTokenRows = 32;
 
 // Workgroups that keep the chip's 256 CUs busy, and the fewest keys that repay
 // the writing and reading of a part.
-constexpr uint64_t kFullGrid = 512;
+constexpr uint64_t kFullGrid = 768;
 constexpr uint64_t kTokenGrid = 1024;
 constexpr uint64_t kFewestKeys = 256;
+constexpr uint64_t kFewestTokenKeys = 128;
 
 struct Plan {
   bool token;
@@ -574,7 +575,8 @@ Plan plan_of(const SparHipAttention& a) {
   }
   const uint64_t wanted = grid / std::max<uint64_t>(1, plan.row_tiles * batch_heads);
   plan.splits = static_cast<uint32_t>(
-      std::max<uint64_t>(1, std::min({wanted, seen / kFewestKeys, uint64_t{kMostParts}})));
+      std::max<uint64_t>(1, std::min({wanted, seen / (plan.token ? kFewestTokenKeys : kFewestKeys),
+                                          uint64_t{kMostParts}})));
   const uint64_t piece = 16 / element_size(a);
   plan.pitch = static_cast<uint32_t>((a.extent + piece - 1) / piece * piece);
   if (plan.splits > 1) {

@@ -524,7 +524,7 @@ __global__ __launch_bounds__(1024) void norm_weight_kernel(T* first, T* second, 
 // ---------------------------------------------------------------- launchers
 
 // Heads a lane turns with one cos and sin: as many as leave the chip full.
-constexpr uint64_t kFullLanes = 256 * 2048;
+constexpr uint64_t kFullLanes = 1 << 16;
 
 bool valid_rotary(const SparHipRotary* rotary, uint64_t extent) {
   return rotary != nullptr && rotary->rotary_extent % 2 == 0 && rotary->rotary_extent <= extent &&
