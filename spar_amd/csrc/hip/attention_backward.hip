@@ -138,8 +138,6 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
   }
   delta = quarter_sum(delta);
   if (quarter == 0 && r < call.rows) saved.delta[place.at] = delta;
-  // What is subtracted from scores and from dP, where their products start.
-  const typename Mma<T>::Acc from_log_sum = -log_sum, from_delta = -delta;
   Along<T, DP> dq;
   dq.clear();
   const T* key_base = saved.key.data + b * saved.key.batch + key_head * saved.key.head;
@@ -183,12 +181,12 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
                          (newest - k0 < call.window || k1 < call.sinks);
       const T* key_rows = keys.value[i % 2] + kb * kBlock * DP;
       const T* value_rows = values.value[i % 2] + kb * kBlock * DP;
-      typename Mma<T>::Acc s = from_log_sum, dp = from_delta;
+      typename Mma<T>::Acc s{0, 0, 0, 0}, dp{0, 0, 0, 0};
       products(lane, key_rows, q, s, value_rows, g, dp);
       Across<1, T, DP> across(lane, key_rows);
       T ds[4];
 #pragma unroll
-      for (int v = 0; v < 4; ++v) ds[v] = exp2_of(s[v]) * dp[v];
+      for (int v = 0; v < 4; ++v) ds[v] = exp2_of(s[v] - log_sum) * (dp[v] - delta);
       if (!whole) {
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
@@ -235,7 +233,7 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(Cal
   constexpr int RT = RB * kBlock;
   constexpr int W = Vec16<T>::width;
   __shared__ Tile<T, RT, DP, READS> queries, output_gradients;
-  __shared__ alignas(16) T from_log_sums[2][RT], from_deltas[2][RT];  // negated
+  __shared__ alignas(16) T log_sums[2][RT], deltas[2][RT];
   __shared__ int32_t tokens[2][RT];
   const uint32_t batch_head = blockIdx.x % call.batch_heads;
   const uint32_t rest = blockIdx.x / call.batch_heads;
@@ -335,8 +333,8 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(Cal
   const auto finish = [&](uint32_t i) {
     if (threadIdx.x < RT) {
       tokens[i % 2][threadIdx.x] = next_token;
-      from_log_sums[i % 2][threadIdx.x] = next_log_sum * static_cast<T>(-kLog2E);
-      from_deltas[i % 2][threadIdx.x] = -next_delta;
+      log_sums[i % 2][threadIdx.x] = next_log_sum * static_cast<T>(kLog2E);
+      deltas[i % 2][threadIdx.x] = next_delta;
     }
     queries.finish(next_queries, i % 2);
     output_gradients.finish(next_gradients, i % 2);
@@ -367,20 +365,15 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(Cal
                          (newest - wave_key < call.window || last_key < call.sinks);
       const T* query_rows = queries.value[i % 2] + rb * kBlock * DP;
       const T* gradient_rows = output_gradients.value[i % 2] + rb * kBlock * DP;
-      typename Mma<T>::Acc s, dp;
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int row = rb * kBlock + Mma<T>::row_of(v, quarter);
-        s[v] = from_log_sums[i % 2][row];
-        dp[v] = from_deltas[i % 2][row];
-      }
+      typename Mma<T>::Acc s{0, 0, 0, 0}, dp{0, 0, 0, 0};
       products(lane, query_rows, k, s, gradient_rows, x, dp);
       Across<1, T, DP> across_gradients(lane, gradient_rows);
       T p[4], ds[4];
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        p[v] = exp2_of(s[v]);
-        ds[v] = p[v] * dp[v];
+        const int row = rb * kBlock + Mma<T>::row_of(v, quarter);
+        p[v] = exp2_of(s[v] - log_sums[i % 2][row]);
+        ds[v] = p[v] * (dp[v] - deltas[i % 2][row]);
       }
       if (!whole) {
 #pragma unroll
