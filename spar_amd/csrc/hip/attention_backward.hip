@@ -482,10 +482,12 @@ struct Plan {
   uint64_t bytes;
 };
 
-// At most this many splits of the rows behind a sink tile's window, each of this part
-// of the rows that a tile of keys has in its window.
-constexpr uint64_t kMostLater = 256;
+// Splits of the rows behind a sink tile's window: each of this part of the rows that a
+// tile of keys has in its window, at most so many, and no more in all than keep the
+// chip busy several times over (their parts take memory).
 constexpr uint64_t kLaterShare = 2;
+constexpr uint64_t kMostLater = 256;
+constexpr uint64_t kMostLaterGroups = 2048;
 // Workgroups that fill the chip, and the fewest rows that repay a part.
 constexpr uint64_t kFullGrid = 512;
 constexpr uint64_t kFewestRows = 64;
@@ -514,6 +516,10 @@ Plan plan_of(const SparHipAttention& a) {
     plan.later = static_cast<uint32_t>(std::min(
         kMostLater, std::max((behind + share - 1) / share,
                              std::min<uint64_t>(plan.main, behind * group / kFewestRows))));
+    plan.later = static_cast<uint32_t>(std::min<uint64_t>(
+        plan.later,
+        std::max<uint64_t>(1, kMostLaterGroups / std::max<uint64_t>(
+                                                     1, plan.sink_tiles * batch_heads))));
   }
   const uint64_t parts = (plan.main > 1 ? uint64_t{plan.key_tiles} * plan.main : 0) +
                          uint64_t{plan.sink_tiles} * plan.later;
@@ -564,7 +570,9 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& quer
 
 bool fits(const SparHipAttention& a, const Plan& plan) {
   const uint64_t batch_heads = a.batch * a.key_heads;
-  return (static_cast<uint64_t>(plan.key_tiles) * plan.main +
+  return batch_heads * std::min(a.keys, plan.main > 1 ? a.keys : a.sinks) <=
+             kIndex32Limit / a.extent * (kThreads / 8) &&
+         (static_cast<uint64_t>(plan.key_tiles) * plan.main +
           static_cast<uint64_t>(plan.sink_tiles) * plan.later) * batch_heads <= kIndex32Limit &&
          static_cast<uint64_t>(plan.row_tiles) * batch_heads <= kIndex32Limit;
 }

@@ -787,6 +787,7 @@ extern "C" SparHipStatus spar_hip_launch_head_norm_rotary_forward(
     if (!sane(batch, parts[p].heads, tokens, extent)) return invalid();
     heads += parts[p].heads;
   }
+  if (!sane(batch, heads, tokens, extent)) return invalid();
   if (batch == 0 || tokens == 0 || heads == 0) return ok();
   if (!complete_rotary(rotary)) return invalid();
   for (int p = 0; p < part_count; ++p) {
@@ -832,6 +833,7 @@ extern "C" SparHipStatus spar_hip_launch_head_norm_rotary_backward(
     }
     heads += parts[p].heads;
   }
+  if (!sane(batch, heads, tokens, extent)) return invalid();
   const bool empty = batch == 0 || tokens == 0 || heads == 0;
   if (!empty) {
     uint64_t need = 0;

@@ -125,6 +125,17 @@ Rotation rotation_of(const Tensor& heads, const Tensor& positions, const Tensor&
           shared ? 0 : static_cast<std::size_t>(read.strides()[0]), magnitude, layout};
 }
 
+// For a backward: what the program changes in the positions later has no part in it.
+Rotation snapshot_of(const Rotation& rotation) {
+  Rotation copy{rotation};
+  copy.positions = rotation.positions.clone();
+  copy.frequencies = rotation.frequencies.clone();
+  if (copy.position_stride != 0) {
+    copy.position_stride = static_cast<std::size_t>(copy.positions.strides()[0]);
+  }
+  return copy;
+}
+
 Tensor turned(const Tensor& heads, const Rotation& rotation, bool inverse, const char* name) {
   const Tensor x{readable(heads.detach())};
   Tensor output{ordered_like(x)};
@@ -284,9 +295,10 @@ Tensor rotary_embedding(const Tensor& heads, const Tensor& positions, const Tens
   const Rotation rotation{rotation_of(heads, positions, frequencies, layout, magnitude, name)};
   Tensor output{turned(heads, rotation, false, name)};
   if (heads.requires_grad()) {
-    detail::record_operation(output, {heads}, [rotation](const Tensor& gradient) {
-      return std::vector<Tensor>{turned(gradient, rotation, true, "rotary_embedding backward")};
-    });
+    detail::record_operation(
+        output, {heads}, [saved = snapshot_of(rotation)](const Tensor& gradient) {
+          return std::vector<Tensor>{turned(gradient, saved, true, "rotary_embedding backward")};
+        });
   }
   return output;
 }
@@ -335,8 +347,11 @@ std::pair<Tensor, Tensor> query_key_norm_rotary(const Tensor& query, const Tenso
                                                       epsilon, hip::dtype_tag(query.dtype()),
                                                       query.device().index()),
              name, query.device());
-  record_head_norm(q_output, q, query_weight, qw, q_rows, rotation);
-  record_head_norm(k_output, k, key_weight, kw, k_rows, rotation);
+  const bool tracked{q.requires_grad() || k.requires_grad() || query_weight.requires_grad() ||
+                     key_weight.requires_grad()};
+  const Rotation saved{tracked ? snapshot_of(rotation) : rotation};
+  record_head_norm(q_output, q, query_weight, qw, q_rows, saved);
+  record_head_norm(k_output, k, key_weight, kw, k_rows, saved);
   return {q_output, k_output};
 }
 
@@ -373,6 +388,8 @@ Tensor window_attention(const Tensor& query, const Tensor& key, const Tensor& va
   const bool grad_query{q.requires_grad()}, grad_key{k.requires_grad()},
       grad_value{v.requires_grad()};
   const bool tracked{grad_query || grad_key || grad_value};
+  // The backward's own: the program may go on counting in its lengths.
+  if (tokens && tracked) tokens = tokens->clone();
   Tensor output{ordered_like(q)};
   const Device device{query.device()};
   const SparHipAttention shape{

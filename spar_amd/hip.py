@@ -56,8 +56,19 @@ class AdamwTensor(ctypes.Structure):
                 ("second_correction", ctypes.c_double)]
 
 
+def _words(*names):
+    """Fields of 64 bits each; a name in brackets is a SparHipHeads.  Flat, since
+    nested structures take several times as long to make."""
+    fields = []
+    for name in names:
+        parts = ([name[0]] + [f"{name[0]}_{axis}_stride" for axis in ("batch", "head", "token")]
+                 if isinstance(name, tuple) else [name])
+        fields += [(part, ctypes.c_uint64) for part in parts]
+    return fields
+
+
 class Heads(ctypes.Structure):
-    _fields_ = [("data", ctypes.c_void_p), ("strides", ctypes.c_uint64 * 3)]
+    _fields_ = _words(("data",))
 
 
 class Rotary(ctypes.Structure):
@@ -67,17 +78,6 @@ class Rotary(ctypes.Structure):
                 ("layout", ctypes.c_int)]
 
 
-def _words(*names):
-    """Fields of 64 bits each; a name in brackets is a SparHipHeads."""
-    fields = []
-    for name in names:
-        parts = ([name[0]] + [f"{name[0]}_{axis}_stride" for axis in ("batch", "head", "token")]
-                 if isinstance(name, tuple) else [name])
-        fields += [(part, ctypes.c_uint64) for part in parts]
-    return fields
-
-
-# Flat, since nested structures take several times as long to make.
 class HeadNorm(ctypes.Structure):
     _fields_ = _words(("output",), "denominator", ("input",), "weight", "heads")
 
@@ -245,7 +245,7 @@ def u64_array(values) -> ctypes.Array:
 def heads(data, strides) -> Heads:
     """A [batch, heads, tokens, extent] tensor: its first element's address and
     its (batch, head, token) strides in elements."""
-    return Heads(data, tuple(strides))
+    return Heads(data or 0, *strides)
 
 
 def rotary(positions, position_stride, position_dtype, frequencies, rotary_extent, magnitude=1.0,

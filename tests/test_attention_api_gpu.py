@@ -231,6 +231,29 @@ def test_refusals(sp):
             call()
 
 
+def test_backward_keeps_positions_and_lengths_as_they_were(sp):
+    """A program that counts its positions and lengths on between forward and backward."""
+    rng = np.random.default_rng(17)
+    x = rng.standard_normal((2, 2, 9, 32))
+
+    def gradient(changes):
+        leaf = put(sp, x, grad=True)
+        weight = put(sp, np.ones(32), grad=True)
+        positions, lengths = put(sp, np.arange(9)), put(sp, np.array([9, 6]))
+        freq = put(sp, oracle.frequencies(32))
+        turned = sp.rotary_embedding(leaf, positions, freq)
+        query, key = sp.query_key_norm_rotary(turned, turned, weight, weight, positions, freq)
+        out = sp.window_attention(query, key, turned, 4, 1, lengths=lengths)
+        if changes:
+            sp.copy_values(positions, put(sp, np.arange(9) + 100))
+            sp.copy_values(lengths, put(sp, np.array([1, 1])))
+        sp.sum(sp.multiply(out, out)).backward()
+        return get(sp, leaf.grad()), get(sp, weight.grad())
+
+    for a, b in zip(gradient(False), gradient(True)):
+        assert np.array_equal(a, b)
+
+
 def test_results_after_the_inputs_are_gone(sp):
     """A graph keeps what its backward reads, although the program drops it."""
     rng = np.random.default_rng(16)

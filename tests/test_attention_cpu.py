@@ -61,6 +61,10 @@ def test_head_norm_refuses(changes):
     assert norm_forward(**changes) == 1
 
 
+def test_head_norm_refuses_too_many_heads_in_all():
+    assert norm_forward(heads=(1 << 24) - 1, count=2) == 1
+
+
 def test_head_norm_of_nothing_succeeds():
     assert norm_forward(tokens=0, output=None) == 0
     assert norm_forward(heads=0, output=None) == 0
@@ -129,6 +133,15 @@ def test_attention_refuses_small_workspaces():
     assert hip.status_of("spar_hip_attention_workspace", None, shape, 0).code == 1
     assert hip.status_of("spar_hip_attention_workspace", ctypes.byref(ctypes.c_uint64()), shape,
                          2).code == 1
+
+
+def test_parts_of_many_sinks_stay_bounded():
+    """A tile of 64 sinks has a part [2, 64, extent] for each split of its later rows;
+    2048 such parts at most once the tiles are many."""
+    shape = attention(batch=1, query_heads=8, key_heads=8, queries=131071, keys=131071,
+                      extent=128, window=1024, sinks=4096)
+    parts = hip.attention_workspace(shape, 1) - 8 * 131071 * 4 // 16 * 16
+    assert 0 < parts <= 2048 * 2 * 64 * 128 * 4 + 16
 
 
 def test_attention_of_nothing_succeeds():

@@ -285,6 +285,9 @@ ATTENTION = [  # (batch, heads, key heads, queries, keys, extent), window, sinks
     ((2, 2, 1, 5, 0, 40), 3, 1, None),     # no keys at all
     ((1, 8, 1, 300, 300, 64), 50, 70, None),  # sinks of two tiles, rows of one head group
     ((1, 5, 5, 256, 256, 3), 100, 0, None),
+    ((1, 1, 1, 200, 200, 254), 64, 40, None),  # sinks that two waves share, odd pieces
+    ((1, 7, 1, 90, 90, 64), 0, 0, None),       # a group that does not divide a tile of rows
+    ((2, 3, 1, 400, 400, 48), 1000, 3, [400, 399]),  # a window that reaches over all keys
 ]
 
 
@@ -428,6 +431,30 @@ def test_cache_offsets_beyond_32_bits(hip):
              space(hip, need).ptr, need, 0)
     want = oracle.Attention(q, k, v)
     assert_within(out.numpy(), want.output, want.output_bound)
+    _alive.clear()
+    hip.call("spar_hip_empty_cache", 0)
+
+
+def test_rotary_offsets_beyond_32_bits(hip):
+    """Two heads 2^32 + 4096 elements apart, turned in place."""
+    d, t = 64, 5
+    step = (1 << 32) + 4096
+    x = np.random.default_rng(6).standard_normal((1, 2, t, d)).astype(F32)
+    buffer = space(hip, (step + t * d) * 4)
+    for head in range(2):
+        part = np.ascontiguousarray(x[0, head])
+        hip.call("spar_hip_copy_host_to_device", buffer.address(head * step * 4),
+                 part.ctypes.data, part.nbytes, 0)
+    view = hip.heads(buffer.ptr, (0, step, d))
+    freq = oracle.frequencies(d)
+    hip.call("spar_hip_launch_rotary", view, view, 1, 2, t, d,
+             rotary_of(hip, np.arange(t), freq, "half", 1.0, shared=True), 0, 0, 0)
+    want, size = oracle.turn(x, np.arange(t), freq, "half")
+    for head in range(2):
+        got = np.empty((t, d), F32)
+        hip.call("spar_hip_copy_device_to_host", got.ctypes.data, buffer.address(head * step * 4),
+                 got.nbytes, 0)
+        assert_within(got, want[0, head], oracle.TURN * half_step(F32) * size[0, head])
     _alive.clear()
     hip.call("spar_hip_empty_cache", 0)
 
