@@ -7,6 +7,7 @@ there is no fallback path.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import os
 from pathlib import Path
@@ -257,20 +258,22 @@ def rotary(positions, position_stride, position_dtype, frequencies, rotary_exten
 def head_norms(*parts):
     """Parts of spar_hip_launch_head_norm_rotary_forward, each (output, output
     strides, denominator, input, input strides, weight, heads)."""
-    return (HeadNorm * len(parts))(*[
-        HeadNorm(output or 0, *output_strides, denominator or 0, source or 0, *strides,
-                 weight or 0, count)
-        for output, output_strides, denominator, source, strides, weight, count in parts])
+    words = array.array("Q")
+    for output, output_strides, denominator, source, strides, weight, count in parts:
+        words.extend((output or 0, *output_strides, denominator or 0, source or 0, *strides,
+                      weight or 0, count))
+    return (HeadNorm * len(parts)).from_buffer(words)
 
 
 def head_norm_gradients(*parts):
     """Parts of spar_hip_launch_head_norm_rotary_backward, each (input gradient,
     its strides, weight gradient, output gradient, its strides, input, its
     strides, weight, denominator, heads)."""
-    return (HeadNormGradient * len(parts))(*[
-        HeadNormGradient(dx or 0, *dx_strides, dw or 0, dy or 0, *dy_strides, x or 0, *strides,
-                         weight or 0, denominator or 0, count)
-        for dx, dx_strides, dw, dy, dy_strides, x, strides, weight, denominator, count in parts])
+    words = array.array("Q")
+    for dx, dx_strides, dw, dy, dy_strides, x, strides, weight, denominator, count in parts:
+        words.extend((dx or 0, *dx_strides, dw or 0, dy or 0, *dy_strides, x or 0, *strides,
+                      weight or 0, denominator or 0, count))
+    return (HeadNormGradient * len(parts)).from_buffer(words)
 
 
 def head_norm_rotary_workspace(batch, tokens, heads, extent, dtype) -> int:
