@@ -464,6 +464,52 @@ void with_padded_width(uint64_t extent, Body&& body) {
   }
 }
 
+// The pieces along the heads of the four rows row_of(v, quarter) of a block of 16, read
+// from memory in the order in which results lie along a head: what a product that
+// contracts those rows takes from the lane.  head_of(row) is the row's head.
+template <typename T, int DP>
+struct AcrossOperand {
+  using L = Lane<T, DP>;
+  static constexpr int W = L::W;
+  T value[4][DP / 16];
+
+  template <Reads READS, typename HeadOf>
+  __device__ __forceinline__ void load(uint32_t extent, int quarter, int column,
+                                       HeadOf&& head_of) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const T* head = head_of(Mma<T>::row_of(v, quarter));
+#pragma unroll
+      for (int c = 0; c < L::kChunks; ++c) {
+        const auto piece = load_piece<READS>(head, 16 * W * c + W * column, extent);
+#pragma unroll
+        for (int j = 0; j < W; ++j) value[v][c * W + j] = piece[j];
+      }
+      if constexpr (L::kRest != 0) {
+        const uint32_t d = 16 * W * L::kChunks + 2 * column;
+        value[v][L::kChunks * W] = head[d < extent ? d : 0];
+        value[v][L::kChunks * W + 1] = head[d + 1 < extent ? d + 1 : 0];
+      }
+    }
+  }
+  __device__ __forceinline__ void add_to(Along<T, DP>& out, const T (&weight)[4]) const {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+#pragma unroll
+      for (int j = 0; j < DP / 16; ++j) {
+        out.block[j] = Mma<T>::step(value[v][j], weight[v], out.block[j]);
+      }
+    }
+  }
+};
+
+// Whether tiles of 64 rows leave so much of the chip idle that workgroups of 16 rows,
+// whose waves share the keys, are faster, although every wave reads its keys itself:
+// the forward of 8 heads of 128 with 256 tokens 26 us in 32 tiles and 12 us in 128,
+// of 16 heads of 64 with 512 tokens and a window of 128 15 us in 128 tiles and 11 us in
+// 512, of 2 heads with 634 queries of 3057 keys 23 us in 220 tiles and 24 us in 960.
+inline bool spreads(uint64_t tiles) { return tiles < 192; }
+
 // COUNT pieces read from LDS AHEAD uses before their own: the reads' latency (about
 // 128 cycles) passes under the matrix instructions of the pieces before.  Left to
 // itself the compiler reads a piece right before its use, into registers that the

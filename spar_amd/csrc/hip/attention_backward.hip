@@ -72,6 +72,29 @@ struct Place {
   }
 };
 
+// What dq of a row is made from, as the row's four lanes hold it.
+template <typename T, int DP>
+struct QueryRow {
+  Operand<T, DP> q, g;  // scaled by scale * log2(e); the output gradient
+  T delta = T(0);       // do . o
+  T log_sum;            // log2 of the row's sum
+
+  template <Reads READS>
+  __device__ __forceinline__ void load(const Call& call, const Saved<T>& saved,
+                                       const Place& place, uint32_t b, bool held, int quarter) {
+    Operand<T, DP> out;
+    q.template load<READS>(place.of(saved.query, b), call.extent, quarter);
+    g.template load<READS>(place.of(saved.output_gradient, b), call.extent, quarter);
+    out.template load<READS>(place.of(saved.output, b), call.extent, quarter);
+    log_sum = saved.logsumexp[place.at] * static_cast<T>(kLog2E);
+    q.finish(held, call.extent, quarter, static_cast<T>(call.scale * kLog2E));
+    g.finish(held, call.extent, quarter, T(1));
+#pragma unroll
+    for (int i = 0; i < DP / 4; ++i) delta += out.value[i] * g.value[i];
+    delta = quarter_sum(delta);
+  }
+};
+
 // s += a_rows a and dp += b_rows b of a block of 16 rows each, side by side: two sums
 // take turns in the matrix units.
 template <typename T, int DP>
@@ -123,21 +146,9 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
   const uint32_t r = wave_row + column;
   const int32_t token = call.token(r, first);
   const Place place(call, b, key_head, r < call.rows ? r : 0);
-  Operand<T, DP> q, g;
-  T delta = T(0), log_sum;
-  {
-    Operand<T, DP> out;
-    q.template load<READS>(place.of(saved.query, b), call.extent, quarter);
-    g.template load<READS>(place.of(saved.output_gradient, b), call.extent, quarter);
-    out.template load<READS>(place.of(saved.output, b), call.extent, quarter);
-    log_sum = saved.logsumexp[place.at] * static_cast<T>(kLog2E);
-    q.finish(token >= 0, call.extent, quarter, static_cast<T>(call.scale * kLog2E));
-    g.finish(token >= 0, call.extent, quarter, T(1));
-#pragma unroll
-    for (int i = 0; i < DP / 4; ++i) delta += out.value[i] * g.value[i];
-  }
-  delta = quarter_sum(delta);
-  if (quarter == 0 && r < call.rows) saved.delta[place.at] = delta;
+  QueryRow<T, DP> row;
+  row.template load<READS>(call, saved, place, b, token >= 0, quarter);
+  if (quarter == 0 && r < call.rows) saved.delta[place.at] = row.delta;
   Along<T, DP> dq;
   dq.clear();
   const T* key_base = saved.key.data + b * saved.key.batch + key_head * saved.key.head;
@@ -182,11 +193,11 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
       const T* key_rows = keys.value[i % 2] + kb * kBlock * DP;
       const T* value_rows = values.value[i % 2] + kb * kBlock * DP;
       typename Mma<T>::Acc s{0, 0, 0, 0}, dp{0, 0, 0, 0};
-      products(lane, key_rows, q, s, value_rows, g, dp);
+      products(lane, key_rows, row.q, s, value_rows, row.g, dp);
       Across<1, T, DP> across(lane, key_rows);
       T ds[4];
 #pragma unroll
-      for (int v = 0; v < 4; ++v) ds[v] = exp2_of(s[v] - log_sum) * (dp[v] - delta);
+      for (int v = 0; v < 4; ++v) ds[v] = exp2_of(s[v] - row.log_sum) * (dp[v] - row.delta);
       if (!whole) {
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
@@ -205,6 +216,88 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
     for (auto& x : run) x *= static_cast<T>(call.scale);
     store_piece(target, d, call.extent, run);
   });
+}
+
+// The same for grids that tiles of 64 rows do not fill: a workgroup's waves share 16
+// rows and take every fourth block of 16 keys, straight from memory; their sums meet
+// in LDS.
+template <typename T, int DP, Reads READS>
+__global__ __launch_bounds__(kThreads) void query_spread_kernel(Call call, Saved<T> saved,
+                                                                Heads<T> gradient,
+                                                                uint32_t row_tiles) {
+  constexpr int W = Vec16<T>::width;
+  __shared__ alignas(16) T sums[kWaves][kBlock][DP + W];
+  const uint32_t batch_head = blockIdx.x % call.batch_heads;
+  const uint32_t row_tile = row_tiles - 1 - blockIdx.x / call.batch_heads;
+  const uint32_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int quarter = threadIdx.x % kWave / kBlock, column = threadIdx.x % kBlock;
+
+  const int32_t first = call.length(b) - call.queries;
+  const uint32_t begin_row = row_tile * kBlock;
+  const uint32_t end_row = begin_row + kBlock < call.rows ? begin_row + kBlock : call.rows;
+  const int32_t oldest = call.token(begin_row, first);
+  const int32_t newest = call.token(end_row - 1, first);
+  const Keys seen(call, oldest < 0 ? 0 : oldest, newest);
+  const uint32_t blocks = seen.tiles(kBlock);
+  const uint32_t r = begin_row + column;
+  const int32_t token = call.token(r, first);
+  const Place place(call, b, key_head, r < call.rows ? r : 0);
+  QueryRow<T, DP> row;
+  row.template load<READS>(call, saved, place, b, token >= 0, quarter);
+  if (wave == 0 && quarter == 0 && r < call.rows) saved.delta[place.at] = row.delta;
+  Along<T, DP> dq;
+  dq.clear();
+  const T* key_base = saved.key.data + b * saved.key.batch + key_head * saved.key.head;
+  const T* value_base = saved.value.data + b * saved.value.batch + key_head * saved.value.head;
+
+  for (uint32_t i = wave; i < blocks; i += kWaves) {
+    int32_t begin, end;
+    seen.tile(i, kBlock, begin, end);
+    // Keys behind the run repeat its block's first; no row sees them.
+    const auto at_key = [&](int32_t k) { return static_cast<uint64_t>(k < end ? k : begin); };
+    const uint64_t own = at_key(begin + column);
+    Operand<T, DP> k, x;
+    AcrossOperand<T, DP> across;
+    k.template load<READS>(key_base + own * saved.key.token, call.extent, quarter);
+    x.template load<READS>(value_base + own * saved.value.token, call.extent, quarter);
+    across.template load<READS>(call.extent, quarter, column, [&](int n) {
+      return key_base + at_key(begin + n) * saved.key.token;
+    });
+    typename Mma<T>::Acc s{0, 0, 0, 0}, dp{0, 0, 0, 0};
+#pragma unroll
+    for (int step = 0; step < DP / 4; ++step) {
+      s = Mma<T>::step(k.value[step], row.q.value[step], s);
+      dp = Mma<T>::step(x.value[step], row.g.value[step], dp);
+    }
+    T ds[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int32_t at = begin + Mma<T>::row_of(v, quarter);
+      const bool visible = (at < end) & call.sees(token, at);
+      ds[v] = exp2_of(s[v] - row.log_sum) * (dp[v] - row.delta);
+      ds[v] = visible ? ds[v] : T(0);
+    }
+    across.add_to(dq, ds);
+  }
+  dq.visit(quarter, [&](uint32_t d, auto& run) {
+    for (auto& y : run) sums[wave][column][d++] = y;
+  });
+  __syncthreads();
+  constexpr int kPieces = DP / W;
+  for (int at = threadIdx.x; at < kBlock * kPieces; at += kThreads) {
+    const int c = at / kPieces, d = at % kPieces * W;
+    if (begin_row + c >= call.rows) continue;
+    T run[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      run[j] = sums[0][c][d + j];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) run[j] += sums[w][c][d + j];
+      run[j] *= static_cast<T>(call.scale);
+    }
+    store_piece(Place(call, b, key_head, begin_row + c).of(gradient, b), d, call.extent, run);
+  }
 }
 
 constexpr uint32_t kKeyTile = kWaves * kBlock;
@@ -477,6 +570,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Call call, Heads<T> key_
 // ---------------------------------------------------------------- launchers
 
 struct Plan {
+  bool spread;  // query_spread_kernel
   uint32_t row_tiles, key_tiles, main, sink_tiles, later;
   uint64_t delta_bytes;  // a multiple of 16
   uint64_t bytes;
@@ -498,6 +592,8 @@ Plan plan_of(const SparHipAttention& a) {
   const uint64_t group = a.query_heads / a.key_heads;
   const uint64_t batch_heads = a.batch * a.key_heads;
   plan.row_tiles = ceil_div_u32(a.queries * group, kWaves * kBlock);
+  plan.spread = spreads(plan.row_tiles * batch_heads);
+  if (plan.spread) plan.row_tiles = ceil_div_u32(a.queries * group, kBlock);
   plan.key_tiles = ceil_div_u32(a.keys, kKeyTile);
   plan.main = 1;
   plan.delta_bytes =
@@ -548,7 +644,13 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& quer
     constexpr Reads READS = decltype(reads)::value;
     constexpr int kBlocks = tile_blocks<T, DP>();
     constexpr int kKeyBlocks = sizeof(T) == 4 && DP <= 128 ? 2 : 1;
-    if (call.rows != 0) {
+    if (call.rows != 0 && plan.spread) {
+      // It reads pieces at any address alike.
+      constexpr Reads kReads = READS == Reads::Aligned ? Reads::Pieces : READS;
+      query_spread_kernel<T, DP, kReads>
+          <<<plan.row_tiles * call.batch_heads, kThreads, 0, stream>>>(
+              call, saved, heads_of<T>(query_gradient), plan.row_tiles);
+    } else if (call.rows != 0) {
       query_kernel<T, DP, kBlocks, READS>
           <<<plan.row_tiles * call.batch_heads, kThreads, 0, stream>>>(
               call, saved, heads_of<T>(query_gradient), plan.row_tiles);

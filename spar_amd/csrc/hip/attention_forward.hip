@@ -10,8 +10,9 @@
 // Two kernels.  tile_kernel: a workgroup of four waves with 16 or 32 rows each
 // shares tiles of keys and values in LDS; bound by the matrix units (4 extent
 // operations per visible pair).  token_kernel, for up to kTokenRows rows (a token
-// or a few per sequence): a workgroup's waves take different keys of the same 16
-// rows straight from memory into registers; bound by reading the visible cache.
+// or a few per sequence) and where tiles would leave the chip idle: a workgroup's
+// waves take different keys of the same 16 rows straight from memory into registers;
+// bound by reading the visible cache.
 // Either splits the keys of a row tile over several workgroups where the rows alone
 // do not fill the chip; combine_kernel joins the parts in their order.
 #include <hip/hip_runtime.h>
@@ -299,24 +300,10 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
     const auto at_key = [&](int32_t k) { return static_cast<uint64_t>(k < end ? k : begin); };
     Operand<T, DP> k;
     k.template load<READS>(key_base + at_key(begin + column) * key.token, call.extent, quarter);
-    using Out = Along<T, DP>;
-    T v[4][DP / 16];  // pieces of the four keys whose weights this lane holds
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const T* head =
-          value_base + at_key(begin + Mma<T>::row_of(n, quarter)) * value.token;
-#pragma unroll
-      for (int c = 0; c < Out::kChunks; ++c) {
-        const auto piece = load_piece<READS>(head, 16 * W * c + W * column, call.extent);
-#pragma unroll
-        for (int j = 0; j < W; ++j) v[n][c * W + j] = piece[j];
-      }
-      if constexpr (Out::kRest != 0) {
-        const uint32_t d = 16 * W * Out::kChunks + 2 * column;
-        v[n][Out::kChunks * W] = head[d < call.extent ? d : 0];
-        v[n][Out::kChunks * W + 1] = head[d + 1 < call.extent ? d + 1 : 0];
-      }
-    }
+    AcrossOperand<T, DP> v;
+    v.template load<READS>(call.extent, quarter, column, [&](int n) {
+      return value_base + at_key(begin + n) * value.token;
+    });
     typename Mma<T>::Acc s = row.start;
 #pragma unroll
     for (int step = 0; step < DP / 4; ++step) {
@@ -333,13 +320,7 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
       score[0][n] = visible ? s[n] : lowest<T>();
     }
     row.template take<1>(score);
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-#pragma unroll
-      for (int j = 0; j < DP / 16; ++j) {
-        row.out.block[j] = Mma<T>::step(v[n][j], score[0][n], row.out.block[j]);
-      }
-    }
+    v.add_to(row.out, score[0]);
   }
   const T total = quarter_sum(row.total);
   if (quarter == 0) {
@@ -582,7 +563,9 @@ Plan plan_of(const SparHipAttention& a) {
   const uint64_t rows = a.queries * (a.query_heads / a.key_heads);
   const uint64_t batch_heads = a.batch * a.key_heads;
   plan.rows = a.batch * a.query_heads * a.queries;
-  plan.token = rows <= kTokenRows;
+  plan.token = rows <= kTokenRows ||
+               spreads((rows + kWaves * kBlock - 1) / (kWaves * kBlock) * batch_heads *
+                       std::max<uint64_t>(1, most_seen(a) / kFewestKeys));
   uint64_t grid = kTokenGrid;
   uint64_t seen = most_seen(a);
   if (plan.token) {

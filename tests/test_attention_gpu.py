@@ -297,6 +297,42 @@ def test_attention(hip, shape, window, sinks, lengths, dtype):
     check(hip, shape, dtype, window, sinks, lengths)
 
 
+def check_in_tiles(hip, shape, dtype, window=0, sinks=0, lengths=None, **more):
+    """The same shape for so many sequences that tiles of 64 rows fill the chip, which
+    then take them: the shape's sequences over and over, each repetition the same bits."""
+    b, h, hk, t, s, d = shape
+    times = -(-192 // (b * hk * -(-t * h // hk // 64)))
+    q, k, v, g = inputs(*shape, dtype)
+    want = oracle.Attention(q, k, v, window, sinks, more.get("scale"), lengths, dtype)
+    lengths = None if lengths is None else np.tile(np.asarray(lengths), times)
+    output, logsumexp, made = attend(hip, *(np.tile(x, (times, 1, 1, 1)) for x in (q, k, v)), window,
+                                     sinks, lengths=lengths,
+                                     gradient=np.tile(g, (times, 1, 1, 1)), out_fill=7.0, **more)
+    for x in (output, logsumexp, *made):
+        assert np.array_equal(x, np.tile(x[:b], (times,) + (1,) * (x.ndim - 1)))
+    assert_within(output[:b], want.output, want.output_bound, "output")
+    assert_within(logsumexp[:b], want.logsumexp, want.logsumexp_bound, "logsumexp")
+    gradients, bounds = want.backward(g)
+    for name, x, y, bound in zip(("dq", "dk", "dv"), made, gradients, bounds):
+        assert_within(x[:b], y, bound, name)
+
+
+@pytest.mark.parametrize("shape,window,sinks,lengths",
+                         [case for case in ATTENTION if case[0][3] * case[0][1] // case[0][2] > 32],
+                         ids=str)
+@pytest.mark.parametrize("dtype", [F32, F64])
+def test_attention_in_tiles(hip, shape, window, sinks, lengths, dtype):
+    check_in_tiles(hip, shape, dtype, window, sinks, lengths)
+
+
+@pytest.mark.parametrize("orders,gap,offset", [(("heads", "heads"), 4, 4),
+                                               (("tokens", "heads"), 3, 1)])
+@pytest.mark.parametrize("extent", [64, 66])
+def test_attention_layouts_in_tiles(hip, orders, gap, offset, extent):
+    check_in_tiles(hip, (2, 6, 2, 80, 90, extent), F32, 21, 3, np.array([90, 61], np.int64),
+                   orders=orders, gap=gap, offset=offset, scale=0.3)
+
+
 @pytest.mark.parametrize("orders,gap,offset", [(("heads", "heads"), 0, 0),
                                                (("tokens", "heads"), 3, 1),
                                                (("heads", "tokens"), 1, 3)])
