@@ -696,8 +696,9 @@ struct SparHipStatus spar_hip_attention_workspace(uint64_t* bytes,
  * `queries` tokens, key and value key_heads heads of `keys` tokens.  logsumexp
  * [batch, query_heads, queries], contiguous, is kept for the backward (-inf where
  * no key is seen); it may be NULL.  Keys and values that no query sees are not
- * used, whatever they hold.  Replaces the reference's scores, mask and softmax
- * over whole [queries, keys] matrices (nn/attention.cpp:122-135). */
+ * used, whatever they hold; a NaN or infinity in one that some query sees may also
+ * reach other queries that read its key head.  Replaces the reference's scores, mask
+ * and softmax over whole [queries, keys] matrices (nn/attention.cpp:122-135). */
 struct SparHipStatus spar_hip_launch_attention_forward(
     const struct SparHipHeads* output, void* logsumexp, const struct SparHipHeads* query,
     const struct SparHipHeads* key, const struct SparHipHeads* value,
@@ -706,7 +707,8 @@ struct SparHipStatus spar_hip_launch_attention_forward(
 
 /* Its backward from the saved output and logsumexp: the gradients of query, key
  * and value (zeros for queries that see nothing and for keys that no query
- * sees), sums in a fixed order. */
+ * sees), sums in a fixed order.  A NaN or infinity in an input that takes part may
+ * reach every gradient of its key head and of the query heads that read it. */
 struct SparHipStatus spar_hip_launch_attention_backward(
     const struct SparHipHeads* query_gradient, const struct SparHipHeads* key_gradient,
     const struct SparHipHeads* value_gradient, const struct SparHipHeads* output_gradient,

@@ -540,14 +540,14 @@ __device__ __forceinline__ void run_queue(Queue<AHEAD, Piece>& queue, Read&& rea
   }
 }
 
-// out += tile^T weights: over BLOCKS blocks of 16 rows of a tile, of each of which the
-// lane has the weights of row_of(v, quarter), v < 4.
-template <int BLOCKS, typename T, int DP>
+// out += block^T weights of a block of 16 rows of a tile, of which the lane has the
+// weights of row_of(v, quarter), v < 4.
+template <typename T, int DP>
 struct Across {
   using L = Lane<T, DP>;
   static constexpr int W = L::W;
   static constexpr int kPerRow = L::kChunks + (L::kRest != 0);
-  static constexpr int kCount = BLOCKS * 4 * kPerRow;
+  static constexpr int kCount = 4 * kPerRow;
   static constexpr int kAhead = kCount < 2 ? kCount : 2;
   const L& lane;
   const T* rows;
@@ -558,29 +558,26 @@ struct Across {
     fill_queue(queue, [&](int i) { return read(i); });
   }
   __device__ __forceinline__ typename L::Piece read(int i) const {
-    const int block = i / (4 * kPerRow), v = i / kPerRow % 4, c = i % kPerRow;
-    const T* from = rows + block * kBlock * DP;
+    const int v = i / kPerRow, c = i % kPerRow;
     if (L::kRest != 0 && c == L::kChunks) {
-      const T* rest = lane.rest(from, v);
+      const T* rest = lane.rest(rows, v);
       typename L::Piece piece{};
       piece[0] = rest[0];
       piece[1] = rest[1];
       return piece;
     }
-    return lane.across(from, v, c);
+    return lane.across(rows, v, c);
   }
-  // weight(block, v)
-  template <typename Weight>
-  __device__ __forceinline__ void run(Along<T, DP>& out, Weight&& weight) {
+  __device__ __forceinline__ void run(Along<T, DP>& out, const T (&weight)[4]) {
     run_queue<kCount>(
         queue, [&](int i) { return read(i); },
         [&](int at, const typename L::Piece& piece) {
-          const int b = at / (4 * kPerRow), v = at / kPerRow % 4, c = at % kPerRow;
+          const int v = at / kPerRow, c = at % kPerRow;
           const int pieces = L::kRest != 0 && c == L::kChunks ? 2 : W;
 #pragma unroll
           for (int n = 0; n < W; ++n) {
             if (n >= pieces) continue;
-            out.block[c * W + n] = Mma<T>::step(piece[n], weight(b, v), out.block[c * W + n]);
+            out.block[c * W + n] = Mma<T>::step(piece[n], weight[v], out.block[c * W + n]);
           }
         });
   }

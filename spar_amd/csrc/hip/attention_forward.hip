@@ -7,7 +7,7 @@
 // they lie, and rescaling O takes no exchange between lanes (attention.hpp).
 // Scores carry scale * log2(e), folded into q, so that weights are powers of two.
 //
-// Two kernels.  tile_kernel: a workgroup of four waves with 16 or 32 rows each
+// Two kernels.  tile_kernel: a workgroup of four waves with 16 rows each
 // shares tiles of keys and values in LDS; bound by the matrix units (4 extent
 // operations per visible pair).  token_kernel, for up to kTokenRows rows (a token
 // or a few per sequence) and where tiles would leave the chip idle: a workgroup's
@@ -56,15 +56,9 @@ struct Row {
   // The base, and the lowest value where no score has been seen.
   __device__ __forceinline__ T top() const { return limit == lowest<T>() ? limit : -start[0]; }
 
-  // Turns the scores of KB blocks of keys into weights.
-  template <int KB>
-  __device__ __forceinline__ void take(T (&score)[KB][4]) {
-    T high = score[0][0];
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-#pragma unroll
-      for (int v = kb == 0 ? 1 : 0; v < 4; ++v) high = larger(high, score[kb][v]);
-    }
+  // Turns the scores of a block of keys into weights.
+  __device__ __forceinline__ void take(T (&score)[4]) {
+    T high = larger(larger(score[0], score[1]), larger(score[2], score[3]));
     if (__any(high > limit)) {
       high = quarter_max(high);
       const bool grows = high > limit;
@@ -75,18 +69,12 @@ struct Row {
       start -= step;
       limit = grows ? T(kSlack) : limit;
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-#pragma unroll
-        for (int v = 0; v < 4; ++v) score[kb][v] -= step;
-      }
+      for (int v = 0; v < 4; ++v) score[v] -= step;
     }
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        score[kb][v] = exp2_of(score[kb][v]);
-        total += score[kb][v];
-      }
+    for (int v = 0; v < 4; ++v) {
+      score[v] = exp2_of(score[v]);
+      total += score[v];
     }
   }
 };
@@ -133,7 +121,13 @@ __device__ __forceinline__ const T* head_row(const Heads<const T>& heads, const 
 
 // Workgroups of one key head follow each other at a distance of batch * key heads,
 // a multiple of the 8 dies in common sizes, so that they share a die's cache; the
-// last rows, which see most, come first.
+// last rows, which see most, come first.  A wave passes over blocks of 16 keys that none
+// of its rows sees, and forms masks only for those that an edge of the window, of the
+// sinks or of the diagonal cuts.  The matrix units are busy 83% of the time at heads of
+// 128: 32 of them with 8192 tokens, window 1024 and 4 sinks in 1.02 ms, 128 TFLOP/s of
+// visible pairs; 72% at heads of 64, 256 of them with 1024 tokens and window 256 in
+// 180 us, 84 TFLOP/s, where cut blocks are a tenth of the work and the softmax's vector
+// instructions, some 45 a block, weigh twice as much.
 template <typename T, int DP, int KB, Reads READS>
 __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(
     Call call, Results<T> results, Heads<const T> query, Heads<const T> key, Heads<const T> value,
@@ -203,47 +197,38 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(
     seen.tile(i, KT, begin, end);
     __syncthreads();
     if (i + 1 < end_tile) start(i + 1);
-    const int32_t last = begin + KT - 1;
-    const bool any = begin <= newest && ((oldest < 0 ? 0 : oldest) - last < call.window ||
-                                         begin < call.sinks);
-    if (any) {
-      const T* key_rows = keys.value[i % 2];
-      const T* value_rows = values.value[i % 2];
-      typename Mma<T>::Acc s[KB];
 #pragma unroll
-      for (int n = 0; n < KB; ++n) s[n] = row.start;
-      const auto read = [&](int p) { return lane.along(key_rows + p % KB * kBlock * DP, p / KB); };
+    for (int kb = 0; kb < KB; ++kb) {
+      const int32_t k0 = begin + kb * kBlock, k1 = k0 + kBlock - 1;
+      const bool any = k0 < end && k0 <= newest &&
+                       ((oldest < 0 ? 0 : oldest) - k1 < call.window || k0 < call.sinks);
+      if (!any) continue;
+      const T* key_rows = keys.value[i % 2] + kb * kBlock * DP;
+      const T* value_rows = values.value[i % 2] + kb * kBlock * DP;
+      typename Mma<T>::Acc s = row.start;
+      const auto read = [&](int p) { return lane.along(key_rows, p); };
       Queue<2, typename Vec16<T>::type> queue;
       fill_queue(queue, read);
-      run_queue<KB * DP / (4 * W)>(queue, read,
-                                   [&](int p, const typename Vec16<T>::type& piece) {
+      run_queue<DP / (4 * W)>(queue, read, [&](int p, const typename Vec16<T>::type& piece) {
 #pragma unroll
-        for (int x = 0; x < W; ++x) {
-          s[p % KB] = Mma<T>::step(piece[x], q.value[p / KB * W + x], s[p % KB]);
-        }
+        for (int x = 0; x < W; ++x) s = Mma<T>::step(piece[x], q.value[p * W + x], s);
       });
-      Across<KB, T, DP> across(lane, value_rows);
-      const bool whole = last <= oldest && last < end &&
-                         (newest - begin < call.window || last < call.sinks);
-      T score[KB][4];
+      Across<T, DP> across(lane, value_rows);
+      const bool whole = k1 <= oldest && k1 < end &&
+                         (newest - k0 < call.window || k1 < call.sinks);
+      T score[4];
 #pragma unroll
-      for (int n = 0; n < KB; ++n) {
-#pragma unroll
-        for (int v = 0; v < 4; ++v) score[n][v] = s[n][v];
-      }
+      for (int v = 0; v < 4; ++v) score[v] = s[v];
       if (!whole) {
 #pragma unroll
-        for (int n = 0; n < KB; ++n) {
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const int32_t at = begin + n * kBlock + Mma<T>::row_of(v, lane.quarter);
-            const bool visible = (at < end) & call.sees(token, at);
-            score[n][v] = visible ? score[n][v] : lowest<T>();
-          }
+        for (int v = 0; v < 4; ++v) {
+          const int32_t at = k0 + Mma<T>::row_of(v, lane.quarter);
+          const bool visible = (at < end) & call.sees(token, at);
+          score[v] = visible ? score[v] : lowest<T>();
         }
       }
-      row.template take<KB>(score);
-      across.run(row.out, [&](int n, int v) { return score[n][v]; });
+      row.take(score);
+      across.run(row.out, score);
     }
     if (i + 1 < end_tile) finish(i + 1);
   }
@@ -252,7 +237,12 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(
 }
 
 // Four waves with the same 16 rows and every fourth block of 16 keys, read into
-// the operands' layout from memory; at the end the waves' rows meet in LDS.
+// the operands' layout from memory; at the end the waves' rows meet in LDS.  Nothing is
+// shared between waves before that, so no wave waits for another.  Bound by reading the
+// cache: 4 sequences of about 50000 tokens in 8 key heads of 128 in 345 us, 5.5 TB/s;
+// 16 sequences with a window of 1024 in 4 key heads of 64 in 10.4 us, 3.3 TB/s, where the
+// launch, a few blocks per wave and their latency show (16 waves a workgroup without
+// splits and their join: 17.7 us against 10.4 + 3).
 template <typename T, int DP, Reads READS>
 __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> results,
                                                          Heads<const T> query, Heads<const T> key,
@@ -312,15 +302,15 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
     const int32_t last = begin + kBlock - 1;
     const bool whole = last <= oldest && last < end &&
                        (newest - begin < call.window || last < call.sinks);
-    T score[1][4];
+    T score[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       const int32_t at = begin + Mma<T>::row_of(n, quarter);
       const bool visible = whole | ((at < end) & call.sees(token, at));
-      score[0][n] = visible ? s[n] : lowest<T>();
+      score[n] = visible ? s[n] : lowest<T>();
     }
-    row.template take<1>(score);
-    v.add_to(row.out, score[0]);
+    row.take(score);
+    v.add_to(row.out, score);
   }
   const T total = quarter_sum(row.total);
   if (quarter == 0) {
@@ -379,7 +369,8 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
 
 // The parts of a row: o = sum 2^(w - top) o_part / sum 2^(w - top), w the log2 of a
 // part's sum.  Few parts: kLanes lanes side by side along a row's head take them in
-// their order.
+// their order, all loaded before the first is used (16384 rows of 128 in 3 parts 7.5 us,
+// 256 rows of 64 in 8 parts 3 us).
 constexpr uint32_t kFewParts = 8;
 
 template <typename T>
@@ -461,7 +452,7 @@ __global__ __launch_bounds__(kThreads) void combine_few_kernel(Call call, Result
 }
 
 // Many parts: a workgroup per row, the parts dealt out to its runs of lanes, whose
-// sums meet in a tree.
+// sums meet in a tree (128 rows of 128 in 32 parts 6 us, latency).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void combine_kernel(Call call, Results<T> results) {
   constexpr int W = Vec16<T>::width;
@@ -534,8 +525,8 @@ static_assert(kThreads >= SPAR_HIP_ATTENTION_MAX_EXTENT);
 // of 64 rows would leave half of its matrix work unused.
 constexpr uint64_t kTokenRows = 32;
 
-// Workgroups that keep the chip's 256 CUs busy, and the fewest keys that repay
-// the writing and reading of a part.
+// Workgroups that fill the chip (three or four to each of its 256 CUs), which row tiles
+// are split up to, and the fewest keys that repay the writing and reading of a part.
 constexpr uint64_t kFullGrid = 768;
 constexpr uint64_t kTokenGrid = 1024;
 constexpr uint64_t kFewestKeys = 256;

@@ -84,7 +84,8 @@ struct RotaryScaling final {
 ///            behind them are not read.
 /// A query or key of another sequence or head never changes a result; a NaN or
 /// infinity in a key or value that some query of its head sees may also reach
-/// other queries of that head.
+/// other queries of that head, and one in any input that takes part the gradients
+/// of its key head and of the query heads that read it.
 [[nodiscard]] Tensor window_attention(const Tensor& query, const Tensor& key, const Tensor& value,
                                       std::size_t window = 0, std::size_t sinks = 0,
                                       std::optional<double> scale = std::nullopt,
