@@ -2,7 +2,8 @@
 // dP = do v^T and delta = do . o per row,
 //   dS = P (dP - delta),  dq = scale dS k,  dk = scale dS^T q,  dv = P^T do.
 //
-// Two kernels, so that every gradient has one writer and sums in a fixed order.
+// Two kernels (each in a form for large and one for small grids), so that every gradient
+// has one writer and sums in a fixed order.
 // query_kernel keeps 16 rows per wave and walks the keys they see (as the forward
 // does); it also leaves delta behind.  key_kernel keeps 16 keys per wave and walks
 // the rows that see them, the heads of a group among them.  Each recomputes S and
@@ -36,12 +37,16 @@ struct Saved {
 // window (none for one split), then of the rows behind the windows of the sinks' tiles.
 template <typename T>
 struct Splits {
-  T* parts;  // [batch head][tile][split][dk, dv][64][extent], and the same of the sinks
+  // [batch head][tile][split][dk, dv][tile_keys][extent], and the same of the sinks
+  T* parts;
+  uint32_t tile_keys;
   uint32_t key_tiles, main;    // splits of a tile's window: at least 1
   uint32_t sink_tiles, later;  // splits of the rows behind it
   uint32_t extent;
 
-  __device__ __forceinline__ uint64_t size() const;  // of a part
+  __device__ __forceinline__ uint64_t size() const {  // of a part
+    return static_cast<uint64_t>(2 * tile_keys) * extent;
+  }
   __device__ __forceinline__ T* main_part(uint32_t batch_head, uint32_t tile,
                                           uint32_t split) const {
     return parts + ((static_cast<uint64_t>(batch_head) * key_tiles + tile) * main + split) * size();
@@ -319,10 +324,74 @@ __host__ __device__ inline int sink_blocks(int32_t sinks) {
   return sinks <= kBlock ? 1 : sinks <= 2 * kBlock ? 2 : kWaves;
 }
 
-template <typename T>
-__device__ __forceinline__ uint64_t Splits<T>::size() const {
-  return static_cast<uint64_t>(2 * kKeyTile) * extent;
-}
+// What a workgroup of either key kernel has to do: a tile of keys, and the rows that see
+// one of them, through the window or behind it as sinks.
+struct KeyTile {
+  uint32_t batch_head, b, key_head;
+  uint32_t tile, split, parts;
+  bool behind;
+  int32_t length, first;  // tokens of the sequence; the token of query 0
+  int32_t begin_key;
+  uint32_t begin_row, end_row;
+
+  // The tiles of keys come first, the short splits of the sinks' later rows last.
+  template <typename T>
+  __device__ __forceinline__ KeyTile(const Call& call, const Splits<T>& splits,
+                                     int32_t tile_keys) {
+    batch_head = blockIdx.x % call.batch_heads;
+    const uint32_t rest = blockIdx.x / call.batch_heads;
+    const uint32_t main_groups = splits.key_tiles * splits.main;
+    behind = rest >= main_groups;
+    parts = behind ? splits.later : splits.main;
+    tile = (behind ? rest - main_groups : rest) / parts;
+    split = (behind ? rest - main_groups : rest) % parts;
+    b = batch_head / call.key_heads;
+    key_head = batch_head % call.key_heads;
+    length = call.length(b);
+    first = length - call.queries;
+    begin_key = static_cast<int32_t>(tile) * tile_keys;
+    const int32_t end_key = begin_key + tile_keys < length ? begin_key + tile_keys : length;
+    int32_t low = begin_key, high = end_key - 1 + call.window;  // tokens [low, high)
+    if (high > length) high = length;
+    if (behind) {
+      low = high;
+      high = length;
+      if (begin_key >= call.sinks) low = high;
+    }
+    if (low < first) low = first;
+    if (low < 0) low = 0;
+    if (high < low || begin_key >= length) high = low;
+    begin_row = static_cast<uint32_t>(low - first) * call.group.divisor;
+    end_row = static_cast<uint32_t>(high - first) * call.group.divisor;
+    if (begin_row >= end_row) begin_row = end_row = 0;
+  }
+  // This split's share of so many blocks of rows.
+  __device__ __forceinline__ uint32_t share(uint32_t blocks, uint32_t of) const {
+    return static_cast<uint32_t>(static_cast<uint64_t>(blocks) * of / parts);
+  }
+  // Keys whose gradients it yields end here.
+  __device__ __forceinline__ int32_t end_key(const Call& call) const {
+    return behind ? call.sinks : static_cast<int32_t>(call.keys);
+  }
+  // Where the gradients of key `at` of the tile go: a part, or the result.
+  template <typename T>
+  __device__ __forceinline__ void targets(const Call& call, const Splits<T>& splits,
+                                          const Heads<T>& key_gradient,
+                                          const Heads<T>& value_gradient, uint32_t at,
+                                          uint32_t own, T*& dk, T*& dv) const {
+    if (behind || splits.main > 1) {
+      T* part = behind ? splits.later_part(call.batch_heads, batch_head, tile, split)
+                       : splits.main_part(batch_head, tile, split);
+      dk = part + static_cast<uint64_t>(at) * call.extent;
+      dv = dk + static_cast<uint64_t>(splits.tile_keys) * call.extent;
+    } else {
+      dk = key_gradient.data + b * key_gradient.batch + key_head * key_gradient.head +
+           own * key_gradient.token;
+      dv = value_gradient.data + b * value_gradient.batch + key_head * value_gradient.head +
+           own * value_gradient.token;
+    }
+  }
+};
 
 // dk and dv of 64 keys, 16 per wave, over tiles of the rows that see them.  Bound by the
 // matrix units, busy 77% of the time at heads of 128 (8 extent operations per visible
@@ -336,41 +405,18 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(
   __shared__ Tile<T, RT, DP, READS> queries, output_gradients;
   __shared__ alignas(16) T log_sums[2][RT], deltas[2][RT];
   __shared__ int32_t tokens[2][RT];
-  const uint32_t batch_head = blockIdx.x % call.batch_heads;
-  const uint32_t rest = blockIdx.x / call.batch_heads;
-  // The tiles of keys come first, the short splits of the sinks' later rows last.
-  const uint32_t main_groups = splits.key_tiles * splits.main;
-  const bool behind = rest >= main_groups;
-  const uint32_t parts = behind ? splits.later : splits.main;
-  const uint32_t tile = (behind ? rest - main_groups : rest) / parts;
-  const uint32_t split = (behind ? rest - main_groups : rest) % parts;
-  const uint32_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
+  const KeyTile work(call, splits, kKeyTile);
+  const uint32_t b = work.b, key_head = work.key_head;
+  const bool behind = work.behind;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const Lane<T, DP> lane(threadIdx.x % kWave);
   const int quarter = lane.quarter, column = lane.column;
 
-  const int32_t length = call.length(b);
-  const int32_t first = length - call.queries;
-  const int32_t begin_key = static_cast<int32_t>(tile) * kKeyTile;
-  const int32_t end_key = begin_key + kKeyTile < length ? begin_key + kKeyTile : length;
-  // Tokens that see a key of the tile through the window, or behind it as sinks.
-  int32_t low = begin_key, high = end_key - 1 + call.window;  // [low, high)
-  if (high > length) high = length;
-  if (behind) {
-    low = high;
-    high = length;
-    if (begin_key >= call.sinks) low = high;
-  }
-  if (low < first) low = first;
-  if (low < 0) low = 0;
-  if (high < low || begin_key >= length) high = low;
-  uint32_t begin_row = static_cast<uint32_t>(low - first) * call.group.divisor;
-  uint32_t end_row = static_cast<uint32_t>(high - first) * call.group.divisor;
-  if (begin_row >= end_row) begin_row = end_row = 0;
+  const int32_t length = work.length, first = work.first, begin_key = work.begin_key;
+  const uint32_t begin_row = work.begin_row, end_row = work.end_row;
   uint32_t tiles = (end_row - begin_row + RT - 1) / RT;
-  const uint32_t begin_tile =
-      static_cast<uint32_t>(static_cast<uint64_t>(tiles) * split / parts);
-  tiles = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / parts);
+  const uint32_t begin_tile = work.share(tiles, work.split);
+  tiles = work.share(tiles, work.split + 1);
 
   // Behind the window a tile with few sinks gives its waves the same keys and every
   // second or fourth block of rows.
@@ -492,25 +538,124 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(
     if (i + 1 < tiles) finish(i + 1);
   }
 
-  T* dk_target;
-  T* dv_target;
-  if (own >= static_cast<int32_t>(behind ? call.sinks : call.keys)) return;
-  if (behind || splits.main > 1) {
-    T* part = behind ? splits.later_part(call.batch_heads, batch_head, tile, split)
-                     : splits.main_part(batch_head, tile, split);
-    dk_target = part + static_cast<uint64_t>(wave * kBlock + column) * call.extent;
-    dv_target = dk_target + static_cast<uint64_t>(kKeyTile) * call.extent;
-  } else {
-    dk_target = key_gradient.data + b * key_gradient.batch + key_head * key_gradient.head +
-                own * key_gradient.token;
-    dv_target = value_gradient.data + b * value_gradient.batch + key_head * value_gradient.head +
-                own * value_gradient.token;
-  }
+  if (own >= work.end_key(call)) return;
+  T *dk_target, *dv_target;
+  work.targets(call, splits, key_gradient, value_gradient, wave * kBlock + column, own, dk_target,
+               dv_target);
   dk.visit(quarter, [&](uint32_t d, auto& run) {
     for (auto& y : run) y *= static_cast<T>(call.scale);
     store_piece(dk_target, d, call.extent, run);
   });
   dv.visit(quarter, [&](uint32_t d, auto& run) { store_piece(dv_target, d, call.extent, run); });
+}
+
+// The same for grids that tiles of 64 keys do not fill: a workgroup's waves share 16
+// keys and take every fourth block of 16 rows, straight from memory; their sums meet
+// in LDS.  Bound by the latency of a block's loads, about 3 us a block.
+template <typename T, int DP, Reads READS>
+__global__ __launch_bounds__(kThreads) void key_spread_kernel(Call call, Saved<T> saved,
+                                                              Heads<T> key_gradient,
+                                                              Heads<T> value_gradient,
+                                                              Splits<T> splits) {
+  constexpr int W = Vec16<T>::width;
+  __shared__ alignas(16) T sums[kWaves][kBlock][DP + W];
+  const KeyTile work(call, splits, kBlock);
+  const uint32_t b = work.b, key_head = work.key_head;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int quarter = threadIdx.x % kWave / kBlock, column = threadIdx.x % kBlock;
+  const uint32_t begin_row = work.begin_row, end_row = work.end_row;
+  const uint32_t blocks = (end_row - begin_row + kBlock - 1) / kBlock;
+  const uint32_t end_block = work.share(blocks, work.split + 1);
+
+  const int32_t own = work.begin_key + column;
+  const bool keeps = own < work.length;
+  Operand<T, DP> k, x;
+  {
+    const uint64_t at = static_cast<uint32_t>(own) < call.keys ? own : 0;
+    k.template load<READS>(
+        saved.key.data + b * saved.key.batch + key_head * saved.key.head + at * saved.key.token,
+        call.extent, quarter);
+    x.template load<READS>(saved.value.data + b * saved.value.batch +
+                               key_head * saved.value.head + at * saved.value.token,
+                           call.extent, quarter);
+    k.finish(keeps, call.extent, quarter, static_cast<T>(call.scale * kLog2E));
+    x.finish(keeps, call.extent, quarter, T(1));
+  }
+  Along<T, DP> dk, dv;
+  dk.clear();
+  dv.clear();
+
+  for (uint32_t i = work.share(blocks, work.split) + wave; i < end_block; i += kWaves) {
+    const uint32_t row0 = begin_row + i * kBlock;
+    // Rows behind the last repeat the block's first; their token sees nothing.
+    const auto place_of = [&](uint32_t j) {
+      return Place(call, b, key_head, row0 + j < end_row ? row0 + j : row0);
+    };
+    const Place read = place_of(column);
+    Operand<T, DP> q, g;
+    q.template load<READS>(read.of(saved.query, b), call.extent, quarter);
+    g.template load<READS>(read.of(saved.output_gradient, b), call.extent, quarter);
+    T log_sum[4], delta[4];
+    int32_t token[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const uint32_t j = Mma<T>::row_of(v, quarter);
+      const Place place = place_of(j);
+      log_sum[v] = saved.logsumexp[place.at] * static_cast<T>(kLog2E);
+      delta[v] = saved.delta[place.at];
+      token[v] = row0 + j < end_row ? work.first + static_cast<int32_t>(place.t) : -1;
+    }
+    typename Mma<T>::Acc s{0, 0, 0, 0}, dp{0, 0, 0, 0};
+#pragma unroll
+    for (int step = 0; step < DP / 4; ++step) {
+      s = Mma<T>::step(q.value[step], k.value[step], s);
+      dp = Mma<T>::step(g.value[step], x.value[step], dp);
+    }
+    T p[4], ds[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const bool visible = call.sees(token[v], own);
+      p[v] = exp2_of(s[v] - log_sum[v]);
+      ds[v] = p[v] * (dp[v] - delta[v]);
+      p[v] = visible ? p[v] : T(0);
+      ds[v] = visible ? ds[v] : T(0);
+    }
+    AcrossOperand<T, DP> across;
+    across.template load<READS>(call.extent, quarter, column, [&](int n) {
+      return place_of(n).of(saved.output_gradient, b);
+    });
+    across.add_to(dv, p);
+    across.template load<READS>(call.extent, quarter, column,
+                                [&](int n) { return place_of(n).of(saved.query, b); });
+    across.add_to(dk, ds);
+  }
+
+  const auto join = [&](const Along<T, DP>& sum, bool keys, T factor) {
+    sum.visit(quarter, [&](uint32_t d, auto& run) {
+      for (auto& y : run) sums[wave][column][d++] = y;
+    });
+    __syncthreads();
+    constexpr int kPieces = DP / W;
+    for (int at = threadIdx.x; at < kBlock * kPieces; at += kThreads) {
+      const int c = at / kPieces, d = at % kPieces * W;
+      if (work.begin_key + c >= work.end_key(call)) continue;
+      T run[W];
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        run[j] = sums[0][c][d + j];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) run[j] += sums[w][c][d + j];
+        run[j] *= factor;
+      }
+      T *dk_target, *dv_target;
+      work.targets(call, splits, key_gradient, value_gradient, c, work.begin_key + c, dk_target,
+                   dv_target);
+      store_piece(keys ? dk_target : dv_target, d, call.extent, run);
+    }
+    __syncthreads();
+  };
+  join(dk, true, static_cast<T>(call.scale));
+  join(dv, false, T(1));
 }
 
 // dk and dv of the first `keys` keys from their parts in a fixed order: eight lanes to
@@ -529,16 +674,18 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Call call, Heads<T> key_
   const uint32_t within = inside ? static_cast<uint32_t>(at - batch_head * per_head) : 0;
   const uint32_t key = within / call.extent, d = within % call.extent;
   const uint32_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
-  const uint32_t tile = key / kKeyTile;
+  const bool spread = splits.tile_keys == kBlock;
+  const uint32_t tile = spread ? key / kBlock : key / kKeyTile;
+  const uint32_t at_key = spread ? key % kBlock : key % kKeyTile;
   const uint64_t row = static_cast<uint64_t>(call.extent);
-  const uint64_t value_part = kKeyTile * row;
+  const uint64_t value_part = splits.tile_keys * row;
   T* dk = key_gradient.data + b * key_gradient.batch + key_head * key_gradient.head +
           key * key_gradient.token + d;
   T* dv = value_gradient.data + b * value_gradient.batch + key_head * value_gradient.head +
           key * value_gradient.token + d;
   T sum_k = T(0), sum_v = T(0);
   if (splits.main > 1) {
-    const T* from = splits.main_part(batch_head, tile, 0) + key % kKeyTile * row + d;
+    const T* from = splits.main_part(batch_head, tile, 0) + at_key * row + d;
 #pragma unroll 4
     for (uint32_t s = run; s < splits.main; s += kRuns) {
       sum_k += from[s * splits.size()];
@@ -549,10 +696,12 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Call call, Heads<T> key_
     sum_v = *dv;
   }
   if (splits.later != 0 && key < static_cast<uint32_t>(call.sinks)) {
-    const int blocks = sink_blocks(call.sinks - static_cast<int32_t>(tile * kKeyTile));
+    // key_kernel's waves that take turns leave a part each.
+    const int blocks =
+        spread ? kWaves : sink_blocks(call.sinks - static_cast<int32_t>(tile * kKeyTile));
     const uint32_t turns = kWaves / blocks;
-    const T* from = splits.later_part(call.batch_heads, batch_head, tile, 0) +
-                    key % kKeyTile * row + d;
+    const T* from =
+        splits.later_part(call.batch_heads, batch_head, tile, 0) + at_key * row + d;
 #pragma unroll 4
     for (uint32_t s = run; s < splits.later * turns; s += kRuns) {
       const uint64_t part = s / turns * splits.size() + s % turns * blocks * kBlock * row;
@@ -578,7 +727,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Call call, Heads<T> key_
 // ---------------------------------------------------------------- launchers
 
 struct Plan {
-  bool spread;  // query_spread_kernel
+  bool spread;      // query_spread_kernel
+  bool key_spread;  // key_spread_kernel
+  uint32_t tile_keys;
   uint32_t row_tiles, key_tiles, main, sink_tiles, later;
   uint64_t delta_bytes;  // a multiple of 16
   uint64_t bytes;
@@ -590,9 +741,22 @@ struct Plan {
 constexpr uint64_t kLaterShare = 2;
 constexpr uint64_t kMostLater = 256;
 constexpr uint64_t kMostLaterGroups = 2048;
-// Workgroups that fill the chip, and the fewest rows that repay a part.
+// Workgroups that fill the chip, and the fewest rows that repay a part of either kernel:
+// two parts of 256 rows of key_spread_kernel (8 heads of 128) 15 + 9 us against 20 us
+// for one, of 348 float64 rows (heads of 72) 28 + 7 us against 38.
 constexpr uint64_t kFullGrid = 512;
 constexpr uint64_t kFewestRows = 64;
+constexpr uint64_t kFewestSpreadRows = 160;
+// key_spread_kernel is for tiles of 16 keys whose rows are at most so many for each tile:
+// more rows want the rows shared in LDS and more parts.  Kernel and join, key_kernel's
+// first: 48 heads of 64 with 128 tokens 24 and 10 us; 16 heads of 64 with 512 tokens and
+// a window of 128 35 and 21 us; 8 heads of 64 with 1472 tokens 101 and 81 us; 2 key
+// heads, each for 4 heads of 128, with 1024 keys and 256 tokens 42 and 46 us; 8 such key
+// heads with 512 tokens 81 and 103 us.
+constexpr uint64_t kMostSpreadRows = 4;
+// Its operands and sums stay in registers up to this many bytes of a head (4 heads of 160
+// with 210 float64 tokens 81 us against 65).
+constexpr uint64_t kMostSpreadBytes = 1024;
 
 Plan plan_of(const SparHipAttention& a) {
   Plan plan{};
@@ -602,24 +766,32 @@ Plan plan_of(const SparHipAttention& a) {
   plan.row_tiles = ceil_div_u32(a.queries * group, kWaves * kBlock);
   plan.spread = spreads(plan.row_tiles * batch_heads);
   if (plan.spread) plan.row_tiles = ceil_div_u32(a.queries * group, kBlock);
-  plan.key_tiles = ceil_div_u32(a.keys, kKeyTile);
+  const auto rows_of = [&](uint64_t tile_keys) {  // that see a tile through the window
+    return group * (a.window == 0 ? a.queries : std::min(a.queries, a.window + tile_keys));
+  };
+  plan.key_spread = spreads(ceil_div_u32(a.keys, kKeyTile) * batch_heads) &&
+                    rows_of(kBlock) <=
+                        kMostSpreadRows * ceil_div_u32(a.keys, kBlock) * batch_heads &&
+                    a.extent * element <= kMostSpreadBytes;
+  plan.tile_keys = plan.key_spread ? kBlock : kKeyTile;
+  plan.key_tiles = ceil_div_u32(a.keys, plan.tile_keys);
   plan.main = 1;
   plan.delta_bytes =
       (a.batch * a.query_heads * a.queries * element + 15) / 16 * 16;
-  const uint64_t rows =
-      group * (a.window == 0 ? a.queries : std::min(a.queries, a.window + kKeyTile));
+  const uint64_t fewest = plan.key_spread ? kFewestSpreadRows : kFewestRows;
   if (plan.key_tiles != 0) {
-    plan.main = static_cast<uint32_t>(std::max<uint64_t>(
-        1, std::min(kFullGrid / (plan.key_tiles * batch_heads), rows / kFewestRows)));
+    plan.main = static_cast<uint32_t>(
+        std::max<uint64_t>(1, std::min(kFullGrid / (plan.key_tiles * batch_heads),
+                                       rows_of(plan.tile_keys) / fewest)));
   }
   const uint64_t sinks = std::min(a.sinks, a.keys);
   if (a.window != 0 && sinks != 0 && a.keys > a.window) {
-    plan.sink_tiles = ceil_div_u32(sinks, kKeyTile);
+    plan.sink_tiles = ceil_div_u32(sinks, plan.tile_keys);
     const uint64_t behind = std::min(a.queries, a.keys - a.window);
-    const uint64_t share = (a.window + kKeyTile) / kLaterShare;
+    const uint64_t share = (a.window + plan.tile_keys) / kLaterShare;
     plan.later = static_cast<uint32_t>(std::min(
         kMostLater, std::max((behind + share - 1) / share,
-                             std::min<uint64_t>(plan.main, behind * group / kFewestRows))));
+                             std::min<uint64_t>(plan.main, behind * group / fewest))));
     plan.later = static_cast<uint32_t>(std::min<uint64_t>(
         plan.later,
         std::max<uint64_t>(1, kMostLaterGroups / std::max<uint64_t>(
@@ -627,7 +799,7 @@ Plan plan_of(const SparHipAttention& a) {
   }
   const uint64_t parts = (plan.main > 1 ? uint64_t{plan.key_tiles} * plan.main : 0) +
                          uint64_t{plan.sink_tiles} * plan.later;
-  plan.bytes = plan.delta_bytes + batch_heads * parts * 2 * kKeyTile * a.extent * element;
+  plan.bytes = plan.delta_bytes + batch_heads * parts * 2 * plan.tile_keys * a.extent * element;
   return plan;
 }
 
@@ -643,8 +815,8 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& quer
                        static_cast<const T*>(logsumexp), static_cast<T*>(workspace)};
   const Heads<T> dk = heads_of<T>(key_gradient), dv = heads_of<T>(value_gradient);
   const Splits<T> splits{
-      reinterpret_cast<T*>(static_cast<char*>(workspace) + plan.delta_bytes), plan.key_tiles,
-      plan.main, plan.sink_tiles, plan.later, call.extent};
+      reinterpret_cast<T*>(static_cast<char*>(workspace) + plan.delta_bytes), plan.tile_keys,
+      plan.key_tiles, plan.main, plan.sink_tiles, plan.later, call.extent};
   const uint32_t key_groups = plan.key_tiles * plan.main + plan.sink_tiles * plan.later;
   with_width<T>(a, {&output_gradient, &output, &query, &key, &value},
                 [&](auto width, auto reads) {
@@ -663,7 +835,13 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& quer
           <<<plan.row_tiles * call.batch_heads, kThreads, 0, stream>>>(
               call, saved, heads_of<T>(query_gradient), plan.row_tiles);
     }
-    if (call.keys != 0) {
+    if (call.keys != 0 && plan.key_spread) {
+      if constexpr (DP * sizeof(T) <= kMostSpreadBytes) {
+        constexpr Reads kReads = READS == Reads::Aligned ? Reads::Pieces : READS;
+        key_spread_kernel<T, DP, kReads>
+            <<<key_groups * call.batch_heads, kThreads, 0, stream>>>(call, saved, dk, dv, splits);
+      }
+    } else if (call.keys != 0) {
       key_kernel<T, DP, kKeyBlocks, READS>
           <<<key_groups * call.batch_heads, kThreads, 0, stream>>>(call, saved, dk, dv, splits);
     }

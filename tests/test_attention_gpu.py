@@ -297,11 +297,12 @@ def test_attention(hip, shape, window, sinks, lengths, dtype):
     check(hip, shape, dtype, window, sinks, lengths)
 
 
-def check_in_tiles(hip, shape, dtype, window=0, sinks=0, lengths=None, **more):
-    """The same shape for so many sequences that tiles of 64 rows fill the chip, which
-    then take them: the shape's sequences over and over, each repetition the same bits."""
+def check_in_tiles(hip, shape, dtype, window=0, sinks=0, lengths=None, of_keys=False, **more):
+    """The same shape for so many sequences that tiles of 64 rows (or `of_keys`) fill the
+    chip, which then take them: the shape's sequences over and over, each repetition the
+    same bits."""
     b, h, hk, t, s, d = shape
-    times = -(-192 // (b * hk * -(-t * h // hk // 64)))
+    times = -(-192 // (b * hk * -(-s // 64 if of_keys else -t * h // hk // 64)))
     q, k, v, g = inputs(*shape, dtype)
     want = oracle.Attention(q, k, v, window, sinks, more.get("scale"), lengths, dtype)
     lengths = None if lengths is None else np.tile(np.asarray(lengths), times)
@@ -323,6 +324,23 @@ def check_in_tiles(hip, shape, dtype, window=0, sinks=0, lengths=None, **more):
 @pytest.mark.parametrize("dtype", [F32, F64])
 def test_attention_in_tiles(hip, shape, window, sinks, lengths, dtype):
     check_in_tiles(hip, shape, dtype, window, sinks, lengths)
+
+
+@pytest.mark.parametrize("shape,window,sinks,lengths",
+                         [case for case in ATTENTION if 16 <= case[0][4] <= 200], ids=str)
+@pytest.mark.parametrize("dtype", [F32, F64])
+def test_attention_in_tiles_of_keys(hip, shape, window, sinks, lengths, dtype):
+    check_in_tiles(hip, shape, dtype, window, sinks, lengths, of_keys=True)
+
+
+@pytest.mark.parametrize("shape,window,sinks,lengths", [
+    ((1, 6, 6, 350, 350, 40), 330, 20, None),         # sinks of two tiles of 16 keys
+    ((2, 8, 4, 250, 250, 72), 200, 3, [250, 101]),
+    ((1, 5, 5, 333, 500, 66), 0, 0, None),
+], ids=str)
+@pytest.mark.parametrize("dtype", [F32, F64])
+def test_rows_of_few_keys_are_split(hip, shape, window, sinks, lengths, dtype):
+    check(hip, shape, dtype, window, sinks, lengths)
 
 
 @pytest.mark.parametrize("orders,gap,offset", [(("heads", "heads"), 4, 4),
