@@ -97,6 +97,10 @@ struct Call {
                                    : static_cast<const int32_t*>(lengths)[b];
     return static_cast<int32_t>(n < 0 ? 0 : n > keys ? keys : n);
   }
+  // Queries of all heads and sequences.
+  __host__ __device__ __forceinline__ uint64_t all_rows() const {
+    return static_cast<uint64_t>(batch_heads) * rows;
+  }
   // Token of its sequence that row r's query is, less than 0 where it sees nothing.
   __device__ __forceinline__ int32_t token(uint32_t r, int32_t first) const {
     return r < rows ? first + static_cast<int32_t>(group.div(r)) : -1;

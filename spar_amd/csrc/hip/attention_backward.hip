@@ -15,7 +15,8 @@
 // Rows of a tile of keys are split over several workgroups where the tiles alone do
 // not fill the chip; and the sinks, which every later row sees, have thousands of
 // rows where other keys have the window's: those behind a tile's own window are split
-// too.  Splits write parts, which join_kernel adds in their order.
+// too; so are the keys of few rows.  Splits write parts, which join_kernel and
+// query_join_kernel add in their order.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -235,11 +236,17 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
 template <typename T, int DP, Reads READS>
 __global__ __launch_bounds__(kThreads) void query_spread_kernel(Call call, Saved<T> saved,
                                                                 Heads<T> gradient,
-                                                                uint32_t row_tiles) {
+                                                                uint32_t row_tiles, T* parts,
+                                                                uint32_t splits) {
   constexpr int W = Vec16<T>::width;
   __shared__ alignas(16) T sums[kWaves][kBlock][DP + W];
   const uint32_t batch_head = blockIdx.x % call.batch_heads;
-  const uint32_t row_tile = row_tiles - 1 - blockIdx.x / call.batch_heads;
+  const uint32_t rest = blockIdx.x / call.batch_heads;
+  uint32_t split = 0, row_tile = row_tiles - 1 - rest;
+  if (splits != 1) {
+    split = rest % splits;
+    row_tile = row_tiles - 1 - rest / splits;
+  }
   const uint32_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int quarter = threadIdx.x % kWave / kBlock, column = threadIdx.x % kBlock;
@@ -250,19 +257,24 @@ __global__ __launch_bounds__(kThreads) void query_spread_kernel(Call call, Saved
   const int32_t oldest = call.token(begin_row, first);
   const int32_t newest = call.token(end_row - 1, first);
   const Keys seen(call, oldest < 0 ? 0 : oldest, newest);
-  const uint32_t blocks = seen.tiles(kBlock);
+  uint32_t begin_block = 0, end_block = seen.tiles(kBlock);
+  if (splits != 1) {
+    const uint64_t blocks = end_block;
+    begin_block = static_cast<uint32_t>(blocks * split / splits);
+    end_block = static_cast<uint32_t>(blocks * (split + 1) / splits);
+  }
   const uint32_t r = begin_row + column;
   const int32_t token = call.token(r, first);
   const Place place(call, b, key_head, r < call.rows ? r : 0);
   QueryRow<T, DP> row;
   row.template load<READS>(call, saved, place, b, token >= 0, quarter);
-  if (wave == 0 && quarter == 0 && r < call.rows) saved.delta[place.at] = row.delta;
+  if (split == 0 && wave == 0 && quarter == 0 && r < call.rows) saved.delta[place.at] = row.delta;
   Along<T, DP> dq;
   dq.clear();
   const T* key_base = saved.key.data + b * saved.key.batch + key_head * saved.key.head;
   const T* value_base = saved.value.data + b * saved.value.batch + key_head * saved.value.head;
 
-  for (uint32_t i = wave; i < blocks; i += kWaves) {
+  for (uint32_t i = begin_block + wave; i < end_block; i += kWaves) {
     int32_t begin, end;
     seen.tile(i, kBlock, begin, end);
     // Keys behind the run repeat its block's first; no row sees them.
@@ -307,8 +319,29 @@ __global__ __launch_bounds__(kThreads) void query_spread_kernel(Call call, Saved
       for (int w = 1; w < kWaves; ++w) run[j] += sums[w][c][d + j];
       run[j] *= static_cast<T>(call.scale);
     }
-    store_piece(Place(call, b, key_head, begin_row + c).of(gradient, b), d, call.extent, run);
+    const Place to(call, b, key_head, begin_row + c);
+    T* target = splits == 1 ? to.of(gradient, b)
+                            : parts + (split * call.all_rows() + to.at) * call.extent;
+    store_piece(target, d, call.extent, run);
   }
+}
+
+// dq from its parts, in their order: a lane per element.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void query_join_kernel(Call call, Heads<T> gradient,
+                                                              const T* parts, uint32_t splits) {
+  const uint64_t at = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const uint64_t all = call.all_rows() * call.extent;
+  if (at >= all) return;
+  T sum = parts[at];
+#pragma unroll 4
+  for (uint32_t s = 1; s < splits; ++s) sum += parts[s * all + at];
+  const uint64_t row = at / call.extent, batch_head = row / call.queries;
+  const uint32_t heads = call.key_heads * call.group.divisor;
+  const uint64_t b = batch_head / heads, head = batch_head - b * heads;
+  gradient.data[b * gradient.batch + head * gradient.head +
+                (row - batch_head * call.queries) * gradient.token + (at - row * call.extent)] =
+      sum;
 }
 
 constexpr uint32_t kKeyTile = kWaves * kBlock;
@@ -728,6 +761,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Call call, Heads<T> key_
 
 struct Plan {
   bool spread;      // query_spread_kernel
+  uint32_t query_splits;
   bool key_spread;  // key_spread_kernel
   uint32_t tile_keys;
   uint32_t row_tiles, key_tiles, main, sink_tiles, later;
@@ -747,6 +781,10 @@ constexpr uint64_t kMostLaterGroups = 2048;
 constexpr uint64_t kFullGrid = 512;
 constexpr uint64_t kFewestRows = 64;
 constexpr uint64_t kFewestSpreadRows = 160;
+// Keys that repay a part of query_spread_kernel: 2 heads of 64 with 634 queries of 3057
+// keys 67 us in one part, 27 + 5 in six; 4 heads of 128 that share a key head with 1024
+// tokens 49 and 38 + 5 in two; 2 heads of 64 that see 516 keys 19 and 19 + 4 in two.
+constexpr uint64_t kFewestQueryKeys = 384;
 // key_spread_kernel is for tiles of 16 keys whose rows are at most so many for each tile:
 // more rows want the rows shared in LDS and more parts.  Kernel and join, key_kernel's
 // first: 48 heads of 64 with 128 tokens 24 and 10 us; 16 heads of 64 with 512 tokens and
@@ -765,7 +803,13 @@ Plan plan_of(const SparHipAttention& a) {
   const uint64_t batch_heads = a.batch * a.key_heads;
   plan.row_tiles = ceil_div_u32(a.queries * group, kWaves * kBlock);
   plan.spread = spreads(plan.row_tiles * batch_heads);
-  if (plan.spread) plan.row_tiles = ceil_div_u32(a.queries * group, kBlock);
+  plan.query_splits = 1;
+  if (plan.spread) {
+    plan.row_tiles = ceil_div_u32(a.queries * group, kBlock);
+    plan.query_splits = static_cast<uint32_t>(std::max<uint64_t>(
+        1, std::min(kFullGrid / std::max<uint64_t>(1, plan.row_tiles * batch_heads),
+                    most_seen(a) / kFewestQueryKeys)));
+  }
   const auto rows_of = [&](uint64_t tile_keys) {  // that see a tile through the window
     return group * (a.window == 0 ? a.queries : std::min(a.queries, a.window + tile_keys));
   };
@@ -799,7 +843,11 @@ Plan plan_of(const SparHipAttention& a) {
   }
   const uint64_t parts = (plan.main > 1 ? uint64_t{plan.key_tiles} * plan.main : 0) +
                          uint64_t{plan.sink_tiles} * plan.later;
-  plan.bytes = plan.delta_bytes + batch_heads * parts * 2 * plan.tile_keys * a.extent * element;
+  // The parts of dq and those of dk and dv take turns in one place.
+  const uint64_t query_parts =
+      plan.query_splits > 1 ? plan.query_splits * a.batch * a.query_heads * a.queries : 0;
+  plan.bytes = plan.delta_bytes +
+               std::max(batch_heads * parts * 2 * plan.tile_keys, query_parts) * a.extent * element;
   return plan;
 }
 
@@ -828,8 +876,14 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& quer
       // It reads pieces at any address alike.
       constexpr Reads kReads = READS == Reads::Aligned ? Reads::Pieces : READS;
       query_spread_kernel<T, DP, kReads>
-          <<<plan.row_tiles * call.batch_heads, kThreads, 0, stream>>>(
-              call, saved, heads_of<T>(query_gradient), plan.row_tiles);
+          <<<plan.row_tiles * call.batch_heads * plan.query_splits, kThreads, 0, stream>>>(
+              call, saved, heads_of<T>(query_gradient), plan.row_tiles, splits.parts,
+              plan.query_splits);
+      if (plan.query_splits > 1) {
+        query_join_kernel<T>
+            <<<ceil_div_u32(call.all_rows() * call.extent, kThreads), kThreads, 0, stream>>>(
+                call, heads_of<T>(query_gradient), splits.parts, plan.query_splits);
+      }
     } else if (call.rows != 0) {
       query_kernel<T, DP, kBlocks, READS>
           <<<plan.row_tiles * call.batch_heads, kThreads, 0, stream>>>(

@@ -337,9 +337,11 @@ def test_attention_in_tiles_of_keys(hip, shape, window, sinks, lengths, dtype):
     ((1, 6, 6, 350, 350, 40), 330, 20, None),         # sinks of two tiles of 16 keys
     ((2, 8, 4, 250, 250, 72), 200, 3, [250, 101]),
     ((1, 5, 5, 333, 500, 66), 0, 0, None),
+    ((1, 4, 2, 200, 1500, 64), 0, 0, None),           # and the keys of few rows
+    ((2, 4, 2, 70, 1100, 40), 800, 5, [1100, 400]),
 ], ids=str)
 @pytest.mark.parametrize("dtype", [F32, F64])
-def test_rows_of_few_keys_are_split(hip, shape, window, sinks, lengths, dtype):
+def test_work_of_small_grids_is_split(hip, shape, window, sinks, lengths, dtype):
     check(hip, shape, dtype, window, sinks, lengths)
 
 
