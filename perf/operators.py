@@ -15,7 +15,9 @@ the heads of its queries, keys and values between the projections.
 
 With `own` false, run() computes a case from elementary torch operations;
 with `own` true it calls the framework's C ABI on the same tensors, whose
-values are complete when run() is called.  A case is a dict of plain values.
+values are complete when run() is called; its outputs are complete once the
+device has been synchronised (the framework has a stream of its own).  A case is
+a dict of plain values.
 `listed()` gives the named cases and `draw(rng)` one more of the same ranges.
 """
 import math
@@ -333,6 +335,16 @@ def _strides(x):
     return x.stride(0), x.stride(2), x.stride(1)
 
 
+def _scratch(state, name, like, count, dtype=None):
+    """Device memory that calls write and read but do not return.  The state keeps it,
+    as a program does: torch would hand memory dropped here to kernels of its own
+    stream while the framework's stream still works in it."""
+    held = state.setdefault("scratch", {})
+    if name not in held:
+        held[name] = torch.empty(count, dtype=dtype or like.dtype, device=like.device)
+    return held[name]
+
+
 def _own_rotary(state):
     from spar_amd import hip
 
@@ -370,7 +382,7 @@ def _own_norm(state):
                         state["frequencies"].data_ptr(), case["rotary"], state["magnitude"],
                         hip.ROTARY_HALF if case["layout"] == "half" else hip.ROTARY_INTERLEAVED)
     made = {"query": query.new_empty(b, t, h, d), "key": query.new_empty(b, t, hk, d)}
-    saved = query.new_empty(b * t * (h + hk))
+    saved = _scratch(state, "denominators", query, b * t * (h + hk))
     split = saved.data_ptr() + b * t * h * saved.element_size()
     parts = hip.head_norms(
         (made["query"].data_ptr(), _strides(made["query"]), saved.data_ptr(), query.data_ptr(),
@@ -384,7 +396,7 @@ def _own_norm(state):
             made[name + "_gradient"] = torch.empty_like(like)
             made[name + "_weight_gradient"] = query.new_empty(d)
         need = hip.head_norm_rotary_workspace(b, t, h + hk, d, dtype)
-        workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
+        workspace = _scratch(state, "backward", query, need, torch.uint8)
         gradients = hip.head_norm_gradients(
             (made["query_gradient"].data_ptr(), _strides(made["query_gradient"]),
              made["query_weight_gradient"].data_ptr(), state["query_gradient"].data_ptr(),
@@ -418,9 +430,9 @@ def _own_attention(state):
                           None if lengths is None else lengths.data_ptr(), hip.INT32,
                           hip.dtype_tag(case["dtype"]))
     output = torch.empty_like(query)
-    saved = query.new_empty(b, h, t) if case["train"] else None
+    saved = _scratch(state, "logsumexp", query, b * h * t) if case["train"] else None
     need = hip.attention_workspace(shape, 0)
-    workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
+    workspace = _scratch(state, "forward", query, need, torch.uint8)
     key, value = cached(state["key"]), cached(state["value"])
     hip.call("spar_hip_launch_attention_forward", heads(output),
              None if saved is None else saved.data_ptr(), heads(query), key, value, shape,
@@ -428,7 +440,7 @@ def _own_attention(state):
     made = {"output": output}
     if case["train"]:
         need = hip.attention_workspace(shape, 1)
-        workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
+        workspace = _scratch(state, "backward", query, need, torch.uint8)
         made["query_gradient"] = torch.empty_like(query)
         made["key_gradient"] = torch.empty_like(state["key"])
         made["value_gradient"] = torch.empty_like(state["value"])
