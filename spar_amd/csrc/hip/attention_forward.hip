@@ -31,7 +31,9 @@ struct Results {
   Heads<T> output;
   T* logsumexp;
   T* part_output;  // [split][batch][query head][query][pitch]
-  T* part_weight;  // [split][batch][query head][query]: log2 of the sum
+  T* part_top;     // [split][batch][query head][query]: the row's base
+  T* part_total;   // the same: its sum.  Two numbers, since the sum is lost in the
+                   // rounding of a large base
   uint32_t splits;
   uint32_t pitch;     // the extent rounded up to whole pieces
   uint64_t all_rows;  // batch * query heads * queries
@@ -40,55 +42,21 @@ struct Results {
 // At most this many parts of a row: one for each thread that joins them.
 constexpr uint32_t kMostParts = kThreads;
 
-// A row's running softmax and output: weights are 2^(score - base), `total` each
-// lane's own part of their sum.  Scores come with the base already taken off: their
-// product starts from `start`.  The base follows the row's maximum only when that has
-// grown by 2^kSlack, so that the output is rarely rescaled; sums of weights up to
-// 2^kSlack lose nothing in floating point.
-template <typename T, int DP>
-struct Row {
-  static constexpr int kSlack = 8;
-  typename Mma<T>::Acc start{0, 0, 0, 0};  // -base; the same in the row's four lanes
-  T limit = lowest<T>();  // of scores: kSlack, or the lowest before the first is seen
-  T total = T(0);
-  Along<T, DP> out;
-
-  // The base, and the lowest value where no score has been seen.
-  __device__ __forceinline__ T top() const { return limit == lowest<T>() ? limit : -start[0]; }
-
-  // Turns the scores of a block of keys into weights.
-  __device__ __forceinline__ void take(T (&score)[4]) {
-    T high = larger(larger(score[0], score[1]), larger(score[2], score[3]));
-    if (__any(high > limit)) {
-      high = quarter_max(high);
-      const bool grows = high > limit;
-      const T step = grows ? high : T(0);
-      const T shrink = limit == lowest<T>() ? T(1) : exp2_of(-step);
-      total *= shrink;
-      out.scale(shrink);
-      start -= step;
-      limit = grows ? T(kSlack) : limit;
-#pragma unroll
-      for (int v = 0; v < 4; ++v) score[v] -= step;
-    }
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      score[v] = exp2_of(score[v]);
-      total += score[v];
-    }
-  }
-};
+// ln of a sum of powers of two over a base; no sum where no key is seen.
+template <typename T>
+__device__ __forceinline__ T logsumexp_of(T top, T sum) {
+  return sum == T(0) ? lowest<T>() : (top + log2_of(sum)) * static_cast<T>(kLn2);
+}
 
 // Writes a finished row: `sum` is its whole total.
 template <typename T, int DP>
 __device__ __forceinline__ void write_row(const Call& call, const Results<T>& results, uint32_t b,
-                                          uint32_t key_head, uint32_t r, uint32_t split, T base,
+                                          uint32_t key_head, uint32_t r, uint32_t split, T top,
                                           T sum, const Along<T, DP>& out, int quarter) {
   if (r >= call.rows) return;
   const uint32_t t = call.group.div(r);
   const uint32_t head = key_head * call.group.divisor + (r - t * call.group.divisor);
   const T over = sum == T(0) ? T(0) : T(1) / sum;
-  const T weight = sum == T(0) ? lowest<T>() : base + log2_of(sum);
   const uint64_t row =
       (static_cast<uint64_t>(b) * call.key_heads * call.group.divisor + head) * call.queries + t;
   T* target;
@@ -96,12 +64,15 @@ __device__ __forceinline__ void write_row(const Call& call, const Results<T>& re
     target = results.output.data + b * results.output.batch + head * results.output.head +
              t * results.output.token;
     if (quarter == 0 && results.logsumexp != nullptr) {
-      results.logsumexp[row] = weight * static_cast<T>(kLn2);
+      results.logsumexp[row] = logsumexp_of(top, sum);
     }
   } else {
     const uint64_t at = split * results.all_rows + row;
     target = results.part_output + at * results.pitch;
-    if (quarter == 0) results.part_weight[at] = weight;
+    if (quarter == 0) {
+      results.part_top[at] = top;
+      results.part_total[at] = sum;
+    }
   }
   out.visit(quarter, [&](uint32_t d, auto& run) {
     for (auto& x : run) x *= over;
@@ -205,7 +176,7 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(
       if (!any) continue;
       const T* key_rows = keys.value[i % 2] + kb * kBlock * DP;
       const T* value_rows = values.value[i % 2] + kb * kBlock * DP;
-      typename Mma<T>::Acc s = row.start;
+      typename Mma<T>::Acc s{0, 0, 0, 0};
       const auto read = [&](int p) { return lane.along(key_rows, p); };
       Queue<2, typename Vec16<T>::type> queue;
       fill_queue(queue, read);
@@ -294,7 +265,7 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
     v.template load<READS>(call.extent, quarter, column, [&](int n) {
       return value_base + at_key(begin + n) * value.token;
     });
-    typename Mma<T>::Acc s = row.start;
+    typename Mma<T>::Acc s{0, 0, 0, 0};
 #pragma unroll
     for (int step = 0; step < DP / 4; ++step) {
       s = Mma<T>::step(k.value[step], q.value[step], s);
@@ -350,25 +321,27 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
     const uint32_t head = key_head * call.group.divisor + (out_row - t * call.group.divisor);
     const uint64_t place =
         (static_cast<uint64_t>(b) * call.key_heads * call.group.divisor + head) * call.queries + t;
-    const T weight = sum == T(0) ? lowest<T>() : base + log2_of(sum);
     T* target;
     if (results.splits == 1) {
       target = results.output.data + b * results.output.batch + head * results.output.head +
                t * results.output.token;
       if (d == 0 && results.logsumexp != nullptr) {
-        results.logsumexp[place] = weight * static_cast<T>(kLn2);
+        results.logsumexp[place] = logsumexp_of(base, sum);
       }
     } else {
       const uint64_t part = split * results.all_rows + place;
       target = results.part_output + part * results.pitch;
-      if (d == 0) results.part_weight[part] = weight;
+      if (d == 0) {
+        results.part_top[part] = top;
+        results.part_total[part] = sum;
+      }
     }
     store_piece(target, d, call.extent, run);
   }
 }
 
-// The parts of a row: o = sum 2^(w - top) o_part / sum 2^(w - top), w the log2 of a
-// part's sum.  Few parts: kLanes lanes side by side along a row's head take them in
+// The parts of a row: o = sum w o_part / sum w, w = 2^(part's base - largest base) times
+// the part's sum.  Few parts: kLanes lanes side by side along a row's head take them in
 // their order, all loaded before the first is used (16384 rows of 128 in 3 parts 7.5 us,
 // 256 rows of 64 in 8 parts 3 us).
 constexpr uint32_t kFewParts = 8;
@@ -384,12 +357,6 @@ __device__ __forceinline__ T* output_row(const Call& call, const Results<T>& res
          t * results.output.token;
 }
 
-// The larger, or a NaN (the weight of a row with a NaN score).
-template <typename T>
-__device__ __forceinline__ T top_of(T a, T b) {
-  return ((a > b) | (a != a)) ? a : b;
-}
-
 template <typename T>
 __global__ __launch_bounds__(kThreads) void combine_few_kernel(Call call, Results<T> results) {
   constexpr int W = Vec16<T>::width;
@@ -400,7 +367,7 @@ __global__ __launch_bounds__(kThreads) void combine_few_kernel(Call call, Result
   // All loads first, of the last part again where there are fewer.
   constexpr int kPieces = SPAR_HIP_ATTENTION_MAX_EXTENT / (kLanes * W);
   const uint32_t lane = threadIdx.x % kLanes;
-  T weight[kFewParts];
+  T weight[kFewParts], part_total[kFewParts];
   typename Vec16<T>::type piece[kFewParts];
   const auto part_of = [&](uint32_t s) {
     return (s < results.splits ? s : results.splits - 1) * results.all_rows + row;
@@ -413,19 +380,21 @@ __global__ __launch_bounds__(kThreads) void combine_few_kernel(Call call, Result
     }
   };
 #pragma unroll
-  for (uint32_t s = 0; s < kFewParts; ++s) weight[s] = results.part_weight[part_of(s)];
+  for (uint32_t s = 0; s < kFewParts; ++s) {
+    weight[s] = results.part_top[part_of(s)];
+    part_total[s] = results.part_total[part_of(s)];
+  }
   load(lane * W);
   T top = lowest<T>();
 #pragma unroll
   for (uint32_t s = 0; s < kFewParts; ++s) {
-    if (s >= results.splits) weight[s] = lowest<T>();
-    top = top_of(weight[s], top);
+    top = larger(weight[s], top);
   }
   const T base = top == lowest<T>() ? T(0) : top;
   T sum = T(0);
 #pragma unroll
   for (uint32_t s = 0; s < kFewParts; ++s) {
-    weight[s] = exp2_of(weight[s] - base);
+    weight[s] = s < results.splits ? exp2_of(weight[s] - base) * part_total[s] : T(0);
     sum += weight[s];
   }
   const T over = sum == T(0) ? T(0) : T(1) / sum;
@@ -446,8 +415,7 @@ __global__ __launch_bounds__(kThreads) void combine_few_kernel(Call call, Result
     store_piece(target, d, call.extent, run);
   }
   if (lane == 0 && results.logsumexp != nullptr) {
-    results.logsumexp[row] =
-        (sum == T(0) ? lowest<T>() : base + log2_of(sum)) * static_cast<T>(kLn2);
+    results.logsumexp[row] = logsumexp_of(base, sum);
   }
 }
 
@@ -463,20 +431,23 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(Call call, Results<T>
   __shared__ T waves[kWaves];
   const uint64_t row = blockIdx.x;
   const uint32_t split = threadIdx.x;
-  const T weight = split < results.splits ? results.part_weight[split * results.all_rows + row]
-                                          : lowest<T>();
-  T top = weight;
+  T part_top = lowest<T>(), part_total = T(0);
+  if (split < results.splits) {
+    part_top = results.part_top[split * results.all_rows + row];
+    part_total = results.part_total[split * results.all_rows + row];
+  }
+  T top = part_top;
 #pragma unroll
   for (int mask = kWave / 2; mask > 0; mask >>= 1) {
-    top = top_of(__shfl_xor(top, mask, kWave), top);
+    top = larger(__shfl_xor(top, mask, kWave), top);
   }
   if (threadIdx.x % kWave == 0) waves[threadIdx.x / kWave] = top;
   __syncthreads();
   top = waves[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) top = top_of(waves[w], top);
+  for (int w = 1; w < kWaves; ++w) top = larger(waves[w], top);
   const T base = top == lowest<T>() ? T(0) : top;
-  weights[split] = exp2_of(weight - base);
+  weights[split] = exp2_of(part_top - base) * part_total;
   __syncthreads();
   T sum = T(0);
   for (uint32_t s = 0; s < results.splits; ++s) sum += weights[s];
@@ -513,8 +484,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(Call call, Results<T>
   T* target = output_row(call, results, row);
   if (threadIdx.x < call.extent) target[threadIdx.x] = outs[0][threadIdx.x] * over;
   if (threadIdx.x == 0 && results.logsumexp != nullptr) {
-    results.logsumexp[row] =
-        (sum == T(0) ? lowest<T>() : base + log2_of(sum)) * static_cast<T>(kLn2);
+    results.logsumexp[row] = logsumexp_of(base, sum);
   }
 }
 static_assert(kThreads >= SPAR_HIP_ATTENTION_MAX_EXTENT);
@@ -575,7 +545,7 @@ Plan plan_of(const SparHipAttention& a) {
   const uint64_t piece = 16 / element_size(a);
   plan.pitch = static_cast<uint32_t>((a.extent + piece - 1) / piece * piece);
   if (plan.splits > 1) {
-    plan.bytes = plan.splits * plan.rows * (plan.pitch + 1) * element_size(a);
+    plan.bytes = plan.splits * plan.rows * (plan.pitch + 2) * element_size(a);
   }
   return plan;
 }
@@ -585,11 +555,12 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& outp
            void* logsumexp, const SparHipHeads& query, const SparHipHeads& key,
            const SparHipHeads& value, void* workspace, hipStream_t stream) {
   const Call call = call_of(a);
-  Results<T> results{heads_of<T>(output), static_cast<T*>(logsumexp), nullptr, nullptr,
+  Results<T> results{heads_of<T>(output), static_cast<T*>(logsumexp), nullptr, nullptr, nullptr,
                      plan.splits, plan.pitch, plan.rows};
   if (plan.splits > 1) {
     results.part_output = static_cast<T*>(workspace);
-    results.part_weight = results.part_output + plan.splits * plan.rows * plan.pitch;
+    results.part_top = results.part_output + plan.splits * plan.rows * plan.pitch;
+    results.part_total = results.part_top + plan.splits * plan.rows;
   }
   const uint32_t grid = plan.row_tiles * call.batch_heads * plan.splits;
   const auto q = heads_of<const T>(query), k = heads_of<const T>(key),
