@@ -705,9 +705,12 @@ struct SparHipStatus spar_hip_launch_attention_forward(
     const struct SparHipAttention* attention, void* workspace, uint64_t workspace_bytes,
     int device);
 
-/* Its backward from the saved output and logsumexp: the gradients of query, key
- * and value (zeros for queries that see nothing and for keys that no query
- * sees), sums in a fixed order.  A NaN or infinity in an input that takes part may
+/* Its backward from the saved output: the gradients of query, key and value (zeros
+ * for queries that see nothing and for keys that no query sees), sums in a fixed
+ * order.  The softmax's weights are formed from the scores again, their maximum and sum
+ * with them, so that they are right for scores of any size, where one rounded logsumexp
+ * would not do; `logsumexp`, as the forward left it, must be given but is not read.
+ * A NaN or infinity in an input that takes part may
  * reach every gradient of its key head and of the query heads that read it. */
 struct SparHipStatus spar_hip_launch_attention_backward(
     const struct SparHipHeads* query_gradient, const struct SparHipHeads* key_gradient,

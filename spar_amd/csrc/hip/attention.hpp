@@ -152,6 +152,11 @@ __device__ __forceinline__ T lowest() {
   return -static_cast<T>(__builtin_huge_val());
 }
 
+template <typename T>
+__device__ __forceinline__ T lowest_finite() {
+  return sizeof(T) == 4 ? static_cast<T>(-__FLT_MAX__) : static_cast<T>(-__DBL_MAX__);
+}
+
 // Sums and maxima over the four quarters of a wave, which hold one column's rows: the
 // halves and then the quarters of a half change places in registers, each lane
 // combining both.  A maximum passes over NaN.
@@ -438,6 +443,16 @@ struct Along {
   }
 };
 
+// 2^(base - next), of a row's old and new base.  A base is the score it was taken from
+// in float32, and that rounded up to a whole number in float64, where the power is then
+// an exponent: a second exponential in double would take 20 registers.
+__device__ __forceinline__ float base_of(float score) { return score; }
+__device__ __forceinline__ double base_of(double score) { return __builtin_ceil(score); }
+__device__ __forceinline__ float shrink_of(float base, float next) { return exp2_of(base - next); }
+__device__ __forceinline__ double shrink_of(double base, double next) {
+  return __builtin_ldexp(1.0, static_cast<int>(larger(base - next, -2000.0)));
+}
+
 // A row's running softmax, and its sum of weights times what the keys bring: weights are
 // 2^(score - base), `total` each lane's own part of their sum.  The base follows the
 // row's maximum only when that has grown by 2^kSlack, so that the sum is rarely
@@ -448,26 +463,20 @@ struct Along {
 template <typename T, int DP>
 struct Row {
   static constexpr int kSlack = 8;
-  T base = T(0);          // the same in the row's four lanes
-  T limit = lowest<T>();  // base + kSlack, or the lowest before the first score is seen
+  T base = lowest_finite<T>();  // the same in the row's four lanes; this before a score is seen
   T total = T(0);
   Along<T, DP> out;
-
-  // The base, and the lowest value where no score has been seen.
-  __device__ __forceinline__ T top() const { return limit == lowest<T>() ? limit : base; }
 
   // Turns the scores of a block of keys into weights.
   __device__ __forceinline__ void take(T (&score)[4]) {
     T high = larger(larger(score[0], score[1]), larger(score[2], score[3]));
-    if (__any(high > limit)) {
+    if (__any(high > base + T(kSlack))) {
       high = quarter_max(high);
-      const bool grows = high > limit;
-      const T next = grows ? high : base;
-      const T shrink = limit == lowest<T>() ? T(1) : exp2_of(base - next);
+      const T next = high > base + T(kSlack) ? base_of(high) : base;
+      const T shrink = shrink_of(base, next);
       total *= shrink;
       out.scale(shrink);
       base = next;
-      limit = grows ? next + T(kSlack) : limit;
     }
 #pragma unroll
     for (int v = 0; v < 4; ++v) {

@@ -1,16 +1,28 @@
-// Attention backward from the saved output and logsumexp: with P the weights,
-// dP = do v^T and delta = do . o per row,
+// Attention backward from the saved output: with P the weights, dP = do v^T and
+// delta = do . o per row,
 //   dS = P (dP - delta),  dq = scale dS k,  dk = scale dS^T q,  dv = P^T do.
 //
 // Two kernels (each in a form for large and one for small grids), so that every gradient
 // has one writer and sums in a fixed order.
 // query_kernel keeps 16 rows per wave and walks the keys they see (as the forward
-// does); it also leaves delta behind.  key_kernel keeps 16 keys per wave and walks
+// does, with the running maximum and sum of the softmax); it also leaves delta and the
+// softmax's base and sum behind.  key_kernel keeps 16 keys per wave and walks
 // the rows that see them, the heads of a group among them.  Each recomputes S and
 // dP: seven products instead of the five that one kernel with shared sums of dq
 // would need, for results that do not depend on the order of workgroups.  In both,
 // P and dS pass from the products that yield them into those that consume them in
 // registers (attention.hpp).
+//
+// Weights.  P = 2^(s - base) / sum with scores of the very same bits in both kernels, so
+// that a weight is at most 1 whatever a score's size.  (From the forward's logsumexp it
+// would be 2^(what rounding s and logsumexp has lost): off by 1e-4 at scores of 1000,
+// by half at 1e6, 0 or infinite from 1e9 on.)  The query is the one operand that both
+// kernels could not scale alike, resident in one and in LDS in the other: of
+// scale * log2(e) the power of two, exact in either operand, goes into the resident one
+// and the rest, between 1 and 2, is multiplied into the finished score.  Finding
+// maximum and sum again costs some 16 vector instructions a block in query_kernel and the
+// factors 8 in key_kernel: 229 against 223 us and 312 against 308 at heads of 64, 0.7%
+// of either at heads of 128.
 //
 // Rows of a tile of keys are split over several workgroups where the tiles alone do
 // not fill the chip; and the sinks, which every later row sees, have thousands of
@@ -20,6 +32,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "attention.hpp"
 
@@ -30,9 +43,23 @@ namespace {
 template <typename T>
 struct Saved {
   Heads<const T> query, key, value, output, output_gradient;
-  const T* logsumexp;  // [batch][query head][query]
-  T* delta;            // the same
+  T* statistics;  // [kStatistics][batch][query head][query]
+  T power, rest;  // scale * log2(e), its power of two and what remains
+
+  __device__ __forceinline__ T& of(int statistic, const Call& call, uint64_t row) const {
+    return statistics[statistic * call.all_rows() + row];
+  }
 };
+
+// Of a row: do . o, what its weights are powers of two over, and 1 / their sum (0 where
+// there is none).
+constexpr int kDelta = 0, kBase = 1, kOver = 2, kStatistics = 3;
+
+// 1 / a sum of weights.
+template <typename T>
+__device__ __forceinline__ T over_of(T sum) {
+  return sum == T(0) ? T(0) : T(1) / sum;
+}
 
 // How the rows of tiles of keys are split, and where the parts lie: of every tile's
 // window (none for one split), then of the rows behind the windows of the sinks' tiles.
@@ -81,9 +108,8 @@ struct Place {
 // What dq of a row is made from, as the row's four lanes hold it.
 template <typename T, int DP>
 struct QueryRow {
-  Operand<T, DP> q, g;  // scaled by scale * log2(e); the output gradient
+  Operand<T, DP> q, g;  // scaled by saved.power; the output gradient
   T delta = T(0);       // do . o
-  T log_sum;            // log2 of the row's sum
 
   template <Reads READS>
   __device__ __forceinline__ void load(const Call& call, const Saved<T>& saved,
@@ -92,8 +118,7 @@ struct QueryRow {
     q.template load<READS>(place.of(saved.query, b), call.extent, quarter);
     g.template load<READS>(place.of(saved.output_gradient, b), call.extent, quarter);
     out.template load<READS>(place.of(saved.output, b), call.extent, quarter);
-    log_sum = saved.logsumexp[place.at] * static_cast<T>(kLog2E);
-    q.finish(held, call.extent, quarter, static_cast<T>(call.scale * kLog2E));
+    q.finish(held, call.extent, quarter, saved.power);
     g.finish(held, call.extent, quarter, T(1));
 #pragma unroll
     for (int i = 0; i < DP / 4; ++i) delta += out.value[i] * g.value[i];
@@ -157,11 +182,10 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
   const uint32_t r = wave_row + column;
   const int32_t token = call.token(r, first);
   const Place place(call, b, key_head, r < call.rows ? r : 0);
-  QueryRow<T, DP> row;
-  row.template load<READS>(call, saved, place, b, token >= 0, quarter);
-  if (quarter == 0 && r < call.rows) saved.delta[place.at] = row.delta;
-  Along<T, DP> dq;
-  dq.clear();
+  QueryRow<T, DP> own;
+  own.template load<READS>(call, saved, place, b, token >= 0, quarter);
+  Row<T, DP> row;  // its sum is dq
+  row.out.clear();
   const T* key_base = saved.key.data + b * saved.key.batch + key_head * saved.key.head;
   const T* value_base = saved.value.data + b * saved.value.batch + key_head * saved.value.head;
 
@@ -204,30 +228,51 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
       const T* key_rows = keys.value[i % 2] + kb * kBlock * DP;
       const T* value_rows = values.value[i % 2] + kb * kBlock * DP;
       typename Mma<T>::Acc s{0, 0, 0, 0}, dp{0, 0, 0, 0};
-      products(lane, key_rows, row.q, s, value_rows, row.g, dp);
+      products(lane, key_rows, own.q, s, value_rows, own.g, dp);
       Across<T, DP> across(lane, key_rows);
-      T ds[4];
+      T weight[4], ds[4];
 #pragma unroll
-      for (int v = 0; v < 4; ++v) ds[v] = exp2_of(s[v] - row.log_sum) * (dp[v] - row.delta);
+      for (int v = 0; v < 4; ++v) {
+        weight[v] = s[v] * saved.rest;
+        ds[v] = dp[v] - own.delta;
+      }
       if (!whole) {
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
           const int32_t at = k0 + Mma<T>::row_of(v, quarter);
           const bool visible = (at < end) & call.sees(token, at);
+          weight[v] = visible ? weight[v] : lowest<T>();
           ds[v] = visible ? ds[v] : T(0);
         }
       }
-      across.run(dq, ds);
+      row.take(weight);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) ds[v] *= weight[v];
+      across.run(row.out, ds);
     }
     if (i + 1 < tiles) finish(i + 1);
   }
+  const T over = over_of(quarter_sum(row.total));
   if (r >= call.rows) return;
+  if (quarter == 0) {
+    saved.of(kDelta, call, place.at) = own.delta;
+    saved.of(kBase, call, place.at) = row.base;
+    saved.of(kOver, call, place.at) = over;
+  }
   T* target = place.of(gradient, b);
-  dq.visit(quarter, [&](uint32_t d, auto& run) {
-    for (auto& x : run) x *= static_cast<T>(call.scale);
+  row.out.visit(quarter, [&](uint32_t d, auto& run) {
+    for (auto& x : run) x = x * over * static_cast<T>(call.scale);
     store_piece(target, d, call.extent, run);
   });
 }
+
+// Parts of dq [split][batch][query head][query][extent], without the scale and the
+// weights' sum, and their bases and sums [split][batch][query head][query].
+template <typename T>
+struct QueryParts {
+  T *dq, *top, *total;
+  uint32_t splits;
+};
 
 // The same for grids that tiles of 64 rows do not fill: a workgroup's waves share 16
 // rows and take every fourth block of 16 keys, straight from memory; their sums meet
@@ -236,10 +281,12 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
 template <typename T, int DP, Reads READS>
 __global__ __launch_bounds__(kThreads) void query_spread_kernel(Call call, Saved<T> saved,
                                                                 Heads<T> gradient,
-                                                                uint32_t row_tiles, T* parts,
-                                                                uint32_t splits) {
+                                                                uint32_t row_tiles,
+                                                                QueryParts<T> parts) {
   constexpr int W = Vec16<T>::width;
   __shared__ alignas(16) T sums[kWaves][kBlock][DP + W];
+  __shared__ T tops[kWaves][kBlock], totals[kWaves][kBlock];
+  const uint32_t splits = parts.splits;
   const uint32_t batch_head = blockIdx.x % call.batch_heads;
   const uint32_t rest = blockIdx.x / call.batch_heads;
   uint32_t split = 0, row_tile = row_tiles - 1 - rest;
@@ -266,11 +313,13 @@ __global__ __launch_bounds__(kThreads) void query_spread_kernel(Call call, Saved
   const uint32_t r = begin_row + column;
   const int32_t token = call.token(r, first);
   const Place place(call, b, key_head, r < call.rows ? r : 0);
-  QueryRow<T, DP> row;
-  row.template load<READS>(call, saved, place, b, token >= 0, quarter);
-  if (split == 0 && wave == 0 && quarter == 0 && r < call.rows) saved.delta[place.at] = row.delta;
-  Along<T, DP> dq;
-  dq.clear();
+  QueryRow<T, DP> held;
+  held.template load<READS>(call, saved, place, b, token >= 0, quarter);
+  if (split == 0 && wave == 0 && quarter == 0 && r < call.rows) {
+    saved.of(kDelta, call, place.at) = held.delta;
+  }
+  Row<T, DP> row;
+  row.out.clear();
   const T* key_base = saved.key.data + b * saved.key.batch + key_head * saved.key.head;
   const T* value_base = saved.value.data + b * saved.value.batch + key_head * saved.value.head;
 
@@ -290,20 +339,28 @@ __global__ __launch_bounds__(kThreads) void query_spread_kernel(Call call, Saved
     typename Mma<T>::Acc s{0, 0, 0, 0}, dp{0, 0, 0, 0};
 #pragma unroll
     for (int step = 0; step < DP / 4; ++step) {
-      s = Mma<T>::step(k.value[step], row.q.value[step], s);
-      dp = Mma<T>::step(x.value[step], row.g.value[step], dp);
+      s = Mma<T>::step(k.value[step], held.q.value[step], s);
+      dp = Mma<T>::step(x.value[step], held.g.value[step], dp);
     }
-    T ds[4];
+    T weight[4], ds[4];
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const int32_t at = begin + Mma<T>::row_of(v, quarter);
       const bool visible = (at < end) & call.sees(token, at);
-      ds[v] = exp2_of(s[v] - row.log_sum) * (dp[v] - row.delta);
-      ds[v] = visible ? ds[v] : T(0);
+      weight[v] = visible ? s[v] * saved.rest : lowest<T>();
+      ds[v] = visible ? dp[v] - held.delta : T(0);
     }
-    across.add_to(dq, ds);
+    row.take(weight);
+#pragma unroll
+    for (int v = 0; v < 4; ++v) ds[v] *= weight[v];
+    across.add_to(row.out, ds);
   }
-  dq.visit(quarter, [&](uint32_t d, auto& run) {
+  const T total = quarter_sum(row.total);
+  if (quarter == 0) {
+    tops[wave][column] = row.base;
+    totals[wave][column] = total;
+  }
+  row.out.visit(quarter, [&](uint32_t d, auto& run) {
     for (auto& y : run) sums[wave][column][d++] = y;
   });
   __syncthreads();
@@ -311,45 +368,91 @@ __global__ __launch_bounds__(kThreads) void query_spread_kernel(Call call, Saved
   for (int at = threadIdx.x; at < kBlock * kPieces; at += kThreads) {
     const int c = at / kPieces, d = at % kPieces * W;
     if (begin_row + c >= call.rows) continue;
-    T run[W];
+    T top = tops[0][c];
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      run[j] = sums[0][c][d + j];
+    for (int w = 1; w < kWaves; ++w) top = larger(tops[w][c], top);
+      T sum = T(0);
+    T run[W] = {};
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) run[j] += sums[w][c][d + j];
-      run[j] *= static_cast<T>(call.scale);
+    for (int w = 0; w < kWaves; ++w) {
+      const T shrink = exp2_of(tops[w][c] - top);
+      sum += totals[w][c] * shrink;
+#pragma unroll
+      for (int j = 0; j < W; ++j) run[j] += sums[w][c][d + j] * shrink;
     }
     const Place to(call, b, key_head, begin_row + c);
-    T* target = splits == 1 ? to.of(gradient, b)
-                            : parts + (split * call.all_rows() + to.at) * call.extent;
-    store_piece(target, d, call.extent, run);
+    if (splits == 1) {
+      const T over = over_of(sum);
+      if (d == 0) {
+        saved.of(kBase, call, to.at) = top;
+        saved.of(kOver, call, to.at) = over;
+      }
+#pragma unroll
+      for (int j = 0; j < W; ++j) run[j] = run[j] * over * static_cast<T>(call.scale);
+      store_piece(to.of(gradient, b), d, call.extent, run);
+    } else {
+      const uint64_t part = split * call.all_rows() + to.at;
+      if (d == 0) {
+        parts.top[part] = top;
+        parts.total[part] = sum;
+      }
+      store_piece(parts.dq + part * call.extent, d, call.extent, run);
+    }
   }
 }
 
-// dq from its parts, in their order: a lane per element.
+// dq from its parts, in their order, and the row's base and sum: a lane per element.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void query_join_kernel(Call call, Heads<T> gradient,
-                                                              const T* parts, uint32_t splits) {
+__global__ __launch_bounds__(kThreads) void query_join_kernel(Call call, Saved<T> saved,
+                                                              Heads<T> gradient,
+                                                              QueryParts<T> parts) {
   const uint64_t at = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const uint64_t all = call.all_rows() * call.extent;
+  const uint64_t rows = call.all_rows(), all = rows * call.extent;
   if (at >= all) return;
-  T sum = parts[at];
-#pragma unroll 4
-  for (uint32_t s = 1; s < splits; ++s) sum += parts[s * all + at];
   const uint64_t row = at / call.extent, batch_head = row / call.queries;
+  T top = parts.top[row];
+#pragma unroll 4
+  for (uint32_t s = 1; s < parts.splits; ++s) top = larger(parts.top[s * rows + row], top);
+  T sum = T(0), total = T(0);
+#pragma unroll 4
+  for (uint32_t s = 0; s < parts.splits; ++s) {
+    const T shrink = exp2_of(parts.top[s * rows + row] - top);
+    total += parts.total[s * rows + row] * shrink;
+    sum += parts.dq[s * all + at] * shrink;
+  }
+  const T over = over_of(total);
+  if (at == row * call.extent) {
+    saved.of(kBase, call, row) = top;
+    saved.of(kOver, call, row) = over;
+  }
   const uint32_t heads = call.key_heads * call.group.divisor;
   const uint64_t b = batch_head / heads, head = batch_head - b * heads;
   gradient.data[b * gradient.batch + head * gradient.head +
                 (row - batch_head * call.queries) * gradient.token + (at - row * call.extent)] =
-      sum;
+      sum * over * static_cast<T>(call.scale);
+}
+
+// A token's bits as a value of the heads' type, and back.
+template <typename T>
+__device__ __forceinline__ T bits_of(int32_t token) {
+  if constexpr (sizeof(T) == 4) {
+    return __int_as_float(token);
+  } else {
+    return __longlong_as_double(token);
+  }
+}
+__device__ __forceinline__ int32_t token_of(float bits) { return __float_as_int(bits); }
+__device__ __forceinline__ int32_t token_of(double bits) {
+  return static_cast<int32_t>(__double_as_longlong(bits));
 }
 
 constexpr uint32_t kKeyTile = kWaves * kBlock;
 
-// Its operands and sums take a third more registers than the other kernels'.
-template <typename T, int DP>
+// Its operands and sums take a third more registers than the other kernels'; float32
+// tiles that go to LDS directly leave room for a fourth wave.
+template <typename T, int DP, Reads READS>
 constexpr int key_waves() {
-  return DP * sizeof(T) <= 256 ? 3 : DP * sizeof(T) <= 512 ? 2 : 1;
+  return DP * sizeof(T) <= 256 ? (sizeof(T) == 4 && READS == Reads::Aligned ? 4 : 3) : DP * sizeof(T) <= 512 ? 2 : 1;
 }
 
 // Blocks of 16 keys that share a tile's waves, for so many sinks in the tile.
@@ -431,13 +534,13 @@ struct KeyTile {
 // pair; two waves per SIMD, all that the two sums' registers leave room for): the calls
 // at query_kernel in 2.16 ms, 120 TFLOP/s, and 350 us, 87 TFLOP/s.
 template <typename T, int DP, int RB, Reads READS>
-__global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(
+__global__ __launch_bounds__(kThreads, (key_waves<T, DP, READS>())) void key_kernel(
     Call call, Saved<T> saved, Heads<T> key_gradient, Heads<T> value_gradient,
     Splits<T> splits) {
   constexpr int RT = RB * kBlock;
   __shared__ Tile<T, RT, DP, READS> queries, output_gradients;
-  __shared__ alignas(16) T log_sums[2][RT], deltas[2][RT];
-  __shared__ int32_t tokens[2][RT];
+  // Of the tile's rows, and their tokens' bits behind.
+  __shared__ alignas(16) T statistics[2][kStatistics + 1][RT];
   const KeyTile work(call, splits, kKeyTile);
   const uint32_t b = work.b, key_head = work.key_head;
   const bool behind = work.behind;
@@ -465,7 +568,7 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(
     const uint64_t at = static_cast<uint32_t>(own) < call.keys ? own : 0;
     k.template load<READS>(key_base + at * saved.key.token, call.extent, quarter);
     x.template load<READS>(value_base + at * saved.value.token, call.extent, quarter);
-    k.finish(keeps, call.extent, quarter, static_cast<T>(call.scale * kLog2E));
+    k.finish(keeps, call.extent, quarter, saved.power);
     x.finish(keeps, call.extent, quarter, T(1));
   }
   Along<T, DP> dk, dv;
@@ -474,8 +577,10 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(
 
   // Rows of a tile behind the last repeat the tile's first; their token sees nothing.
   typename Tile<T, RT, DP, READS>::Stage next_queries, next_gradients;
-  T next_log_sum, next_delta;
-  int32_t next_token;
+  // A thread brings one of a row's statistics, or its token.
+  static_assert((kStatistics + 1) * RT <= kThreads);
+  const uint32_t which = threadIdx.x / RT, its_row = threadIdx.x % RT;
+  T next_statistic;
   // Offsets of a tile's rows from the first head of the query of its first row,
   // `extra` heads behind which that row is.
   const uint32_t group = call.group.divisor;
@@ -494,12 +599,14 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(
                            [&](uint32_t j) { return offset(saved.output_gradient, j); });
   const auto start = [&](uint32_t i) {
     const uint32_t row0 = begin_row + i * RT;
-    if (threadIdx.x < RT) {
-      const bool row = row0 + threadIdx.x < end_row;
-      const Place place(call, b, key_head, row ? row0 + threadIdx.x : row0);
-      next_token = row ? first + static_cast<int32_t>(place.t) : -1;
-      next_log_sum = saved.logsumexp[place.at];
-      next_delta = saved.delta[place.at];
+    if (which <= kStatistics) {
+      const bool row = row0 + its_row < end_row;
+      const Place place(call, b, key_head, row ? row0 + its_row : row0);
+      if (which == kStatistics) {
+        next_statistic = bits_of<T>(row ? first + static_cast<int32_t>(place.t) : -1);
+      } else {
+        next_statistic = saved.of(which, call, place.at);
+      }
     }
     const uint32_t t0 = call.group.div(row0), extra = row0 - t0 * group;
     const bool whole = even && row0 + RT <= end_row;
@@ -511,11 +618,7 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(
                            [&](uint32_t j) { return offset(saved.output_gradient, at(j)); });
   };
   const auto finish = [&](uint32_t i) {
-    if (threadIdx.x < RT) {
-      tokens[i % 2][threadIdx.x] = next_token;
-      log_sums[i % 2][threadIdx.x] = next_log_sum * static_cast<T>(kLog2E);
-      deltas[i % 2][threadIdx.x] = next_delta;
-    }
+    if (which <= kStatistics) statistics[i % 2][which][its_row] = next_statistic;
     queries.finish(next_queries, i % 2);
     output_gradients.finish(next_gradients, i % 2);
   };
@@ -552,14 +655,15 @@ __global__ __launch_bounds__(kThreads, (key_waves<T, DP>())) void key_kernel(
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int row = rb * kBlock + Mma<T>::row_of(v, quarter);
-        p[v] = exp2_of(s[v] - log_sums[i % 2][row]);
-        ds[v] = p[v] * (dp[v] - deltas[i % 2][row]);
+        p[v] = exp2_of(s[v] * saved.rest - statistics[i % 2][kBase][row]) *
+               statistics[i % 2][kOver][row];
+        ds[v] = p[v] * (dp[v] - statistics[i % 2][kDelta][row]);
       }
       if (!whole) {
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const bool visible =
-              call.sees(tokens[i % 2][rb * kBlock + Mma<T>::row_of(v, quarter)], own);
+          const int row = rb * kBlock + Mma<T>::row_of(v, quarter);
+          const bool visible = call.sees(token_of(statistics[i % 2][kStatistics][row]), own);
           p[v] = visible ? p[v] : T(0);
           ds[v] = visible ? ds[v] : T(0);
         }
@@ -611,7 +715,7 @@ __global__ __launch_bounds__(kThreads) void key_spread_kernel(Call call, Saved<T
     x.template load<READS>(saved.value.data + b * saved.value.batch +
                                key_head * saved.value.head + at * saved.value.token,
                            call.extent, quarter);
-    k.finish(keeps, call.extent, quarter, static_cast<T>(call.scale * kLog2E));
+    k.finish(keeps, call.extent, quarter, saved.power);
     x.finish(keeps, call.extent, quarter, T(1));
   }
   Along<T, DP> dk, dv;
@@ -628,14 +732,15 @@ __global__ __launch_bounds__(kThreads) void key_spread_kernel(Call call, Saved<T
     Operand<T, DP> q, g;
     q.template load<READS>(read.of(saved.query, b), call.extent, quarter);
     g.template load<READS>(read.of(saved.output_gradient, b), call.extent, quarter);
-    T log_sum[4], delta[4];
+    T base[4], over[4], delta[4];
     int32_t token[4];
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const uint32_t j = Mma<T>::row_of(v, quarter);
       const Place place = place_of(j);
-      log_sum[v] = saved.logsumexp[place.at] * static_cast<T>(kLog2E);
-      delta[v] = saved.delta[place.at];
+      base[v] = saved.of(kBase, call, place.at);
+      over[v] = saved.of(kOver, call, place.at);
+      delta[v] = saved.of(kDelta, call, place.at);
       token[v] = row0 + j < end_row ? work.first + static_cast<int32_t>(place.t) : -1;
     }
     typename Mma<T>::Acc s{0, 0, 0, 0}, dp{0, 0, 0, 0};
@@ -648,7 +753,7 @@ __global__ __launch_bounds__(kThreads) void key_spread_kernel(Call call, Saved<T
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const bool visible = call.sees(token[v], own);
-      p[v] = exp2_of(s[v] - log_sum[v]);
+      p[v] = exp2_of(s[v] * saved.rest - base[v]) * over[v];
       ds[v] = p[v] * (dp[v] - delta[v]);
       p[v] = visible ? p[v] : T(0);
       ds[v] = visible ? ds[v] : T(0);
@@ -765,7 +870,8 @@ struct Plan {
   bool key_spread;  // key_spread_kernel
   uint32_t tile_keys;
   uint32_t row_tiles, key_tiles, main, sink_tiles, later;
-  uint64_t delta_bytes;  // a multiple of 16
+  uint64_t rows;             // batch * query heads * queries
+  uint64_t statistic_bytes;  // a multiple of 16
   uint64_t bytes;
 };
 
@@ -774,7 +880,7 @@ struct Plan {
 // chip busy several times over (their parts take memory).
 constexpr uint64_t kLaterShare = 2;
 constexpr uint64_t kMostLater = 256;
-constexpr uint64_t kMostLaterGroups = 2048;
+constexpr uint64_t kMostLaterGroups = 2000;
 // Workgroups that fill the chip, and the fewest rows that repay a part of either kernel:
 // two parts of 256 rows of key_spread_kernel (8 heads of 128) 15 + 9 us against 20 us
 // for one, of 348 float64 rows (heads of 72) 28 + 7 us against 38.
@@ -820,8 +926,8 @@ Plan plan_of(const SparHipAttention& a) {
   plan.tile_keys = plan.key_spread ? kBlock : kKeyTile;
   plan.key_tiles = ceil_div_u32(a.keys, plan.tile_keys);
   plan.main = 1;
-  plan.delta_bytes =
-      (a.batch * a.query_heads * a.queries * element + 15) / 16 * 16;
+  plan.rows = a.batch * a.query_heads * a.queries;
+  plan.statistic_bytes = (kStatistics * plan.rows * element + 15) / 16 * 16;
   const uint64_t fewest = plan.key_spread ? kFewestSpreadRows : kFewestRows;
   if (plan.key_tiles != 0) {
     plan.main = static_cast<uint32_t>(
@@ -845,26 +951,43 @@ Plan plan_of(const SparHipAttention& a) {
                          uint64_t{plan.sink_tiles} * plan.later;
   // The parts of dq and those of dk and dv take turns in one place.
   const uint64_t query_parts =
-      plan.query_splits > 1 ? plan.query_splits * a.batch * a.query_heads * a.queries : 0;
-  plan.bytes = plan.delta_bytes +
-               std::max(batch_heads * parts * 2 * plan.tile_keys, query_parts) * a.extent * element;
+      plan.query_splits > 1 ? plan.query_splits * plan.rows * (a.extent + 2) : 0;
+  plan.bytes = plan.statistic_bytes +
+               std::max(batch_heads * parts * 2 * plan.tile_keys * a.extent, query_parts) * element;
   return plan;
+}
+
+// scale * log2(e) as a power of two and a rest in [1, 2).
+template <typename T>
+void split_scale(double scale, T& power, T& rest) {
+  const T whole = static_cast<T>(scale * kLog2E);
+  power = whole;
+  rest = T(1);
+  if (whole == T(0) || !__builtin_isfinite(whole)) return;
+  int exponent;
+  rest = 2 * std::frexp(whole, &exponent);
+  power = std::ldexp(T(1), exponent - 1);
 }
 
 template <typename T>
 void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& query_gradient,
            const SparHipHeads& key_gradient, const SparHipHeads& value_gradient,
-           const SparHipHeads& output_gradient, const SparHipHeads& output, const void* logsumexp,
+           const SparHipHeads& output_gradient, const SparHipHeads& output,
            const SparHipHeads& query, const SparHipHeads& key, const SparHipHeads& value,
            void* workspace, hipStream_t stream) {
   const Call call = call_of(a);
-  const Saved<T> saved{heads_of<const T>(query), heads_of<const T>(key), heads_of<const T>(value),
-                       heads_of<const T>(output), heads_of<const T>(output_gradient),
-                       static_cast<const T*>(logsumexp), static_cast<T*>(workspace)};
+  Saved<T> saved{heads_of<const T>(query), heads_of<const T>(key), heads_of<const T>(value),
+                 heads_of<const T>(output), heads_of<const T>(output_gradient),
+                 static_cast<T*>(workspace), T(0), T(0)};
+  split_scale(a.scale, saved.power, saved.rest);
   const Heads<T> dk = heads_of<T>(key_gradient), dv = heads_of<T>(value_gradient);
   const Splits<T> splits{
-      reinterpret_cast<T*>(static_cast<char*>(workspace) + plan.delta_bytes), plan.tile_keys,
+      reinterpret_cast<T*>(static_cast<char*>(workspace) + plan.statistic_bytes),
+      plan.tile_keys,
       plan.key_tiles, plan.main, plan.sink_tiles, plan.later, call.extent};
+  T* const query_tops = splits.parts + plan.query_splits * plan.rows * a.extent;
+  const QueryParts<T> query_parts{splits.parts, query_tops,
+                                  query_tops + plan.query_splits * plan.rows, plan.query_splits};
   const uint32_t key_groups = plan.key_tiles * plan.main + plan.sink_tiles * plan.later;
   with_width<T>(a, {&output_gradient, &output, &query, &key, &value},
                 [&](auto width, auto reads) {
@@ -877,12 +1000,11 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& quer
       constexpr Reads kReads = READS == Reads::Aligned ? Reads::Pieces : READS;
       query_spread_kernel<T, DP, kReads>
           <<<plan.row_tiles * call.batch_heads * plan.query_splits, kThreads, 0, stream>>>(
-              call, saved, heads_of<T>(query_gradient), plan.row_tiles, splits.parts,
-              plan.query_splits);
+              call, saved, heads_of<T>(query_gradient), plan.row_tiles, query_parts);
       if (plan.query_splits > 1) {
         query_join_kernel<T>
             <<<ceil_div_u32(call.all_rows() * call.extent, kThreads), kThreads, 0, stream>>>(
-                call, heads_of<T>(query_gradient), splits.parts, plan.query_splits);
+                call, saved, heads_of<T>(query_gradient), query_parts);
       }
     } else if (call.rows != 0) {
       query_kernel<T, DP, kBlocks, READS>
@@ -976,11 +1098,11 @@ extern "C" SparHipStatus spar_hip_launch_attention_backward(
   if (enter(device, guard) != hipSuccess) return runtime(guard.error);
   if (a.dtype == SPAR_HIP_FLOAT32) {
     attention::start<float>(a, plan, *query_gradient, *key_gradient, *value_gradient,
-                            *output_gradient, *output, logsumexp, *query, *key, *value, workspace,
+                            *output_gradient, *output, *query, *key, *value, workspace,
                             guard.stream);
   } else {
     attention::start<double>(a, plan, *query_gradient, *key_gradient, *value_gradient,
-                             *output_gradient, *output, logsumexp, *query, *key, *value, workspace,
+                             *output_gradient, *output, *query, *key, *value, workspace,
                              guard.stream);
   }
   return finish(guard);

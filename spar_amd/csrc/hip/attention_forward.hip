@@ -203,7 +203,7 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(
     }
     if (i + 1 < end_tile) finish(i + 1);
   }
-  write_row(call, results, b, key_head, r, split, row.top(), quarter_sum(row.total), row.out,
+  write_row(call, results, b, key_head, r, split, row.base, quarter_sum(row.total), row.out,
             lane.quarter);
 }
 
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
   }
   const T total = quarter_sum(row.total);
   if (quarter == 0) {
-    tops[wave][column] = row.top();
+    tops[wave][column] = row.base;
     totals[wave][column] = total;
   }
   row.out.visit(quarter, [&](uint32_t d, auto& run) {
@@ -303,13 +303,12 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
     if (out_row >= call.rows) continue;
     T top = tops[0][c];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = tops[w][c] > top ? tops[w][c] : top;
-    const T base = top == lowest<T>() ? T(0) : top;
-    T sum = T(0);
+    for (int w = 1; w < kWaves; ++w) top = larger(tops[w][c], top);
+      T sum = T(0);
     T run[W] = {};
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const T shrink = exp2_of(tops[w][c] - base);
+      const T shrink = exp2_of(tops[w][c] - top);
       sum += totals[w][c] * shrink;
 #pragma unroll
       for (int j = 0; j < W; ++j) run[j] += outs[w][c][d + j] * shrink;
@@ -326,7 +325,7 @@ __global__ __launch_bounds__(kThreads) void token_kernel(Call call, Results<T> r
       target = results.output.data + b * results.output.batch + head * results.output.head +
                t * results.output.token;
       if (d == 0 && results.logsumexp != nullptr) {
-        results.logsumexp[place] = logsumexp_of(base, sum);
+        results.logsumexp[place] = logsumexp_of(top, sum);
       }
     } else {
       const uint64_t part = split * results.all_rows + place;
@@ -385,16 +384,15 @@ __global__ __launch_bounds__(kThreads) void combine_few_kernel(Call call, Result
     part_total[s] = results.part_total[part_of(s)];
   }
   load(lane * W);
-  T top = lowest<T>();
+  T top = lowest_finite<T>();
 #pragma unroll
   for (uint32_t s = 0; s < kFewParts; ++s) {
     top = larger(weight[s], top);
   }
-  const T base = top == lowest<T>() ? T(0) : top;
   T sum = T(0);
 #pragma unroll
   for (uint32_t s = 0; s < kFewParts; ++s) {
-    weight[s] = s < results.splits ? exp2_of(weight[s] - base) * part_total[s] : T(0);
+    weight[s] = s < results.splits ? exp2_of(weight[s] - top) * part_total[s] : T(0);
     sum += weight[s];
   }
   const T over = sum == T(0) ? T(0) : T(1) / sum;
@@ -415,7 +413,7 @@ __global__ __launch_bounds__(kThreads) void combine_few_kernel(Call call, Result
     store_piece(target, d, call.extent, run);
   }
   if (lane == 0 && results.logsumexp != nullptr) {
-    results.logsumexp[row] = logsumexp_of(base, sum);
+    results.logsumexp[row] = logsumexp_of(top, sum);
   }
 }
 
@@ -431,7 +429,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(Call call, Results<T>
   __shared__ T waves[kWaves];
   const uint64_t row = blockIdx.x;
   const uint32_t split = threadIdx.x;
-  T part_top = lowest<T>(), part_total = T(0);
+  T part_top = lowest_finite<T>(), part_total = T(0);
   if (split < results.splits) {
     part_top = results.part_top[split * results.all_rows + row];
     part_total = results.part_total[split * results.all_rows + row];
@@ -446,8 +444,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(Call call, Results<T>
   top = waves[0];
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) top = larger(waves[w], top);
-  const T base = top == lowest<T>() ? T(0) : top;
-  weights[split] = exp2_of(part_top - base) * part_total;
+  weights[split] = exp2_of(part_top - top) * part_total;
   __syncthreads();
   T sum = T(0);
   for (uint32_t s = 0; s < results.splits; ++s) sum += weights[s];
@@ -484,7 +481,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(Call call, Results<T>
   T* target = output_row(call, results, row);
   if (threadIdx.x < call.extent) target[threadIdx.x] = outs[0][threadIdx.x] * over;
   if (threadIdx.x == 0 && results.logsumexp != nullptr) {
-    results.logsumexp[row] = logsumexp_of(base, sum);
+    results.logsumexp[row] = logsumexp_of(top, sum);
   }
 }
 static_assert(kThreads >= SPAR_HIP_ATTENTION_MAX_EXTENT);
