@@ -316,10 +316,15 @@ struct Tile {
                                (__attribute__((address_space(3))) T*)(value[to]))) +
                            wave * kWave * 16;
       const auto load = [&](int j, uint32_t offset) {
+// m0 is named, although the compiler does not give it out and warns of it: it
+// writes it for instructions of its own.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                      :
                      : "s"(lds + j * kThreads * 16), "v"(offset), "s"(base)
-                     : "memory");
+                     : "memory", "m0");
+#pragma clang diagnostic pop
       };
       if (whole) {
 #pragma unroll
