@@ -58,6 +58,18 @@ def kernels(tmp_path_factory):
     return {name: code for name, code in found.items() if "attention" in name}
 
 
+def test_no_masked_block_is_empty(kernels):
+    """A short-circuited condition that selects between a matrix product's result and a
+    constant has been compiled to a block that saves and restores the mask of lanes around
+    nothing: the selected value was always the constant.  None of the kernels has one."""
+    assert any("tile_kernel" in name for name in kernels)
+    assert any("key_kernel" in name for name in kernels)
+    for name, code in kernels.items():
+        for first, second in zip(code, code[1:]):
+            saves = re.match(r"s_(and|or|andn2)_saveexec_b64|s_and_b64 exec", first)
+            assert not (saves and re.match(r"s_(or|mov)_b64 exec", second)), (name, first, second)
+
+
 def test_m0_is_written_by_the_loads_to_lds_alone(kernels):
     for name, code in kernels.items():
         for i, instruction in enumerate(code):
