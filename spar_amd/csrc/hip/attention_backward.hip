@@ -796,21 +796,27 @@ __global__ __launch_bounds__(kThreads) void key_spread_kernel(Call call, Saved<T
   join(dv, false, T(1));
 }
 
-// dk and dv of the first `keys` keys from their parts in a fixed order: eight lanes to
-// an element take every eighth part each, and their sums meet in a tree (4 to 7 us).
+// dk and dv of the first `keys` keys from their parts in a fixed order, of a launch's
+// elements from `first` on: eight lanes to an element take every eighth part each, and
+// their sums meet in a tree (4 to 7 us).
+constexpr uint32_t kJoinRuns = 8;
+constexpr uint64_t kJoinGroups = uint64_t{1} << 22;  // of a launch
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_kernel(Call call, Heads<T> key_gradient,
                                                         Heads<T> value_gradient,
-                                                        Splits<T> splits, uint32_t keys) {
-  constexpr uint32_t kRuns = 8, kLanes = kThreads / kRuns;
+                                                        Splits<T> splits, uint32_t keys,
+                                                        uint64_t first) {
+  constexpr uint32_t kRuns = kJoinRuns, kLanes = kThreads / kRuns;
   __shared__ T sums[2][kRuns][kLanes];
   const uint32_t lane = threadIdx.x % kLanes, run = threadIdx.x / kLanes;
   const uint64_t per_head = static_cast<uint64_t>(keys) * call.extent;
-  const uint64_t at = static_cast<uint64_t>(blockIdx.x) * kLanes + lane;
+  const uint64_t at = first + static_cast<uint64_t>(blockIdx.x) * kLanes + lane;
   const bool inside = at < per_head * call.batch_heads;
   const uint32_t batch_head = inside ? static_cast<uint32_t>(at / per_head) : 0;
-  const uint32_t within = inside ? static_cast<uint32_t>(at - batch_head * per_head) : 0;
-  const uint32_t key = within / call.extent, d = within % call.extent;
+  const uint64_t within = inside ? at - batch_head * per_head : 0;  // may pass 32 bits
+  const uint32_t key = static_cast<uint32_t>(within / call.extent);
+  const uint32_t d = static_cast<uint32_t>(within - static_cast<uint64_t>(key) * call.extent);
   const uint32_t b = batch_head / call.key_heads, key_head = batch_head % call.key_heads;
   const bool spread = splits.tile_keys == kBlock;
   const uint32_t tile = spread ? key / kBlock : key / kKeyTile;
@@ -1025,18 +1031,17 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& quer
   const uint32_t joined = plan.main > 1     ? call.keys
                           : plan.later != 0 ? static_cast<uint32_t>(std::min(a.sinks, a.keys))
                                             : 0;
-  if (joined != 0) {
-    join_kernel<T><<<ceil_div_u32(static_cast<uint64_t>(call.batch_heads) * joined * a.extent,
-                                  kThreads / 8),
-                     kThreads, 0, stream>>>(call, dk, dv, splits, joined);
+  const uint64_t elements = static_cast<uint64_t>(call.batch_heads) * joined * a.extent;
+  constexpr uint64_t kLaunch = kJoinGroups * (kThreads / kJoinRuns);
+  for (uint64_t at = 0; at < elements; at += kLaunch) {
+    join_kernel<T><<<ceil_div_u32(std::min(kLaunch, elements - at), kThreads / kJoinRuns),
+                     kThreads, 0, stream>>>(call, dk, dv, splits, joined, at);
   }
 }
 
 bool fits(const SparHipAttention& a, const Plan& plan) {
   const uint64_t batch_heads = a.batch * a.key_heads;
-  return batch_heads * std::min(a.keys, plan.main > 1 ? a.keys : a.sinks) <=
-             kIndex32Limit / a.extent * (kThreads / 8) &&
-         (static_cast<uint64_t>(plan.key_tiles) * plan.main +
+  return (static_cast<uint64_t>(plan.key_tiles) * plan.main +
           static_cast<uint64_t>(plan.sink_tiles) * plan.later) * batch_heads <= kIndex32Limit &&
          static_cast<uint64_t>(plan.row_tiles) * batch_heads <= kIndex32Limit;
 }
