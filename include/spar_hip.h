@@ -204,7 +204,9 @@ struct SparHipHeadNormGradient {
  * sequence b is its token p = length(b) - queries + i, length(b) = lengths[b]
  * clamped to [0, keys] (keys where lengths is NULL), and sees key j when
  *   j <= p  and  (window == 0  or  p - j < window  or  j < sinks);
- * queries with p < 0 see nothing. */
+ * queries with p < 0 see nothing.  Calls of 2^24 workgroups or more are refused: one
+ * for each key head of a sequence and every 64 queries of its heads or keys, or 16
+ * where they are few. */
 struct SparHipAttention {
   uint64_t batch;
   uint64_t query_heads;

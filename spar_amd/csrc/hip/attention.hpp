@@ -76,6 +76,10 @@ Heads<T> heads_of(const SparHipHeads& heads) {
 constexpr uint64_t kMostKeys = uint64_t{1} << 30;
 constexpr int32_t kNoWindow = 1 << 30;
 
+// Workgroups of a launch: its work-items are counted in 32 bits, and those behind are
+// dropped without an error.
+constexpr uint64_t kMostGroups = (uint64_t{1} << 32) / kThreads - 1;
+
 // The shape of a call, as the kernels take it.
 struct Call {
   const void* lengths;

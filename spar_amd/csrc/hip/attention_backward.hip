@@ -1042,8 +1042,8 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& quer
 bool fits(const SparHipAttention& a, const Plan& plan) {
   const uint64_t batch_heads = a.batch * a.key_heads;
   return (static_cast<uint64_t>(plan.key_tiles) * plan.main +
-          static_cast<uint64_t>(plan.sink_tiles) * plan.later) * batch_heads <= kIndex32Limit &&
-         static_cast<uint64_t>(plan.row_tiles) * batch_heads <= kIndex32Limit;
+          static_cast<uint64_t>(plan.sink_tiles) * plan.later) * batch_heads <= kMostGroups &&
+         static_cast<uint64_t>(plan.row_tiles) * batch_heads * plan.query_splits <= kMostGroups;
 }
 
 }  // namespace

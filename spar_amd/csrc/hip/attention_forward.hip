@@ -607,7 +607,7 @@ extern "C" SparHipStatus spar_hip_launch_attention_forward(
   }
   const attention::Plan plan = attention::plan_of(a);
   if (static_cast<uint64_t>(plan.row_tiles) * a.batch * a.key_heads * plan.splits >
-          kIndex32Limit ||
+          attention::kMostGroups ||
       (plan.bytes != 0 &&
        (workspace == nullptr || workspace_bytes < plan.bytes || !aligned16(workspace)))) {
     return invalid();
