@@ -339,17 +339,18 @@ __global__ __launch_bounds__(kThreads) void norm_forward_kernel(NormParts<T> par
   if (u < units) unit = unit_at<HALF>(u, turn.half, turn.extent);
   const bool other = group >= first_groups;
   const NormPart<T>& part = parts.part[other ? 1 : 0];
-  const uint32_t heads = parts.heads[other ? 1 : 0];
+  const uint32_t heads = other ? parts.heads[1] : parts.heads[0];
   const uint32_t groups = other ? by_groups.divisor - first_groups : first_groups;
   if (other) group -= first_groups;
   const T* source = part.input.data + b * part.input.batch + t * part.input.token;
   T* target = part.output.data + b * part.output.batch + t * part.output.token;
   T x[K][8], w[8];
-  // A head behind the last is read as the last, and not written.
+  // In the place of a head behind the last the first of these is read, and not written:
+  // any other may be written meanwhile, where the output is the input itself.
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const uint32_t head = group + k * groups;
-    load_unit<T, NT>(x[k], source + (head < heads ? head : heads - 1) * part.input.head, unit);
+    load_unit<T, NT>(x[k], source + (head < heads ? head : group) * part.input.head, unit);
   }
   load_unit<T, false>(w, part.weight, unit);
   T c[4], s[4];
@@ -433,7 +434,8 @@ __global__ __launch_bounds__(kThreads, 3) void norm_backward_kernel(NormGradient
     T x[K][8], g[K][8], over[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const uint32_t head = group + k * groups < heads ? group + k * groups : heads - 1;
+      // As in the forward: a head behind the last is the first of these.
+      const uint32_t head = group + k * groups < heads ? group + k * groups : group;
       load_unit<T, NT>(x[k], source + head * part.input.head, unit);
       load_unit<T, NT>(g[k], gradient + head * part.output_gradient.head, unit);
       over[k] = part.denominator[(b * heads + head) * rows.tokens + t];
