@@ -81,7 +81,8 @@ struct RotaryScaling final {
 ///   scale    1 / sqrt(extent) where not given
 ///   lengths  Int32 or Int64 [batch], the tokens of each sequence in the keys,
 ///            clamped to [0, keys]; all keys where not given.  Keys and values
-///            behind them are not read.
+///            behind them have no part in any result, whatever they hold (their
+///            memory may be read).
 /// A query or key of another sequence or head never changes a result; a NaN or
 /// infinity in a key or value that some query of its head sees may also reach
 /// other queries of that head, and one in any input that takes part the gradients
