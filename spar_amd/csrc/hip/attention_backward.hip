@@ -266,6 +266,11 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
   });
 }
 
+// The spread kernels' operands and sums stay in registers up to this many bytes of a head
+// (key_spread_kernel for 4 heads of 160 with 210 float64 tokens 81 us against key_kernel's
+// 65).
+constexpr uint64_t kMostSpreadBytes = 1024;
+
 // Parts of dq [split][batch][query head][query][extent], without the scale and the
 // weights' sum, and their bases and sums [split][batch][query head][query].
 template <typename T>
@@ -284,6 +289,10 @@ __global__ __launch_bounds__(kThreads) void query_spread_kernel(Call call, Saved
                                                                 uint32_t row_tiles,
                                                                 QueryParts<T> parts) {
   constexpr int W = Vec16<T>::width;
+  // A block's keys, values and keys again are asked for at once where registers hold them,
+  // and eight pieces at a time where not (4 heads of 160 with 210 float64
+  // tokens: forward and backward 153 us against 181).
+  constexpr bool kTogether = DP * sizeof(T) <= kMostSpreadBytes;
   __shared__ alignas(16) T sums[kWaves][kBlock][DP + W];
   __shared__ T tops[kWaves][kBlock], totals[kWaves][kBlock];
   const uint32_t splits = parts.splits;
@@ -329,18 +338,36 @@ __global__ __launch_bounds__(kThreads) void query_spread_kernel(Call call, Saved
     // Keys behind the run repeat its block's first; no row sees them.
     const auto at_key = [&](int32_t k) { return static_cast<uint64_t>(k < end ? k : begin); };
     const uint64_t own = at_key(begin + column);
-    Operand<T, DP> k, x;
-    AcrossOperand<T, DP> across;
-    k.template load<READS>(key_base + own * saved.key.token, call.extent, quarter);
-    x.template load<READS>(value_base + own * saved.value.token, call.extent, quarter);
-    across.template load<READS>(call.extent, quarter, column, [&](int n) {
-      return key_base + at_key(begin + n) * saved.key.token;
-    });
     typename Mma<T>::Acc s{0, 0, 0, 0}, dp{0, 0, 0, 0};
+    AcrossOperand<T, DP> across;
+    const auto load_across = [&]() {
+      across.template load<READS>(call.extent, quarter, column, [&](int n) {
+        return key_base + at_key(begin + n) * saved.key.token;
+      });
+    };
+    if constexpr (kTogether) {
+      Operand<T, DP> k, x;
+      k.template load<READS>(key_base + own * saved.key.token, call.extent, quarter);
+      x.template load<READS>(value_base + own * saved.value.token, call.extent, quarter);
+      load_across();
 #pragma unroll
-    for (int step = 0; step < DP / 4; ++step) {
-      s = Mma<T>::step(k.value[step], held.q.value[step], s);
-      dp = Mma<T>::step(x.value[step], held.g.value[step], dp);
+      for (int step = 0; step < DP / 4; ++step) {
+        s = Mma<T>::step(k.value[step], held.q.value[step], s);
+        dp = Mma<T>::step(x.value[step], held.g.value[step], dp);
+      }
+    } else {
+      const auto product = [&](const T* head, const Operand<T, DP>& with,
+                               typename Mma<T>::Acc& sum) {
+#pragma unroll
+        for (int n = 0; n < DP / (4 * W); ++n) {
+          const auto piece = load_piece<READS>(head, 4 * W * n + W * quarter, call.extent);
+#pragma unroll
+          for (int w = 0; w < W; ++w) sum = Mma<T>::step(piece[w], with.value[n * W + w], sum);
+          if (READS != Reads::Single && n % 8 == 7) keep_order();
+        }
+      };
+      product(key_base + own * saved.key.token, held.q, s);
+      product(value_base + own * saved.value.token, held.g, dp);
     }
     T weight[4], ds[4];
 #pragma unroll
@@ -353,6 +380,7 @@ __global__ __launch_bounds__(kThreads) void query_spread_kernel(Call call, Saved
     row.take(weight);
 #pragma unroll
     for (int v = 0; v < 4; ++v) ds[v] *= weight[v];
+    if constexpr (!kTogether) load_across();
     across.add_to(row.out, ds);
   }
   const T total = quarter_sum(row.total);
@@ -904,9 +932,6 @@ constexpr uint64_t kFewestQueryKeys = 384;
 // heads, each for 4 heads of 128, with 1024 keys and 256 tokens 42 and 46 us; 8 such key
 // heads with 512 tokens 81 and 103 us.
 constexpr uint64_t kMostSpreadRows = 4;
-// Its operands and sums stay in registers up to this many bytes of a head (4 heads of 160
-// with 210 float64 tokens 81 us against 65).
-constexpr uint64_t kMostSpreadBytes = 1024;
 
 Plan plan_of(const SparHipAttention& a) {
   Plan plan{};
