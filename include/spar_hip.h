@@ -699,8 +699,10 @@ struct SparHipStatus spar_hip_attention_workspace(uint64_t* bytes,
  * [batch, query_heads, queries], contiguous, is kept for the backward (-inf where
  * no key is seen); it may be NULL.  Keys and values that no query sees are not
  * used, whatever they hold; a NaN or infinity in one that some query sees may also
- * reach other queries that read its key head.  Replaces the reference's scores, mask
- * and softmax over whole [queries, keys] matrices (nn/attention.cpp:122-135). */
+ * reach other queries that read its key head.  Weights are divided by their sum after
+ * the product and may reach 2^8 before: the visible values times 2^8 must add up to a
+ * finite number of the dtype.  Replaces the reference's scores, mask and softmax over
+ * whole [queries, keys] matrices (nn/attention.cpp:122-135). */
 struct SparHipStatus spar_hip_launch_attention_forward(
     const struct SparHipHeads* output, void* logsumexp, const struct SparHipHeads* query,
     const struct SparHipHeads* key, const struct SparHipHeads* value,
@@ -712,8 +714,9 @@ struct SparHipStatus spar_hip_launch_attention_forward(
  * order.  The softmax's weights are formed from the scores again, their maximum and sum
  * with them, so that they are right for scores of any size, where one rounded logsumexp
  * would not do; `logsumexp`, as the forward left it, must be given but is not read.
- * A NaN or infinity in an input that takes part may
- * reach every gradient of its key head and of the query heads that read it. */
+ * A NaN or infinity in an input that takes part may reach every gradient of its key
+ * head and of the query heads that read it.  The sums of dq are divided as the output's
+ * are, and have the same bound. */
 struct SparHipStatus spar_hip_launch_attention_backward(
     const struct SparHipHeads* query_gradient, const struct SparHipHeads* key_gradient,
     const struct SparHipHeads* value_gradient, const struct SparHipHeads* output_gradient,

@@ -41,9 +41,8 @@ template <typename T> struct Mma;
 // float32 reaches 154 TFLOP/s, twice what the vector units do without packed
 // instructions; products and sums are IEEE single.  Vector instructions of any wave
 // take their time, 4 cycles each, from the same pipeline (one per matrix instruction
-// leaves 138 TFLOP/s, two 124), so the kernels count them: products start from what
-// would be subtracted from them, masks are formed for tiles at an edge alone, and
-// addresses move in scalar registers.
+// leaves 138 TFLOP/s, two 124), so the kernels count them: masks are formed for
+// tiles at an edge alone, and addresses move in scalar registers.
 template <> struct Mma<float> {
   using Acc = f32x4;
   __device__ static __forceinline__ Acc step(float a, float b, Acc c) {

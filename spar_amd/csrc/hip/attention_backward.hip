@@ -150,11 +150,11 @@ __device__ __forceinline__ void products(const Lane<T, DP>& lane, const T* a_row
 }
 
 // dq and delta of 64 rows, 16 per wave, over tiles of the keys they see.  Bound by the
-// matrix units, busy 86% of the time at heads of 128 (6 extent operations per visible
-// pair): 32 heads of 128 with 8192 tokens, window 1024 and 4 sinks in 1.49 ms,
-// 131 TFLOP/s of visible pairs; 256 heads of 64 with 1024 tokens and window 256 in
-// 255 us, 90 TFLOP/s, where the blocks of 16 keys that the window's edges cut and a
-// block of sinks are a tenth of the work and the vector instructions weigh twice as much.
+// matrix units, busy in 88% of the CUs' cycles at heads of 128 (6 extent operations per
+// visible pair): 32 heads of 128 with 8192 tokens, window 1024 and 4 sinks in 1.49 ms,
+// 130 TFLOP/s of visible pairs; 256 heads of 64 with 1024 tokens and window 256 in
+// 228 us, 100 TFLOP/s and 73%, where the blocks of 16 keys that the window's edges cut and
+// a block of sinks are a tenth of the work and the vector instructions weigh twice as much.
 template <typename T, int DP, int KB, Reads READS>
 __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void query_kernel(
     Call call, Saved<T> saved, Heads<T> gradient, uint32_t row_tiles) {
@@ -281,7 +281,7 @@ struct QueryParts {
 
 // The same for grids that tiles of 64 rows do not fill: a workgroup's waves share 16
 // rows and take every fourth block of 16 keys, straight from memory; their sums meet
-// in LDS.  18 heads of 72 with 333 float64 tokens and a window of 100 in 20 us, five
+// in LDS.  18 heads of 72 with 333 float64 tokens and a window of 100 in 23 us, five
 // blocks a wave with the latency of their loads (query_kernel: 31 us).
 template <typename T, int DP, Reads READS>
 __global__ __launch_bounds__(kThreads) void query_spread_kernel(Call call, Saved<T> saved,
@@ -480,7 +480,9 @@ constexpr uint32_t kKeyTile = kWaves * kBlock;
 // tiles that go to LDS directly leave room for a fourth wave.
 template <typename T, int DP, Reads READS>
 constexpr int key_waves() {
-  return DP * sizeof(T) <= 256 ? (sizeof(T) == 4 && READS == Reads::Aligned ? 4 : 3) : DP * sizeof(T) <= 512 ? 2 : 1;
+  constexpr int row = DP * sizeof(T);
+  if (row <= 256) return sizeof(T) == 4 && READS == Reads::Aligned ? 4 : 3;
+  return row <= 512 ? 2 : 1;
 }
 
 // Blocks of 16 keys that share a tile's waves, for so many sinks in the tile.
@@ -558,9 +560,9 @@ struct KeyTile {
 };
 
 // dk and dv of 64 keys, 16 per wave, over tiles of the rows that see them.  Bound by the
-// matrix units, busy 77% of the time at heads of 128 (8 extent operations per visible
-// pair; two waves per SIMD, all that the two sums' registers leave room for): the calls
-// at query_kernel in 2.16 ms, 120 TFLOP/s, and 350 us, 87 TFLOP/s.
+// matrix units, busy in 81% of the CUs' cycles at heads of 128 (8 extent operations per
+// visible pair; two waves per SIMD, all that the two sums' registers leave room for): the calls
+// at query_kernel in 2.18 ms, 119 TFLOP/s, and 311 us, 98 TFLOP/s and 70%.
 template <typename T, int DP, int RB, Reads READS>
 __global__ __launch_bounds__(kThreads, (key_waves<T, DP, READS>())) void key_kernel(
     Call call, Saved<T> saved, Heads<T> key_gradient, Heads<T> value_gradient,

@@ -94,11 +94,11 @@ __device__ __forceinline__ const T* head_row(const Heads<const T>& heads, const 
 // a multiple of the 8 dies in common sizes, so that they share a die's cache; the
 // last rows, which see most, come first.  A wave passes over blocks of 16 keys that none
 // of its rows sees, and forms masks only for those that an edge of the window, of the
-// sinks or of the diagonal cuts.  The matrix units are busy 83% of the time at heads of
-// 128: 32 of them with 8192 tokens, window 1024 and 4 sinks in 1.02 ms, 128 TFLOP/s of
-// visible pairs; 72% at heads of 64, 256 of them with 1024 tokens and window 256 in
-// 180 us, 84 TFLOP/s, where cut blocks are a tenth of the work and the softmax's vector
-// instructions, some 45 a block, weigh twice as much.
+// sinks or of the diagonal cuts.  The matrix units are busy in 87% of the CUs'
+// cycles at heads of 128: 32 of them with 8192 tokens, window 1024 and 4 sinks in 1.02 ms,
+// 127 TFLOP/s of visible pairs; in 68% at heads of 64, 256 of them with 1024 tokens and
+// window 256 in 163 us, 94 TFLOP/s, where cut blocks are a tenth of the work and the
+// vector instructions, some 57 a block, weigh twice as much.
 template <typename T, int DP, int KB, Reads READS>
 __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(
     Call call, Results<T> results, Heads<const T> query, Heads<const T> key, Heads<const T> value,
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void tile_kernel(
 // Four waves with the same 16 rows and every fourth block of 16 keys, read into
 // the operands' layout from memory; at the end the waves' rows meet in LDS.  Nothing is
 // shared between waves before that, so no wave waits for another.  Bound by reading the
-// cache: 4 sequences of about 50000 tokens in 8 key heads of 128 in 345 us, 5.5 TB/s;
+// cache: 4 sequences of about 50000 tokens in 8 key heads of 128 in 340 us, 5.5 TB/s;
 // 16 sequences with a window of 1024 in 4 key heads of 64 in 10.4 us, 3.3 TB/s, where the
 // launch, a few blocks per wave and their latency show (16 waves a workgroup without
 // splits and their join: 17.7 us against 10.4 + 3).
@@ -492,8 +492,10 @@ static_assert(kThreads >= SPAR_HIP_ATTENTION_MAX_EXTENT);
 // of 64 rows would leave half of its matrix work unused.
 constexpr uint64_t kTokenRows = 32;
 
-// Workgroups that fill the chip (three or four to each of its 256 CUs), which row tiles
-// are split up to, and the fewest keys that repay the writing and reading of a part.
+// Workgroups that row tiles are split up to, and the fewest keys that repay the writing
+// and reading of a part: three tiles and four tokens to each of the 256 CUs.  (Of
+// token_kernel a CU holds as many in float32 up to heads of 64, three at 96, two at 128
+// and one above, and the others wait for them to end.)
 constexpr uint64_t kFullGrid = 768;
 constexpr uint64_t kTokenGrid = 1024;
 constexpr uint64_t kFewestKeys = 256;

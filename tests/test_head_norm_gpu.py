@@ -4,8 +4,8 @@ import pytest
 
 from tests import attention_oracle as oracle
 from tests.attention_oracle import assert_within, half_step
-from tests.test_attention_gpu import (F32, F64, View, _release_buffers, device, rotary_of,  # noqa: F401
-                                      space, tag)
+from tests.test_attention_gpu import _release_buffers  # noqa: F401
+from tests.test_attention_gpu import F32, F64, View, device, rotary_of, space, tag
 
 pytestmark = pytest.mark.gpu
 
