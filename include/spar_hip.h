@@ -222,6 +222,74 @@ struct SparHipAttention {
   int dtype;           /* of heads: SPAR_HIP_FLOAT32 or SPAR_HIP_FLOAT64 */
 };
 
+/* Keys and values of several sequences in pages of page_tokens tokens each, of a
+ * call's dtype.  Token t of row b (a sequence, or a prefix that several share) is token
+ * t % page_tokens of page table[b * table_stride + t / page_tokens], whose head h starts
+ * at data[page * strides[0] + h * strides[1] + token * strides[2]] of key and of value
+ * (their strides: page, head, token).  Where table is NULL row b is page b and holds
+ * page_tokens tokens: a contiguous cache.  A row has room for table_pages *
+ * page_tokens tokens, fewer than 2^30.  A page whose number is not in [0, pages) holds
+ * nothing: its tokens are neither seen nor written. */
+struct SparHipPages {
+  struct SparHipHeads key;
+  struct SparHipHeads value;
+  uint64_t pages;
+  uint64_t page_tokens;
+  const int32_t* table;  /* in device memory, or NULL                            */
+  uint64_t table_stride; /* elements between rows                                */
+  uint64_t table_pages;  /* entries of a row that may be used; 1 without a table */
+};
+
+/* What a cache attention call computes: sequence b has lengths[b] tokens of its own in
+ * row b of the cache and goes on behind prefix b / (batch / prefixes), of
+ * prefix_lengths[...] tokens (lengths are clamped to [0, what a row has room for], which
+ * they also are where NULL).  Query i of sequence b is its own token p = length - queries
+ * + i and sees its prefix and its own tokens j <= p; queries with p < 0 see nothing. */
+struct SparHipCacheAttention {
+  uint64_t batch;
+  uint64_t prefixes;    /* divides batch; not read where no prefix is given */
+  uint64_t query_heads; /* a multiple of key_heads: query head h reads key head
+                           h / (query_heads / key_heads) */
+  uint64_t key_heads;
+  uint64_t queries;     /* per sequence */
+  uint64_t extent;      /* of a head; at most SPAR_HIP_ATTENTION_MAX_EXTENT */
+  double scale;         /* of the scores; finite */
+  const void* lengths;        /* [batch] in device memory, or NULL    */
+  const void* prefix_lengths; /* [prefixes] in device memory, or NULL */
+  int length_dtype;     /* of both: SPAR_HIP_INT32 or SPAR_HIP_INT64 */
+  int dtype;            /* of heads: SPAR_HIP_FLOAT32 or SPAR_HIP_FLOAT64 */
+};
+
+/* Most beams and picks of a group of spar_hip_launch_beam_select. */
+#define SPAR_HIP_MAX_BEAMS 64
+
+/* What a beam selection chooses from: groups * beams rows of `vocabulary` logits,
+ * row_stride elements apart, with a score each.  The total of token k of row r is
+ * scores[r] + logits[r][k] - log(sum of exp(logits[r])), in double, and -infinity where
+ * that is NaN; in a row that has ended (ended[r] != 0) scores[r] for end_token and
+ * -infinity for every other token. */
+struct SparHipBeams {
+  uint64_t groups;
+  uint64_t beams;      /* rows of a group; at most SPAR_HIP_MAX_BEAMS */
+  uint64_t vocabulary; /* fewer than 2^31 */
+  uint64_t picks;      /* of a group; at most SPAR_HIP_MAX_BEAMS, beams * vocabulary */
+  uint64_t row_stride; /* at least vocabulary */
+  const int32_t* ended; /* [groups * beams] in device memory, or NULL: none has */
+  int64_t end_token;    /* of [0, vocabulary) where ended is given; negative: none ends */
+  int dtype;            /* of logits and scores: SPAR_HIP_FLOAT32 or SPAR_HIP_FLOAT64 */
+};
+
+/* One state of spar_hip_launch_reorder: row i of output, row_elements elements at
+ * output + i * output_stride, becomes row parents[i] of input. */
+struct SparHipReorder {
+  void* output;
+  uint64_t output_stride; /* in elements, at least row_elements */
+  const void* input;
+  uint64_t input_stride;  /* in elements, any */
+  uint64_t row_elements;
+  uint64_t element_size;  /* 4 or 8 bytes */
+};
+
 /* ---------------------------------------------------------------- runtime */
 
 /* Number of visible HIP devices (replaces the cudaGetDeviceCount check in
@@ -724,6 +792,76 @@ struct SparHipStatus spar_hip_launch_attention_backward(
     const struct SparHipHeads* key, const struct SparHipHeads* value,
     const struct SparHipAttention* attention, void* workspace, uint64_t workspace_bytes,
     int device);
+
+/* ------------------------------------------- decoding: cache, prefixes, beams */
+
+/* As in the section above: nothing is allocated and nothing copied from the host, so
+ * that calls may be captured into a graph; outputs must not overlap inputs unless that is
+ * said; a workspace is device memory of at least the bytes its query returns, 16-byte
+ * aligned, one for each of two calls that may run at once.  These operators have no
+ * backward: they serve. */
+
+/* Writes the keys and values of `tokens` new tokens of every sequence to the cache, the
+ * keys turned by their positions, and with them the queries' heads, turned, to
+ * query_output (both NULL: no queries; query_output may be query itself).  query, key
+ * and value are [batch, heads, tokens, extent] heads of query_heads, key_heads and
+ * key_heads heads.  Token t of sequence b goes to token places[b * place_stride + t]
+ * (SPAR_HIP_INT32 or SPAR_HIP_INT64) of row b of the cache, and nowhere where that is
+ * negative, behind the row's room or in a page that holds nothing; the rest of the cache
+ * is left as it was.  Two tokens of one call must not share a place in the pages: either
+ * may be found there, or a part of each.  rotary is NULL where heads are not turned; its
+ * positions are apart from the places, which count from the end of a shared prefix.
+ * No reference counterpart (its cache is a concatenation of tensors). */
+struct SparHipStatus spar_hip_launch_cache_append(
+    const struct SparHipPages* cache, const struct SparHipHeads* query_output,
+    const struct SparHipHeads* query, uint64_t query_heads, const struct SparHipHeads* key,
+    const struct SparHipHeads* value, uint64_t batch, uint64_t key_heads, uint64_t tokens,
+    uint64_t extent, const void* places, uint64_t place_stride, int place_dtype,
+    const struct SparHipRotary* rotary, int dtype, int device);
+
+/* Bytes of the workspace of spar_hip_launch_cache_attention; prefix may be NULL. */
+struct SparHipStatus spar_hip_cache_attention_workspace(
+    uint64_t* bytes, const struct SparHipPages* cache, const struct SparHipPages* prefix,
+    const struct SparHipCacheAttention* attention);
+
+/* output = softmax(scale * query [prefix keys; own keys]^T) [prefix values; own values]
+ * over what each query sees, and zeros for queries that see nothing.  The keys and values
+ * of a prefix are read once for all sequences that share it, whose queries are the rows of
+ * one product; prefix is NULL where there is none.  query and output have query_heads
+ * heads of `queries` tokens.  Keys and values that no query sees are not used, whatever they
+ * hold.  A NaN or infinity in one that some query sees may also reach other queries of its
+ * head, in a prefix those of all sequences that share it, but never a query that
+ * sees nothing.  Weights are divided by their sum after the product, as in
+ * spar_hip_launch_attention_forward, with the same bound. */
+struct SparHipStatus spar_hip_launch_cache_attention(
+    const struct SparHipHeads* output, const struct SparHipHeads* query,
+    const struct SparHipPages* cache, const struct SparHipPages* prefix,
+    const struct SparHipCacheAttention* attention, void* workspace, uint64_t workspace_bytes,
+    int device);
+
+/* Bytes of the workspace of spar_hip_launch_beam_select. */
+struct SparHipStatus spar_hip_beam_select_workspace(uint64_t* bytes,
+                                                    const struct SparHipBeams* beams);
+
+/* The best `picks` tokens of the rows of each group, best first: the largest totals, of
+ * equal totals the lowest row, in a row the largest logit, of equal ones the lowest token;
+ * totals of -infinity come in the order of rows and tokens alone.  Outputs are [groups, picks], contiguous: the totals
+ * rounded to the dtype, the rows picks go on from (of all groups * beams), their tokens,
+ * and whether they have ended (1 where the row had or the token is end_token, else 0; may
+ * be NULL).  One pass over the logits; log-probabilities are not written anywhere.
+ * No reference counterpart (it decodes greedily or by sampling on the host). */
+struct SparHipStatus spar_hip_launch_beam_select(
+    void* picked_scores, int64_t* parents, int64_t* tokens, int32_t* picked_ended,
+    const void* logits, const void* scores, const struct SparHipBeams* beams, void* workspace,
+    uint64_t workspace_bytes, int device);
+
+/* Rows of `state_count` states (host memory, read before the call returns; at most 2^16)
+ * in the order of their parents: `rows` numbers in device memory, of [0, source_rows).
+ * An output row whose parent lies outside becomes zeros.  Outputs must not overlap
+ * inputs or each other. */
+struct SparHipStatus spar_hip_launch_reorder(const struct SparHipReorder* states,
+                                             uint64_t state_count, const int64_t* parents,
+                                             uint64_t rows, uint64_t source_rows, int device);
 
 /* ---------------------------------------------- optimizer and gradient norm */
 

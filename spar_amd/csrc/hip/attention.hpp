@@ -351,6 +351,33 @@ struct Tile {
       }
     }
   }
+  // The same for rows that lie anywhere: head_of(row) is the row's head.
+  template <typename HeadOf>
+  __device__ __forceinline__ void start_rows(Stage& stage, int to, uint32_t extent,
+                                             HeadOf&& head_of) {
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+                             (__attribute__((address_space(3))) T*)(value[to]))) +
+                         wave * kWave * 16;
+#pragma unroll
+    for (int j = 0; j < kShare; ++j) {
+      if (!holds(j, wave)) continue;
+      const uint32_t at = threadIdx.x + j * kThreads;
+      const uint32_t row = at / kPieces, d = (at % kPieces ^ row % kMix<kPieces>) * W;
+      const T* head = head_of(j, row);
+      if constexpr (kDirect) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                     :
+                     : "s"(lds + j * kThreads * 16), "v"(head + (d < extent ? d : 0))
+                     : "memory", "m0");
+#pragma clang diagnostic pop
+      } else {
+        stage.piece[j] = load_piece<READS>(head, d, extent);
+      }
+    }
+  }
   __device__ __forceinline__ void finish(const Stage& stage, int to) {
     if constexpr (kDirect) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

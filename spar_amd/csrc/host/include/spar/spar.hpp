@@ -4,6 +4,7 @@
 
 #include "spar/attention.hpp"
 #include "spar/core.hpp"
+#include "spar/decoding.hpp"
 #include "spar/loss.hpp"
 #include "spar/ops.hpp"
 #include "spar/optim.hpp"

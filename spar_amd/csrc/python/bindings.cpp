@@ -357,6 +357,42 @@ PYBIND11_MODULE(_spar, m) {
         py::arg("value"), py::arg("window") = 0, py::arg("sinks") = 0,
         py::arg("scale") = py::none(), py::arg("lengths") = py::none(),
         py::call_guard<py::gil_scoped_release>());
+  py::class_<spar::PagedCache>(m, "PagedCache")
+      .def(py::init([](const Tensor& key, const Tensor& value, const std::optional<Tensor>& table) {
+             return spar::PagedCache{key, value, table};
+           }),
+           py::arg("key"), py::arg("value"), py::arg("table") = py::none())
+      .def_readwrite("key", &spar::PagedCache::key)
+      .def_readwrite("value", &spar::PagedCache::value)
+      .def_readwrite("table", &spar::PagedCache::table);
+  py::class_<spar::CacheRotation>(m, "CacheRotation")
+      .def(py::init([](const Tensor& positions, const Tensor& frequencies,
+                       spar::RotaryLayout layout, double magnitude) {
+             return spar::CacheRotation{positions, frequencies, layout, magnitude};
+           }),
+           py::arg("positions"), py::arg("frequencies"),
+           py::arg("layout") = spar::RotaryLayout::Half, py::arg("magnitude") = 1.0)
+      .def_readwrite("positions", &spar::CacheRotation::positions)
+      .def_readwrite("frequencies", &spar::CacheRotation::frequencies)
+      .def_readwrite("layout", &spar::CacheRotation::layout)
+      .def_readwrite("magnitude", &spar::CacheRotation::magnitude);
+  py::class_<spar::BeamSelection>(m, "BeamSelection")
+      .def_readonly("scores", &spar::BeamSelection::scores)
+      .def_readonly("parents", &spar::BeamSelection::parents)
+      .def_readonly("tokens", &spar::BeamSelection::tokens)
+      .def_readonly("ended", &spar::BeamSelection::ended);
+  m.def("cache_append", &spar::cache_append, py::arg("cache"), py::arg("key"), py::arg("value"),
+        py::arg("places"), py::arg("rotation") = py::none(), py::arg("query") = py::none(),
+        py::call_guard<py::gil_scoped_release>());
+  m.def("cache_attention", &spar::cache_attention, py::arg("query"), py::arg("cache"),
+        py::arg("lengths") = py::none(), py::arg("prefix") = py::none(),
+        py::arg("prefix_lengths") = py::none(), py::arg("scale") = py::none(),
+        py::call_guard<py::gil_scoped_release>());
+  m.def("beam_select", &spar::beam_select, py::arg("logits"), py::arg("scores"), py::arg("picks"),
+        py::arg("end_token") = py::none(), py::arg("ended") = py::none(),
+        py::call_guard<py::gil_scoped_release>());
+  m.def("reorder", &spar::reorder, py::arg("states"), py::arg("parents"),
+        py::call_guard<py::gil_scoped_release>());
   m.def("reduce_gradient_to_shape", [](const Tensor& g, const std::vector<std::int64_t>& s) {
     return spar::detail::reduce_gradient_to_shape(g, to_shape(s));
   });

@@ -97,6 +97,32 @@ class Attention(ctypes.Structure):
                 ("length_dtype", ctypes.c_int), ("dtype", ctypes.c_int)]
 
 
+class Pages(ctypes.Structure):
+    _fields_ = _words(("key",), ("value",), "pages", "page_tokens", "table", "table_stride",
+                      "table_pages")
+
+
+class CacheAttention(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_uint64), ("prefixes", ctypes.c_uint64),
+                ("query_heads", ctypes.c_uint64), ("key_heads", ctypes.c_uint64),
+                ("queries", ctypes.c_uint64), ("extent", ctypes.c_uint64),
+                ("scale", ctypes.c_double), ("lengths", ctypes.c_void_p),
+                ("prefix_lengths", ctypes.c_void_p), ("length_dtype", ctypes.c_int),
+                ("dtype", ctypes.c_int)]
+
+
+class Beams(ctypes.Structure):
+    _fields_ = [("groups", ctypes.c_uint64), ("beams", ctypes.c_uint64),
+                ("vocabulary", ctypes.c_uint64), ("picks", ctypes.c_uint64),
+                ("row_stride", ctypes.c_uint64), ("ended", ctypes.c_void_p),
+                ("end_token", ctypes.c_int64), ("dtype", ctypes.c_int)]
+
+
+class Reorder(ctypes.Structure):
+    _fields_ = _words("output", "output_stride", "input", "input_stride", "row_elements",
+                      "element_size")
+
+
 class HipError(RuntimeError):
     def __init__(self, name: str, status: Status, message: str):
         super().__init__(f"{name} failed: {message} (code {status.code}, hip error {status.hip_error})")
@@ -113,6 +139,9 @@ _U64P = ctypes.POINTER(ctypes.c_uint64)
 _HEADS = ctypes.POINTER(Heads)
 _ROTARY = ctypes.POINTER(Rotary)
 _ATTENTION = ctypes.POINTER(Attention)
+_PAGES = ctypes.POINTER(Pages)
+_CACHE_ATTENTION = ctypes.POINTER(CacheAttention)
+_BEAMS = ctypes.POINTER(Beams)
 
 # name -> argument types (every entry point returns Status except error_string and
 # norm_max_extent)
@@ -185,6 +214,14 @@ SIGNATURES = {
                                           _I],
     "spar_hip_launch_attention_backward": [_HEADS, _HEADS, _HEADS, _HEADS, _HEADS, _P, _HEADS,
                                            _HEADS, _HEADS, _ATTENTION, _P, _U64, _I],
+    "spar_hip_launch_cache_append": [_PAGES, _HEADS, _HEADS, _U64, _HEADS, _HEADS, _U64, _U64, _U64,
+                                     _U64, _P, _U64, _I, _ROTARY, _I, _I],
+    "spar_hip_cache_attention_workspace": [_U64P, _PAGES, _PAGES, _CACHE_ATTENTION],
+    "spar_hip_launch_cache_attention": [_HEADS, _HEADS, _PAGES, _PAGES, _CACHE_ATTENTION, _P, _U64,
+                                        _I],
+    "spar_hip_beam_select_workspace": [_U64P, _BEAMS],
+    "spar_hip_launch_beam_select": [_P, _P, _P, _P, _P, _P, _BEAMS, _P, _U64, _I],
+    "spar_hip_launch_reorder": [ctypes.POINTER(Reorder), _U64, _P, _U64, _U64, _I],
     "spar_hip_gradient_norm_summary": [ctypes.POINTER(NormSummary), _P, _U64, _I, _I],
     "spar_hip_launch_gradient_norm_summary": [_P, _P, _U64, _I, _I],
     "spar_hip_launch_gradient_norm_summaries": [_P, _P, _U64P, _U64, _I, _I],
@@ -293,6 +330,45 @@ def attention_workspace(shape, backward) -> int:
     need = ctypes.c_uint64(0)
     call("spar_hip_attention_workspace", ctypes.byref(need), shape, backward)
     return need.value
+
+
+def pages(key, key_strides, value, value_strides, count, page_tokens, table=None, table_stride=0,
+          table_pages=1) -> Pages:
+    """A cache of `count` pages: the first elements of its keys and values with their
+    (page, head, token) strides, and the table's address (None: row b is page b)."""
+    return Pages(key or 0, *key_strides, value or 0, *value_strides, count, page_tokens, table or 0,
+                 table_stride, table_pages)
+
+
+def cache_attention(batch, prefixes, query_heads, key_heads, queries, extent, scale, lengths,
+                    prefix_lengths, length_dtype, dtype) -> CacheAttention:
+    return CacheAttention(batch, prefixes, query_heads, key_heads, queries, extent, scale, lengths,
+                          prefix_lengths, length_dtype, dtype)
+
+
+def cache_attention_workspace(cache, prefix, shape) -> int:
+    need = ctypes.c_uint64(0)
+    call("spar_hip_cache_attention_workspace", ctypes.byref(need), cache, prefix, shape)
+    return need.value
+
+
+def beams(groups, beams, vocabulary, picks, row_stride, ended, end_token, dtype) -> Beams:
+    return Beams(groups, beams, vocabulary, picks, row_stride, ended, end_token, dtype)
+
+
+def beam_select_workspace(shape) -> int:
+    need = ctypes.c_uint64(0)
+    call("spar_hip_beam_select_workspace", ctypes.byref(need), shape)
+    return need.value
+
+
+def reorders(*states):
+    """States of spar_hip_launch_reorder, each (output, output stride, input, input
+    stride, row elements, element size)."""
+    words = array.array("Q")
+    for output, output_stride, source, source_stride, elements, size in states:
+        words.extend((output or 0, output_stride, source or 0, source_stride, elements, size))
+    return (Reorder * len(states)).from_buffer(words) if states else None
 
 
 def dtype_tag(dtype) -> int:
