@@ -18,13 +18,16 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kPieces = 4;               // 16-byte pieces of a lane's share of a chunk
-constexpr uint32_t kKept = 512;          // candidates a wave holds
+constexpr int kPieces = 8;               // 16-byte pieces of a lane's share of a chunk
 constexpr uint32_t kMostParts = kWave;   // of a row
 constexpr uint32_t kNone = ~0U;          // no token
 
 template <typename T>
 constexpr uint32_t kChunk = kWave * kPieces * Vec16<T>::width;
+
+// Candidates a wave holds: what half a chunk brings at most behind the best so far.
+template <typename T>
+constexpr uint32_t kKept = kChunk<T> / 2 + SPAR_HIP_MAX_BEAMS;
 
 // Whole numbers in the order of the values (of any but NaN; -0 before +0).
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -58,16 +61,22 @@ __device__ __forceinline__ T infinity() {
   return static_cast<T>(__builtin_huge_val());
 }
 
+// Passes over NaN.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_fmaxf(a, b); }
+__device__ __forceinline__ double larger(double a, double b) { return __builtin_fmax(a, b); }
+
 __device__ __forceinline__ uint32_t count_of(bool flag) {
   return static_cast<uint32_t>(__popcll(__ballot(flag)));
 }
 
-// The largest key that at least `wanted` of the wave's keys reach: bit by bit, from the
-// top.  counted(key) is how many reach it.
-template <typename Key, typename Counted>
+// The largest key that at least `wanted` of the wave's keys reach, of its BITS highest bits:
+// bit by bit, from the top.  counted(key) is how many reach it.
+template <typename Key, int BITS = 8 * sizeof(Key), typename Counted>
 __device__ __forceinline__ Key kth_largest(uint32_t wanted, Counted&& counted) {
   Key found = 0;
-  for (Key bit = Key{1} << (8 * sizeof(Key) - 1); bit != 0; bit >>= 1) {
+  Key bit = Key{1} << (8 * sizeof(Key) - 1);
+#pragma unroll 1
+  for (int i = 0; i < BITS; ++i, bit >>= 1) {
     if (counted(found | bit) >= wanted) found |= bit;
   }
   return found;
@@ -81,44 +90,40 @@ struct Rows {
   uint32_t vocabulary;
   uint32_t parts;   // of a row
   uint32_t picks;
+  uint32_t slots;   // of a part's candidates, at least picks
   double* maxima;   // [row][part]
   double* sums;     // the same
-  T* values;        // [row][part][picks], best in no order
+  T* values;        // [row][part][slot], in no order
   uint32_t* tokens; // the same, kNone behind the last
 };
 
 // What a wave has kept, in LDS: the candidates in the order of their finding.
 template <typename T>
 struct Kept {
-  T value[kKept];
-  uint32_t token[kKept];
+  T value[kKept<T>];
+  uint32_t token[kKept<T>];
 };
 
 // Keeps the best `picks` of `count` candidates (more than picks): those above the
 // picks-th largest value, and of those equal to it the lowest tokens.  Returns that value.
-template <typename T>
+// The loops over bits stay loops: unrolled, they would be most of a kernel that runs its
+// code once.
+template <typename T, int SHARE>
 __device__ __forceinline__ T compact(Kept<T>& kept, uint32_t count, uint32_t picks, int lane) {
   using Key = decltype(key_of(T(0)));
-  constexpr int kShare = kKept / kWave;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  Key key[kShare];
-  uint32_t token[kShare];
-  T value[kShare];
+  Key key[SHARE];
+  uint32_t token[SHARE];
 #pragma unroll
-  for (int i = 0; i < kShare; ++i) {
+  for (int i = 0; i < SHARE; ++i) {
     const uint32_t at = lane + i * kWave;
-    const bool held = at < count;
-    value[i] = held ? kept.value[at] : T(0);
-    token[i] = held ? kept.token[at] : kNone;
-    key[i] = held ? key_of(value[i]) : Key{0};
+    token[i] = at < count ? kept.token[at] : kNone;
+    key[i] = at < count ? key_of(kept.value[at]) : Key{0};
   }
-  const uint32_t used = (count + kWave - 1) / kWave;
   const auto counted = [&](auto&& flag) {
     uint32_t n = 0;
 #pragma unroll
-    for (int i = 0; i < kShare; ++i) {
-      if (static_cast<uint32_t>(i) < used) n += count_of(flag(i));
-    }
+    for (int i = 0; i < SHARE; ++i) n += count_of(flag(i));
     return n;
   };
   const Key border = kth_largest<Key>(
@@ -131,13 +136,12 @@ __device__ __forceinline__ T compact(Kept<T>& kept, uint32_t count, uint32_t pic
   });
   uint32_t next = 0;
 #pragma unroll
-  for (int i = 0; i < kShare; ++i) {
-    if (static_cast<uint32_t>(i) >= used) continue;
+  for (int i = 0; i < SHARE; ++i) {
     const bool stays = (key[i] > border) | ((key[i] == border) & (token[i] <= last));
     const uint64_t mask = __ballot(stays);
     if (stays) {
       const uint32_t to = next + __popcll(mask & ((uint64_t{1} << lane) - 1));
-      kept.value[to] = value[i];
+      kept.value[to] = value_of(key[i]);
       kept.token[to] = token[i];
     }
     next += static_cast<uint32_t>(__popcll(mask));
@@ -145,6 +149,11 @@ __device__ __forceinline__ T compact(Kept<T>& kept, uint32_t count, uint32_t pic
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   return value_of(border);
 }
+// Most waves hold few candidates, all a wave has room for hardly any.
+constexpr int kFew = 2;
+template <typename T>
+constexpr int kAll = kKept<T> / kWave;
+static_assert(kKept<float> % kWave == 0 && kKept<double> % kWave == 0);
 
 // The largest value below x.
 template <typename T>
@@ -154,22 +163,29 @@ __device__ __forceinline__ T below(T x) {
 }
 
 // A wave per part of a row: chunks of the part one after the other, the next one's loads in
-// flight.  A candidate is what exceeds `bar`, which follows the picks-th best so far; its
-// first value comes from the lanes' maxima of the first chunk.
+// flight.  A candidate is what exceeds `bar`, below which the row's picks-th best cannot lie;
+// it comes from the lanes' maxima of the first chunk, and waves of a workgroup that read the
+// same row share the highest of theirs.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void row_kernel(Rows<T> rows, uint32_t waves,
-                                                       FastDiv by_parts) {
+__global__ __launch_bounds__(kThreads, 2) void row_kernel(Rows<T> rows, uint32_t waves,
+                                                          FastDiv by_parts) {
   constexpr int W = Vec16<T>::width;
   constexpr int E = kPieces * W;
   using Key = decltype(key_of(T(0)));
   __shared__ Kept<T> all_kept[kWaves];
+  __shared__ T bars[kWaves];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
   const uint32_t id = blockIdx.x * kWaves + wave;
+  bars[wave] = -infinity<T>();
+  __syncthreads();
   if (id >= waves) return;
   const uint32_t row = by_parts.div(id);
   const uint32_t part = id - row * rows.parts;
   if (rows.ended != nullptr && rows.ended[row] != 0) return;
+  bool shares[kWaves];
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) shares[w] = by_parts.div(blockIdx.x * kWaves + w) == row;
   Kept<T>& kept = all_kept[wave];
   const T* logits = rows.logits + row * rows.stride;
   const uint32_t chunks = (rows.vocabulary + kChunk<T> - 1) / kChunk<T>;
@@ -189,11 +205,10 @@ __global__ __launch_bounds__(kThreads) void row_kernel(Rows<T> rows, uint32_t wa
 #pragma unroll
         for (int j = 0; j < W; ++j) x[p * W + j] = piece[j];
       }
-    } else {
+    } else {  // and the row's last token in the place of those behind
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const uint32_t token = first + i / W * kWave * W + i % W;
-        x[i] = token < rows.vocabulary ? logits[token] : -infinity<T>();
+        x[i] = logits[min(first + i / W * kWave * W + i % W, rows.vocabulary - 1)];
       }
     }
   };
@@ -202,56 +217,82 @@ __global__ __launch_bounds__(kThreads) void row_kernel(Rows<T> rows, uint32_t wa
   T bar = -infinity<T>();
   uint32_t count = 0;
   T x[E], next[E];
-  if (begin < end) load(x, begin);
+  load(x, begin);
+  // Waited for here (vmcnt(0)), or the loop's first use of it would wait for the next chunk's
+  // loads in every round.
+  __builtin_amdgcn_s_waitcnt(0x0f70);
   for (uint32_t chunk = begin; chunk < end; ++chunk) {
     if (chunk + 1 < end) load(next, chunk + 1);
-    T high = x[0];
+    if ((chunk + 1) * static_cast<uint64_t>(kChunk<T>) > rows.vocabulary) {
 #pragma unroll
-    for (int i = 1; i < E; ++i) high = x[i] > high || high != high ? x[i] : high;
+      for (int i = 0; i < E; ++i) {
+        const uint32_t token = chunk * kChunk<T> + (i / W * kWave + lane) * W + i % W;
+        if (token >= rows.vocabulary) x[i] = -infinity<T>();
+      }
+    }
+    T highs[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      highs[h] = x[h * E / 2];
+#pragma unroll
+      for (int i = 1; i < E / 2; ++i) highs[h] = larger(highs[h], x[h * E / 2 + i]);
+    }
+    const T high = larger(highs[0], highs[1]);
     if (high > top) {
       sum *= static_cast<double>(exp_of(top - high));
       top = high;
     }
-    T part_sum = T(0);
 #pragma unroll
-    for (int i = 0; i < E; ++i) part_sum += exp_of(x[i] - top);
-    sum += static_cast<double>(part_sum);
+    for (int h = 0; h < 2; ++h) {
+      T part_sum = T(0);
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) part_sum += exp_of(x[h * E / 2 + i] - top);
+      sum += static_cast<double>(part_sum);
+    }
 
     if (chunk == begin) {
-      // picks lanes hold a value of this size or more each.
+      // picks lanes hold a value of this size or more each; sign, exponent and 7 bits do.
       const Key key = high > -infinity<T>() ? key_of(high) : Key{0};
-      const Key border =
-          kth_largest<Key>(picks, [&](Key at) { return count_of(key >= at); });
+      const Key border = kth_largest<Key, sizeof(T) == 4 ? 16 : 19>(
+          picks, [&](Key at) { return count_of(key >= at); });
       if (border != 0) bar = below(value_of(border));
+      if (lane == 0) *const_cast<volatile T*>(&bars[wave]) = bar;
     }
-    if (__any(high > bar)) {
+    // A bar that another wave has not set yet is -infinity: no harm but more candidates.
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
+    for (int w = 0; w < kWaves; ++w) {
+      const T other = *const_cast<const volatile T*>(&bars[w]);
+      bar = shares[w] ? larger(bar, other) : bar;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (!__any(highs[h] > bar)) continue;
+      if (count + count_of(highs[h] > bar) * (E / 2) > kKept<T>) {
+        // Tokens to come are larger than those before: an equal value does not count.
+        bar = compact<T, kAll<T>>(kept, count, picks, lane);
+        count = picks;
+      }
+#pragma unroll
+      for (int i = h * E / 2; i < (h + 1) * E / 2; ++i) {
         const uint64_t mask = __ballot(x[i] > bar);
         if (mask == 0) continue;
-        if (count + kWave > kKept) {
-          bar = below(compact(kept, count, picks, lane));
-          count = picks;
-        }
         if (x[i] > bar) {
-          const uint32_t to =
-              count + __popcll(__ballot(x[i] > bar) & ((uint64_t{1} << lane) - 1));
+          const uint32_t to = count + __popcll(mask & ((uint64_t{1} << lane) - 1));
           kept.value[to] = x[i];
           kept.token[to] = chunk * kChunk<T> + (i / W * kWave + lane) * W + i % W;
         }
-        count += count_of(x[i] > bar);
-      }
-      // Tokens of later chunks are larger: an equal value no longer counts.
-      if (count > picks && chunk + 1 < end) {
-        bar = compact(kept, count, picks, lane);
-        count = picks;
+        count += static_cast<uint32_t>(__popcll(mask));
       }
     }
 #pragma unroll
     for (int i = 0; i < E; ++i) x[i] = next[i];
   }
-  if (count > picks) {
-    compact(kept, count, picks, lane);
+  if (count > rows.slots) {
+    if (count <= kFew * kWave) {
+      compact<T, kFew>(kept, count, picks, lane);
+    } else {
+      compact<T, kAll<T>>(kept, count, picks, lane);
+    }
     count = picks;
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -267,8 +308,8 @@ __global__ __launch_bounds__(kThreads) void row_kernel(Rows<T> rows, uint32_t wa
     rows.maxima[id] = static_cast<double>(most);
     rows.sums[id] = sum;
   }
-  const uint64_t base = static_cast<uint64_t>(id) * picks;
-  if (static_cast<uint32_t>(lane) < picks) {
+  const uint64_t base = static_cast<uint64_t>(id) * rows.slots;
+  if (static_cast<uint32_t>(lane) < rows.slots) {
     const bool held = static_cast<uint32_t>(lane) < count;
     rows.values[base + lane] = held ? kept.value[lane] : T(0);
     rows.tokens[base + lane] = held ? kept.token[lane] : kNone;
@@ -292,7 +333,8 @@ __device__ __forceinline__ bool precedes(const Candidate& a, const Candidate& b)
 
 constexpr int kGroupThreads = 512;
 constexpr int kGroupWaves = kGroupThreads / kWave;
-constexpr uint32_t kListed = 1024;  // candidates in LDS
+constexpr uint32_t kBatch = 4096;   // candidates whose totals are held
+constexpr uint32_t kListed = 1024;  // candidates in LDS that may be the best
 
 template <typename T>
 struct Picked {
@@ -302,6 +344,9 @@ struct Picked {
   int32_t* ended;  // or nullptr
 };
 
+// A workgroup per group.  Candidates are read while the rows' sums are joined; the picks-th
+// best of each wave's lanes bounds what can be among the group's best, which few pass, and
+// those are ranked by counting.
 template <typename T>
 __global__ __launch_bounds__(kGroupThreads) void group_kernel(Picked<T> picked, Rows<T> rows,
                                                               const T* scores, uint32_t beams,
@@ -310,111 +355,150 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(Picked<T> picked, 
   __shared__ Candidate list[kListed], best[SPAR_HIP_MAX_BEAMS];
   __shared__ double score_of[SPAR_HIP_MAX_BEAMS], log_sum[SPAR_HIP_MAX_BEAMS];
   __shared__ bool has_ended[SPAR_HIP_MAX_BEAMS];
+  __shared__ uint32_t keys[kBatch], passed[kBatch];
   __shared__ uint32_t bars[kGroupWaves];
-  __shared__ uint32_t listed;
+  __shared__ uint32_t listed, count;
   const uint32_t group = blockIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
   const uint32_t picks = rows.picks;
+  const uint32_t per_row = by_row.divisor;  // parts * slots
+  const uint32_t all = beams * per_row;
+  const uint64_t first_row = static_cast<uint64_t>(group) * beams;
 
+  // The first candidates are on their way while the rows' sums are joined.
+  constexpr int kShare = kBatch / kGroupThreads;
+  T value[kShare];
+  uint32_t token[kShare];
+#pragma unroll
+  for (int j = 0; j < kShare; ++j) {
+    const uint32_t i = j * kGroupThreads + threadIdx.x;
+    const uint64_t from = first_row * per_row + (i < all ? i : 0);
+    value[j] = rows.values[from];
+    token[j] = rows.tokens[from];
+  }
   for (uint32_t r = wave; r < beams; r += kGroupWaves) {
-    const uint32_t row = group * beams + r;
+    const uint64_t row = first_row + r;
     const bool ended = rows.ended != nullptr && rows.ended[row] != 0;
     double top = -__DBL_MAX__, sum = 0.0;
     if (!ended && static_cast<uint32_t>(lane) < rows.parts) {
-      top = rows.maxima[static_cast<uint64_t>(row) * rows.parts + lane];
-      sum = rows.sums[static_cast<uint64_t>(row) * rows.parts + lane];
+      top = rows.maxima[row * rows.parts + lane];
+      sum = rows.sums[row * rows.parts + lane];
     }
+    const T score = scores[row];
     double most = top;
-#pragma unroll
+#pragma unroll 1
     for (int mask = kWave / 2; mask > 0; mask >>= 1) {
       most = fmax(most, __shfl_xor(most, mask, kWave));
     }
-    sum = wave_sum(sum * exp(top - most));
+    sum *= exp(top - most);
+#pragma unroll 1
+    for (int mask = kWave / 2; mask > 0; mask >>= 1) sum += __shfl_xor(sum, mask, kWave);
     if (lane == 0) {
-      score_of[r] = static_cast<double>(scores[row]);
+      score_of[r] = static_cast<double>(score);
       log_sum[r] = most + log(sum);
       has_ended[r] = ended;
     }
   }
-  if (threadIdx.x == 0) listed = 0;
+  if (threadIdx.x == 0) listed = count = 0;
   __syncthreads();
 
-  const uint32_t per_row = rows.parts * picks;
-  const uint32_t all = beams * per_row;
-  // Candidate i of the group; its total is -infinity where there is none.
-  const auto candidate = [&](uint32_t i) {
-    Candidate c{-infinity<double>(), 0.0, 0, 0};
-    if (i >= all) return c;
-    c.row = by_row.div(i);
-    const uint32_t at = i - c.row * per_row;
+  // Candidate i, of these; its total is -infinity where there is none.
+  const auto made = [&](uint32_t i, T value, uint32_t token) {
+    Candidate c{-infinity<double>(), static_cast<double>(value), by_row.div(i), token};
     if (has_ended[c.row]) {
-      if (at != 0) return c;
+      if (i != c.row * per_row) return c;
       c.token = static_cast<uint32_t>(end_token);
       c.total = score_of[c.row];
-    } else {
-      const uint64_t from = static_cast<uint64_t>(group * beams + c.row) * per_row + at;
-      c.token = rows.tokens[from];
-      if (c.token == kNone) return c;
-      c.logit = static_cast<double>(rows.values[from]);
+    } else if (token != kNone) {
       c.total = score_of[c.row] + (c.logit - log_sum[c.row]);
     }
     if (c.total != c.total) c.total = -infinity<double>();
     return c;
   };
-  // In single precision: rounding keeps the order, so that what lies below the picks-th
-  // largest of these is not among the best.
-  const auto coarse = [](double total) { return key_of(static_cast<float>(total)); };
+  const auto candidate = [&](uint32_t i) {
+    const uint64_t from = first_row * per_row + i;
+    return made(i, rows.values[from], rows.tokens[from]);
+  };
+  // Totals in single precision: rounding keeps the order, so that what lies below the
+  // picks-th largest of these is not among the best; of its bits the first do.
+  const auto coarse = [](const Candidate& c) { return key_of(static_cast<float>(c.total)); };
   const uint32_t nothing = key_of(-infinity<float>());
 
   uint32_t high = nothing;
-  for (uint32_t i = threadIdx.x; i < all; i += kGroupThreads) {
-    const uint32_t key = coarse(candidate(i).total);
-    high = key > high ? key : high;
+#pragma unroll
+  for (int j = 0; j < kShare; ++j) {
+    const uint32_t i = j * kGroupThreads + threadIdx.x;
+    if (j * kGroupThreads >= all) break;
+    const uint32_t key = i < all ? coarse(made(i, value[j], token[j])) : 0;
+    keys[i] = key;
+    high = max(high, key);
+  }
+#pragma unroll 1
+  for (uint32_t i = kBatch + threadIdx.x; i < all; i += kGroupThreads) {
+    high = max(high, coarse(candidate(i)));
   }
   const uint32_t border =
-      kth_largest<uint32_t>(picks, [&](uint32_t at) { return count_of(high >= at); });
+      kth_largest<uint32_t, 20>(picks, [&](uint32_t at) { return count_of(high >= at); });
   if (lane == 0) bars[wave] = border;
   __syncthreads();
   uint32_t bar = nothing;
 #pragma unroll
-  for (int w = 0; w < kGroupWaves; ++w) bar = bars[w] > bar ? bars[w] : bar;
+  for (int w = 0; w < kGroupWaves; ++w) bar = max(bar, bars[w]);
 
-  // Keeps the best picks of the list; all threads.
+  // Keeps the best picks of the list; all threads.  Returns how many it keeps.
   const auto choose = [&]() {
-    const uint32_t count = listed;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < count; i += kGroupThreads) {
-      const Candidate c = list[i];
+    const uint32_t count = listed;  // of all, the best so far among them
+    constexpr uint32_t kLanes = 8;  // to rank a candidate
+    const uint32_t part = threadIdx.x % kLanes;
+    for (uint32_t first = 0; first < count; first += kGroupThreads / kLanes) {
+      const uint32_t i = first + threadIdx.x / kLanes;
+      const Candidate c = list[i < count ? i : 0];
       uint32_t before = 0;
-      for (uint32_t j = 0; j < count && before < picks; ++j) before += precedes(list[j], c);
-      if (before < picks) best[before] = c;
+#pragma unroll 2
+      for (uint32_t j = part; j < count; j += kLanes) before += precedes(list[j], c);
+      before += __shfl_xor(before, 1, kWave);
+      before += __shfl_xor(before, 2, kWave);
+      before += __shfl_xor(before, 4, kWave);
+      if (part == 0 && i < count && before < picks) best[before] = c;
     }
-    const uint32_t chosen = count < picks ? count : picks;
+    const uint32_t kept = count < picks ? count : picks;
     __syncthreads();
-    if (threadIdx.x < chosen) list[threadIdx.x] = best[threadIdx.x];
-    if (threadIdx.x == 0) listed = chosen;
+    if (threadIdx.x < kept) list[threadIdx.x] = best[threadIdx.x];
+    if (threadIdx.x == 0) listed = kept;
     __syncthreads();
-    return chosen;
+    return kept;
   };
-  for (uint32_t first = 0; first < all; first += kGroupThreads) {
-    const Candidate c = candidate(first + threadIdx.x);
-    const uint32_t key = coarse(c.total);
-    const bool taken = (c.total > -infinity<double>()) & (key >= bar);
-    const uint64_t mask = __ballot(taken);
-    if (mask != 0) {
-      uint32_t base = 0;
-      if (lane == 0) base = atomicAdd(&listed, static_cast<uint32_t>(__popcll(mask)));
-      base = __builtin_amdgcn_readfirstlane(base);
-      if (taken) list[base + __popcll(mask & ((uint64_t{1} << lane) - 1))] = c;
+  // A batch's candidates that may be the best, first by number and then as they are, so many
+  // at once as the list has room for.
+  uint32_t chosen = 0;
+  for (uint32_t base = 0; base < all; base += kBatch) {
+    const uint32_t end = min(base + kBatch, all);
+#pragma unroll 1
+    for (uint32_t first = base; first < end; first += kGroupThreads) {
+      const uint32_t i = first + threadIdx.x;
+      const bool taken = i < end && (i < kBatch ? keys[i] : coarse(candidate(i))) >= bar;
+      const uint64_t mask = __ballot(taken);
+      if (mask == 0) continue;
+      uint32_t to = 0;
+      if (lane == 0) to = atomicAdd(&count, static_cast<uint32_t>(__popcll(mask)));
+      to = __builtin_amdgcn_readfirstlane(to) + __popcll(mask & ((uint64_t{1} << lane) - 1));
+      if (taken) passed[to] = i;
     }
     __syncthreads();
-    const uint32_t count = listed;
+    const uint32_t found = count;
+    for (uint32_t first = 0; first < found; first += kListed - SPAR_HIP_MAX_BEAMS) {
+      const uint32_t last = min(first + kListed - SPAR_HIP_MAX_BEAMS, found);
+      for (uint32_t i = first + threadIdx.x; i < last; i += kGroupThreads) {
+        const Candidate c = candidate(passed[i]);
+        if (c.total > -infinity<double>()) list[atomicAdd(&listed, 1U)] = c;
+      }
+      chosen = choose();
+    }
+    if (threadIdx.x == 0) count = 0;
     __syncthreads();
-    if (count > kListed - kGroupThreads) choose();
   }
-  __syncthreads();
-  const uint32_t chosen = choose();
 
   const auto write = [&](uint32_t i, double total, uint32_t r, uint32_t token) {
     const uint64_t at = static_cast<uint64_t>(group) * picks + i;
@@ -519,12 +603,13 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(States states, const 
 
 // ---------------------------------------------------------------- launchers
 
-// Waves that a call's rows are split up to: 16 for each of the 256 CUs.
-constexpr uint64_t kFullWaves = 4096;
+// Waves that a call's rows are split up to: eight for each of the 256 CUs, which are as many
+// as a CU holds.
+constexpr uint64_t kFullWaves = 2048;
 constexpr uint64_t kMostGroups = (uint64_t{1} << 32) / kGroupThreads - 1;
 
 struct Plan {
-  uint64_t rows, parts;
+  uint64_t rows, parts, slots;
   uint64_t bytes;
 };
 
@@ -537,7 +622,10 @@ Plan plan_of(const SparHipBeams& b) {
   plan.parts = std::max<uint64_t>(
       1, std::min({chunks, uint64_t{kMostParts}, kFullWaves / std::max<uint64_t>(1, plan.rows)}));
   const uint64_t waves = plan.rows * plan.parts;
-  plan.bytes = waves * 2 * sizeof(double) + waves * b.picks * (size + sizeof(uint32_t));
+  // Room for a few more than the picks, which a part of one chunk mostly finds: they need
+  // not be told apart before the group's choice.
+  plan.slots = std::min<uint64_t>(2 * b.picks, SPAR_HIP_MAX_BEAMS);
+  plan.bytes = waves * 2 * sizeof(double) + waves * plan.slots * (size + sizeof(uint32_t));
   return plan;
 }
 
@@ -563,13 +651,14 @@ void start(const SparHipBeams& b, const Plan& plan, void* picked_scores, int64_t
   rows.vocabulary = static_cast<uint32_t>(b.vocabulary);
   rows.parts = static_cast<uint32_t>(plan.parts);
   rows.picks = static_cast<uint32_t>(b.picks);
+  rows.slots = static_cast<uint32_t>(plan.slots);
   rows.maxima = static_cast<double*>(workspace);
   rows.sums = rows.maxima + waves;
   rows.values = reinterpret_cast<T*>(rows.sums + waves);
-  rows.tokens = reinterpret_cast<uint32_t*>(rows.values + waves * b.picks);
+  rows.tokens = reinterpret_cast<uint32_t*>(rows.values + waves * plan.slots);
   FastDiv by_parts, by_row;
   by_parts.init(rows.parts);
-  by_row.init(rows.parts * rows.picks);
+  by_row.init(rows.parts * rows.slots);
   row_kernel<T><<<ceil_div_u32(waves, kWaves), kThreads, 0, stream>>>(
       rows, static_cast<uint32_t>(waves), by_parts);
   const Picked<T> picked{static_cast<T*>(picked_scores), parents, tokens, picked_ended};
