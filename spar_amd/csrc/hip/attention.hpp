@@ -264,14 +264,14 @@ struct Operand {
 template <int PIECES>
 constexpr int kMix = PIECES % 16 == 0 ? 16 : 8;
 
-// Tiles of ROWS heads in LDS, two of them: one is used while the next one arrives.
+// Tiles of ROWS heads in LDS, two or more of them: one is used while the next arrive.
 // Piece p of row r lies at piece p ^ (r % 16) of the row (r % 8 where 16 pieces do not
 // divide a row), so that 16 lanes that read one piece of 16 rows each, and 16 lanes
 // that read 16 pieces of one row, both spread over the 64 banks without padding (with
 // r % 8 every such read takes half as long again): so aligned heads go from memory
 // to LDS directly, 64 neighbouring pieces of LDS per instruction, each lane asking
 // for the piece that belongs there.  Others pass through registers.
-template <typename T, int ROWS, int DP, Reads READS>
+template <typename T, int ROWS, int DP, Reads READS, int BUFFERS = 2>
 struct Tile {
   static constexpr int W = Vec16<T>::width;
   static constexpr int kPieces = DP / W;
@@ -279,7 +279,7 @@ struct Tile {
   static constexpr int kShare = (kAll + kThreads - 1) / kThreads;  // pieces per thread
   static constexpr bool kDirect = READS == Reads::Aligned;
   static_assert(kAll % kWave == 0 && kPieces % 8 == 0);
-  alignas(16) T value[2][ROWS * DP];
+  alignas(16) T value[BUFFERS][ROWS * DP];
 
   struct Stage {
     typename Vec16<T>::type piece[kDirect ? 1 : kShare];

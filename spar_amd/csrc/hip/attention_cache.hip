@@ -42,7 +42,9 @@ struct Side {
   uint32_t rows;         // of a unit
   uint32_t row_tiles;
   uint32_t splits;
+  uint32_t least;        // blocks of 16 keys that are worth a part
   uint32_t first_part;
+  bool whole;            // a page holds whole blocks of keys
 
   __device__ __forceinline__ int32_t length(uint32_t u) const {
     if (lengths == nullptr) return static_cast<int32_t>(cache.room);
@@ -92,27 +94,57 @@ __device__ __forceinline__ T* part_row(const Call& call, const Results<T>& resul
   return results.part_output + at * results.pitch;
 }
 
-// The keys of a block of SIZE from `begin` on, found through the table.  `page` is what the
-// lane found for key begin + lane (WHOLE: the block's only page).
-template <typename T, int SIZE, bool WHOLE>
+// The run of blocks of SIZE keys that part `split` of a side takes of the first `high`:
+// equal shares, of fewer parts where those would be small.
+template <int SIZE, typename T>
+__device__ __forceinline__ void share_of(const Side<T>& side, int32_t high, uint32_t split,
+                                         uint32_t& begin, uint32_t& end) {
+  const uint32_t blocks = static_cast<uint32_t>(high + SIZE - 1) / SIZE;
+  const uint32_t share = max((blocks + side.splits - 1) / side.splits,
+                             (side.least * kBlock + SIZE - 1) / SIZE);
+  begin = min(split * share, blocks);
+  end = min(begin + share, blocks);
+}
+
+// The keys of a block of SIZE from `begin` on, below `end`, found through the table.
+template <typename T, int SIZE>
 struct Finder {
   const Pages<const T>& cache;
   uint32_t u;
+  bool whole;
+  // Where a page holds whole blocks: the next 64 entries of the row, one in each lane.  A
+  // block's page is then known without a load of its own, behind which loads of keys
+  // would have to be waited for.
+  int32_t window = 0;
+  uint32_t window_first = 0, window_end = 0;
 
-  __device__ __forceinline__ int32_t look(int32_t begin, int32_t end, int lane) const {
-    const int32_t key = WHOLE ? begin : begin + lane;
-    if (key >= end || (!WHOLE && lane >= SIZE)) return -1;
+  __device__ __forceinline__ Finder(const Pages<const T>& cache_, uint32_t u_, bool whole_)
+      : cache(cache_), u(u_), whole(whole_) {}
+
+  __device__ __forceinline__ int32_t only_page(int32_t begin) {
+    if (cache.table == nullptr) return static_cast<int32_t>(u);
+    const uint32_t entry = cache.page_tokens.div(static_cast<uint32_t>(begin));
+    if (entry >= window_end) {
+      const uint32_t last = cache.page_tokens.div(cache.room) - 1;
+      window_first = entry;
+      window_end = entry + kWave;
+      window = cache.page_at(u, min(entry + threadIdx.x % kWave, last));
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), here and not at every use
+    }
+    return __builtin_amdgcn_readlane(window, entry - window_first);
+  }
+  // Where it does not: what the table names for key begin + lane of the block (for its last
+  // key where that is behind it), asked for a block ahead.
+  __device__ __forceinline__ int32_t page_of(int32_t begin, int32_t end, int lane) const {
+    const int32_t key = min(begin + lane % SIZE, end - 1);
     return cache.page_at(u, cache.page_tokens.div(static_cast<uint32_t>(key)));
   }
-  // Which of the block's keys are there, a bit each.
+  // Which of the block's keys are there, a bit each; `page` as found by either.
   __device__ __forceinline__ uint64_t present(int32_t page, int32_t begin, int32_t end) const {
     constexpr uint64_t kAll = (uint64_t{1} << SIZE) - 1;
-    if constexpr (WHOLE) {
-      const int32_t count = end - begin;
-      const uint64_t inside = count >= SIZE ? kAll : (uint64_t{1} << count) - 1;
-      return page < 0 ? 0 : inside;
-    }
-    return __ballot(page >= 0) & kAll;
+    const int32_t count = end - begin;
+    const uint64_t inside = count >= SIZE ? kAll : (uint64_t{1} << count) - 1;
+    return __ballot(cache.held(page)) & inside;
   }
   __device__ __forceinline__ uint32_t slot(int32_t key) const {
     const uint32_t k = static_cast<uint32_t>(key);
@@ -125,15 +157,33 @@ struct Finder {
   }
 };
 
-template <typename T, int DP, int KB, Reads READS, bool WHOLE>
-__global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void cache_tile_kernel(
-    Call call, Results<T> results, Heads<const T> query, Side<T> side) {
+template <typename T, int DP, Reads READS>
+struct TileSpace {
+  static constexpr int KB = tile_blocks<T, DP>();
+  // Three tiles, two of them on their way, where a CU's 160 KB hold them for all workgroups
+  // that its registers hold, and every wave has as many loads of a tile.
+  static constexpr int kTileBytes = 2 * KB * kBlock * DP * sizeof(T);
+  static constexpr int kBuffers =
+      READS == Reads::Aligned && KB * kBlock * DP * sizeof(T) / 16 % kThreads == 0 &&
+              3 * kTileBytes * tile_waves<T, DP>() <= 160 * 1024
+          ? 3
+          : 2;
+  Tile<T, KB * kBlock, DP, READS, kBuffers> keys, values;
+};
+
+// A workgroup's 64 rows and its share of the keys, in tiles that its waves share.
+template <typename T, int DP, Reads READS>
+__device__ __forceinline__ void tile_part(TileSpace<T, DP, READS>& space, const Call& call,
+                                          const Results<T>& results, const Heads<const T>& query,
+                                          const Side<T>& side, uint32_t index) {
+  constexpr int KB = TileSpace<T, DP, READS>::KB;
   constexpr int KT = KB * kBlock;
   constexpr int W = Vec16<T>::width;
   constexpr uint32_t kRows = kWaves * kBlock;
-  __shared__ Tile<T, KT, DP, READS> keys, values;
-  const uint32_t unit = blockIdx.x % side.units;
-  const uint32_t rest = blockIdx.x / side.units;
+  auto& keys = space.keys;
+  auto& values = space.values;
+  const uint32_t unit = index % side.units;
+  const uint32_t rest = index / side.units;
   // Row tiles side by side: they read the same keys.
   const uint32_t split = rest / side.row_tiles;
   const uint32_t row_tile = side.row_tiles - 1 - (rest - split * side.row_tiles);
@@ -149,64 +199,100 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void cache_tile_ke
   const int32_t high =
       side.own ? row_at(call, side, u, key_head, end_row - 1, side_length).limit + 1
                : side_length;
-  const uint32_t tiles = static_cast<uint32_t>(high + KT - 1) / KT;
-  const uint32_t begin_tile =
-      static_cast<uint32_t>(static_cast<uint64_t>(tiles) * split / side.splits);
-  const uint32_t end_tile =
-      static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / side.splits);
+  uint32_t begin_tile, end_tile;
+  share_of<KT>(side, high, split, begin_tile, end_tile);
 
-  const Finder<T, KT, WHOLE> finder{side.cache, u};
-  typename Tile<T, KT, DP, READS>::Stage next_keys, next_values;
-  if constexpr (WHOLE) {
-    keys.prepare(next_keys, call.extent, [&](uint32_t j) { return j * side.cache.key.token; });
-    values.prepare(next_values, call.extent,
-                   [&](uint32_t j) { return j * side.cache.value.token; });
-  }
-  int32_t page = -1;          // found for the next tile to start
-  uint64_t present = 0, next_present = 0;
+  constexpr int B = TileSpace<T, DP, READS>::kBuffers;
+  using KeyTile = Tile<T, KT, DP, READS, B>;
+  Finder<T, KT> finder(side.cache, u, side.whole);
+  typename KeyTile::Stage next_keys, next_values;
+  keys.prepare(next_keys, call.extent, [&](uint32_t j) { return j * side.cache.key.token; });
+  values.prepare(next_values, call.extent, [&](uint32_t j) { return j * side.cache.value.token; });
+  int32_t page = 0;                           // found for the next tile to start
+  // Where pages hold whole tiles: the next tile's place in its page.
+  const T* key_at = nullptr;
+  const T* value_at = nullptr;
+  int32_t page_left = 0;  // tokens
+  bool page_held = false;
+  constexpr uint64_t kAll = (uint64_t{1} << KT) - 1;
+  uint64_t present[B] = {};                   // of the current tile and those behind it
+  int to = 0;                                 // buffer of the next tile to start
   const auto look = [&](uint32_t i) {
-    page = i < end_tile ? finder.look(static_cast<int32_t>(i) * KT, high, wave_lane) : -1;
+    if (!side.whole && i < end_tile) {
+      page = finder.page_of(static_cast<int32_t>(i) * KT, high, wave_lane);
+    }
   };
   // Starts tile i, whose pages have been looked up, and looks for those of the next.
   const auto start = [&](uint32_t i) {
     const int32_t begin = static_cast<int32_t>(i) * KT;
-    next_present = finder.present(page, begin, high);
-    if constexpr (WHOLE) {
-      const int32_t at = __builtin_amdgcn_readfirstlane(page);
-      if (at >= 0) {
+    uint64_t there;
+    if (side.whole) {
+      if (page_left <= 0) {
+        const int32_t only = finder.only_page(begin);
         const uint32_t slot = finder.slot(begin);
-        const uint32_t count = static_cast<uint32_t>(high - begin);
+        page_held = side.cache.held(only);
+        page_left = static_cast<int32_t>(side.cache.page_tokens.divisor - slot);
+        key_at = finder.head(side.cache.key, key_head, only, slot);
+        value_at = finder.head(side.cache.value, key_head, only, slot);
+      }
+      const uint32_t count = static_cast<uint32_t>(high - begin);
+      there = !page_held ? 0 : count >= KT ? kAll : (uint64_t{1} << count) - 1;
+      if (page_held) {
         // Rows behind the last key repeat the tile's first, and no row sees them.
         const auto in = [&](uint32_t j) { return static_cast<uint64_t>(j < count ? j : 0); };
-        keys.start(next_keys, i % 2, finder.head(side.cache.key, key_head, at, slot),
-                   count >= KT, call.extent,
+        keys.start(next_keys, to, key_at, count >= KT, call.extent,
                    [&](uint32_t j) { return in(j) * side.cache.key.token; });
-        values.start(next_values, i % 2, finder.head(side.cache.value, key_head, at, slot),
-                     count >= KT, call.extent,
+        values.start(next_values, to, value_at, count >= KT, call.extent,
                      [&](uint32_t j) { return in(j) * side.cache.value.token; });
       }
+      key_at += KT * side.cache.key.token;
+      value_at += KT * side.cache.value.token;
+      page_left -= KT;
     } else {
+      there = finder.present(page, begin, high);
       const uint32_t slot = finder.slot(begin + wave_lane % KT);
       const auto row = [&](const PageHeads<const T>& heads) {
         return [&](int, uint32_t j) {
           const int32_t at = __shfl(page, j, kWave);
           const uint32_t in = __shfl(slot, j, kWave);
-          return at < 0 ? reinterpret_cast<const T*>(kNothing)
-                        : finder.head(heads, key_head, at, in);
+          return (there >> j & 1U) != 0 ? finder.head(heads, key_head, at, in)
+                                        : reinterpret_cast<const T*>(kNothing);
         };
       };
-      keys.start_rows(next_keys, i % 2, call.extent, row(side.cache.key));
-      values.start_rows(next_values, i % 2, call.extent, row(side.cache.value));
+      keys.start_rows(next_keys, to, call.extent, row(side.cache.key));
+      values.start_rows(next_values, to, call.extent, row(side.cache.value));
     }
+    present[B - 1] = there;
+    to = to + 1 < B ? to + 1 : 0;
     look(i + 1);
   };
-  const auto finish = [&](uint32_t i) {
-    keys.finish(next_keys, i % 2);
-    values.finish(next_values, i % 2);
-    present = next_present;
+  // Waits for the tile behind the current one, which becomes the current one: for all loads
+  // but those of a tile started after it.
+  const auto finish = [&](int at) {
+    if constexpr (B > 2) {
+      if (present[B - 1] != 0) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * KeyTile::kShare) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+    } else {
+      keys.finish(next_keys, at);
+      values.finish(next_values, at);
+    }
+#pragma unroll
+    for (int n = 0; n + 1 < B; ++n) present[n] = present[n + 1];
+    present[B - 1] = 0;
   };
   look(begin_tile);
-  if (begin_tile < end_tile) start(begin_tile);
+#pragma unroll
+  for (int n = 0; n + 1 < B; ++n) {
+    if (n != 0) {
+#pragma unroll
+      for (int m = 0; m + 1 < B; ++m) present[m] = present[m + 1];
+      present[B - 1] = 0;
+    }
+    if (begin_tile + n < end_tile) start(begin_tile + n);
+  }
 
   const uint32_t wave_row = begin_row + wave * kBlock;
   const uint32_t r = wave_row + lane.column;
@@ -230,19 +316,20 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void cache_tile_ke
   q.finish(limit >= 0, call.extent, lane.quarter, static_cast<T>(call.scale * kLog2E));
   Row<T, DP> row;
   row.out.clear();
-  if (begin_tile < end_tile) finish(begin_tile);
+  int at = 0;  // buffer of the current tile
+  if (begin_tile < end_tile) finish(at);
 
   for (uint32_t i = begin_tile; i < end_tile; ++i) {
     const int32_t begin = static_cast<int32_t>(i) * KT;
     __syncthreads();
-    if (i + 1 < end_tile) start(i + 1);
+    if (i + B - 1 < end_tile) start(i + B - 1);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       const int32_t k0 = begin + kb * kBlock, k1 = k0 + kBlock - 1;
-      const uint32_t there = static_cast<uint32_t>(present >> (kb * kBlock)) & 0xffffU;
+      const uint32_t there = static_cast<uint32_t>(present[0] >> (kb * kBlock)) & 0xffffU;
       if (there == 0 || k0 > newest) continue;
-      const T* key_rows = keys.value[i % 2] + kb * kBlock * DP;
-      const T* value_rows = values.value[i % 2] + kb * kBlock * DP;
+      const T* key_rows = keys.value[at] + kb * kBlock * DP;
+      const T* value_rows = values.value[at] + kb * kBlock * DP;
       typename Mma<T>::Acc s{0, 0, 0, 0};
       const auto read = [&](int p) { return lane.along(key_rows, p); };
       Queue<2, typename Vec16<T>::type> queue;
@@ -267,12 +354,14 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void cache_tile_ke
       row.take(score);
       across.run(row.out, score);
     }
-    if (i + 1 < end_tile) finish(i + 1);
+    at = at + 1 < B ? at + 1 : 0;
+    if (i + 1 < end_tile) finish(at);
   }
   const T total = quarter_sum(row.total);
   if (!held) return;
   T* target = part_row(call, results, row_place, side.first_part + split, row.base, total,
                        lane.quarter == 0);
+  if (begin_tile >= end_tile && results.splits != 1) return;
   const T over = total == T(0) ? T(0) : T(1) / total;
   row.out.visit(lane.quarter, [&](uint32_t d, auto& run) {
     // No weights: nothing, also where what they would have met is not finite.
@@ -281,16 +370,25 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void cache_tile_ke
   });
 }
 
-template <typename T, int DP, Reads READS, bool WHOLE>
-__global__ __launch_bounds__(kThreads) void cache_token_kernel(Call call, Results<T> results,
-                                                               Heads<const T> query,
-                                                               Side<T> side) {
+template <typename T, int DP>
+struct TokenSpace {
+  T outs[kWaves][kBlock][DP + Vec16<T>::width];
+  T tops[kWaves][kBlock], totals[kWaves][kBlock];
+};
+
+// A workgroup's 16 rows and its share of the keys, of which each wave takes every fourth
+// block from memory.
+template <typename T, int DP, Reads READS>
+__device__ __forceinline__ void token_part(TokenSpace<T, DP>& space, const Call& call,
+                                           const Results<T>& results,
+                                           const Heads<const T>& query, const Side<T>& side,
+                                           uint32_t index) {
   constexpr int W = Vec16<T>::width;
-  constexpr int kPitch = DP + W;
-  __shared__ T outs[kWaves][kBlock][kPitch];
-  __shared__ T tops[kWaves][kBlock], totals[kWaves][kBlock];
-  const uint32_t unit = blockIdx.x % side.units;
-  const uint32_t rest = blockIdx.x / side.units;
+  auto& outs = space.outs;
+  auto& tops = space.tops;
+  auto& totals = space.totals;
+  const uint32_t unit = index % side.units;
+  const uint32_t rest = index / side.units;
   const uint32_t split = rest / side.row_tiles;
   const uint32_t row_tile = side.row_tiles - 1 - (rest - split * side.row_tiles);
   const uint32_t u = unit / call.key_heads, key_head = unit % call.key_heads;
@@ -304,18 +402,24 @@ __global__ __launch_bounds__(kThreads) void cache_token_kernel(Call call, Result
   const int32_t high =
       side.own ? row_at(call, side, u, key_head, end_row - 1, side_length).limit + 1
                : side_length;
-  const uint32_t blocks = static_cast<uint32_t>(high + kBlock - 1) / kBlock;
-  const uint32_t begin_block =
-      static_cast<uint32_t>(static_cast<uint64_t>(blocks) * split / side.splits);
-  const uint32_t end_block =
-      static_cast<uint32_t>(static_cast<uint64_t>(blocks) * (split + 1) / side.splits);
+  uint32_t begin_block, end_block;
+  share_of<kBlock>(side, high, split, begin_block, end_block);
+  if (begin_block >= end_block && results.splits != 1) {
+    if (threadIdx.x < end_row - begin_row) {
+      part_row(call, results, row_at(call, side, u, key_head, begin_row + threadIdx.x, side_length),
+               side.first_part + split, lowest_finite<T>(), T(0), true);
+    }
+    return;
+  }
 
-  const Finder<T, kBlock, WHOLE> finder{side.cache, u};
+  Finder<T, kBlock> finder(side.cache, u, side.whole);
+  int32_t next = 0;  // page found for the wave's next block
   const auto look = [&](uint32_t i) {
-    return i < end_block ? finder.look(static_cast<int32_t>(i) * kBlock, high, lane % kBlock)
-                         : -1;
+    if (!side.whole && i < end_block) {
+      next = finder.page_of(static_cast<int32_t>(i) * kBlock, high, lane);
+    }
   };
-  int32_t page = look(begin_block + wave);
+  look(begin_block + wave);
 
   const uint32_t r = begin_row + column;
   const bool held = r < side.rows;
@@ -337,14 +441,13 @@ __global__ __launch_bounds__(kThreads) void cache_token_kernel(Call call, Result
 
   for (uint32_t i = begin_block + wave; i < end_block; i += kWaves) {
     const int32_t begin = static_cast<int32_t>(i) * kBlock;
-    const uint32_t there =
-        static_cast<uint32_t>(finder.present(page, begin, high)) & 0xffffU;
-    const int32_t found = page;
-    page = look(i + kWaves);
+    const int32_t found = side.whole ? finder.only_page(begin) : next;
+    const uint32_t there = static_cast<uint32_t>(finder.present(found, begin, high));
+    look(i + kWaves);
     if (there == 0) continue;
     Operand<T, DP> k;
     AcrossOperand<T, DP> v;
-    if constexpr (WHOLE) {
+    if (side.whole) {
       const int32_t at = __builtin_amdgcn_readfirstlane(found);
       const uint32_t slot = finder.slot(begin);
       const uint32_t count = static_cast<uint32_t>(high - begin);
@@ -359,12 +462,14 @@ __global__ __launch_bounds__(kThreads) void cache_token_kernel(Call call, Result
       const uint32_t slot = finder.slot(begin + column);
       const T* nothing = reinterpret_cast<const T*>(kNothing);
       k.template load<READS>(
-          found < 0 ? nothing : finder.head(side.cache.key, key_head, found, slot), call.extent,
-          quarter);
+          (there >> column & 1U) != 0 ? finder.head(side.cache.key, key_head, found, slot)
+                                      : nothing,
+          call.extent, quarter);
       v.template load<READS>(call.extent, quarter, column, [&](int n) {
         const int32_t at = __shfl(found, n, kWave);
         const uint32_t in = __shfl(slot, n, kWave);
-        return at < 0 ? nothing : finder.head(side.cache.value, key_head, at, in);
+        return (there >> n & 1U) != 0 ? finder.head(side.cache.value, key_head, at, in)
+                                      : nothing;
       });
     }
     typename Mma<T>::Acc s{0, 0, 0, 0};
@@ -423,20 +528,322 @@ __global__ __launch_bounds__(kThreads) void cache_token_kernel(Call call, Result
   }
 }
 
+// Up to four rows (a token of a group of four query heads): products of 4 keys with 4 rows,
+// sixteen of them side by side in the 4x4x1 matrix instruction, where 16x16x4 would leave
+// three quarters or more of its columns unused.  The instruction takes one value per lane of
+// each operand (lane l: block l / 4, row or column l % 4) and adds one product to each of a
+// block's 4x4 results (lane l: column l % 4; the lane's four values are the rows).
+//   Scores: block b contracts d = 64 c + 4 b + i, i < 4, of keys 4 g + l % 4; the blocks'
+//   sums are added up across the wave and leave key 4 g + l / 16 of row l % 4 in each lane.
+//   Values: that lane's weight meets d = 64 c + 4 (l % 16) + i of its key as it stands.  The
+//   quarters' sums over their keys are added up once at the end.
+constexpr int kFewRows = 4;
+
+__device__ __forceinline__ f32x4 few_step(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_4x4x1f32(a, b, c, 0, 0, 0);
+}
+
+// Of four values in every lane, value l / 16, summed over the lanes of all quarters with
+// this l % 16.
+__device__ __forceinline__ float scattered_sum(const f32x4& x) {
+  const auto swapped = [](float a, float b, auto&& swap) {
+    const auto both = swap(__float_as_uint(a), __float_as_uint(b));
+    return __uint_as_float(both[0]) + __uint_as_float(both[1]);
+  };
+  const auto halves = [](uint32_t a, uint32_t b) {
+    return __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  };
+  const auto quarters = [](uint32_t a, uint32_t b) {
+    return __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  };
+  const float even = swapped(x[0], x[2], halves), odd = swapped(x[1], x[3], halves);
+  return swapped(even, odd, quarters);
+}
+
+// x of the lane that is LANES further in its row of 16, around its end.
+template <int LANES>
+__device__ __forceinline__ float rotated(float x) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x120 + LANES, 0xf,
+                                                     0xf, true));
+}
+
+template <int DP>
+constexpr int kFewChunks = (DP + 63) / 64;
+
+template <int DP>
+struct FewSpace {
+  float outs[kWaves][kFewRows][kFewChunks<DP> * 64 + 4];
+  float tops[kWaves][kFewRows], totals[kWaves][kFewRows];
+};
+
+// A workgroup's rows and its share of the keys, of which each wave takes every fourth block
+// of 16 from memory.
+template <int DP, Reads READS>
+__device__ __forceinline__ void few_part(FewSpace<DP>& space, const Call& call,
+                                         const Results<float>& results,
+                                         const Heads<const float>& query,
+                                         const Side<float>& side, uint32_t index) {
+  constexpr int C = kFewChunks<DP>;
+  constexpr int G = kBlock / 4;  // groups of four keys
+  // Beside tiles, whose products fill the matrix units whenever they may: the short work
+  // between two reads goes first.
+  __builtin_amdgcn_s_setprio(3);
+  const uint32_t unit = index % side.units, split = index / side.units;
+  const uint32_t u = unit / call.key_heads, key_head = unit % call.key_heads;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave;
+  const int quarter = lane / kBlock, column = lane % 4;
+
+  const int32_t side_length = side.length(u);
+  const int32_t high =
+      side.own ? row_at(call, side, u, key_head, side.rows - 1, side_length).limit + 1
+               : side_length;
+  uint32_t begin_block, end_block;
+  share_of<kBlock>(side, high, split, begin_block, end_block);
+  const bool held = static_cast<uint32_t>(column) < side.rows;
+  const RowAt row_place =
+      row_at(call, side, u, key_head, held ? column : side.rows - 1, side_length);
+  if (begin_block >= end_block && results.splits != 1) {
+    if (threadIdx.x < side.rows) {
+      part_row(call, results, row_place, side.first_part + split, lowest_finite<float>(), 0.0F,
+               true);
+    }
+    return;
+  }
+
+  Finder<float, kBlock> finder(side.cache, u, side.whole);
+  int32_t next = 0;  // page found for the wave's next block
+  const auto look = [&](uint32_t i) {
+    if (!side.whole && i < end_block) {
+      next = finder.page_of(static_cast<int32_t>(i) * kBlock, high, lane);
+    }
+  };
+  look(begin_block + wave);
+
+  const int32_t limit = held ? row_place.limit : -1;
+  int32_t oldest = held ? limit : INT32_MAX;
+  oldest = min(oldest, __shfl_xor(oldest, 1, kWave));
+  oldest = min(oldest, __shfl_xor(oldest, 2, kWave));
+  oldest = __builtin_amdgcn_readfirstlane(oldest);
+  const uint32_t key_d = lane / 4 * 4, value_d = lane % kBlock * 4;
+  const float* query_row = query.data + row_place.b * query.batch +
+                           row_place.head * query.head + row_place.t * query.token;
+  f32x4 q[C], out[C][4];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    q[c] = load_piece<READS>(query_row, 64 * c + key_d, call.extent);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool inside = (limit >= 0) & (64 * c + key_d + i < call.extent);
+      q[c][i] = inside ? q[c][i] * static_cast<float>(call.scale * kLog2E) : 0.0F;
+      out[c][i] = f32x4{0, 0, 0, 0};
+    }
+  }
+  float base = lowest_finite<float>(), total = 0.0F;
+
+  for (uint32_t i = begin_block + wave; i < end_block; i += kWaves) {
+    const int32_t begin = static_cast<int32_t>(i) * kBlock;
+    const int32_t found = side.whole ? finder.only_page(begin) : next;
+    const uint32_t there = static_cast<uint32_t>(finder.present(found, begin, high));
+    look(i + kWaves);
+    if (there == 0) continue;
+    f32x4 k[G][C], v[G][C];
+    if (side.whole) {
+      const int32_t at = __builtin_amdgcn_readfirstlane(found);
+      const uint32_t slot = finder.slot(begin);
+      const uint32_t count = static_cast<uint32_t>(high - begin);
+      const auto in = [&](uint32_t n) { return static_cast<uint64_t>(n < count ? n : 0); };
+      const float* key_base = finder.head(side.cache.key, key_head, at, slot);
+      const float* value_base = finder.head(side.cache.value, key_head, at, slot);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float* head = key_base + in(4 * g + column) * side.cache.key.token;
+#pragma unroll
+        for (int c = 0; c < C; ++c) k[g][c] = load_piece<READS>(head, 64 * c + key_d, call.extent);
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float* head = value_base + in(4 * g + quarter) * side.cache.value.token;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          v[g][c] = load_piece<READS>(head, 64 * c + value_d, call.extent);
+        }
+      }
+    } else {
+      const uint32_t slot = finder.slot(begin + lane % kBlock);
+      const auto head_of = [&](const PageHeads<const float>& heads, int n) {
+        const int32_t at = __shfl(found, n, kWave);
+        const uint32_t in = __shfl(slot, n, kWave);
+        return (there >> n & 1U) != 0 ? finder.head(heads, key_head, at, in)
+                                      : reinterpret_cast<const float*>(kNothing);
+      };
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float* head = head_of(side.cache.key, 4 * g + column);
+#pragma unroll
+        for (int c = 0; c < C; ++c) k[g][c] = load_piece<READS>(head, 64 * c + key_d, call.extent);
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float* head = head_of(side.cache.value, 4 * g + quarter);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          v[g][c] = load_piece<READS>(head, 64 * c + value_d, call.extent);
+        }
+      }
+    }
+    const bool whole = (begin + kBlock - 1 <= oldest) & (there == 0xffffU);
+    float score[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      f32x4 s{0, 0, 0, 0};
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) s = few_step(k[g][c][n], q[c][n], s);
+      }
+      float sum = scattered_sum(s);
+      sum += rotated<8>(sum);
+      sum += rotated<4>(sum);
+      const int at = 4 * g + quarter;
+      const bool visible = whole | ((begin + at <= limit) & ((there >> at & 1U) != 0));
+      score[g] = visible ? sum : lowest<float>();
+    }
+    float top = larger(larger(score[0], score[1]), larger(score[2], score[3]));
+    constexpr float kSlack = Row<float, DP>::kSlack;
+    if (__any(top > base + kSlack)) {
+      top = quarter_max(top);
+      const float next = top > base + kSlack ? top : base;
+      const float shrink = exp2_of(base - next);
+      total *= shrink;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+#pragma unroll
+          for (int m = 0; m < 4; ++m) out[c][n][m] *= shrink;
+        }
+      }
+      base = next;
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float weight = exp2_of(score[g] - base);
+      total += weight;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) out[c][n] = few_step(v[g][c][n], weight, out[c][n]);
+      }
+    }
+  }
+  total = quarter_sum(total);
+  if (lane < kFewRows) {
+    space.tops[wave][lane] = base;
+    space.totals[wave][lane] = total;
+  }
+  // out[c][n][m] is d = 64 c + 16 (l % 16 / 4) + 4 m + n of row l % 4, over the quarter's keys.
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    f32x4 piece;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) piece[n] = scattered_sum(out[c][n]);
+    const int d = 64 * c + lane % kBlock / 4 * 16 + 4 * quarter;
+    *reinterpret_cast<f32x4*>(&space.outs[wave][column][d]) = piece;
+  }
+  __syncthreads();
+  // Lane by lane over the rows' pieces: the waves in order.
+  constexpr int kPieces = C * 16;
+  const int r = threadIdx.x / kPieces, d = threadIdx.x % kPieces * 4;
+  if (static_cast<uint32_t>(r) >= side.rows || static_cast<uint32_t>(d) >= call.extent) return;
+  float most = space.tops[0][r];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) most = larger(space.tops[w][r], most);
+  float sum = 0.0F;
+  float run[4] = {};
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float shrink = exp2_of(space.tops[w][r] - most);
+    const float part = space.totals[w][r];
+    sum += part * shrink;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) run[j] += part == 0.0F ? 0.0F : space.outs[w][r][d + j] * shrink;
+  }
+  const float over = sum == 0.0F ? 0.0F : 1.0F / sum;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) run[j] *= over;
+  const RowAt place = row_at(call, side, u, key_head, r, side_length);
+  float* target = part_row(call, results, place, side.first_part + split, most, sum, d == 0);
+  store_piece(target, d, call.extent, run);
+}
+static_assert(kThreads >= kFewRows * kFewChunks<SPAR_HIP_ATTENTION_MAX_EXTENT> * 16);
+
+// How a side is computed.
+enum class Kind { Few, Tokens, Tiles };
+
+template <typename T, int DP, Reads READS, Kind KIND>
+struct Space {
+  using type = TokenSpace<T, DP>;
+};
+template <typename T, int DP, Reads READS>
+struct Space<T, DP, READS, Kind::Tiles> {
+  using type = TileSpace<T, DP, READS>;
+};
+template <typename T, int DP, Reads READS>
+struct Space<T, DP, READS, Kind::Few> {
+  using type = FewSpace<DP>;
+};
+
+template <typename T, int DP, Reads READS, Kind KIND>
+__device__ __forceinline__ void side_part(char* space, const Call& call, const Results<T>& results,
+                                          const Heads<const T>& query, const Side<T>& side,
+                                          uint32_t index) {
+  constexpr Reads kReads = READS == Reads::Aligned ? Reads::Pieces : READS;
+  auto& mine = *reinterpret_cast<typename Space<T, DP, READS, KIND>::type*>(space);
+  if constexpr (KIND == Kind::Tiles) {
+    tile_part<T, DP, READS>(mine, call, results, query, side, index);
+  } else if constexpr (KIND == Kind::Tokens) {
+    token_part<T, DP, kReads>(mine, call, results, query, side, index);
+  } else {
+    few_part<DP, kReads>(mine, call, results, query, side, index);
+  }
+}
+
+// The prefixes' workgroups come first: their products keep the matrix units busy while the
+// others, which fill what room they leave on a CU, read the sequences' own keys.
+template <typename T, int DP, Reads READS, Kind PREFIX, Kind OWN>
+__global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void cache_kernel(
+    Call call, Results<T> results, Heads<const T> query, Side<T> prefix, Side<T> own,
+    uint32_t prefix_groups) {
+  constexpr size_t kPrefixBytes = sizeof(typename Space<T, DP, READS, PREFIX>::type);
+  constexpr size_t kOwnBytes = sizeof(typename Space<T, DP, READS, OWN>::type);
+  __shared__ alignas(16) char space[kPrefixBytes > kOwnBytes ? kPrefixBytes : kOwnBytes];
+  const bool mine = blockIdx.x >= prefix_groups;
+  const uint32_t index = mine ? blockIdx.x - prefix_groups : blockIdx.x;
+  if constexpr (PREFIX == OWN) {
+    const Side<T>& side = mine ? own : prefix;
+    side_part<T, DP, READS, OWN>(space, call, results, query, side, index);
+  } else if (mine) {
+    side_part<T, DP, READS, OWN>(space, call, results, query, own, index);
+  } else {
+    side_part<T, DP, READS, PREFIX>(space, call, results, query, prefix, index);
+  }
+}
+
 // ---------------------------------------------------------------- launchers
 
 // As in the forward over a contiguous cache: up to this many rows of a unit the waves share
 // rows and split keys; workgroups that row tiles are split up to, and the fewest keys that
 // repay a part.
 constexpr uint64_t kTokenRows = 32;
-constexpr uint64_t kFullGrid = 768;
-constexpr uint64_t kTokenGrid = 1024;
+constexpr uint64_t kFullGrid = 512;
+constexpr uint64_t kTokenGrid = 512;
 constexpr uint64_t kFewestKeys = 256;
-constexpr uint64_t kFewestTokenKeys = 128;
+constexpr uint64_t kFewestTokenKeys = 64;
 
 struct SidePlan {
-  bool token;
-  uint64_t units, rows, row_tiles, splits;
+  Kind kind;
+  uint64_t units, rows, row_tiles, splits, least;
   uint64_t groups() const { return units * row_tiles * splits; }
 };
 
@@ -458,17 +865,26 @@ SidePlan side_plan(const SparHipCacheAttention& a, uint64_t rows_of_cache, uint6
   plan.units = rows_of_cache * a.key_heads;
   plan.rows = sharers * a.queries * (a.query_heads / a.key_heads);
   constexpr uint64_t kRows = kWaves * kBlock;
-  plan.token = plan.rows <= kTokenRows ||
-               spreads((plan.rows + kRows - 1) / kRows * plan.units *
-                       std::max<uint64_t>(1, room / kFewestKeys));
-  const uint64_t tile_rows = plan.token ? kBlock : kRows;
-  plan.row_tiles = (plan.rows + tile_rows - 1) / tile_rows;
-  const uint64_t wanted = (plan.token ? kTokenGrid : kFullGrid) /
-                          std::max<uint64_t>(1, plan.row_tiles * plan.units);
-  plan.splits = std::max<uint64_t>(
-      1, std::min({wanted, room / (plan.token ? kFewestTokenKeys : kFewestKeys),
-                   uint64_t{kMostParts / 2}}));
+  const bool tiles = plan.rows > kTokenRows &&
+                     !spreads((plan.rows + kRows - 1) / kRows * plan.units *
+                              std::max<uint64_t>(1, room / kFewestKeys));
+  const bool few = a.dtype == SPAR_HIP_FLOAT32 && plan.rows <= kFewRows;
+  plan.kind = tiles ? Kind::Tiles : few ? Kind::Few : Kind::Tokens;
   return plan;
+}
+
+// Workgroups of a side whose kind is settled.
+void divide(SidePlan& plan, uint64_t room) {
+  constexpr uint64_t kRows = kWaves * kBlock;
+  const bool tiles = plan.kind == Kind::Tiles;
+  const uint64_t tile_rows = tiles ? kRows : kBlock;
+  const uint64_t least = tiles ? kFewestKeys : kFewestTokenKeys;
+  plan.row_tiles = (plan.rows + tile_rows - 1) / tile_rows;
+  const uint64_t wanted = (tiles ? kFullGrid : kTokenGrid) /
+                          std::max<uint64_t>(1, plan.row_tiles * plan.units);
+  plan.splits =
+      std::max<uint64_t>(1, std::min({wanted, room / least, uint64_t{kMostParts / 2}}));
+  plan.least = least / kBlock;
 }
 
 Plan plan_of(const SparHipCacheAttention& a, const SparHipPages& cache,
@@ -478,7 +894,11 @@ Plan plan_of(const SparHipCacheAttention& a, const SparHipPages& cache,
   plan.own = side_plan(a, a.batch, 1, room_of(&cache));
   if (room_of(prefix) != 0) {
     plan.prefix = side_plan(a, a.prefixes, a.batch / a.prefixes, room_of(prefix));
+    // There is no launch of fewer rows before more: a prefix has the more rows.
+    if (plan.prefix.kind < plan.own.kind) plan.prefix.kind = plan.own.kind;
+    divide(plan.prefix, room_of(prefix));
   }
+  divide(plan.own, room_of(&cache));
   plan.parts = static_cast<uint32_t>(plan.own.splits + plan.prefix.splits);
   const uint64_t size = a.dtype == SPAR_HIP_FLOAT32 ? sizeof(float) : sizeof(double);
   const uint64_t piece = 16 / size;
@@ -490,7 +910,7 @@ Plan plan_of(const SparHipCacheAttention& a, const SparHipPages& cache,
 // A launch counts its workgroups in 32 bits of work-items.
 bool fits(const Plan& plan) {
   return plan.own.groups() <= kMostGroups && plan.prefix.groups() <= kMostGroups &&
-         plan.rows <= kMostGroups;
+         plan.own.groups() + plan.prefix.groups() <= kMostGroups && plan.rows <= kMostGroups;
 }
 
 // Whether a cache's keys and values go to LDS directly.
@@ -500,9 +920,8 @@ bool pages_aligned(const SparHipPages& cache) {
 }
 
 template <typename T>
-void start_side(const SparHipCacheAttention& a, const SparHipPages& cache, const SidePlan& plan,
-                const Call& call, const Results<T>& results, const Heads<const T>& query,
-                bool own, uint32_t first_part, hipStream_t stream) {
+Side<T> side_of(const SparHipCacheAttention& a, const SparHipPages& cache, const SidePlan& plan,
+                bool own, uint32_t first_part, int block) {
   Side<T> side{};
   side.cache = pages_of<const T>(cache);
   side.lengths = own ? a.lengths : a.prefix_lengths;
@@ -514,38 +933,11 @@ void start_side(const SparHipCacheAttention& a, const SparHipPages& cache, const
   side.rows = static_cast<uint32_t>(plan.rows);
   side.row_tiles = static_cast<uint32_t>(plan.row_tiles);
   side.splits = static_cast<uint32_t>(plan.splits);
+  side.least = static_cast<uint32_t>(plan.least);
   side.first_part = first_part;
-  const uint32_t grid = static_cast<uint32_t>(plan.groups());
-  const bool pieces = a.extent % Vec16<T>::width == 0;
-  with_padded_width(a.extent, [&](auto width) {
-    constexpr int DP = decltype(width)::value;
-    if (plan.token) {
-      const bool whole = cache.table == nullptr || cache.page_tokens % kBlock == 0;
-      if (pieces && whole) {
-        cache_token_kernel<T, DP, Reads::Pieces, true>
-            <<<grid, kThreads, 0, stream>>>(call, results, query, side);
-      } else if (pieces) {
-        cache_token_kernel<T, DP, Reads::Pieces, false>
-            <<<grid, kThreads, 0, stream>>>(call, results, query, side);
-      } else {
-        cache_token_kernel<T, DP, Reads::Single, false>
-            <<<grid, kThreads, 0, stream>>>(call, results, query, side);
-      }
-      return;
-    }
-    constexpr int KB = tile_blocks<T, DP>();
-    const bool whole = cache.table == nullptr || cache.page_tokens % (KB * kBlock) == 0;
-    if (pieces && pages_aligned<T>(cache) && whole) {
-      cache_tile_kernel<T, DP, KB, Reads::Aligned, true>
-          <<<grid, kThreads, 0, stream>>>(call, results, query, side);
-    } else if (pieces && pages_aligned<T>(cache)) {
-      cache_tile_kernel<T, DP, KB, Reads::Aligned, false>
-          <<<grid, kThreads, 0, stream>>>(call, results, query, side);
-    } else {
-      cache_tile_kernel<T, DP, KB, Reads::Single, false>
-          <<<grid, kThreads, 0, stream>>>(call, results, query, side);
-    }
-  });
+  side.whole = cache.table == nullptr ||
+               cache.page_tokens % (plan.kind == Kind::Tiles ? block : kBlock) == 0;
+  return side;
 }
 
 template <typename T>
@@ -573,12 +965,51 @@ void start(const SparHipCacheAttention& a, const Plan& plan, const SparHipHeads&
     results.part_total = results.part_top + plan.parts * plan.rows;
   }
   const auto q = heads_of<const T>(query);
-  if (plan.prefix.splits != 0) {
-    start_side<T>(a, *prefix, plan.prefix, call, results, q, false, 0, stream);
-  }
-  start_side<T>(a, cache, plan.own, call, results, q, true,
-                static_cast<uint32_t>(plan.prefix.splits), stream);
-  if (plan.parts > 1) join_parts(call, results, stream);
+  const bool shared = plan.prefix.splits != 0;
+  // Only tiles ask for heads at multiples of 16 bytes.
+  const auto reads_pieces = [&](const SparHipPages& pages, const SidePlan& side) {
+    return side.kind != Kind::Tiles || pages_aligned<T>(pages);
+  };
+  const bool pieces = a.extent % Vec16<T>::width == 0 && reads_pieces(cache, plan.own) &&
+                      (!shared || reads_pieces(*prefix, plan.prefix));
+  const uint32_t before_own = static_cast<uint32_t>(plan.prefix.groups());
+  const uint32_t grid = static_cast<uint32_t>(plan.prefix.groups() + plan.own.groups());
+  with_padded_width(a.extent, [&](auto width) {
+    constexpr int DP = decltype(width)::value;
+    constexpr int block = tile_blocks<T, DP>() * kBlock;
+    const Side<T> before =
+        shared ? side_of<T>(a, *prefix, plan.prefix, false, 0, block) : Side<T>{};
+    const Side<T> own = side_of<T>(a, cache, plan.own, true,
+                                   static_cast<uint32_t>(plan.prefix.splits), block);
+    const auto launch = [&](auto kernel) {
+      kernel<<<grid, kThreads, 0, stream>>>(call, results, q, before, own, before_own);
+    };
+    const auto with_kinds = [&](auto reads) {
+      constexpr Reads READS = decltype(reads)::value;
+      const Kind kind = plan.own.kind, prefix_kind = shared ? plan.prefix.kind : kind;
+      if (kind == Kind::Tiles) {
+        launch(cache_kernel<T, DP, READS, Kind::Tiles, Kind::Tiles>);
+      } else if (kind == Kind::Tokens && prefix_kind == Kind::Tiles) {
+        launch(cache_kernel<T, DP, READS, Kind::Tiles, Kind::Tokens>);
+      } else if (kind == Kind::Tokens) {
+        launch(cache_kernel<T, DP, READS, Kind::Tokens, Kind::Tokens>);
+      } else if constexpr (std::is_same_v<T, float>) {
+        if (prefix_kind == Kind::Tiles) {
+          launch(cache_kernel<T, DP, READS, Kind::Tiles, Kind::Few>);
+        } else if (prefix_kind == Kind::Tokens) {
+          launch(cache_kernel<T, DP, READS, Kind::Tokens, Kind::Few>);
+        } else {
+          launch(cache_kernel<T, DP, READS, Kind::Few, Kind::Few>);
+        }
+      }
+    };
+    if (pieces) {
+      with_kinds(std::integral_constant<Reads, Reads::Aligned>{});
+    } else {
+      with_kinds(std::integral_constant<Reads, Reads::Single>{});
+    }
+  });
+  if (plan.parts > 1) join_parts<T, true>(call, results, stream);
 }
 
 bool valid_call(const SparHipCacheAttention* a, const SparHipPages* cache,

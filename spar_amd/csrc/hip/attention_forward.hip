@@ -407,7 +407,7 @@ void start(const SparHipAttention& a, const Plan& plan, const SparHipHeads& outp
     tile_kernel<T, DP, tile_blocks<T, DP>(), READS>
         <<<grid, kThreads, 0, stream>>>(call, results, q, k, v, plan.row_tiles);
   });
-  if (plan.splits > 1) join_parts(call, results, stream);
+  if (plan.splits > 1) join_parts<T, false>(call, results, stream);
 }
 
 }  // namespace

@@ -50,7 +50,8 @@ __device__ __forceinline__ T* output_row(const Call& call, const Results<T>& res
          t * results.output.token;
 }
 
-template <typename T>
+// EMPTY: parts of no weight (a total of 0) hold nothing but that.
+template <typename T, bool EMPTY>
 __global__ __launch_bounds__(kThreads) void combine_few_kernel(Call call, Results<T> results) {
   constexpr int W = Vec16<T>::width;
   constexpr uint32_t kLanes = 32;
@@ -99,7 +100,7 @@ __global__ __launch_bounds__(kThreads) void combine_few_kernel(Call call, Result
     typename Vec16<T>::type x = {};
 #pragma unroll
     for (uint32_t s = 0; s < kFewParts; ++s) {
-      if (s < results.splits) x += piece[s] * weight[s];
+      if (s < results.splits && !(EMPTY && part_total[s] == T(0))) x += piece[s] * weight[s];
     }
     T run[W];
 #pragma unroll
@@ -113,12 +114,13 @@ __global__ __launch_bounds__(kThreads) void combine_few_kernel(Call call, Result
 
 // Many parts: a workgroup per row, the parts dealt out to its runs of lanes, whose
 // sums meet in a tree (128 rows of 128 in 32 parts 6 us, latency).
-template <typename T>
+template <typename T, bool EMPTY>
 __global__ __launch_bounds__(kThreads) void combine_kernel(Call call, Results<T> results) {
   constexpr int W = Vec16<T>::width;
   constexpr uint32_t kLanes = SPAR_HIP_ATTENTION_MAX_EXTENT / W / 2;  // two pieces each
   constexpr uint32_t kRuns = kThreads / kLanes;
   __shared__ T weights[kMostParts];
+  __shared__ T totals[EMPTY ? kMostParts : 1];
   __shared__ alignas(16) T outs[kRuns][SPAR_HIP_ATTENTION_MAX_EXTENT];
   __shared__ T waves[kWaves];
   const uint64_t row = blockIdx.x;
@@ -139,6 +141,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(Call call, Results<T>
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) top = larger(waves[w], top);
   weights[split] = exp2_of(part_top - top) * part_total;
+  if constexpr (EMPTY) totals[split] = part_total;
   __syncthreads();
   T sum = T(0);
   for (uint32_t s = 0; s < results.splits; ++s) sum += weights[s];
@@ -147,6 +150,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(Call call, Results<T>
   typename Vec16<T>::type x[2] = {};
 #pragma unroll 4
   for (uint32_t s = run; s < results.splits; s += kRuns) {
+    if (EMPTY && totals[s] == T(0)) continue;
     const T* part = results.part_output + (s * results.all_rows + row) * results.pitch;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -180,13 +184,13 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(Call call, Results<T>
 }
 static_assert(kThreads >= SPAR_HIP_ATTENTION_MAX_EXTENT);
 
-template <typename T>
+template <typename T, bool EMPTY>
 void join_parts(const Call& call, const Results<T>& results, hipStream_t stream) {
   if (results.splits <= kFewParts) {
-    combine_few_kernel<T>
+    combine_few_kernel<T, EMPTY>
         <<<ceil_div_u32(results.all_rows * 32, kThreads), kThreads, 0, stream>>>(call, results);
   } else {
-    combine_kernel<T>
+    combine_kernel<T, EMPTY>
         <<<static_cast<uint32_t>(results.all_rows), kThreads, 0, stream>>>(call, results);
   }
 }

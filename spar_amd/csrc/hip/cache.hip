@@ -70,7 +70,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Append<T> append, Turn
     const uint32_t at = static_cast<uint32_t>(place);
     const uint32_t entry = append.cache.page_tokens.div(at);
     const int32_t page = append.cache.page_at(static_cast<uint32_t>(b), entry);
-    if (page < 0) return;
+    if (!append.cache.held(page)) return;
     const PageHeads<T>& to = value ? append.cache.value : append.cache.key;
     target = to.data + static_cast<uint64_t>(page) * to.page +
              (at - entry * append.cache.page_tokens.divisor) * to.token;

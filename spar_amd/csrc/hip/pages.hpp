@@ -25,11 +25,13 @@ struct Pages {
   uint32_t room;  // tokens of a row
   FastDiv page_tokens;
 
-  // The page of entry `entry` of row b, less than 0 where it holds nothing.
+  // The number that entry `entry` of row b names; held() says whether there is such a page.
+  // A load's value is not looked at before that, so that it may be on its way meanwhile.
   __device__ __forceinline__ int32_t page_at(uint32_t b, uint32_t entry) const {
-    const int32_t page =
-        table == nullptr ? static_cast<int32_t>(b) : table[b * table_stride + entry];
-    return static_cast<uint32_t>(page) < pages ? page : -1;
+    return table == nullptr ? static_cast<int32_t>(b) : table[b * table_stride + entry];
+  }
+  __device__ __forceinline__ bool held(int32_t page) const {
+    return static_cast<uint32_t>(page) < pages;
   }
 };
 
