@@ -24,8 +24,10 @@ namespace spar_hip {
 namespace attention {
 namespace {
 
-// What stands in the place of a key that is not there.
-alignas(16) __device__ const double kNothing[SPAR_HIP_ATTENTION_MAX_EXTENT] = {};
+// What stands in the place of a key that is not there: zeros.  Not const, for which it would
+// lie in another address space than the caches, and pointers to either could be followed by
+// flat loads alone.
+alignas(16) __device__ double kNothing[SPAR_HIP_ATTENTION_MAX_EXTENT] = {};
 
 // One side of the keys: row u of its cache is read by `sharers` sequences from u *
 // sharers on, whose queries are the rows of its products: row r = (s * queries + t) *
@@ -577,14 +579,15 @@ struct FewSpace {
 };
 
 // A workgroup's rows and its share of the keys, of which each wave takes every fourth block
-// of 16 from memory.
+// from memory: the next block's loads are in flight while one is used.
 template <int DP, Reads READS>
 __device__ __forceinline__ void few_part(FewSpace<DP>& space, const Call& call,
                                          const Results<float>& results,
                                          const Heads<const float>& query,
                                          const Side<float>& side, uint32_t index) {
   constexpr int C = kFewChunks<DP>;
-  constexpr int G = kBlock / 4;  // groups of four keys
+  constexpr int SIZE = C == 1 ? 16 : 8;  // keys of a block
+  constexpr int G = SIZE / 4;            // groups of four keys
   // Beside tiles, whose products fill the matrix units whenever they may: the short work
   // between two reads goes first.
   __builtin_amdgcn_s_setprio(3);
@@ -599,7 +602,7 @@ __device__ __forceinline__ void few_part(FewSpace<DP>& space, const Call& call,
       side.own ? row_at(call, side, u, key_head, side.rows - 1, side_length).limit + 1
                : side_length;
   uint32_t begin_block, end_block;
-  share_of<kBlock>(side, high, split, begin_block, end_block);
+  share_of<SIZE>(side, high, split, begin_block, end_block);
   const bool held = static_cast<uint32_t>(column) < side.rows;
   const RowAt row_place =
       row_at(call, side, u, key_head, held ? column : side.rows - 1, side_length);
@@ -610,15 +613,6 @@ __device__ __forceinline__ void few_part(FewSpace<DP>& space, const Call& call,
     }
     return;
   }
-
-  Finder<float, kBlock> finder(side.cache, u, side.whole);
-  int32_t next = 0;  // page found for the wave's next block
-  const auto look = [&](uint32_t i) {
-    if (!side.whole && i < end_block) {
-      next = finder.page_of(static_cast<int32_t>(i) * kBlock, high, lane);
-    }
-  };
-  look(begin_block + wave);
 
   const int32_t limit = held ? row_place.limit : -1;
   int32_t oldest = held ? limit : INT32_MAX;
@@ -641,58 +635,71 @@ __device__ __forceinline__ void few_part(FewSpace<DP>& space, const Call& call,
   }
   float base = lowest_finite<float>(), total = 0.0F;
 
-  for (uint32_t i = begin_block + wave; i < end_block; i += kWaves) {
-    const int32_t begin = static_cast<int32_t>(i) * kBlock;
-    const int32_t found = side.whole ? finder.only_page(begin) : next;
-    const uint32_t there = static_cast<uint32_t>(finder.present(found, begin, high));
-    look(i + kWaves);
-    if (there == 0) continue;
+  // A block of keys and values on its way.  However few of its keys there are, it is as
+  // many loads: in the place of those that are not, ones that are harmless.
+  struct Stage {
     f32x4 k[G][C], v[G][C];
-    if (side.whole) {
-      const int32_t at = __builtin_amdgcn_readfirstlane(found);
-      const uint32_t slot = finder.slot(begin);
-      const uint32_t count = static_cast<uint32_t>(high - begin);
-      const auto in = [&](uint32_t n) { return static_cast<uint64_t>(n < count ? n : 0); };
-      const float* key_base = finder.head(side.cache.key, key_head, at, slot);
-      const float* value_base = finder.head(side.cache.value, key_head, at, slot);
+    int32_t begin;
+    uint32_t there;
+  };
+  const float* nothing = reinterpret_cast<const float*>(kNothing);
+  Finder<float, SIZE> finder(side.cache, u, side.whole);
+  int32_t next = 0;  // page found for the next block to fetch
+  const auto look = [&](uint32_t i) {
+    next = finder.page_of(static_cast<int32_t>(min(i, end_block - 1)) * SIZE, high, lane);
+  };
+  const auto load = [&](Stage& stage, auto&& key_of, auto&& value_of) {
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const float* head = key_base + in(4 * g + column) * side.cache.key.token;
+    for (int g = 0; g < G; ++g) {
+      const float* head = key_of(4 * g + column);
 #pragma unroll
-        for (int c = 0; c < C; ++c) k[g][c] = load_piece<READS>(head, 64 * c + key_d, call.extent);
-      }
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const float* head = value_base + in(4 * g + quarter) * side.cache.value.token;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-          v[g][c] = load_piece<READS>(head, 64 * c + value_d, call.extent);
-        }
-      }
-    } else {
-      const uint32_t slot = finder.slot(begin + lane % kBlock);
-      const auto head_of = [&](const PageHeads<const float>& heads, int n) {
-        const int32_t at = __shfl(found, n, kWave);
-        const uint32_t in = __shfl(slot, n, kWave);
-        return (there >> n & 1U) != 0 ? finder.head(heads, key_head, at, in)
-                                      : reinterpret_cast<const float*>(kNothing);
-      };
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const float* head = head_of(side.cache.key, 4 * g + column);
-#pragma unroll
-        for (int c = 0; c < C; ++c) k[g][c] = load_piece<READS>(head, 64 * c + key_d, call.extent);
-      }
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const float* head = head_of(side.cache.value, 4 * g + quarter);
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-          v[g][c] = load_piece<READS>(head, 64 * c + value_d, call.extent);
-        }
+      for (int c = 0; c < C; ++c) {
+        stage.k[g][c] = load_piece<READS>(head, 64 * c + key_d, call.extent);
       }
     }
-    const bool whole = (begin + kBlock - 1 <= oldest) & (there == 0xffffU);
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float* head = value_of(4 * g + quarter);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        stage.v[g][c] = load_piece<READS>(head, 64 * c + value_d, call.extent);
+      }
+    }
+  };
+  const auto fetch = [&](auto whole, Stage& stage, uint32_t i) {
+    const int32_t begin = static_cast<int32_t>(i) * SIZE;
+    stage.begin = begin;
+    if constexpr (decltype(whole)::value) {
+      const int32_t page = finder.only_page(begin);
+      stage.there = static_cast<uint32_t>(finder.present(page, begin, high));
+      const uint32_t slot = finder.slot(begin);
+      const uint32_t count = stage.there != 0 ? static_cast<uint32_t>(high - begin) : 1;
+      const auto in = [&](uint32_t n) { return static_cast<uint64_t>(n < count ? n : 0); };
+      const float* key_base =
+          stage.there != 0 ? finder.head(side.cache.key, key_head, page, slot) : nothing;
+      const float* value_base =
+          stage.there != 0 ? finder.head(side.cache.value, key_head, page, slot) : nothing;
+      load(
+          stage, [&](int n) { return key_base + in(n) * side.cache.key.token; },
+          [&](int n) { return value_base + in(n) * side.cache.value.token; });
+    } else {
+      const int32_t page = next;
+      stage.there = static_cast<uint32_t>(finder.present(page, begin, high));
+      look(i + kWaves);
+      const uint32_t slot = finder.slot(begin + lane % SIZE);
+      const auto head_of = [&](const PageHeads<const float>& heads, int n) {
+        const int32_t at = __shfl(page, n, kWave);
+        const uint32_t in = __shfl(slot, n, kWave);
+        return (stage.there >> n & 1U) != 0 ? finder.head(heads, key_head, at, in) : nothing;
+      };
+      load(
+          stage, [&](int n) { return head_of(side.cache.key, n); },
+          [&](int n) { return head_of(side.cache.value, n); });
+    }
+  };
+  const auto use = [&](const Stage& stage) {
+    constexpr uint32_t kAll = (1U << SIZE) - 1;
+    const bool whole = (stage.begin + SIZE - 1 <= oldest) & (stage.there == kAll);
     float score[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -700,21 +707,24 @@ __device__ __forceinline__ void few_part(FewSpace<DP>& space, const Call& call,
 #pragma unroll
       for (int c = 0; c < C; ++c) {
 #pragma unroll
-        for (int n = 0; n < 4; ++n) s = few_step(k[g][c][n], q[c][n], s);
+        for (int n = 0; n < 4; ++n) s = few_step(stage.k[g][c][n], q[c][n], s);
       }
       float sum = scattered_sum(s);
       sum += rotated<8>(sum);
       sum += rotated<4>(sum);
       const int at = 4 * g + quarter;
-      const bool visible = whole | ((begin + at <= limit) & ((there >> at & 1U) != 0));
+      const bool visible =
+          whole | ((stage.begin + at <= limit) & ((stage.there >> at & 1U) != 0));
       score[g] = visible ? sum : lowest<float>();
     }
-    float top = larger(larger(score[0], score[1]), larger(score[2], score[3]));
+    float top = score[0];
+#pragma unroll
+    for (int g = 1; g < G; ++g) top = larger(top, score[g]);
     constexpr float kSlack = Row<float, DP>::kSlack;
     if (__any(top > base + kSlack)) {
       top = quarter_max(top);
-      const float next = top > base + kSlack ? top : base;
-      const float shrink = exp2_of(base - next);
+      const float risen = top > base + kSlack ? top : base;
+      const float shrink = exp2_of(base - risen);
       total *= shrink;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
@@ -724,7 +734,7 @@ __device__ __forceinline__ void few_part(FewSpace<DP>& space, const Call& call,
           for (int m = 0; m < 4; ++m) out[c][n][m] *= shrink;
         }
       }
-      base = next;
+      base = risen;
     }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -733,9 +743,37 @@ __device__ __forceinline__ void few_part(FewSpace<DP>& space, const Call& call,
 #pragma unroll
       for (int c = 0; c < C; ++c) {
 #pragma unroll
-        for (int n = 0; n < 4; ++n) out[c][n] = few_step(v[g][c][n], weight, out[c][n]);
+        for (int n = 0; n < 4; ++n) out[c][n] = few_step(stage.v[g][c][n], weight, out[c][n]);
       }
     }
+  };
+  // Two blocks in turn; the last ones apart, and the two ways to find pages too: where a
+  // load may or may not have been made, the compiler waits for all.
+  const auto run_over = [&](auto whole) {
+    uint32_t i = begin_block + wave;
+    if (i >= end_block) return;
+    uint32_t left = (end_block - i + kWaves - 1) / kWaves;
+    Stage one, other;
+    if constexpr (!decltype(whole)::value) look(i);
+    fetch(whole, one, i);
+    for (; left > 2; left -= 2, i += 2 * kWaves) {
+      fetch(whole, other, i + kWaves);
+      use(one);
+      fetch(whole, one, i + 2 * kWaves);
+      use(other);
+    }
+    if (left == 2) {
+      fetch(whole, other, i + kWaves);
+      use(one);
+      use(other);
+    } else {
+      use(one);
+    }
+  };
+  if (side.whole) {
+    run_over(std::true_type{});
+  } else {
+    run_over(std::false_type{});
   }
   total = quarter_sum(total);
   if (lane < kFewRows) {
@@ -837,7 +875,7 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void cache_kernel(
 // repay a part.
 constexpr uint64_t kTokenRows = 32;
 constexpr uint64_t kFullGrid = 512;
-constexpr uint64_t kTokenGrid = 512;
+constexpr uint64_t kTokenGrid = 768;
 constexpr uint64_t kFewestKeys = 256;
 constexpr uint64_t kFewestTokenKeys = 64;
 
@@ -935,6 +973,7 @@ Side<T> side_of(const SparHipCacheAttention& a, const SparHipPages& cache, const
   side.splits = static_cast<uint32_t>(plan.splits);
   side.least = static_cast<uint32_t>(plan.least);
   side.first_part = first_part;
+  // (Few rows take blocks of 8 or 16 keys.)
   side.whole = cache.table == nullptr ||
                cache.page_tokens % (plan.kind == Kind::Tiles ? block : kBlock) == 0;
   return side;

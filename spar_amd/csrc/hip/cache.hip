@@ -121,7 +121,7 @@ void start_append(const Append<T>& append, uint64_t batch, uint64_t tokens, cons
   const uint64_t lanes = batch * tokens * units_of(turn.half, turn.extent) * heads;
   const bool stream_out =
       stream_output(batch * tokens * heads * static_cast<uint64_t>(turn.extent) * sizeof(T));
-  constexpr int kMany = 16 / sizeof(T);
+  constexpr int kMany = 8 / sizeof(T);
   with_policy(layout == SPAR_HIP_ROTARY_HALF, [&](auto half) {
     with_policy(stream_out, [&](auto nt) {
       if (lanes >= kMany * kFullLanes) {
