@@ -210,3 +210,25 @@ def test_reorder(hip, rows, source):
         for i, p in enumerate(parents):
             made[i, :width] = before[p, :width] if 0 <= p < source else 0
         assert np.array_equal(to.to_numpy(kind, target.shape), want)
+
+
+@pytest.mark.parametrize("dtype", [F32, F64])
+@pytest.mark.parametrize("beams,picks", [(64, 64), (64, 3), (7, 64)])
+def test_more_equal_totals_than_are_held_at_once(hip, dtype, beams, picks):
+    """All totals of a group are the same: the first tokens of its first beam."""
+    logits = np.zeros((2, beams, 20000), dtype)
+    scores, parents, tokens, _ = select(hip, logits, np.full((2, beams), -1.5), picks)
+    assert (parents == np.array([[0], [beams]])).all()
+    assert (tokens == np.arange(picks)).all()
+    total = -1.5 - np.log(20000.0)
+    bound = half_step(dtype) * abs(total) + oracle.select_bound(logits, dtype)
+    assert (np.abs(scores - total) <= bound).all()
+
+
+@pytest.mark.parametrize("place", [0, 2047, 2048, 4999])
+@pytest.mark.parametrize("dtype", [F32, F64])
+def test_one_logit_outweighs_all(hip, dtype, place):
+    """Its total is its score; others of the row follow far behind."""
+    logits, scores = inputs(1, 2, 5000, dtype, 23)
+    logits[0, 1, place] = 500
+    check(hip, logits, scores, 5)
