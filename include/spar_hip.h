@@ -285,7 +285,7 @@ struct SparHipReorder {
   void* output;
   uint64_t output_stride; /* in elements, at least row_elements */
   const void* input;
-  uint64_t input_stride;  /* in elements, any */
+  uint64_t input_stride;  /* in elements, also less or 0 */
   uint64_t row_elements;
   uint64_t element_size;  /* 4 or 8 bytes */
 };
@@ -857,6 +857,8 @@ struct SparHipStatus spar_hip_launch_beam_select(
 
 /* Rows of `state_count` states (host memory, read before the call returns; at most 2^16)
  * in the order of their parents: `rows` numbers in device memory, of [0, source_rows).
+ * Rows and strides have at most 2^40 elements, and a state at most 2^23 - 1 rows of up to 2^14 bytes,
+ * half as many of up to 2^15 and so on.
  * An output row whose parent lies outside becomes zeros.  Outputs must not overlap
  * inputs or each other. */
 struct SparHipStatus spar_hip_launch_reorder(const struct SparHipReorder* states,

@@ -714,7 +714,7 @@ extern "C" SparHipStatus spar_hip_launch_reorder(const SparHipReorder* states,
   }
   if (state_count == 0 || rows == 0) return ok();
   if (parents == nullptr) return invalid();
-  constexpr uint64_t kMost = uint64_t{1} << 48;  // elements, far beyond memory
+  constexpr uint64_t kMost = uint64_t{1} << 40;  // elements: beyond memory, and no product wraps
   for (uint64_t i = 0; i < state_count; ++i) {
     const SparHipReorder& s = states[i];
     if ((s.element_size != 4 && s.element_size != 8) || s.output_stride < s.row_elements ||

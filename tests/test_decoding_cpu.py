@@ -206,6 +206,12 @@ def test_reorder_refuses(state, changes):
     assert move(state, **changes) == 1
 
 
+@pytest.mark.parametrize("elements,rows", [(1 << 48, 1 << 27), (1 << 47, 1 << 28), (1 << 41, 4)])
+def test_reorder_refuses_more_than_its_products_hold(elements, rows):
+    # 2^48 elements of 8 bytes are 2^37 workgroups of 2^14 bytes a row: 2^64 in all
+    assert move((A, elements, A, elements, elements, 8), rows=rows) == 1
+
+
 def test_reorder_takes():
     assert move() == 0
     assert move((A, 8, A, 8, 8, 4), rows=0, parents=None) == 0
