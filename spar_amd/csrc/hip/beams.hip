@@ -130,10 +130,14 @@ __device__ __forceinline__ T compact(Kept<T>& kept, uint32_t count, uint32_t pic
       picks, [&](Key at) { return counted([&](int i) { return key[i] >= at; }); });
   const uint32_t above = counted([&](int i) { return key[i] > border; });
   // Of the tokens at the border the (picks - above) lowest: those whose complement is
-  // among the largest.
-  const uint32_t last = ~kth_largest<uint32_t>(picks - above, [&](uint32_t at) {
-    return counted([&](int i) { return (key[i] == border) & (~token[i] >= at); });
-  });
+  // among the largest.  Mostly there is one.
+  const uint32_t reached = counted([&](int i) { return key[i] >= border; });
+  uint32_t last = kNone;
+  if (reached != picks) {
+    last = ~kth_largest<uint32_t>(picks - above, [&](uint32_t at) {
+      return counted([&](int i) { return (key[i] == border) & (~token[i] >= at); });
+    });
+  }
   uint32_t next = 0;
 #pragma unroll
   for (int i = 0; i < SHARE; ++i) {
@@ -150,7 +154,8 @@ __device__ __forceinline__ T compact(Kept<T>& kept, uint32_t count, uint32_t pic
   return value_of(border);
 }
 // Most waves hold few candidates, all a wave has room for hardly any.
-constexpr int kFew = 2;
+constexpr int kFew = 2, kMore = 5;
+constexpr uint32_t kWorth = 16;  // lanes with a candidate that are worth a higher bar
 template <typename T>
 constexpr int kAll = kKept<T> / kWave;
 static_assert(kKept<float> % kWave == 0 && kKept<double> % kWave == 0);
@@ -164,8 +169,8 @@ __device__ __forceinline__ T below(T x) {
 
 // A wave per part of a row: chunks of the part one after the other, the next one's loads in
 // flight.  A candidate is what exceeds `bar`, below which the row's picks-th best cannot lie;
-// it comes from the lanes' maxima of the first chunk, and waves of a workgroup that read the
-// same row share the highest of theirs.
+// it comes from the lanes' maxima so far, and waves of a workgroup that read the same row
+// share the highest of theirs.
 template <typename T>
 __global__ __launch_bounds__(kThreads, 2) void row_kernel(Rows<T> rows, uint32_t waves,
                                                           FastDiv by_parts) {
@@ -214,6 +219,7 @@ __global__ __launch_bounds__(kThreads, 2) void row_kernel(Rows<T> rows, uint32_t
   };
   T top = sizeof(T) == 4 ? static_cast<T>(-__FLT_MAX__) : static_cast<T>(-__DBL_MAX__);
   double sum = 0.0;
+  T best = -infinity<T>();  // of the lane
   T bar = -infinity<T>();
   uint32_t count = 0;
   T x[E], next[E];
@@ -250,13 +256,17 @@ __global__ __launch_bounds__(kThreads, 2) void row_kernel(Rows<T> rows, uint32_t
       sum += static_cast<double>(part_sum);
     }
 
-    if (chunk == begin) {
+    best = larger(best, high);
+    if (chunk == begin || count_of(high > bar) >= kWorth) {
       // picks lanes hold a value of this size or more each; sign, exponent and 7 bits do.
-      const Key key = high > -infinity<T>() ? key_of(high) : Key{0};
+      const Key key = best > -infinity<T>() ? key_of(best) : Key{0};
       const Key border = kth_largest<Key, sizeof(T) == 4 ? 16 : 19>(
           picks, [&](Key at) { return count_of(key >= at); });
-      if (border != 0) bar = below(value_of(border));
-      if (lane == 0) *const_cast<volatile T*>(&bars[wave]) = bar;
+      if (border != 0) {
+        const T under = below(value_of(border));
+        bar = larger(bar, under);
+        if (lane == 0) *const_cast<volatile T*>(&bars[wave]) = under;
+      }
     }
     // A bar that another wave has not set yet is -infinity: no harm but more candidates.
 #pragma unroll
@@ -290,6 +300,8 @@ __global__ __launch_bounds__(kThreads, 2) void row_kernel(Rows<T> rows, uint32_t
   if (count > rows.slots) {
     if (count <= kFew * kWave) {
       compact<T, kFew>(kept, count, picks, lane);
+    } else if (count <= kMore * kWave) {
+      compact<T, kMore>(kept, count, picks, lane);
     } else {
       compact<T, kAll<T>>(kept, count, picks, lane);
     }
@@ -335,6 +347,7 @@ constexpr int kGroupThreads = 512;
 constexpr int kGroupWaves = kGroupThreads / kWave;
 constexpr uint32_t kBatch = 4096;   // candidates whose totals are held
 constexpr uint32_t kListed = 1024;  // candidates in LDS that may be the best
+constexpr uint32_t kFewPicks = 16;
 
 template <typename T>
 struct Picked {
@@ -366,17 +379,20 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(Picked<T> picked, 
   const uint32_t all = beams * per_row;
   const uint64_t first_row = static_cast<uint64_t>(group) * beams;
 
-  // The first candidates are on their way while the rows' sums are joined.
+  // A thread's share of a batch of candidates, all on their way at once.
   constexpr int kShare = kBatch / kGroupThreads;
   T value[kShare];
   uint32_t token[kShare];
+  const auto fetch = [&](uint32_t base) {
 #pragma unroll
-  for (int j = 0; j < kShare; ++j) {
-    const uint32_t i = j * kGroupThreads + threadIdx.x;
-    const uint64_t from = first_row * per_row + (i < all ? i : 0);
-    value[j] = rows.values[from];
-    token[j] = rows.tokens[from];
-  }
+    for (int j = 0; j < kShare; ++j) {
+      const uint32_t i = base + j * kGroupThreads + threadIdx.x;
+      const uint64_t from = first_row * per_row + (i < all ? i : 0);
+      value[j] = rows.values[from];
+      token[j] = rows.tokens[from];
+    }
+  };
+  fetch(0);  // they arrive while the rows' sums are joined
   for (uint32_t r = wave; r < beams; r += kGroupWaves) {
     const uint64_t row = first_row + r;
     const bool ended = rows.ended != nullptr && rows.ended[row] != 0;
@@ -416,35 +432,50 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(Picked<T> picked, 
     if (c.total != c.total) c.total = -infinity<double>();
     return c;
   };
-  const auto candidate = [&](uint32_t i) {
-    const uint64_t from = first_row * per_row + i;
-    return made(i, rows.values[from], rows.tokens[from]);
-  };
   // Totals in single precision: rounding keeps the order, so that what lies below the
   // picks-th largest of these is not among the best; of its bits the first do.
-  const auto coarse = [](const Candidate& c) { return key_of(static_cast<float>(c.total)); };
   const uint32_t nothing = key_of(-infinity<float>());
+  const auto coarse = [&](uint32_t base, int j) {
+    const uint32_t i = base + j * kGroupThreads + threadIdx.x;
+    return i < all ? key_of(static_cast<float>(made(i, value[j], token[j]).total)) : 0;
+  };
 
   uint32_t high = nothing;
 #pragma unroll
   for (int j = 0; j < kShare; ++j) {
-    const uint32_t i = j * kGroupThreads + threadIdx.x;
     if (j * kGroupThreads >= all) break;
-    const uint32_t key = i < all ? coarse(made(i, value[j], token[j])) : 0;
-    keys[i] = key;
-    high = max(high, key);
+    keys[j * kGroupThreads + threadIdx.x] = coarse(0, j);
+    high = max(high, keys[j * kGroupThreads + threadIdx.x]);
   }
 #pragma unroll 1
-  for (uint32_t i = kBatch + threadIdx.x; i < all; i += kGroupThreads) {
-    high = max(high, coarse(candidate(i)));
-  }
-  const uint32_t border =
-      kth_largest<uint32_t, 20>(picks, [&](uint32_t at) { return count_of(high >= at); });
-  if (lane == 0) bars[wave] = border;
-  __syncthreads();
-  uint32_t bar = nothing;
+  for (uint32_t base = kBatch; base < all; base += kBatch) {
+    fetch(base);
 #pragma unroll
-  for (int w = 0; w < kGroupWaves; ++w) bar = max(bar, bars[w]);
+    for (int j = 0; j < kShare; ++j) high = max(high, coarse(base, j));
+  }
+  uint32_t bar = nothing;
+  if (picks <= kFewPicks) {
+    const uint32_t border =
+        kth_largest<uint32_t, 20>(picks, [&](uint32_t at) { return count_of(high >= at); });
+    if (lane == 0) bars[wave] = border;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kGroupWaves; ++w) bar = max(bar, bars[w]);
+  } else {  // of all waves' lanes, in every wave
+    passed[threadIdx.x] = high;
+    __syncthreads();
+    uint32_t highs[kGroupWaves];
+#pragma unroll
+    for (int w = 0; w < kGroupWaves; ++w) highs[w] = passed[w * kWave + lane];
+    const uint32_t border = kth_largest<uint32_t, 20>(picks, [&](uint32_t at) {
+      uint32_t n = 0;
+#pragma unroll
+      for (int w = 0; w < kGroupWaves; ++w) n += count_of(highs[w] >= at);
+      return n;
+    });
+    bar = max(bar, border);
+    __syncthreads();
+  }
 
   // Keeps the best picks of the list; all threads.  Returns how many it keeps.
   const auto choose = [&]() {
@@ -470,35 +501,47 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(Picked<T> picked, 
     __syncthreads();
     return kept;
   };
-  // A batch's candidates that may be the best, first by number and then as they are, so many
-  // at once as the list has room for.
-  uint32_t chosen = 0;
-  for (uint32_t base = 0; base < all; base += kBatch) {
-    const uint32_t end = min(base + kBatch, all);
+  // A batch's candidates that may be the best, first by number and then as they are; the
+  // choice waits until the list is full.
+  uint32_t held = 0;  // in the list
 #pragma unroll 1
-    for (uint32_t first = base; first < end; first += kGroupThreads) {
+  for (uint32_t base = 0; base < all; base += kBatch) {
+    if (base != 0) {
+      fetch(base);
+#pragma unroll
+      for (int j = 0; j < kShare; ++j) keys[j * kGroupThreads + threadIdx.x] = coarse(base, j);
+    }
+    const uint32_t end = min(kBatch, all - base);
+#pragma unroll 1
+    for (uint32_t first = 0; first < end; first += kGroupThreads) {
       const uint32_t i = first + threadIdx.x;
-      const bool taken = i < end && (i < kBatch ? keys[i] : coarse(candidate(i))) >= bar;
+      const bool taken = i < end && keys[i] >= bar;
       const uint64_t mask = __ballot(taken);
       if (mask == 0) continue;
       uint32_t to = 0;
       if (lane == 0) to = atomicAdd(&count, static_cast<uint32_t>(__popcll(mask)));
       to = __builtin_amdgcn_readfirstlane(to) + __popcll(mask & ((uint64_t{1} << lane) - 1));
-      if (taken) passed[to] = i;
+      if (taken) passed[to] = base + i;
     }
     __syncthreads();
     const uint32_t found = count;
     for (uint32_t first = 0; first < found; first += kListed - SPAR_HIP_MAX_BEAMS) {
       const uint32_t last = min(first + kListed - SPAR_HIP_MAX_BEAMS, found);
-      for (uint32_t i = first + threadIdx.x; i < last; i += kGroupThreads) {
-        const Candidate c = candidate(passed[i]);
+      if (held + (last - first) > kListed) choose();
+      for (uint32_t at = first + threadIdx.x; at < last; at += kGroupThreads) {
+        const uint32_t i = passed[at];
+        const uint64_t from = first_row * per_row + i;
+        const Candidate c = made(i, rows.values[from], rows.tokens[from]);
         if (c.total > -infinity<double>()) list[atomicAdd(&listed, 1U)] = c;
       }
-      chosen = choose();
+      __syncthreads();
+      held = listed;
+      __syncthreads();
     }
     if (threadIdx.x == 0) count = 0;
     __syncthreads();
   }
+  const uint32_t chosen = choose();
 
   const auto write = [&](uint32_t i, double total, uint32_t r, uint32_t token) {
     const uint64_t at = static_cast<uint64_t>(group) * picks + i;
@@ -606,6 +649,7 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(States states, const 
 // Waves that a call's rows are split up to: eight for each of the 256 CUs, which are as many
 // as a CU holds.
 constexpr uint64_t kFullWaves = 2048;
+constexpr uint64_t kMostCandidates = 8192;
 constexpr uint64_t kMostGroups = (uint64_t{1} << 32) / kGroupThreads - 1;
 
 struct Plan {
@@ -619,12 +663,13 @@ Plan plan_of(const SparHipBeams& b) {
   const uint64_t size = b.dtype == SPAR_HIP_FLOAT32 ? sizeof(float) : sizeof(double);
   const uint64_t chunk = b.dtype == SPAR_HIP_FLOAT32 ? kChunk<float> : kChunk<double>;
   const uint64_t chunks = (b.vocabulary + chunk - 1) / chunk;
-  plan.parts = std::max<uint64_t>(
-      1, std::min({chunks, uint64_t{kMostParts}, kFullWaves / std::max<uint64_t>(1, plan.rows)}));
-  const uint64_t waves = plan.rows * plan.parts;
   // Room for a few more than the picks, which a part of one chunk mostly finds: they need
   // not be told apart before the group's choice.
-  plan.slots = std::min<uint64_t>(2 * b.picks, SPAR_HIP_MAX_BEAMS);
+  plan.slots = std::max<uint64_t>(b.picks, std::min<uint64_t>(2 * b.picks, 32));
+  plan.parts = std::max<uint64_t>(
+      1, std::min({chunks, uint64_t{kMostParts}, kFullWaves / std::max<uint64_t>(1, plan.rows),
+                   kMostCandidates / (b.beams * plan.slots)}));
+  const uint64_t waves = plan.rows * plan.parts;
   plan.bytes = waves * 2 * sizeof(double) + waves * plan.slots * (size + sizeof(uint32_t));
   return plan;
 }

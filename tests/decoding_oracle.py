@@ -107,11 +107,14 @@ def attention(query, cache, lengths=None, prefix=None, prefix_lengths=None, scal
 # ------------------------------------------------------------------- beams
 
 def log_sums(logits):
-    """log(sum(exp)) of rows, NaN where a NaN or +infinity stands."""
+    """log(sum(exp)) of rows, NaN where a NaN or +infinity stands.  Summed in extended
+    precision: along an axis that is not the innermost in memory numpy adds term by term,
+    which puts 60000 equal terms off by 1.4e-13 in double."""
     x = np.asarray(logits, np.float64)
     with np.errstate(invalid="ignore", divide="ignore", over="ignore"):
         top = x.max(-1, keepdims=True)
-        return (top + np.log(np.exp(x - top).sum(-1, keepdims=True)))[..., 0]
+        total = np.exp(x - top).sum(-1, keepdims=True, dtype=np.longdouble)
+        return (top + np.log(total)).astype(np.float64)[..., 0]
 
 
 def select(logits, scores, picks, ended=None, end_token=-1):

@@ -232,3 +232,23 @@ def test_one_logit_outweighs_all(hip, dtype, place):
     logits, scores = inputs(1, 2, 5000, dtype, 23)
     logits[0, 1, place] = 500
     check(hip, logits, scores, 5)
+
+
+@pytest.mark.parametrize("dtype", [F32, F64])
+@pytest.mark.parametrize("beams,picks", [(16, 32), (16, 64), (3, 17), (64, 16)])
+def test_long_parts_of_rows(hip, dtype, beams, picks):
+    """Parts of many chunks each, since a group's candidates are bounded."""
+    logits, scores = inputs(1, beams, 90001, dtype, 24)
+    check(hip, logits, scores, picks)
+
+
+@pytest.mark.parametrize("dtype", [F32, F64])
+@pytest.mark.parametrize("order", ["rising", "falling", "equal", "steps"])
+def test_orders_in_long_parts(hip, dtype, order):
+    """The bar that a chunk sets for the next ones: each better, each worse, equal ones."""
+    v, beams = 60000, 16
+    row = {"rising": np.arange(v) / 8192, "falling": -np.arange(v) / 8192,
+           "equal": np.full(v, 2.5), "steps": np.arange(v) // 2500 % 4 * 0.5}[order]
+    logits = np.broadcast_to(row, (1, beams, v)).astype(dtype)
+    scores = -40.0 * np.arange(beams)[None]
+    check(hip, logits, scores, 64)
