@@ -870,14 +870,15 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void cache_kernel(
 
 // ---------------------------------------------------------------- launchers
 
-// As in the forward over a contiguous cache: up to this many rows of a unit the waves share
-// rows and split keys; workgroups that row tiles are split up to, and the fewest keys that
-// repay a part.
+// Up to this many rows of a unit the waves of a workgroup share rows and split keys; the
+// fewest keys that repay a part.
 constexpr uint64_t kTokenRows = 32;
-constexpr uint64_t kFullGrid = 512;
-constexpr uint64_t kTokenGrid = 768;
 constexpr uint64_t kFewestKeys = 256;
 constexpr uint64_t kFewestTokenKeys = 64;
+// Workgroups that tiles of 64 rows are split up to: two for each CU (three are not all there
+// at once: 264 us for 200 with 64 sequences behind 16384 tokens).
+constexpr uint64_t kCus = 256;
+constexpr uint64_t kFullGrid = 2 * kCus;
 
 struct SidePlan {
   Kind kind;
@@ -911,15 +912,38 @@ SidePlan side_plan(const SparHipCacheAttention& a, uint64_t rows_of_cache, uint6
   return plan;
 }
 
+// Keys that a side's workgroups read at most, one after the other.
+uint64_t reads_of(const SidePlan& plan, uint64_t room) {
+  return plan.units * ((plan.rows + kBlock - 1) / kBlock) * room;
+}
+
+// Workgroups that a side's rows are split up to where its keys are read straight from
+// memory.
+//   Few rows: one for each CU, whose four waves have enough loads in flight between them;
+//   three take 46 us for 39 (one sequence of 4096 behind 16384) to 37 for 34 (16 sequences,
+//   heads of 64), and are equal for 16 sequences with heads of 128.
+//   16 rows: one less than a CU holds (8 rows, heads of 128: two 60 us, three 68, one 65).
+//   Where a CU holds one, all at once: half of them for each side, or all for one that reads
+//   far more than the other (heads of 256: half 70 us, all 82, twice as many 96; without a
+//   prefix all 41, half 55).
+uint64_t grid_of(const SparHipCacheAttention& a, Kind kind, uint64_t reads, uint64_t others) {
+  int waves = 0;
+  with_padded_width(a.extent, [&](auto width) {
+    constexpr int DP = decltype(width)::value;
+    waves = a.dtype == SPAR_HIP_FLOAT32 ? tile_waves<float, DP>() : tile_waves<double, DP>();
+  });
+  if (waves == 1) return others < reads / 4 ? kCus : kCus / 2;
+  return kind == Kind::Few ? kCus : kCus * (waves - 1);
+}
+
 // Workgroups of a side whose kind is settled.
-void divide(SidePlan& plan, uint64_t room) {
+void divide(SidePlan& plan, uint64_t room, uint64_t grid) {
   constexpr uint64_t kRows = kWaves * kBlock;
   const bool tiles = plan.kind == Kind::Tiles;
   const uint64_t tile_rows = tiles ? kRows : kBlock;
   const uint64_t least = tiles ? kFewestKeys : kFewestTokenKeys;
   plan.row_tiles = (plan.rows + tile_rows - 1) / tile_rows;
-  const uint64_t wanted = (tiles ? kFullGrid : kTokenGrid) /
-                          std::max<uint64_t>(1, plan.row_tiles * plan.units);
+  const uint64_t wanted = (tiles ? kFullGrid : grid) / std::max<uint64_t>(1, plan.row_tiles * plan.units);
   plan.splits =
       std::max<uint64_t>(1, std::min({wanted, room / least, uint64_t{kMostParts / 2}}));
   plan.least = least / kBlock;
@@ -934,9 +958,13 @@ Plan plan_of(const SparHipCacheAttention& a, const SparHipPages& cache,
     plan.prefix = side_plan(a, a.prefixes, a.batch / a.prefixes, room_of(prefix));
     // There is no launch of fewer rows before more: a prefix has the more rows.
     if (plan.prefix.kind < plan.own.kind) plan.prefix.kind = plan.own.kind;
-    divide(plan.prefix, room_of(prefix));
   }
-  divide(plan.own, room_of(&cache));
+  const uint64_t own_reads = reads_of(plan.own, room_of(&cache));
+  const uint64_t prefix_reads = reads_of(plan.prefix, room_of(prefix));
+  if (plan.prefix.units != 0) {
+    divide(plan.prefix, room_of(prefix), grid_of(a, plan.prefix.kind, prefix_reads, own_reads));
+  }
+  divide(plan.own, room_of(&cache), grid_of(a, plan.own.kind, own_reads, prefix_reads));
   plan.parts = static_cast<uint32_t>(plan.own.splits + plan.prefix.splits);
   const uint64_t size = a.dtype == SPAR_HIP_FLOAT32 ? sizeof(float) : sizeof(double);
   const uint64_t piece = 16 / size;
@@ -973,7 +1001,7 @@ Side<T> side_of(const SparHipCacheAttention& a, const SparHipPages& cache, const
   side.splits = static_cast<uint32_t>(plan.splits);
   side.least = static_cast<uint32_t>(plan.least);
   side.first_part = first_part;
-  // (Few rows take blocks of 8 or 16 keys.)
+  // Few rows take blocks of 8 keys or of kBlock.
   side.whole = cache.table == nullptr ||
                cache.page_tokens % (plan.kind == Kind::Tiles ? block : kBlock) == 0;
   return side;
