@@ -845,10 +845,10 @@ struct SparHipStatus spar_hip_beam_select_workspace(uint64_t* bytes,
 
 /* The best `picks` tokens of the rows of each group, best first: the largest totals, of
  * equal totals the lowest row, in a row the largest logit, of equal ones the lowest token;
- * totals of -infinity come in the order of rows and tokens alone.  Outputs are [groups, picks], contiguous: the totals
- * rounded to the dtype, the rows picks go on from (of all groups * beams), their tokens,
- * and whether they have ended (1 where the row had or the token is end_token, else 0; may
- * be NULL).  One pass over the logits; log-probabilities are not written anywhere.
+ * totals of -infinity come in the order of rows and tokens alone.  Outputs are
+ * [groups, picks], contiguous: the totals rounded to the dtype, the rows picks go on from
+ * (of all groups * beams), their tokens, and whether they have ended (1 where the row had
+ * or the token is end_token, else 0; may be NULL).  One pass over the logits; log-probabilities are not written anywhere.
  * No reference counterpart (it decodes greedily or by sampling on the host). */
 struct SparHipStatus spar_hip_launch_beam_select(
     void* picked_scores, int64_t* parents, int64_t* tokens, int32_t* picked_ended,
@@ -857,8 +857,8 @@ struct SparHipStatus spar_hip_launch_beam_select(
 
 /* Rows of `state_count` states (host memory, read before the call returns; at most 2^16)
  * in the order of their parents: `rows` numbers in device memory, of [0, source_rows).
- * Rows and strides have at most 2^40 elements, and a state at most 2^23 - 1 rows of up to 2^14 bytes,
- * half as many of up to 2^15 and so on.
+ * Rows and strides have at most 2^40 elements, and a state at most 2^23 - 1 rows of up to
+ * 2^14 bytes, half as many of up to 2^15 and so on.
  * An output row whose parent lies outside becomes zeros.  Outputs must not overlap
  * inputs or each other. */
 struct SparHipStatus spar_hip_launch_reorder(const struct SparHipReorder* states,

@@ -173,7 +173,11 @@ struct TileSpace {
   Tile<T, KB * kBlock, DP, READS, kBuffers> keys, values;
 };
 
-// A workgroup's 64 rows and its share of the keys, in tiles that its waves share.
+// A workgroup's 64 rows and its share of the keys, in tiles that its waves share: every key
+// read once for 64 rows.  Bound by the matrix units: 256 rows a key head over 16384 keys, 8
+// heads of 128, take 152 us, 113 TFLOP/s (the units are busy in 87% of the waves' lives and
+// the softmax's vector instructions take the rest); 4 * 256 tokens behind 4096, 673 us, 115
+// TFLOP/s.  Pages of 5 and 100 tokens, found key by key, take 790.
 template <typename T, int DP, Reads READS>
 __device__ __forceinline__ void tile_part(TileSpace<T, DP, READS>& space, const Call& call,
                                           const Results<T>& results, const Heads<const T>& query,
@@ -379,7 +383,9 @@ struct TokenSpace {
 };
 
 // A workgroup's 16 rows and its share of the keys, of which each wave takes every fourth
-// block from memory.
+// block from memory.  Bound by reading the cache: 16 sequences of up to 4096 tokens, 4 key
+// heads of 128 and 8 rows each, 46 us, 3.7 TB/s: a block's loads are waited for before its
+// products.
 template <typename T, int DP, Reads READS>
 __device__ __forceinline__ void token_part(TokenSpace<T, DP>& space, const Call& call,
                                            const Results<T>& results,
@@ -539,6 +545,9 @@ __device__ __forceinline__ void token_part(TokenSpace<T, DP>& space, const Call&
 //   sums are added up across the wave and leave key 4 g + l / 16 of row l % 4 in each lane.
 //   Values: that lane's weight meets d = 64 c + 4 (l % 16) + i of its key as it stands.  The
 //   quarters' sums over their keys are added up once at the end.
+// Bound by reading the cache: the own tokens of 64 sequences (up to 2048 of 8 heads of 128)
+// take 115 us alone, 5.2 TB/s; in token_part they and their prefix took 294 together, here
+// (and in one launch) 200.
 constexpr int kFewRows = 4;
 
 __device__ __forceinline__ f32x4 few_step(float a, float b, f32x4 c) {
@@ -589,7 +598,7 @@ __device__ __forceinline__ void few_part(FewSpace<DP>& space, const Call& call,
   constexpr int SIZE = C == 1 ? 16 : 8;  // keys of a block
   constexpr int G = SIZE / 4;            // groups of four keys
   // Beside tiles, whose products fill the matrix units whenever they may: the short work
-  // between two reads goes first.
+  // between two reads goes first (199 us for 210).
   __builtin_amdgcn_s_setprio(3);
   const uint32_t unit = index % side.units, split = index / side.units;
   const uint32_t u = unit / call.key_heads, key_head = unit % call.key_heads;
@@ -848,7 +857,10 @@ __device__ __forceinline__ void side_part(char* space, const Call& call, const R
 }
 
 // The prefixes' workgroups come first: their products keep the matrix units busy while the
-// others, which fill what room they leave on a CU, read the sequences' own keys.
+// others, which fill what room they leave on a CU, read the sequences' own keys.  64 sequences
+// behind 16384 tokens: 152 us for the prefix and 115 for the rest apart, 194 together.  In
+// turn by eights all prefix groups came to lie on half of the CUs (1141 us for 673 with 256
+// tokens of 4 sequences).  Registers for a wave more per SIMD: 204.
 template <typename T, int DP, Reads READS, Kind PREFIX, Kind OWN>
 __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void cache_kernel(
     Call call, Results<T> results, Heads<const T> query, Side<T> prefix, Side<T> own,
@@ -870,8 +882,9 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void cache_kernel(
 
 // ---------------------------------------------------------------- launchers
 
-// Up to this many rows of a unit the waves of a workgroup share rows and split keys; the
-// fewest keys that repay a part.
+// Up to this many rows of a unit (and where tiles would be few) the waves of a workgroup share
+// rows and split keys; the fewest keys that repay a part: 64, 128 and 256 are within a tenth
+// of each other, now one now the other ahead; of tiles 128 take 88 us for 82 (heads of 256).
 constexpr uint64_t kTokenRows = 32;
 constexpr uint64_t kFewestKeys = 256;
 constexpr uint64_t kFewestTokenKeys = 64;
@@ -943,7 +956,8 @@ void divide(SidePlan& plan, uint64_t room, uint64_t grid) {
   const uint64_t tile_rows = tiles ? kRows : kBlock;
   const uint64_t least = tiles ? kFewestKeys : kFewestTokenKeys;
   plan.row_tiles = (plan.rows + tile_rows - 1) / tile_rows;
-  const uint64_t wanted = (tiles ? kFullGrid : grid) / std::max<uint64_t>(1, plan.row_tiles * plan.units);
+  const uint64_t wanted =
+      (tiles ? kFullGrid : grid) / std::max<uint64_t>(1, plan.row_tiles * plan.units);
   plan.splits =
       std::max<uint64_t>(1, std::min({wanted, room / least, uint64_t{kMostParts / 2}}));
   plan.least = least / kBlock;

@@ -155,7 +155,10 @@ __device__ __forceinline__ T compact(Kept<T>& kept, uint32_t count, uint32_t pic
 }
 // Most waves hold few candidates, all a wave has room for hardly any.
 constexpr int kFew = 2, kMore = 5;
-constexpr uint32_t kWorth = 16;  // lanes with a candidate that are worth a higher bar
+// Lanes with a candidate that are worth a higher bar.  Without one a chunk brings as many
+// candidates as the first: 1024 rows of 32000 with 32 picks took 54 us for 31.  Where every
+// chunk looks for one, 256 rows with 8 picks take 28 for 25.
+constexpr uint32_t kWorth = 16;
 template <typename T>
 constexpr int kAll = kKept<T> / kWave;
 static_assert(kKept<float> % kWave == 0 && kKept<double> % kWave == 0);
@@ -168,9 +171,10 @@ __device__ __forceinline__ T below(T x) {
 }
 
 // A wave per part of a row: chunks of the part one after the other, the next one's loads in
-// flight.  A candidate is what exceeds `bar`, below which the row's picks-th best cannot lie;
-// it comes from the lanes' maxima so far, and waves of a workgroup that read the same row
-// share the highest of theirs.
+// flight.  Bound by memory: 1024 rows of 32000 with 32 picks in 31 us, 4.3 TB/s, and by the
+// start and the end of 8 chunks a wave.  A candidate is what exceeds `bar`, below which the
+// row's picks-th best cannot lie; it comes from the lanes' maxima so far, and waves of a
+// workgroup that read the same row share the highest of theirs.
 template <typename T>
 __global__ __launch_bounds__(kThreads, 2) void row_kernel(Rows<T> rows, uint32_t waves,
                                                           FastDiv by_parts) {
@@ -265,13 +269,17 @@ __global__ __launch_bounds__(kThreads, 2) void row_kernel(Rows<T> rows, uint32_t
       if (border != 0) {
         const T under = below(value_of(border));
         bar = larger(bar, under);
-        if (lane == 0) *const_cast<volatile T*>(&bars[wave]) = under;
+        if (lane == 0) {
+          __hip_atomic_store(&bars[wave], under, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
       }
     }
-    // A bar that another wave has not set yet is -infinity: no harm but more candidates.
+    // A bar that another wave has not set yet is -infinity, one that it has raised meanwhile
+    // lower than it need be: no harm but more candidates.
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const T other = *const_cast<const volatile T*>(&bars[w]);
+      const T other =
+          __hip_atomic_load(&bars[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
       bar = shares[w] ? larger(bar, other) : bar;
     }
 #pragma unroll
@@ -347,6 +355,8 @@ constexpr int kGroupThreads = 512;
 constexpr int kGroupWaves = kGroupThreads / kWave;
 constexpr uint32_t kBatch = 4096;   // candidates whose totals are held
 constexpr uint32_t kListed = 1024;  // candidates in LDS that may be the best
+// Up to this many picks the best wave's lanes alone set the bar (32 groups of 8 picks 36 us
+// for 38 with all waves' lanes); of more picks too many would pass (32: 18 us for 27).
 constexpr uint32_t kFewPicks = 16;
 
 template <typename T>
@@ -358,8 +368,9 @@ struct Picked {
 };
 
 // A workgroup per group.  Candidates are read while the rows' sums are joined; the picks-th
-// best of each wave's lanes bounds what can be among the group's best, which few pass, and
-// those are ranked by counting.
+// best of the lanes bounds what can be among the group's best, which few pass, and those are
+// ranked by counting.  Bound by latency, one step behind the other: 7 us for 32 groups of
+// 1024 candidates, 18 for one of 8192.
 template <typename T>
 __global__ __launch_bounds__(kGroupThreads) void group_kernel(Picked<T> picked, Rows<T> rows,
                                                               const T* scores, uint32_t beams,
@@ -595,7 +606,10 @@ struct States {
   uint32_t count;
 };
 
-constexpr uint64_t kGroupBytes = 4 * kThreads * 16;  // of a row, to a workgroup
+// A workgroup moves this much of a row, four pieces of a lane on their way at once.  Bound by
+// memory for large states (160 rows of 65536 floats, 42 MB written, in 10 us), by the launch
+// for small ones.
+constexpr uint64_t kGroupBytes = 4 * kThreads * 16;
 
 // from: nullptr for zeros.
 template <typename V>
@@ -649,6 +663,8 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(States states, const 
 // Waves that a call's rows are split up to: eight for each of the 256 CUs, which are as many
 // as a CU holds.
 constexpr uint64_t kFullWaves = 2048;
+// Candidates of a group, which one workgroup goes through: 16 rows of 200000 with 32 picks
+// take 46 us with 4096, 42 with 8192, 47 with 16384 and 183 without a bound.
 constexpr uint64_t kMostCandidates = 8192;
 constexpr uint64_t kMostGroups = (uint64_t{1} << 32) / kGroupThreads - 1;
 
@@ -664,7 +680,8 @@ Plan plan_of(const SparHipBeams& b) {
   const uint64_t chunk = b.dtype == SPAR_HIP_FLOAT32 ? kChunk<float> : kChunk<double>;
   const uint64_t chunks = (b.vocabulary + chunk - 1) / chunk;
   // Room for a few more than the picks, which a part of one chunk mostly finds: they need
-  // not be told apart before the group's choice.
+  // not be told apart before the group's choice (10 picks: 27 us for 29).  Many picks are,
+  // where the group's choice would take longer (32: 45 us for 46, 42 for 52).
   plan.slots = std::max<uint64_t>(b.picks, std::min<uint64_t>(2 * b.picks, 32));
   plan.parts = std::max<uint64_t>(
       1, std::min({chunks, uint64_t{kMostParts}, kFullWaves / std::max<uint64_t>(1, plan.rows),
