@@ -392,8 +392,7 @@ def test_queries_are_turned_in_place(hip):
 
 
 def test_append_far_into_a_large_cache(hip):
-    """Places whose elements are more than 2^32 from the cache's start, and attention over
-    them."""
+    """Places whose elements are more than 2^32 from the cache's start."""
     hk, d, page, pages = 1, 128, 1 << 17, 300  # 300 * 2^24 elements of keys and of values
     count = pages * page * d
     key, value = space(hip, 4 * count), space(hip, 4 * count)
