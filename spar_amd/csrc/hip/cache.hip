@@ -122,23 +122,36 @@ void start_append(const Append<T>& append, uint64_t batch, uint64_t tokens, cons
                   int layout, hipStream_t stream) {
   const uint64_t heads = append.query_heads + 2 * static_cast<uint64_t>(append.key_heads);
   const uint64_t lanes = batch * tokens * units_of(turn.half, turn.extent) * heads;
+  // Past the caches where much is written in whole lines: halves of float32 heads whose lanes
+  // lie side by side ([4, 4096] tokens of 32 + 2 * 8 heads of 128 150 us, through the caches
+  // 160).  Elsewhere a store writes every second 16 bytes or ends in the middle of a line, which
+  // the caches put together: neighbouring pairs 114 us, past the caches 133, in float64 130 and
+  // 255, half of a head of 100 62 and 84.
   const bool stream_out =
+      2 * turn.half == turn.extent && turn.half * sizeof(T) % 128 == 0 &&
       stream_output(batch * tokens * heads * static_cast<uint64_t>(turn.extent) * sizeof(T));
   // Two heads a lane, so that cos and sin serve twice: four take 156 us and eight 154 where
-  // two take 149.  Stores that stay in the caches take 170.  One head of doubles: a lane's
-  // loads are as wide.
+  // two take 149.  One head of doubles: a lane's loads are as wide.
   constexpr int kMany = 8 / sizeof(T);
-  with_policy(layout == SPAR_HIP_ROTARY_HALF, [&](auto half) {
-    with_policy(stream_out, [&](auto nt) {
-      if (lanes >= kMany * kFullLanes) {
-        launch_append<T, decltype(half)::value, decltype(nt)::value, kMany>(append, batch, tokens,
-                                                                            turn, stream);
-      } else {
-        launch_append<T, decltype(half)::value, decltype(nt)::value, 1>(append, batch, tokens,
-                                                                        turn, stream);
-      }
-    });
-  });
+  const bool many = lanes >= kMany * kFullLanes;
+  const auto launch = [&](auto half, auto nt, auto heads_a_lane) {
+    launch_append<T, decltype(half)::value, decltype(nt)::value, decltype(heads_a_lane)::value>(
+        append, batch, tokens, turn, stream);
+  };
+  const auto launch_heads = [&](auto half, auto nt) {
+    if (many) {
+      launch(half, nt, std::integral_constant<int, kMany>{});
+    } else {
+      launch(half, nt, std::integral_constant<int, 1>{});
+    }
+  };
+  if (layout != SPAR_HIP_ROTARY_HALF) {
+    launch_heads(std::false_type{}, std::false_type{});
+  } else if (!(std::is_same_v<T, float> && stream_out)) {
+    launch_heads(std::true_type{}, std::false_type{});
+  } else if constexpr (std::is_same_v<T, float>) {
+    launch_heads(std::true_type{}, std::true_type{});
+  }
 }
 
 }  // namespace
