@@ -888,10 +888,7 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void cache_kernel(
 constexpr uint64_t kTokenRows = 32;
 constexpr uint64_t kFewestKeys = 256;
 constexpr uint64_t kFewestTokenKeys = 64;
-// Workgroups that tiles of 64 rows are split up to: two for each CU (three are not all there
-// at once: 264 us for 200 with 64 sequences behind 16384 tokens).
 constexpr uint64_t kCus = 256;
-constexpr uint64_t kFullGrid = 2 * kCus;
 
 struct SidePlan {
   Kind kind;
@@ -930,8 +927,12 @@ uint64_t reads_of(const SidePlan& plan, uint64_t room) {
   return plan.units * ((plan.rows + kBlock - 1) / kBlock) * room;
 }
 
-// Workgroups that a side's rows are split up to where its keys are read straight from
-// memory.
+// Workgroups that a side's rows are split up to, by what a CU holds of them (`waves` per
+// SIMD).
+//   Tiles: all that a CU holds where they are alone there or the other side is tiles too
+//   (256 tokens of 4 sequences, heads of 64, 602 us, half as many 658); otherwise one less,
+//   which leaves room for those that read (64 sequences behind 16384 tokens: heads of 128
+//   200 us, all that it holds 264; of 64 121 and 136; of 192 195 and 220).
 //   Few rows: one for each CU, whose four waves have enough loads in flight between them;
 //   three take 46 us for 39 (one sequence of 4096 behind 16384) to 37 for 34 (16 sequences,
 //   heads of 64), and are equal for 16 sequences with heads of 128.
@@ -939,13 +940,18 @@ uint64_t reads_of(const SidePlan& plan, uint64_t room) {
 //   Where a CU holds one, all at once: half of them for each side, or all for one that reads
 //   far more than the other (heads of 256: half 70 us, all 82, twice as many 96; without a
 //   prefix all 41, half 55).
-uint64_t grid_of(const SparHipCacheAttention& a, Kind kind, uint64_t reads, uint64_t others) {
-  int waves = 0;
+uint64_t grid_of(const SparHipCacheAttention& a, Kind kind, Kind other, uint64_t reads,
+                 uint64_t other_reads) {
+  uint64_t waves = 0;
   with_padded_width(a.extent, [&](auto width) {
     constexpr int DP = decltype(width)::value;
     waves = a.dtype == SPAR_HIP_FLOAT32 ? tile_waves<float, DP>() : tile_waves<double, DP>();
   });
-  if (waves == 1) return others < reads / 4 ? kCus : kCus / 2;
+  const bool alone = other_reads < reads / 4;
+  if (kind == Kind::Tiles) {
+    return kCus * (alone || other == Kind::Tiles ? waves : std::max<uint64_t>(1, waves - 1));
+  }
+  if (waves == 1) return alone ? kCus : kCus / 2;
   return kind == Kind::Few ? kCus : kCus * (waves - 1);
 }
 
@@ -956,8 +962,7 @@ void divide(SidePlan& plan, uint64_t room, uint64_t grid) {
   const uint64_t tile_rows = tiles ? kRows : kBlock;
   const uint64_t least = tiles ? kFewestKeys : kFewestTokenKeys;
   plan.row_tiles = (plan.rows + tile_rows - 1) / tile_rows;
-  const uint64_t wanted =
-      (tiles ? kFullGrid : grid) / std::max<uint64_t>(1, plan.row_tiles * plan.units);
+  const uint64_t wanted = grid / std::max<uint64_t>(1, plan.row_tiles * plan.units);
   plan.splits =
       std::max<uint64_t>(1, std::min({wanted, room / least, uint64_t{kMostParts / 2}}));
   plan.least = least / kBlock;
@@ -976,9 +981,11 @@ Plan plan_of(const SparHipCacheAttention& a, const SparHipPages& cache,
   const uint64_t own_reads = reads_of(plan.own, room_of(&cache));
   const uint64_t prefix_reads = reads_of(plan.prefix, room_of(prefix));
   if (plan.prefix.units != 0) {
-    divide(plan.prefix, room_of(prefix), grid_of(a, plan.prefix.kind, prefix_reads, own_reads));
+    divide(plan.prefix, room_of(prefix),
+           grid_of(a, plan.prefix.kind, plan.own.kind, prefix_reads, own_reads));
   }
-  divide(plan.own, room_of(&cache), grid_of(a, plan.own.kind, own_reads, prefix_reads));
+  divide(plan.own, room_of(&cache),
+         grid_of(a, plan.own.kind, plan.prefix.kind, own_reads, prefix_reads));
   plan.parts = static_cast<uint32_t>(plan.own.splits + plan.prefix.splits);
   const uint64_t size = a.dtype == SPAR_HIP_FLOAT32 ? sizeof(float) : sizeof(double);
   const uint64_t piece = 16 / size;
