@@ -858,9 +858,10 @@ __device__ __forceinline__ void side_part(char* space, const Call& call, const R
 
 // The prefixes' workgroups come first: their products keep the matrix units busy while the
 // others, which fill what room they leave on a CU, read the sequences' own keys.  64 sequences
-// behind 16384 tokens: 152 us for the prefix and 115 for the rest apart, 194 together.  In
-// turn by eights all prefix groups came to lie on half of the CUs (1141 us for 673 with 256
-// tokens of 4 sequences).  Registers for a wave more per SIMD: 204.
+// behind 16384 tokens: 152 us for the prefix and 115 for the rest apart, 187 to 204 together
+// (from card to card).  In turn by eights all prefix groups came to lie on half of the CUs
+// (1141 us for 673 with 256 tokens of 4 sequences).  With registers for a wave more per SIMD
+// 204 us where this took 193.
 template <typename T, int DP, Reads READS, Kind PREFIX, Kind OWN>
 __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void cache_kernel(
     Call call, Results<T> results, Heads<const T> query, Side<T> prefix, Side<T> own,
