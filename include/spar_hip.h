@@ -808,8 +808,9 @@ struct SparHipStatus spar_hip_launch_attention_backward(
  * key_heads heads.  Token t of sequence b goes to token places[b * place_stride + t]
  * (SPAR_HIP_INT32 or SPAR_HIP_INT64) of row b of the cache, and nowhere where that is
  * negative, behind the row's room or in a page that holds nothing; the rest of the cache
- * is left as it was.  Two tokens of one call must not share a place in the pages: either
- * may be found there, or a part of each.  rotary is NULL where heads are not turned; its
+ * is left as it was.  Two tokens of one call must not share a place in the pages, as they
+ * do where two rows of a table name the page that both write to (beams that go on from one
+ * parent): either may be found there, or a part of each.  rotary is NULL where heads are not turned; its
  * positions are apart from the places, which count from the end of a shared prefix.
  * No reference counterpart (its cache is a concatenation of tensors). */
 struct SparHipStatus spar_hip_launch_cache_append(
@@ -860,7 +861,8 @@ struct SparHipStatus spar_hip_launch_beam_select(
  * Rows and strides have at most 2^40 elements, and a state at most 2^23 - 1 rows of up to
  * 2^14 bytes, half as many of up to 2^15 and so on.
  * An output row whose parent lies outside becomes zeros.  Outputs must not overlap
- * inputs or each other. */
+ * inputs or each other.  Rows of a cache's table that come from one parent name the same
+ * pages, which must not be appended to before each has a page of its own there. */
 struct SparHipStatus spar_hip_launch_reorder(const struct SparHipReorder* states,
                                              uint64_t state_count, const int64_t* parents,
                                              uint64_t rows, uint64_t source_rows, int device);

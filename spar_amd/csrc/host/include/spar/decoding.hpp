@@ -48,7 +48,8 @@ struct CacheRotation final {
 ///   places  Int32 or Int64 [batch, tokens]: the token of its sequence's row that each new
 ///           token becomes; negative or behind the row's room for one that is not written
 ///           (padding).  The rest of the cache stays as it is.  Two tokens must not share a
-///           place in the pages.
+///           place in the pages: rows whose tables name one page, as beams' do that go on
+///           from one parent, need pages of their own for new tokens (see reorder).
 std::optional<Tensor> cache_append(const PagedCache& cache, const Tensor& key,
                                    const Tensor& value, const Tensor& places,
                                    const std::optional<CacheRotation>& rotation = std::nullopt,
@@ -99,7 +100,12 @@ struct BeamSelection final {
 
 /// New tensors with the states' rows (along axis 0) in the order of `parents`, Int64 of any
 /// shape: row i of each is row parents[i] of its state, zeros where there is none.  States of
-/// any dtype and shape, moved in one launch.
+/// any dtype and shape, moved in one launch; those that are not contiguous are copied first.
+/// Where a cache's table is moved and a parent comes twice, both rows name its pages.  They
+/// may share pages that are only read.  Before cache_append the page of the next token must
+/// be another for each: one that no row names and, in the middle of a page, with a copy of
+/// the shared one's tokens, which reorder({key, value}, page numbers) yields as heads [rows,
+/// key heads, page tokens, extent] for cache_append to write (-1 for places to come).
 [[nodiscard]] std::vector<Tensor> reorder(const std::vector<Tensor>& states,
                                           const Tensor& parents);
 
