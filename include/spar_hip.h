@@ -244,7 +244,11 @@ struct SparHipPages {
  * row b of the cache and goes on behind prefix b / (batch / prefixes), of
  * prefix_lengths[...] tokens (lengths are clamped to [0, what a row has room for], which
  * they also are where NULL).  Query i of sequence b is its own token p = length - queries
- * + i and sees its prefix and its own tokens j <= p; queries with p < 0 see nothing. */
+ * + i and sees its prefix and its own tokens j <= p; queries with p < 0 see nothing.
+ * Refused are calls of 2^24 workgroups or more (one for each key head of a sequence and of
+ * a prefix and every 64 queries of its heads, or 16 where they are few), and by the queries
+ * of all heads, of 2^30 or more in a sequence, of more than 2^30 behind a prefix and, where
+ * there is a prefix, of more than 2^27 - 8 in all. */
 struct SparHipCacheAttention {
   uint64_t batch;
   uint64_t prefixes;    /* divides batch; not read where no prefix is given */

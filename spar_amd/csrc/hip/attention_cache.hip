@@ -995,10 +995,11 @@ Plan plan_of(const SparHipCacheAttention& a, const SparHipPages& cache,
   return plan;
 }
 
-// A launch counts its workgroups in 32 bits of work-items.
+// A launch counts its workgroups in 32 bits of work-items.  (Rows are many only where neither
+// side is split: with a prefix they have two parts, without one a single one.)
 bool fits(const Plan& plan) {
   return plan.own.groups() <= kMostGroups && plan.prefix.groups() <= kMostGroups &&
-         plan.own.groups() + plan.prefix.groups() <= kMostGroups && plan.rows <= kMostGroups;
+         plan.own.groups() + plan.prefix.groups() <= kMostGroups && joins(plan.rows, plan.parts);
 }
 
 // Whether a cache's keys and values go to LDS directly.

@@ -38,6 +38,7 @@ __device__ __forceinline__ T logsumexp_of(T top, T sum) {
 // their order, all loaded before the first is used (16384 rows of 128 in 3 parts 7.5 us,
 // 256 rows of 64 in 8 parts 3 us).
 constexpr uint32_t kFewParts = 8;
+constexpr uint32_t kFewLanes = 32;
 
 template <typename T>
 __device__ __forceinline__ T* output_row(const Call& call, const Results<T>& results,
@@ -54,7 +55,7 @@ __device__ __forceinline__ T* output_row(const Call& call, const Results<T>& res
 template <typename T, bool EMPTY>
 __global__ __launch_bounds__(kThreads) void combine_few_kernel(Call call, Results<T> results) {
   constexpr int W = Vec16<T>::width;
-  constexpr uint32_t kLanes = 32;
+  constexpr uint32_t kLanes = kFewLanes;
   const uint64_t row = static_cast<uint64_t>(blockIdx.x) * (kThreads / kLanes) +
                        threadIdx.x / kLanes;
   if (row >= results.all_rows) return;
@@ -184,11 +185,19 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(Call call, Results<T>
 }
 static_assert(kThreads >= SPAR_HIP_ATTENTION_MAX_EXTENT);
 
+// Whether a launch counts the workgroups that join so many parts of `rows` rows.  One part
+// is the output itself and is not joined.
+inline bool joins(uint64_t rows, uint64_t parts) {
+  constexpr uint64_t kRows = kThreads / kFewLanes;  // of a workgroup, few parts
+  return parts <= 1 || rows <= (parts <= kFewParts ? kMostGroups * kRows : kMostGroups);
+}
+
 template <typename T, bool EMPTY>
 void join_parts(const Call& call, const Results<T>& results, hipStream_t stream) {
   if (results.splits <= kFewParts) {
     combine_few_kernel<T, EMPTY>
-        <<<ceil_div_u32(results.all_rows * 32, kThreads), kThreads, 0, stream>>>(call, results);
+        <<<ceil_div_u32(results.all_rows, kThreads / kFewLanes), kThreads, 0, stream>>>(call,
+                                                                                        results);
   } else {
     combine_kernel<T, EMPTY>
         <<<static_cast<uint32_t>(results.all_rows), kThreads, 0, stream>>>(call, results);

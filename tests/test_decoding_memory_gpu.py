@@ -93,3 +93,44 @@ def test_attention_far_into_a_large_cache(hip, page, heads, queries):
     del key, value
     attention._alive.clear()
     hip.call("spar_hip_empty_cache", 0)
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_attention_of_more_rows_than_a_launch_has_workgroups(hip, shared):
+    """2^24 rows and more, of which the last of every sequence see something: without a prefix
+    and behind one, whose parts a second launch joins."""
+    b, h, hk, t, n, d = 64, 8, 2, 32800, 20, 4
+    rows = b * h * t
+    assert rows > 2 ** 24
+    lengths = [n - i % 4 for i in range(b)]
+    cache = attention.Cache(hip, oracle.Pool(random((b, hk, n, d), F32, 1),
+                                             random((b, hk, n, d), F32, 2), lengths, 4))
+    pool = oracle.Pool(random((2, hk, 30, d), F32, 3), random((2, hk, 30, d), F32, 4), [30, 7], 0)
+    prefix = attention.Cache(hip, pool).pages if shared else None
+    seen = random((b, h, n, d), F32, 5)  # the queries that see something, and others
+    query = attention.space(hip, 4 * rows * d)
+    hip.call("spar_hip_launch_fill", query.ptr, rows * d, 0, 1.0, 0)
+    for i in range(b):
+        for j in range(h):
+            at = query.ptr + 4 * d * ((i * h + j) * t + t - n)
+            hip.call("spar_hip_copy_host_to_device", at,
+                     np.ascontiguousarray(seen[i, j]).ctypes.data, 4 * n * d, 0)
+    output = attention.space(hip, 4 * rows * d)
+    hip.call("spar_hip_launch_fill", output.ptr, rows * d, 0, 3.0, 0)
+    strides = (h * t * d, t * d, d)
+    shape = hip.cache_attention(
+        b, 2, h, hk, t, d, 0.5, attention.device(hip, np.array(lengths, np.int32)).ptr,
+        attention.device(hip, np.array([30, 7], np.int32)).ptr if shared else None, hip.INT32, 0)
+    need = hip.cache_attention_workspace(cache.pages, prefix, shape)
+    assert need == (2 * rows * (d + 2) * 4 if shared else 0)
+    workspace = attention.space(hip, need)
+    hip.call("spar_hip_launch_cache_attention", hip.heads(output.ptr, strides),
+             hip.heads(query.ptr, strides), cache.pages, prefix, shape, workspace.ptr, need, 0)
+    got = output.to_numpy(F32, (b, h, t, d))
+    assert not got[:, :, :t - n].any()
+    want, bound = oracle.attention(seen, cache.pool, lengths, pool if shared else None,
+                                   [30, 7] if shared else None, 0.5, F32)
+    assert_within(got[:, :, t - n:], want, bound)
+    del query, output, workspace
+    attention._alive.clear()
+    hip.call("spar_hip_empty_cache", 0)
