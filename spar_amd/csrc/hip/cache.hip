@@ -134,23 +134,25 @@ void start_append(const Append<T>& append, uint64_t batch, uint64_t tokens, cons
   // two take 149.  One head of doubles: a lane's loads are as wide.
   constexpr int kMany = 8 / sizeof(T);
   const bool many = lanes >= kMany * kFullLanes;
-  const auto launch = [&](auto half, auto nt, auto heads_a_lane) {
-    launch_append<T, decltype(half)::value, decltype(nt)::value, decltype(heads_a_lane)::value>(
-        append, batch, tokens, turn, stream);
-  };
-  const auto launch_heads = [&](auto half, auto nt) {
+  // What goes past the caches is more than that many lanes' share.
+  static_assert(kStreamStoreBytes / (8 * sizeof(T)) >= kMany * kFullLanes);
+  if constexpr (std::is_same_v<T, float>) {
+    if (layout == SPAR_HIP_ROTARY_HALF && stream_out) {
+      launch_append<T, true, true, kMany>(append, batch, tokens, turn, stream);
+      return;
+    }
+  }
+  const auto launch_heads = [&](auto half) {
     if (many) {
-      launch(half, nt, std::integral_constant<int, kMany>{});
+      launch_append<T, decltype(half)::value, false, kMany>(append, batch, tokens, turn, stream);
     } else {
-      launch(half, nt, std::integral_constant<int, 1>{});
+      launch_append<T, decltype(half)::value, false, 1>(append, batch, tokens, turn, stream);
     }
   };
-  if (layout != SPAR_HIP_ROTARY_HALF) {
-    launch_heads(std::false_type{}, std::false_type{});
-  } else if (!(std::is_same_v<T, float> && stream_out)) {
-    launch_heads(std::true_type{}, std::false_type{});
-  } else if constexpr (std::is_same_v<T, float>) {
-    launch_heads(std::true_type{}, std::true_type{});
+  if (layout == SPAR_HIP_ROTARY_HALF) {
+    launch_heads(std::true_type{});
+  } else {
+    launch_heads(std::false_type{});
   }
 }
 
