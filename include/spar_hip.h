@@ -269,9 +269,14 @@ struct SparHipCacheAttention {
 
 /* What a beam selection chooses from: groups * beams rows of `vocabulary` logits,
  * row_stride elements apart, with a score each.  The total of token k of row r is
- * scores[r] + logits[r][k] - log(sum of exp(logits[r])), in double, and -infinity where
- * that is NaN; in a row that has ended (ended[r] != 0) scores[r] for end_token and
- * -infinity for every other token. */
+ * scores[r] + logits[r][k] - log(sum of exp(logits[r])), and -infinity where that is NaN;
+ * in a row that has ended (ended[r] != 0) scores[r] for end_token and -infinity for every
+ * other token.  The exponentials, and sums of up to 16 of them, are formed in the dtype;
+ * these are joined, and everything else is done, in double.  So the totals of a row are off
+ * together, by u (8 d + 24 + 6 ceil(vocabulary / 512)) and a few roundings of double at most,
+ * u = 2^-24 or 2^-53 and d the distance between the row's largest and smallest finite
+ * logits (float32: mostly by less than 1e-7): tokens of two rows whose totals are closer than
+ * that may come in either order, the same in every call. */
 struct SparHipBeams {
   uint64_t groups;
   uint64_t beams;      /* rows of a group; at most SPAR_HIP_MAX_BEAMS */

@@ -86,9 +86,11 @@ struct BeamSelection final {
 
 /// The best continuations of every group of beams: logits [groups, beams, vocabulary],
 /// scores [groups, beams] the log-probabilities of the beams so far.  The total of a token
-/// is its beam's score plus log_softmax(logits), in double and -infinity where that is NaN;
-/// picks (at most 64, as beams) are the largest totals of a group, of equal ones the lowest
-/// beam, its largest logit and lowest token first.
+/// is its beam's score plus log_softmax(logits), -infinity where that is NaN; picks (at most
+/// 64, as beams) are the largest totals of a group, of equal ones the lowest beam, its largest
+/// logit and lowest token first.  Totals are added in double to a log-sum whose exponentials
+/// are of the logits' dtype: of Float32 logits it is mostly off by less than 1e-7 (spar_hip.h
+/// has the bound), and two beams' totals that are closer may come in either order.
 ///   end_token  ends a sequence; none where not given
 ///   ended      Int32 [groups, beams]: beams that are not 0 have ended and go on with the
 ///              end token alone (which must be given), at their score

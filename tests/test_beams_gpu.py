@@ -252,3 +252,33 @@ def test_orders_in_long_parts(hip, dtype, order):
     logits = np.broadcast_to(row, (1, beams, v)).astype(dtype)
     scores = -40.0 * np.arange(beams)[None]
     check(hip, logits, scores, 64)
+
+
+@pytest.mark.parametrize("dtype", [F32, F64])
+@pytest.mark.parametrize("vocabulary", [700, 20011])
+def test_rows_closer_than_rounding(hip, dtype, vocabulary):
+    """Beams with the same logits in other orders: which of them comes first is up to the
+    rounding of their sums, but nothing further off than that is chosen or left out, and every
+    call chooses alike."""
+    beams, picks = 6, 20
+    rng = np.random.default_rng(33)
+    row = (3 * rng.standard_normal(vocabulary)).astype(dtype)
+    logits = np.stack([np.stack([row[rng.permutation(vocabulary)] for _ in range(beams)])
+                       for _ in range(3)])
+    scores = np.full((3, beams), -2.0)
+    totals = scores[..., None] + logits - oracle.log_sums(logits)[..., None]
+    off = oracle.select_bound(logits, dtype)
+    got = select(hip, logits, scores, picks)
+    for again in range(2):
+        for x, y in zip(select(hip, logits, scores, picks), got):
+            assert np.array_equal(x, y)
+    for g in range(3):
+        at = got[1][g] - g * beams, got[2][g]
+        assert len(set(zip(*at))) == picks
+        chosen = totals[g][at]
+        assert (np.abs(got[0][g] - chosen) <= off + half_step(dtype) * np.abs(chosen)).all()
+        assert (np.diff(got[0][g]) <= 0).all()
+        assert (chosen[:-1] >= chosen[1:] - 2 * off).all()
+        rest = totals[g].copy()
+        rest[at] = -np.inf
+        assert rest.max() <= chosen.min() + 2 * off
