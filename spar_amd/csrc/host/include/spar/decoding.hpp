@@ -44,7 +44,8 @@ struct CacheRotation final {
 /// cache, whose rows are the batch's sequences; with a rotation the keys are turned on the
 /// way, and with queries [batch, query heads, tokens, extent] these are turned in the same
 /// launch and returned, in the order of their tokens and heads (nothing without queries,
-/// which need a rotation).
+/// which need a rotation).  The cache's keys and values must not overlap each other (nor be
+/// expanded) or what is written to them.
 ///   places  Int32 or Int64 [batch, tokens]: the token of its sequence's row that each new
 ///           token becomes; negative or behind the row's room for one that is not written
 ///           (padding).  The rest of the cache stays as it is.  Two tokens must not share a

@@ -50,6 +50,21 @@ std::size_t validate_cache(const PagedCache& cache, const Tensor& heads, const c
   return extent_of(table, 0);
 }
 
+// A cache that is written: every element has a place of its own.
+void validate_written(const PagedCache& cache, const char* name) {
+  if (cache.key.numel() == 0) return;
+  for (const Tensor* tensor : {&cache.key, &cache.value}) {
+    for (std::size_t axis{0}; axis < 3; ++axis) {
+      if (extent_of(*tensor, axis) > 1 && tensor->strides()[axis] == 0) {
+        refuse(name, "needs caches whose tokens have places of their own");
+      }
+    }
+  }
+  if (first_element(cache.key) == first_element(cache.value)) {
+    refuse(name, "needs keys and values at places of their own");
+  }
+}
+
 // A cache as kernels read it; `table` is what keeps a packed table alive.
 SparHipPages pages_of(const PagedCache& cache, std::optional<Tensor>& table) {
   SparHipPages pages{heads_of(cache.key), heads_of(cache.value), extent_of(cache.key, 0),
@@ -106,6 +121,7 @@ std::optional<Tensor> cache_append(const PagedCache& cache, const Tensor& key,
     q = readable(*query);
     output = ordered_like(*q);
   }
+  validate_written(cache, name);
   const Tensor k{readable(key)}, v{readable(value)};
   const bool dense{places.numel() == 0 || tokens == 1 || places.strides()[1] == 1};
   const Tensor at{dense ? places : places.contiguous()};

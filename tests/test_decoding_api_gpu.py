@@ -312,3 +312,26 @@ def test_refusals(sp):
             put(sp, np.zeros((1, 65), F32)), 2)
     refused("equally many", sp.reorder, [scores, logits.narrow(0, 0, 1)], places)
     refused("rows", sp.reorder, [sp.sum(scores)], places)
+
+
+def test_caches_are_written_at_places_of_their_own(sp):
+    """Expanded caches, and one tensor for keys and values, are read but not written."""
+    b, hk, d, page = 2, 2, 16, 4
+    pool = [put(sp, random((6, hk, page, d), F32, 5 + i)) for i in range(2)]
+    one = [x.narrow(1, 0, 1).expand([6, hk, page, d]) for x in pool]
+    table = put(sp, np.arange(6, dtype=np.int32).reshape(2, 3))
+    x = put(sp, np.ones((b, hk, 1, d), F32))
+    places = put(sp, np.zeros((b, 1), np.int32))
+    for key, value in ((one[0], pool[1]), (pool[0], one[1]), (pool[0], pool[0]),
+                       (pool[0].narrow(0, 0, 1).expand([6, hk, page, d]), pool[1]),
+                       (pool[0].narrow(2, 0, 1).expand([6, hk, page, d]), pool[1])):
+        with pytest.raises(ValueError, match="places of their own"):
+            sp.cache_append(sp.PagedCache(key, value, table), x, x, places)
+    got = get(sp, sp.cache_attention(x, sp.PagedCache(*one, table)))
+    shared = [np.broadcast_to(get(sp, x.narrow(1, 0, 1)), (6, hk, page, d)) for x in pool]
+    held = oracle.Pool(np.zeros((b, hk, 12, d), F32), np.zeros((b, hk, 12, d), F32), [12] * b, page)
+    held.table, (held.key, held.value) = get(sp, table), shared
+    want, bound = oracle.attention(np.ones((b, hk, 1, d), F32), held)
+    assert_within(got, want, bound)
+    sp.cache_append(sp.PagedCache(*pool, table), x, x, places)
+    assert (get(sp, pool[0])[[0, 3], :, 0] == 1).all() and (get(sp, pool[1])[[0, 3], :, 0] == 1).all()
