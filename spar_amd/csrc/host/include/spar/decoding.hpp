@@ -45,7 +45,8 @@ struct CacheRotation final {
 /// way, and with queries [batch, query heads, tokens, extent] these are turned in the same
 /// launch and returned, in the order of their tokens and heads (nothing without queries,
 /// which need a rotation).  The cache's keys and values must not overlap each other (nor be
-/// expanded) or what is written to them.
+/// expanded) or what is written to them; an operation with gradients that has read them reads
+/// them again, as they are then, in its backward.
 ///   places  Int32 or Int64 [batch, tokens]: the token of its sequence's row that each new
 ///           token becomes; negative or behind the row's room for one that is not written
 ///           (padding).  The rest of the cache stays as it is.  Two tokens must not share a

@@ -261,9 +261,10 @@ Tensor subtract(const Tensor& a, const Tensor& b) {
   return output;
 }
 
-// Saved operands alias the inputs (detach, no copy): device tensors are
-// never modified in place by this backend's ops, so a saved alias holds the
-// same values a clone would (elementwise.cpp:140-147 cloned them).
+// Saved operands alias the inputs (detach, no copy): of this backend's ops only
+// an optimizer's step and cache_append modify device tensors in place, and
+// unless one of them runs before the backward a saved alias holds the same
+// values a clone would (elementwise.cpp:140-147 cloned them).
 Tensor multiply(const Tensor& a, const Tensor& b) {
   const Shape output_shape{validate_binary_inputs(a, b)};
   Tensor output{binary_device(a, b, output_shape, SPAR_HIP_MULTIPLY)};
