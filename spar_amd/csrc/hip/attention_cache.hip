@@ -177,7 +177,8 @@ struct TileSpace {
 // read once for 64 rows.  Bound by the matrix units: 256 rows a key head over 16384 keys, 8
 // heads of 128, take 152 us, 113 TFLOP/s (the units are busy in 87% of the waves' lives and
 // the softmax's vector instructions take the rest); 4 * 256 tokens behind 4096, 673 us, 115
-// TFLOP/s.  Pages of 5 and 100 tokens, found key by key, take 790.
+// TFLOP/s.  Pages of 5 and 100 tokens, found key by key, take 782; so are pages of 16 where
+// tiles are 32 keys, at heads up to 64 (256 tokens behind 8192: 714 us, in pages of 32 620).
 template <typename T, int DP, Reads READS>
 __device__ __forceinline__ void tile_part(TileSpace<T, DP, READS>& space, const Call& call,
                                           const Results<T>& results, const Heads<const T>& query,
@@ -886,6 +887,8 @@ __global__ __launch_bounds__(kThreads, (tile_waves<T, DP>())) void cache_kernel(
 // Up to this many rows of a unit (and where tiles would be few) the waves of a workgroup share
 // rows and split keys; the fewest keys that repay a part: 64, 128 and 256 are within a tenth
 // of each other, now one now the other ahead; of tiles 128 take 88 us for 82 (heads of 256).
+// With 256 a prefix of 8192 tokens and 8 key heads is 256 workgroups at most, a wave per SIMD
+// (16 sequences, heads of 128: the prefix alone 38 us with the join, 14 at the units' rate).
 constexpr uint64_t kTokenRows = 32;
 constexpr uint64_t kFewestKeys = 256;
 constexpr uint64_t kFewestTokenKeys = 64;
@@ -931,9 +934,10 @@ uint64_t reads_of(const SidePlan& plan, uint64_t room) {
 // Workgroups that a side's rows are split up to, by what a CU holds of them (`waves` per
 // SIMD).
 //   Tiles: all that a CU holds where they are alone there or the other side is tiles too
-//   (256 tokens of 4 sequences, heads of 64, 602 us, half as many 658); otherwise one less,
-//   which leaves room for those that read (64 sequences behind 16384 tokens: heads of 128
-//   200 us, all that it holds 264; of 64 121 and 136; of 192 195 and 220).
+//   (256 tokens of 4 sequences, heads of 64, 602 us, half as many 658; but 16 tokens of 16
+//   sequences, heads of 128, 361 us, with one less 346); otherwise one less, which leaves room
+//   for those that read (64 sequences behind 16384 tokens: heads of 128 200 us, all that it
+//   holds 264; of 64 121 and 136; of 192 195 and 220).
 //   Few rows: one for each CU, whose four waves have enough loads in flight between them;
 //   three take 46 us for 39 (one sequence of 4096 behind 16384) to 37 for 34 (16 sequences,
 //   heads of 64), and are equal for 16 sequences with heads of 128.
@@ -1024,7 +1028,8 @@ Side<T> side_of(const SparHipCacheAttention& a, const SparHipPages& cache, const
   side.splits = static_cast<uint32_t>(plan.splits);
   side.least = static_cast<uint32_t>(plan.least);
   side.first_part = first_part;
-  // Few rows take blocks of 8 keys or of kBlock.
+  // Few rows take blocks of 8 keys or of kBlock: in pages of 8 they look for every key too, at
+  // no loss (16 sequences 61 us, in pages of 16 as well).
   side.whole = cache.table == nullptr ||
                cache.page_tokens % (plan.kind == Kind::Tiles ? block : kBlock) == 0;
   return side;
@@ -1056,7 +1061,9 @@ void start(const SparHipCacheAttention& a, const Plan& plan, const SparHipHeads&
   }
   const auto q = heads_of<const T>(query);
   const bool shared = plan.prefix.splits != 0;
-  // Only tiles ask for heads at multiples of 16 bytes.
+  // Only tiles ask for heads at multiples of 16 bytes.  Where theirs are not, everything is read
+  // element by element (one token of 16 sequences behind 8192 102 us for 62, of 64 behind 16384
+  // 334 for 211, 256 of 4 behind 4096 876 for 669).
   const auto reads_pieces = [&](const SparHipPages& pages, const SidePlan& side) {
     return side.kind != Kind::Tiles || pages_aligned<T>(pages);
   };
