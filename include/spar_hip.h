@@ -819,9 +819,9 @@ struct SparHipStatus spar_hip_launch_attention_backward(
  * negative, behind the row's room or in a page that holds nothing; the rest of the cache
  * is left as it was.  Two tokens of one call must not share a place in the pages, as they
  * do where two rows of a table name the page that both write to (beams that go on from one
- * parent): either may be found there, or a part of each.  rotary is NULL where heads are not turned; its
- * positions are apart from the places, which count from the end of a shared prefix.
- * No reference counterpart (its cache is a concatenation of tensors). */
+ * parent): either may be found there, or a part of each.  rotary is NULL where heads are
+ * not turned; its positions are apart from the places, which count from the end of a shared
+ * prefix.  No reference counterpart (its cache is a concatenation of tensors). */
 struct SparHipStatus spar_hip_launch_cache_append(
     const struct SparHipPages* cache, const struct SparHipHeads* query_output,
     const struct SparHipHeads* query, uint64_t query_heads, const struct SparHipHeads* key,

@@ -70,8 +70,8 @@ std::optional<Tensor> cache_append(const PagedCache& cache, const Tensor& key,
 ///   scale    1 / sqrt(extent) where not given
 /// Keys and values that no query sees have no part, whatever they hold; a NaN or
 /// infinity in one that some query sees may also reach other queries of its head, in a
-/// prefix those of all sequences that share it.  Calls of more queries than a launch counts
-/// are refused: behind a prefix 2^27 - 8 of all heads and sequences, otherwise 2^30 or less.
+/// prefix those of all sequences that share it.  Refused are calls of more than 2^27 - 8
+/// queries of all heads and sequences behind a prefix, of some 2^30 without one (spar_hip.h).
 [[nodiscard]] Tensor cache_attention(const Tensor& query, const PagedCache& cache,
                                      const std::optional<Tensor>& lengths = std::nullopt,
                                      const std::optional<PagedCache>& prefix = std::nullopt,
